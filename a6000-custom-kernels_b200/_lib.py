@@ -60,6 +60,15 @@ class MoeLayerDesc(ctypes.Structure):
                 ("glu_op", ctypes.c_int32), ("glu_limit", ctypes.c_float), ("norm_w", ctypes.c_int32)]
 
 
+class MoeRouter(ctypes.Structure):
+    _fields_ = [("score", ctypes.c_int32), ("n_group", ctypes.c_int32), ("topk_group", ctypes.c_int32),
+                ("group_score", ctypes.c_int32), ("norm_w", ctypes.c_int32), ("scale", ctypes.c_float)]
+
+
+class MoeMxfp4(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("n_experts", ctypes.c_int64), ("rows", ctypes.c_int64), ("K", ctypes.c_int64)]
+
+
 def _sources():
     out = []
     for d in (CSRC, os.path.join(REPO, "include")):
@@ -131,6 +140,14 @@ def _declare(L):
         "moe_b200_ep_return": (i32, [vp, i32, i64, vp, vp, vp, i64, vp, vp]),
         "moe_b200_prefill_mul_mat_id": (i32, [ctypes.POINTER(MoeTensor), vp, i64, vp, i64, i64, vp, vp, sz,
                                              ctypes.POINTER(i32), vp]),
+        "moe_b200_route_experts": (i32, [ctypes.POINTER(MoeRouter), vp, i32, i64, vp, i64, i64, i64, vp, vp, vp]),
+        "moe_b200_quantize_mxfp4": (i32, [vp, i32, i64, i64, i64, i32, vp, vp]),
+        "moe_b200_dequantize_mxfp4": (i32, [vp, i64, i64, i32, vp, i32, i64, vp]),
+        "moe_b200_mxfp4_packed_size": (sz, [i64, i64, i64]),
+        "moe_b200_mxfp4_pack": (i32, [PT, vp, sz, vp]),
+        "moe_b200_mxfp4_workspace_size": (sz, [ctypes.POINTER(MoeMxfp4), i64, i64, i32, i32]),
+        "moe_b200_mxfp4_mul_mat_id": (i32, [ctypes.POINTER(MoeMxfp4), ctypes.POINTER(MoeMxfp4), vp, vp, i32,
+                                            ctypes.c_float, vp, i32, i64, i32, i64, vp, i64, i64, i32, vp, vp, sz, vp]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(L, name)

@@ -11,6 +11,7 @@ struct LayerArgs;
 struct Layer2Args;
 struct StackArgs;
 struct MmqArgs;
+struct MxArgs;
 
 cudaError_t launch_quantize_act(int act_type, const float *x, void *y, int64_t n_rows, int64_t n_cols,
                                 cudaStream_t st);
@@ -97,5 +98,36 @@ cudaError_t launch_mmq_gather32(const uint8_t *x8, int K, int sk, int k, int ntc
                                 const int4 *chunks, const int32_t *n_chunks, int64_t max_chunks, uint8_t *btiles,
                                 uint32_t bt_stride, cudaStream_t st);
 int launch_mmq(int type, MmqArgs &a, cudaStream_t st, const char **why, cudaError_t *cuda_err);
+
+// Routing with sigmoid / softmax scores, a selection bias and expert groups
+// (moe_router.cu); n_experts <= ROUTE_MAX_EXPERTS, k <= 32, n_group <= 32
+enum : int { ROUTE_SOFTMAX = 0, ROUTE_SIGMOID = 1, ROUTE_SOFTMAX_TOPK = 2 };
+enum : int { ROUTE_GROUP_MAX = 0, ROUTE_GROUP_TOP2 = 1 };
+constexpr int ROUTE_MAX_EXPERTS = 1024;
+constexpr float ROUTE_MIN_SUM = 6.103515625e-5f;   // 2^-14
+struct RouteArgs {
+    const void *logits;      // [tok * row_stride + expert]
+    int64_t row_stride, n_tok;
+    const float *bias;       // [n_experts] or null
+    int32_t n_experts, k, score, n_group, topk_group, group_score, norm_w;
+    float scale;
+    int32_t *ids;            // [tok][k]
+    float *weights;          // [tok][k]
+};
+cudaError_t launch_route(const RouteArgs &a, int logits_type, cudaStream_t st);
+
+// MXFP4 (moe_mx.cu). Element types: MX_F32, MX_F16, MX_BF16; strides in elements.
+cudaError_t launch_mx_quantize(const void *x, int xt, int64_t stride, int64_t n_rows, int64_t n_cols, int planes,
+                               uint8_t *y, cudaStream_t st);
+cudaError_t launch_mx_dequantize(const uint8_t *y, int64_t n_rows, int64_t n_cols, int planes, void *out, int ot,
+                                 int64_t stride, cudaStream_t st);
+cudaError_t launch_mx_pack(const uint8_t *src, int64_t E, int64_t rows, int64_t K, uint8_t *dst, cudaStream_t st);
+cudaError_t launch_mx_quantize_x(const void *x, int xt, int64_t stride, int64_t n_rows, int64_t K, int planes,
+                                 uint8_t *xq, uint32_t *xs, cudaStream_t st);
+// entries per chunk, and whether the product groups the entries itself (no chunk table)
+int mx_chunk_tokens(int64_t n_tok, int64_t k, int64_t n_experts);
+bool mx_direct(int64_t n_tok, int64_t k);
+// units: entries (direct) or the largest possible number of chunks
+cudaError_t launch_mx_product(MxArgs &a, int NT, int64_t units, cudaStream_t st);
 
 }  // namespace moe

@@ -40,6 +40,7 @@
 #include "moe_layer2.cuh"
 #include "moe_stack.cuh"
 #include "moe_mmq.cuh"
+#include "moe_mx.cuh"
 #include "moe_promote.cuh"
 
 namespace {
@@ -2012,6 +2013,233 @@ int moe_b200_fill_quantized(int32_t type, void *dst, int64_t n_rows, int64_t n_c
     if (!type_supported(type)) return fail(MOE_ERR_UNSUPPORTED, "unsupported type %d", type);
     if (n_cols % blck_size(type)) return fail(MOE_ERR_INVALID, "n_cols not a multiple of the block size");
     CK(moe::launch_fill_quantized(type, dst, n_rows, n_cols, seed, sigma, reinterpret_cast<cudaStream_t>(stream)));
+    return MOE_OK;
+}
+
+}  // extern "C"
+
+// ---- MXFP4 ------------------------------------------------------------------
+namespace {
+
+int mx_elem(int32_t t) {
+    return t == MOE_TYPE_F32 ? moe::MX_F32 : t == MOE_TYPE_F16 ? moe::MX_F16 : t == MOE_TYPE_BF16 ? moe::MX_BF16 : -1;
+}
+size_t elem_size(int32_t t) { return t == MOE_TYPE_F32 ? 4 : 2; }
+bool aligned_elem(const void *p, int32_t t) { return reinterpret_cast<uintptr_t>(p) % elem_size(t) == 0; }
+
+constexpr int64_t kMxMaxBlocks = int64_t{1} << 37;   // blocks of one quantise / read-back call (grid limit)
+
+int mx_rows_check(int32_t type, const void *x, int64_t n_rows, int64_t n_cols, int64_t row_stride, int32_t planes,
+                  const void *y) {
+    if (mx_elem(type) < 0) return fail(MOE_ERR_UNSUPPORTED, "element type must be F32, F16 or BF16");
+    if (n_rows < 0 || n_cols < 32 || n_cols % 32 || n_cols > (int64_t{1} << 30))
+        return fail(MOE_ERR_INVALID, "n_cols must be a positive multiple of 32");
+    if (row_stride < n_cols) return fail(MOE_ERR_INVALID, "row stride below n_cols");
+    if (planes < 1 || planes > moe::MX_MAX_PLANES) return fail(MOE_ERR_INVALID, "planes must be 1 or 2");
+    if (n_rows > kMxMaxBlocks / (n_cols / 32)) return fail(MOE_ERR_INVALID, "too many values in one call");
+    if (n_rows && (!x || !y)) return fail(MOE_ERR_INVALID, "null argument");
+    if (!aligned_elem(x, type)) return fail(MOE_ERR_INVALID, "elements not aligned to their size");
+    return MOE_OK;
+}
+
+int64_t mx_row_tiles(int64_t rows) { return (rows + moe::MX_M - 1) / moe::MX_M; }
+int64_t mx_k_tiles(int64_t K) { return (K + moe::MX_KT - 1) / moe::MX_KT; }
+
+int mx_shape_check(int64_t E, int64_t rows, int64_t K) {
+    if (E < 1 || E > 16384 || rows < 1 || K < 32 || K % 32) return fail(MOE_ERR_INVALID, "need 1 <= n_experts <= 16384, rows >= 1, K a multiple of 32");
+    if (rows > (int64_t{1} << 24) || K > (int64_t{1} << 20)) return fail(MOE_ERR_UNSUPPORTED, "rows above 2^24 or K above 2^20");
+    return MOE_OK;
+}
+
+struct MxWs {
+    uint8_t *xq;
+    uint32_t *xs;
+    int32_t *entries, *n_chunks;
+    int4 *chunks;
+    int64_t max_chunks;
+    size_t bytes;
+};
+
+MxWs mx_ws(int64_t E, int64_t K, int64_t n_tok, int64_t k, bool per_pick, int planes, char *base) {
+    MxWs w{};
+    size_t off = 0;
+    auto take = [&](size_t bytes) { char *p = base ? base + off : nullptr; off += align256(bytes); return p; };
+    const size_t x_rows = static_cast<size_t>(per_pick ? n_tok * k : n_tok), KT = static_cast<size_t>(mx_k_tiles(K));
+    w.xq = reinterpret_cast<uint8_t *>(take(x_rows * KT * planes * 64));
+    w.xs = reinterpret_cast<uint32_t *>(take(x_rows * KT * planes * 4));
+    if (!moe::mx_direct(n_tok, k)) {
+        w.max_chunks = moe::mmq_max_chunks(n_tok * k, E, moe::mx_chunk_tokens(n_tok, k, E));
+        w.entries = reinterpret_cast<int32_t *>(take(4 * static_cast<size_t>(n_tok * k)));
+        w.chunks = reinterpret_cast<int4 *>(take(16 * static_cast<size_t>(w.max_chunks)));
+        w.n_chunks = reinterpret_cast<int32_t *>(take(4));
+    }
+    w.bytes = off;
+    return w;
+}
+
+}  // namespace
+
+extern "C" {
+
+int moe_b200_route_experts(const moe_router *r, const void *logits, int32_t logits_type, int64_t row_stride,
+                           const float *bias, int64_t n_tok, int64_t n_experts, int64_t k, int32_t *ids, float *weights,
+                           moe_stream_t stream) {
+    std::lock_guard<std::recursive_mutex> lock(g_mu);
+    if (!r) return fail(MOE_ERR_INVALID, "null argument");
+    if (mx_elem(logits_type) < 0) return fail(MOE_ERR_UNSUPPORTED, "logits must be F32, F16 or BF16");
+    if (r->score < MOE_ROUTE_SOFTMAX || r->score > MOE_ROUTE_SOFTMAX_TOPK) return fail(MOE_ERR_INVALID, "unknown score %d", r->score);
+    if (r->group_score != MOE_ROUTE_GROUP_MAX && r->group_score != MOE_ROUTE_GROUP_TOP2)
+        return fail(MOE_ERR_INVALID, "unknown group_score %d", r->group_score);
+    if (n_experts < 1 || n_experts > moe::ROUTE_MAX_EXPERTS)
+        return fail(MOE_ERR_UNSUPPORTED, "need 1 <= n_experts <= %d", moe::ROUTE_MAX_EXPERTS);
+    if (r->n_group < 1 || r->n_group > 32 || n_experts % r->n_group || r->topk_group < 1 || r->topk_group > r->n_group)
+        return fail(MOE_ERR_INVALID, "need 1 <= topk_group <= n_group <= 32, n_group dividing n_experts");
+    if (k < 1 || k > 32 || k > r->topk_group * (n_experts / r->n_group))
+        return fail(MOE_ERR_INVALID, "need 1 <= k <= min(32, the experts of topk_group groups)");
+    if (n_tok < 0 || n_tok > (int64_t{1} << 32) || row_stride < n_experts)
+        return fail(MOE_ERR_INVALID, "need 0 <= n_tok <= 2^32, row_stride >= n_experts");
+    if (n_tok == 0) return MOE_OK;
+    if (!logits || !ids || !weights || !aligned_elem(logits, logits_type)) return fail(MOE_ERR_INVALID, "null or misaligned argument");
+    moe::RouteArgs a{};
+    a.logits = logits;
+    a.row_stride = row_stride;
+    a.n_tok = n_tok;
+    a.bias = bias;
+    a.n_experts = static_cast<int32_t>(n_experts);
+    a.k = static_cast<int32_t>(k);
+    a.score = r->score;
+    a.n_group = r->n_group;
+    a.topk_group = r->topk_group;
+    a.group_score = r->group_score;
+    a.norm_w = r->norm_w;
+    a.scale = r->scale;
+    a.ids = ids;
+    a.weights = weights;
+    CK(moe::launch_route(a, mx_elem(logits_type), reinterpret_cast<cudaStream_t>(stream)));
+    return MOE_OK;
+}
+
+int moe_b200_quantize_mxfp4(const void *x, int32_t x_type, int64_t n_rows, int64_t n_cols, int64_t row_stride,
+                            int32_t planes, void *y, moe_stream_t stream) {
+    std::lock_guard<std::recursive_mutex> lock(g_mu);
+    const int rc = mx_rows_check(x_type, x, n_rows, n_cols, row_stride, planes, y);
+    if (rc) return rc;
+    CK(moe::launch_mx_quantize(x, mx_elem(x_type), row_stride, n_rows, n_cols, planes, static_cast<uint8_t *>(y),
+                               reinterpret_cast<cudaStream_t>(stream)));
+    return MOE_OK;
+}
+
+int moe_b200_dequantize_mxfp4(const void *y, int64_t n_rows, int64_t n_cols, int32_t planes, void *x, int32_t x_type,
+                              int64_t row_stride, moe_stream_t stream) {
+    std::lock_guard<std::recursive_mutex> lock(g_mu);
+    const int rc = mx_rows_check(x_type, x, n_rows, n_cols, row_stride, planes, y);
+    if (rc) return rc;
+    CK(moe::launch_mx_dequantize(static_cast<const uint8_t *>(y), n_rows, n_cols, planes, x, mx_elem(x_type), row_stride,
+                                 reinterpret_cast<cudaStream_t>(stream)));
+    return MOE_OK;
+}
+
+size_t moe_b200_mxfp4_packed_size(int64_t n_experts, int64_t rows, int64_t K) {
+    if (mx_shape_check(n_experts, rows, K)) return 0;
+    return static_cast<size_t>(n_experts * mx_row_tiles(rows) * mx_k_tiles(K)) * moe::MX_TILE;
+}
+
+int moe_b200_mxfp4_pack(const moe_tensor *src0, void *dst, size_t dst_bytes, moe_stream_t stream) {
+    std::lock_guard<std::recursive_mutex> lock(g_mu);
+    if (!src0 || !src0->data || !dst) return fail(MOE_ERR_INVALID, "null argument");
+    if (src0->type != MOE_TYPE_MXFP4) return fail(MOE_ERR_UNSUPPORTED, "expert type %d is not MXFP4", src0->type);
+    const int64_t K = src0->ne[0], rows = src0->ne[1], E = src0->ne[2];
+    const int rc = mx_shape_check(E, rows, K);
+    if (rc) return rc;
+    const uint64_t rb = static_cast<uint64_t>(K / 32) * 17;
+    if (src0->ne[3] != 1 || src0->nb[1] != rb || src0->nb[2] != rb * static_cast<uint64_t>(rows))
+        return fail(MOE_ERR_UNSUPPORTED, "expert tensor is not contiguous");
+    if (!aligned16(dst)) return fail(MOE_ERR_INVALID, "the packed matrices must be 16-byte aligned");
+    if (dst_bytes < moe_b200_mxfp4_packed_size(E, rows, K))
+        return fail(MOE_ERR_INVALID, "packed buffer too small (%zu < %zu bytes)", dst_bytes, moe_b200_mxfp4_packed_size(E, rows, K));
+    CK(moe::launch_mx_pack(static_cast<const uint8_t *>(src0->data), E, rows, K, static_cast<uint8_t *>(dst),
+                           reinterpret_cast<cudaStream_t>(stream)));
+    return MOE_OK;
+}
+
+size_t moe_b200_mxfp4_workspace_size(const moe_mxfp4 *w, int64_t n_tok, int64_t k, int32_t x_per_pick, int32_t planes) {
+    if (!w || n_tok < 0 || k < 1 || planes < 1 || planes > moe::MX_MAX_PLANES ||
+        mx_shape_check(w->n_experts, w->rows, w->K) || n_tok > (int64_t{1} << 30) / k)
+        return 0;
+    return mx_ws(w->n_experts, w->K, n_tok, k, x_per_pick != 0, planes, nullptr).bytes;
+}
+
+int moe_b200_mxfp4_mul_mat_id(const moe_mxfp4 *w, const moe_mxfp4 *gate, const float *bias, const float *gate_bias,
+                              int32_t glu_op, float glu_limit, const void *x, int32_t x_type, int64_t x_row_stride,
+                              int32_t x_per_pick, int64_t n_tok, const int32_t *ids, int64_t k, int64_t ids_stride,
+                              int32_t planes, float *dst, void *workspace, size_t workspace_bytes, moe_stream_t stream) {
+    std::lock_guard<std::recursive_mutex> lock(g_mu);
+    read_env();
+    if (!w || !w->data) return fail(MOE_ERR_INVALID, "null argument");
+    int rc = mx_shape_check(w->n_experts, w->rows, w->K);
+    if (rc) return rc;
+    if (gate && (!gate->data || gate->n_experts != w->n_experts || gate->rows != w->rows || gate->K != w->K))
+        return fail(MOE_ERR_INVALID, "the gate must have the up matrices' shape");
+    if (gate_bias && !gate) return fail(MOE_ERR_INVALID, "gate_bias without a gate");
+    if (gate && (glu_op < MOE_GLU_SWIGLU || glu_op > MOE_GLU_PRODUCT)) return fail(MOE_ERR_INVALID, "unknown glu_op %d", glu_op);
+    if (!aligned16(w->data) || (gate && !aligned16(gate->data)))
+        return fail(MOE_ERR_INVALID, "the packed matrices must be 16-byte aligned");
+    if (mx_elem(x_type) < 0) return fail(MOE_ERR_UNSUPPORTED, "x must be F32, F16 or BF16");
+    if (planes < 1 || planes > moe::MX_MAX_PLANES) return fail(MOE_ERR_INVALID, "planes must be 1 or 2");
+    if (n_tok < 0 || k < 1 || ids_stride < k || x_row_stride < w->K)
+        return fail(MOE_ERR_INVALID, "need n_tok >= 0, k >= 1, ids_stride >= k, x_row_stride >= K");
+    if (n_tok > (int64_t{1} << 30) / k) return fail(MOE_ERR_UNSUPPORTED, "too many picks in one call");
+    if (n_tok == 0) return MOE_OK;
+    if (!x || !ids || !dst || !aligned_elem(x, x_type)) return fail(MOE_ERR_INVALID, "null or misaligned argument");
+    const bool per_pick = x_per_pick != 0;
+    const MxWs s = mx_ws(w->n_experts, w->K, n_tok, k, per_pick, planes, static_cast<char *>(workspace));
+    if (!workspace || workspace_bytes < s.bytes)
+        return fail(MOE_ERR_INVALID, "workspace too small (%zu < %zu bytes)", workspace_bytes, s.bytes);
+    if (!aligned16(workspace)) return fail(MOE_ERR_INVALID, "workspace must be 16-byte aligned");
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (!g.d_err) {
+        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+        CK(cudaStreamIsCapturing(st, &cap));
+        if (cap != cudaStreamCaptureStatusNone)
+            return fail(MOE_ERR_STATE, "the first call on a device allocates the error word: make it before capture");
+    }
+    rc = ensure_device();
+    if (rc) return rc;
+    const int NT = moe::mx_chunk_tokens(n_tok, k, w->n_experts);
+    const bool direct = moe::mx_direct(n_tok, k);
+    const int64_t units = direct ? n_tok * k : s.max_chunks;
+    moe::MxArgs a{};
+    a.RT = static_cast<int32_t>(mx_row_tiles(w->rows));
+    a.KT = static_cast<int32_t>(mx_k_tiles(w->K));
+    if (units * a.RT > (int64_t{1} << 28)) return fail(MOE_ERR_UNSUPPORTED, "too many tiles in one call");
+    if (!direct)
+        CK(moe::launch_mmq_group(ids, ids_stride, static_cast<int>(n_tok), static_cast<int>(k),
+                                 static_cast<int>(w->n_experts), NT, s.entries, s.chunks, s.n_chunks, g.d_err, st, true));
+    CK(moe::launch_mx_quantize_x(x, mx_elem(x_type), x_row_stride, per_pick ? n_tok * k : n_tok, w->K, planes, s.xq, s.xs, st));
+    a.w = static_cast<const uint8_t *>(w->data);
+    a.gate = gate ? static_cast<const uint8_t *>(gate->data) : nullptr;
+    a.expert_bytes = static_cast<uint64_t>(a.RT) * a.KT * moe::MX_TILE;
+    a.bias = bias;
+    a.gate_bias = gate_bias;
+    a.n_experts = static_cast<int32_t>(w->n_experts);
+    a.rows = static_cast<int32_t>(w->rows);
+    a.glu_op = glu_op;
+    a.glu_limit = glu_limit;
+    a.xq = s.xq;
+    a.xs = s.xs;
+    a.planes = planes;
+    a.k = static_cast<int32_t>(k);
+    a.n_entries = static_cast<int32_t>(n_tok * k);
+    a.per_pick = per_pick ? 1 : 0;
+    a.ids = ids;
+    a.ids_stride = ids_stride;
+    a.entries = s.entries;
+    a.chunks = direct ? nullptr : s.chunks;
+    a.n_chunks = s.n_chunks;
+    a.dst = dst;
+    a.err = g.d_err;
+    a.timeout_ns = g.timeout_ns_kernel;
+    CK(moe::launch_mx_product(a, NT, units, st));
     return MOE_OK;
 }
 

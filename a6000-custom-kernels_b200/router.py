@@ -1,0 +1,58 @@
+"""Routing tokens to experts with the scores of current MoE routers
+(moe_b200_route_experts in include/moe_cache_b200.h)."""
+import ctypes
+
+import torch
+
+from ._call import ELEM, On, dense_rows, need
+from ._lib import MoeRouter, check, lib
+
+SCORES = {"softmax": 0, "sigmoid": 1, "softmax_topk": 2}
+GROUP_SCORES = {"max": 0, "top2": 1}
+
+
+class Router:
+    """How a layer routes: `score` "softmax" (over all experts), "sigmoid" or
+    "softmax_topk" (over the picks); `bias` f32 [n_experts] that only the choice
+    sees; `n_group` groups of consecutive experts, of which the `topk_group`
+    best stay (by their largest selection score, "max", or the sum of their two
+    largest, "top2"); `norm_w` divides the weights by their sum, `scale`
+    multiplies them."""
+
+    def __init__(self, k, score="softmax", bias=None, n_group=1, topk_group=1, group_score="top2", norm_w=False, scale=1.0):
+        need(score in SCORES, f"score must be one of {sorted(SCORES)}")
+        need(group_score in GROUP_SCORES, f"group_score must be one of {sorted(GROUP_SCORES)}")
+        need(bias is None or (isinstance(bias, torch.Tensor) and bias.is_cuda and bias.dtype == torch.float32 and
+                              bias.dim() == 1 and bias.is_contiguous()), "bias must be a contiguous f32 CUDA vector")
+        self.k, self.bias = k, bias
+        self.desc = MoeRouter(SCORES[score], n_group, topk_group, GROUP_SCORES[group_score], int(norm_w), scale)
+        self.ref = ctypes.byref(self.desc)
+
+    def __call__(self, logits, ids=None, weights=None, stream=None):
+        """logits f32 / f16 / bf16 [n_tok, E] -> (ids i32 [n_tok, k], weights f32 [n_tok, k])."""
+        stride, _ = dense_rows(logits, "logits", ELEM)
+        need(logits.dim() == 2, "logits must be [n_tok, n_experts]")
+        n_tok, E = logits.shape
+        dev = logits.device
+        need(self.bias is None or (self.bias.device == dev and self.bias.numel() == E), "bias must be f32 [n_experts] on the logits' device")
+        with On(dev, stream) as st:
+            if ids is None:
+                ids = torch.empty((n_tok, self.k), dtype=torch.int32, device=dev)
+            if weights is None:
+                weights = torch.empty((n_tok, self.k), dtype=torch.float32, device=dev)
+            for name, t, dt in (("ids", ids, torch.int32), ("weights", weights, torch.float32)):
+                need(t.dtype == dt and t.device == dev and t.is_contiguous() and tuple(t.shape) == (n_tok, self.k),
+                     f"{name} must be contiguous {dt} [n_tok, k] on the logits' device")
+            check(lib().moe_b200_route_experts(self.ref, logits.data_ptr(), ELEM[logits.dtype], max(stride, E),
+                                               None if self.bias is None else self.bias.data_ptr(), n_tok, E, self.k,
+                                               ids.data_ptr(), weights.data_ptr(), st))
+        return ids, weights
+
+
+def route_experts(logits, k, score="softmax", bias=None, n_group=1, topk_group=1, group_score="top2", norm_w=False,
+                  scale=1.0, ids=None, weights=None, stream=None):
+    """One routing call (see Router): (ids i32 [n_tok, k], weights f32 [n_tok, k])."""
+    return Router(k, score, bias, n_group, topk_group, group_score, norm_w, scale)(logits, ids, weights, stream)
+
+
+__all__ = ["Router", "route_experts"]

@@ -32,9 +32,9 @@ typedef struct CUstream_st *moe_stream_t;   /* same type as cudaStream_t */
 
 /* ggml_type numbering (ggml.h) for the formats of the path */
 enum {
-    MOE_TYPE_F32 = 0, MOE_TYPE_Q4_0 = 2, MOE_TYPE_Q5_0 = 6, MOE_TYPE_Q8_0 = 8, MOE_TYPE_Q8_1 = 9,
+    MOE_TYPE_F32 = 0, MOE_TYPE_F16 = 1, MOE_TYPE_Q4_0 = 2, MOE_TYPE_Q5_0 = 6, MOE_TYPE_Q8_0 = 8, MOE_TYPE_Q8_1 = 9,
     MOE_TYPE_Q2_K = 10, MOE_TYPE_Q3_K = 11, MOE_TYPE_Q4_K = 12, MOE_TYPE_Q5_K = 13,
-    MOE_TYPE_Q6_K = 14, MOE_TYPE_Q8_K = 15,
+    MOE_TYPE_Q6_K = 14, MOE_TYPE_Q8_K = 15, MOE_TYPE_BF16 = 30, MOE_TYPE_MXFP4 = 39,
 };
 
 /* GLU ops of the fused gate/up epilogue (moe-cache.cu:264-280). The shim maps
@@ -456,6 +456,102 @@ int moe_b200_noalloc_device_error(moe_stream_t stream, int32_t *code);
  * quantizer (the same algorithm as the CPU oracle's). */
 int moe_b200_fill_quantized(int32_t type, void *dst, int64_t n_rows, int64_t n_cols, uint64_t seed,
                             float sigma, moe_stream_t stream);
+
+/* ---- routing (no counterpart in the reference: upstream graph ops) ---------
+ * Router of a MoE layer beyond moe_b200_topk_softmax: scores s of the experts
+ * from the logits l, a selection score c = s + bias, groups, top-k, weights. */
+enum { MOE_ROUTE_SOFTMAX = 0,        /* s = softmax over all experts */
+       MOE_ROUTE_SIGMOID = 1,        /* s = 1 / (1 + exp(-l)) */
+       MOE_ROUTE_SOFTMAX_TOPK = 2 }; /* s = l; weights = softmax over the picks' logits */
+enum { MOE_ROUTE_GROUP_MAX = 0,      /* a group's score: its largest c */
+       MOE_ROUTE_GROUP_TOP2 = 1 };   /* the sum of its two largest c */
+typedef struct {
+    int32_t score;                 /* MOE_ROUTE_* */
+    int32_t n_group, topk_group;   /* n_group groups of consecutive experts, the topk_group best stay (1, 1: no groups) */
+    int32_t group_score;           /* MOE_ROUTE_GROUP_* */
+    int32_t norm_w;                /* divide the k weights by their sum, which counts as at least 2^-14 */
+    float   scale;                 /* then multiply them by this */
+} moe_router;
+
+/* Route n_tok tokens: ids[t][k] the picks in order of c (descending, ties to
+ * the lower id; so are ties of groups), weights[t][k] their scores without the
+ * bias, normalised and scaled as `r` says. logits: [n_tok] rows of n_experts
+ * values of logits_type (MOE_TYPE_F32, _F16 or _BF16), row_stride elements
+ * apart; bias f32 [n_experts] or NULL. Where a bias or groups enter, the ranking
+ * is computed in 64 bits. A logit of +inf counts as the largest number; an
+ * expert whose logit is -inf or NaN, whose bias is -inf or NaN, or whose group
+ * fell out has c = -inf: it is picked only when fewer than k others are left
+ * (lowest ids first), with weight 0. n_experts <= 1024, n_group <= 32, k <=
+ * min(32, experts of topk_group groups). n_tok may be 0. */
+int moe_b200_route_experts(const moe_router *r, const void *logits, int32_t logits_type, int64_t row_stride,
+                           const float *bias, int64_t n_tok, int64_t n_experts, int64_t k, int32_t *ids, float *weights,
+                           moe_stream_t stream);
+
+/* ---- MXFP4 experts (no counterpart in the reference) ---------------------
+ * MXFP4 is ggml's 4-bit microscaled type: blocks of 32 values in 17 bytes, one
+ * scale byte e (the block's scale is 2^(e - 127); 255 makes every value NaN),
+ * then 16 bytes of e2m1 codes (magnitudes 0, 0.5, 1, 1.5, 2, 3, 4, 6; bit 3 is
+ * the sign), value j in the low nibble of byte j and value j + 16 in its high
+ * nibble. The MUL_MAT_ID GEMV, the layer kernels and the hot-expert cache
+ * handle the eight formats of the reference's op; MXFP4 expert tensors run
+ * through moe_b200_mxfp4_mul_mat_id for one token and for prompts alike. */
+
+/* Quantise n_rows rows of n_cols values (x_type MOE_TYPE_F32, _F16 or _BF16;
+ * n_cols a multiple of 32, row_stride in elements) into y: planes x n_rows
+ * rows of n_cols / 32 blocks, contiguous. e = floor(log2 of the block's largest
+ * magnitude) - 2 + 127, at least 0; codes are the nearest of value / scale,
+ * ties to the even code, saturating at 6. A block with an infinity or a NaN
+ * becomes NaN. planes = 2: plane 1 holds, quantised the same way, what plane 0
+ * leaves of x (the difference is exact), so that the planes' sum is about ten
+ * times closer to x than plane 0. n_rows may be 0. */
+int moe_b200_quantize_mxfp4(const void *x, int32_t x_type, int64_t n_rows, int64_t n_cols, int64_t row_stride,
+                            int32_t planes, void *y, moe_stream_t stream);
+
+/* The values that quantised rows stand for: x = the planes' values added in
+ * 32 bits, rounded once to x_type. Layouts as moe_b200_quantize_mxfp4. */
+int moe_b200_dequantize_mxfp4(const void *y, int64_t n_rows, int64_t n_cols, int32_t planes, void *x, int32_t x_type,
+                              int64_t row_stride, moe_stream_t stream);
+
+/* Expert matrices laid out for the tensor cores (see moe_b200_mxfp4_pack):
+ * data 16-byte aligned, moe_b200_mxfp4_packed_size bytes. */
+typedef struct {
+    const void *data;
+    int64_t     n_experts, rows, K;
+} moe_mxfp4;
+
+/* moe_b200_mxfp4_packed_size: bytes of the laid-out form of n_experts matrices
+ * of rows x K values (K a multiple of 32; 0 for a shape the path does not
+ * take): 128-row by 128-value tiles of 8,704 bytes, the last ones padded with
+ * zeros. moe_b200_mxfp4_pack writes it from a contiguous MXFP4 expert tensor
+ * in ggml's layout (device memory, no alignment asked of src0); done once per
+ * tensor, src0 is not needed afterwards. */
+size_t moe_b200_mxfp4_packed_size(int64_t n_experts, int64_t rows, int64_t K);
+int moe_b200_mxfp4_pack(const moe_tensor *src0, void *dst, size_t dst_bytes, moe_stream_t stream);
+
+/* MUL_MAT_ID of MXFP4 experts, any n_tok:
+ *   dst[(t * k + p) * rows + r] = row r of expert ids[t * ids_stride + p] . x
+ * (+ bias[expert][r]), with x's row t, or t * k + p with x_per_pick, quantised
+ * to `planes` MXFP4 planes (1 or 2) as moe_b200_quantize_mxfp4 does. With
+ * `gate` (the shape of w) the GLU is fused: dst = GLU(gate . x + gate_bias,
+ * w . x + bias), glu_op and glu_limit as in moe_fusion_device. x_type
+ * MOE_TYPE_F32, _F16 or _BF16, x_row_stride in elements; biases f32
+ * [n_experts][rows] or NULL. Products run on the 4-bit tensor cores (both
+ * operands MXFP4, 32-bit accumulators); sums over a shared K are added in a
+ * fixed order, so equal calls give equal bits.
+ * An id of -1 marks an empty slot: its row of dst is left as it was. Any other
+ * id outside [0, n_experts) also leaves its row and sets the device error word
+ * (MOE_DERR_BAD_ID). A NaN or an infinity in a block of x makes that row's
+ * outputs NaN and no other's. n_tok may be 0.
+ * Workspace: moe_b200_mxfp4_workspace_size bytes of device memory, 16-byte
+ * aligned, no initialisation needed; calls that overlap on the GPU must not
+ * share one, captured graphs included. Allocates nothing, except that the
+ * first call of a process makes the device error word: not during stream
+ * capture (MOE_ERR_STATE). */
+size_t moe_b200_mxfp4_workspace_size(const moe_mxfp4 *w, int64_t n_tok, int64_t k, int32_t x_per_pick, int32_t planes);
+int moe_b200_mxfp4_mul_mat_id(const moe_mxfp4 *w, const moe_mxfp4 *gate, const float *bias, const float *gate_bias,
+                              int32_t glu_op, float glu_limit, const void *x, int32_t x_type, int64_t x_row_stride,
+                              int32_t x_per_pick, int64_t n_tok, const int32_t *ids, int64_t k, int64_t ids_stride,
+                              int32_t planes, float *dst, void *workspace, size_t workspace_bytes, moe_stream_t stream);
 
 #ifdef __cplusplus
 }
