@@ -145,7 +145,7 @@ def _declare(L):
         "moe_b200_dequantize_mxfp4": (i32, [vp, i64, i64, i32, vp, i32, i64, vp]),
         "moe_b200_mxfp4_packed_size": (sz, [i64, i64, i64]),
         "moe_b200_mxfp4_pack": (i32, [PT, vp, sz, vp]),
-        "moe_b200_mxfp4_workspace_size": (sz, [ctypes.POINTER(MoeMxfp4), i64, i64, i32, i32]),
+        "moe_b200_mxfp4_workspace_size": (sz, [ctypes.POINTER(MoeMxfp4), i64, i64, i32]),
         "moe_b200_mxfp4_mul_mat_id": (i32, [ctypes.POINTER(MoeMxfp4), ctypes.POINTER(MoeMxfp4), vp, vp, i32,
                                             ctypes.c_float, vp, i32, i64, i32, i64, vp, i64, i64, i32, vp, vp, sz, vp]),
     }

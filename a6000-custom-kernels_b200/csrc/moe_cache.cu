@@ -2046,30 +2046,32 @@ int64_t mx_row_tiles(int64_t rows) { return (rows + moe::MX_M - 1) / moe::MX_M; 
 int64_t mx_k_tiles(int64_t K) { return (K + moe::MX_KT - 1) / moe::MX_KT; }
 
 int mx_shape_check(int64_t E, int64_t rows, int64_t K) {
-    if (E < 1 || E > 16384 || rows < 1 || K < 32 || K % 32) return fail(MOE_ERR_INVALID, "need 1 <= n_experts <= 16384, rows >= 1, K a multiple of 32");
+    if (E < 1 || rows < 1 || K < 32 || K % 32) return fail(MOE_ERR_INVALID, "need n_experts >= 1, rows >= 1, K a positive multiple of 32");
+    if (E > moe::mx_max_experts()) return fail(MOE_ERR_UNSUPPORTED, "more than %d experts", static_cast<int>(moe::mx_max_experts()));
     if (rows > (int64_t{1} << 24) || K > (int64_t{1} << 20)) return fail(MOE_ERR_UNSUPPORTED, "rows above 2^24 or K above 2^20");
     return MOE_OK;
 }
 
 struct MxWs {
-    uint8_t *xq;
-    uint32_t *xs;
-    int32_t *entries, *n_chunks;
+    uint8_t *images;
+    int32_t *entries, *n_chunks, *where;
     int4 *chunks;
     int64_t max_chunks;
     size_t bytes;
 };
 
-MxWs mx_ws(int64_t E, int64_t K, int64_t n_tok, int64_t k, bool per_pick, int planes, char *base) {
+MxWs mx_ws(int64_t E, int64_t K, int64_t n_tok, int64_t k, int planes, char *base) {
     MxWs w{};
     size_t off = 0;
     auto take = [&](size_t bytes) { char *p = base ? base + off : nullptr; off += align256(bytes); return p; };
-    const size_t x_rows = static_cast<size_t>(per_pick ? n_tok * k : n_tok), KT = static_cast<size_t>(mx_k_tiles(K));
-    w.xq = reinterpret_cast<uint8_t *>(take(x_rows * KT * planes * 64));
-    w.xs = reinterpret_cast<uint32_t *>(take(x_rows * KT * planes * 4));
-    if (!moe::mx_direct(n_tok, k)) {
-        w.max_chunks = moe::mmq_max_chunks(n_tok * k, E, moe::mx_chunk_tokens(n_tok, k, E));
+    const bool direct = moe::mx_direct(n_tok, k);
+    const int NT = moe::mx_chunk_tokens(n_tok, k, E);
+    w.max_chunks = direct ? n_tok * k : moe::mmq_max_chunks(n_tok * k, E, NT);
+    const size_t images = static_cast<size_t>(moe::mx_images_bytes(w.max_chunks, NT, K, planes));
+    w.images = reinterpret_cast<uint8_t *>(take(images));
+    if (!direct) {
         w.entries = reinterpret_cast<int32_t *>(take(4 * static_cast<size_t>(n_tok * k)));
+        w.where = reinterpret_cast<int32_t *>(take(4 * static_cast<size_t>(n_tok * k)));
         w.chunks = reinterpret_cast<int4 *>(take(16 * static_cast<size_t>(w.max_chunks)));
         w.n_chunks = reinterpret_cast<int32_t *>(take(4));
     }
@@ -2162,11 +2164,11 @@ int moe_b200_mxfp4_pack(const moe_tensor *src0, void *dst, size_t dst_bytes, moe
     return MOE_OK;
 }
 
-size_t moe_b200_mxfp4_workspace_size(const moe_mxfp4 *w, int64_t n_tok, int64_t k, int32_t x_per_pick, int32_t planes) {
+size_t moe_b200_mxfp4_workspace_size(const moe_mxfp4 *w, int64_t n_tok, int64_t k, int32_t planes) {
     if (!w || n_tok < 0 || k < 1 || planes < 1 || planes > moe::MX_MAX_PLANES ||
         mx_shape_check(w->n_experts, w->rows, w->K) || n_tok > (int64_t{1} << 30) / k)
         return 0;
-    return mx_ws(w->n_experts, w->K, n_tok, k, x_per_pick != 0, planes, nullptr).bytes;
+    return mx_ws(w->n_experts, w->K, n_tok, k, planes, nullptr).bytes;
 }
 
 int moe_b200_mxfp4_mul_mat_id(const moe_mxfp4 *w, const moe_mxfp4 *gate, const float *bias, const float *gate_bias,
@@ -2192,7 +2194,7 @@ int moe_b200_mxfp4_mul_mat_id(const moe_mxfp4 *w, const moe_mxfp4 *gate, const f
     if (n_tok == 0) return MOE_OK;
     if (!x || !ids || !dst || !aligned_elem(x, x_type)) return fail(MOE_ERR_INVALID, "null or misaligned argument");
     const bool per_pick = x_per_pick != 0;
-    const MxWs s = mx_ws(w->n_experts, w->K, n_tok, k, per_pick, planes, static_cast<char *>(workspace));
+    const MxWs s = mx_ws(w->n_experts, w->K, n_tok, k, planes, static_cast<char *>(workspace));
     if (!workspace || workspace_bytes < s.bytes)
         return fail(MOE_ERR_INVALID, "workspace too small (%zu < %zu bytes)", workspace_bytes, s.bytes);
     if (!aligned16(workspace)) return fail(MOE_ERR_INVALID, "workspace must be 16-byte aligned");
@@ -2207,15 +2209,11 @@ int moe_b200_mxfp4_mul_mat_id(const moe_mxfp4 *w, const moe_mxfp4 *gate, const f
     if (rc) return rc;
     const int NT = moe::mx_chunk_tokens(n_tok, k, w->n_experts);
     const bool direct = moe::mx_direct(n_tok, k);
-    const int64_t units = direct ? n_tok * k : s.max_chunks;
+    const int64_t units = s.max_chunks;
     moe::MxArgs a{};
     a.RT = static_cast<int32_t>(mx_row_tiles(w->rows));
     a.KT = static_cast<int32_t>(mx_k_tiles(w->K));
-    if (units * a.RT > (int64_t{1} << 28)) return fail(MOE_ERR_UNSUPPORTED, "too many tiles in one call");
-    if (!direct)
-        CK(moe::launch_mmq_group(ids, ids_stride, static_cast<int>(n_tok), static_cast<int>(k),
-                                 static_cast<int>(w->n_experts), NT, s.entries, s.chunks, s.n_chunks, g.d_err, st, true));
-    CK(moe::launch_mx_quantize_x(x, mx_elem(x_type), x_row_stride, per_pick ? n_tok * k : n_tok, w->K, planes, s.xq, s.xs, st));
+    if (units >= (int64_t{1} << 19) || units * a.RT > (int64_t{1} << 28)) return fail(MOE_ERR_UNSUPPORTED, "too many tiles in one call");
     a.w = static_cast<const uint8_t *>(w->data);
     a.gate = gate ? static_cast<const uint8_t *>(gate->data) : nullptr;
     a.expert_bytes = static_cast<uint64_t>(a.RT) * a.KT * moe::MX_TILE;
@@ -2225,8 +2223,8 @@ int moe_b200_mxfp4_mul_mat_id(const moe_mxfp4 *w, const moe_mxfp4 *gate, const f
     a.rows = static_cast<int32_t>(w->rows);
     a.glu_op = glu_op;
     a.glu_limit = glu_limit;
-    a.xq = s.xq;
-    a.xs = s.xs;
+    a.images = s.images;
+    a.where = s.where;
     a.planes = planes;
     a.k = static_cast<int32_t>(k);
     a.n_entries = static_cast<int32_t>(n_tok * k);
@@ -2239,6 +2237,7 @@ int moe_b200_mxfp4_mul_mat_id(const moe_mxfp4 *w, const moe_mxfp4 *gate, const f
     a.dst = dst;
     a.err = g.d_err;
     a.timeout_ns = g.timeout_ns_kernel;
+    CK(moe::launch_mx_prep(x, mx_elem(x_type), x_row_stride, per_pick ? n_tok * k : n_tok, w->K, a, NT, st));
     CK(moe::launch_mx_product(a, NT, units, st));
     return MOE_OK;
 }

@@ -169,6 +169,12 @@ __device__ __forceinline__ uint64_t l2_evict_first_policy() {
     return p;
 }
 
+__device__ __forceinline__ uint64_t l2_evict_last_policy() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+
 // sum of 4 (unsigned byte of a) * (signed byte of b) + c
 __device__ __forceinline__ int dp4a_us(uint32_t a, int b, int c) {
     int d;

@@ -422,12 +422,6 @@ __device__ __forceinline__ MmqTile mmq_tile(const int4 ch, int ti, int row_block
     return T;
 }
 
-__device__ __forceinline__ uint64_t l2_evict_last_policy() {
-    uint64_t p;
-    asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
-    return p;
-}
-
 // Bounded wait that also gives up once another role has aborted; a timeout
 // aborts the block.
 __device__ __forceinline__ bool mmq_wait(MmqCtrl &C, uint64_t *bar, uint32_t parity, const MmqArgs &a) {

@@ -4,6 +4,9 @@
 #include "moe_mmq.cuh"
 #include "moe_mx.cuh"
 
+#include <algorithm>
+#include <type_traits>
+
 #include <cuda_bf16.h>
 
 namespace moe {
@@ -243,40 +246,14 @@ __global__ void mx_pack_kernel(const uint8_t *__restrict__ src, int rows, int nb
 }
 
 // ---------------------------------------------------------------------------
-// quantise the product's activations: per x row, K tile and plane 64 bytes of
-// codes and 4 scale bytes, K padded to whole tiles with zeros
-// ---------------------------------------------------------------------------
-template <int XT, bool VEC>
-__global__ void __launch_bounds__(256) mx_quantize_x_kernel(const typename MxElem<XT>::T *__restrict__ x,
-                                                            int64_t stride, int64_t n_rows, int nb, int KT, int planes,
-                                                            uint8_t *__restrict__ xq, uint8_t *__restrict__ xs) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int64_t g = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 2;   // (row, block), K padded
-    const int i = threadIdx.x & 3;
-    const int64_t row = g / (KT * 4);
-    const int b = static_cast<int>(g - row * (KT * 4));
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (row < n_rows && b < nb) {
-        const typename MxElem<XT>::T *p = x + row * stride + static_cast<int64_t>(b) * 32 + 4 * i;
-        mx_load4<XT, VEC>(p, v);
-        mx_load4<XT, VEC>(p + 16, v + 4);
-    }
-    for (int pl = 0; pl < planes; ++pl) {
-        uint32_t byte;
-        const uint32_t w = mx_quant_block(v, byte);
-        if (row < n_rows) {
-            const int64_t at = (row * KT + b / 4) * planes + pl;
-            *reinterpret_cast<uint32_t *>(xq + at * 64 + (b % 4) * 16 + 4 * i) = w;
-            if (i == 0) xs[at * 4 + b % 4] = static_cast<uint8_t>(byte);
-        }
-        if (pl + 1 < planes) mx_residual(v, w, byte);
-    }
-}
-
-// ---------------------------------------------------------------------------
 // The grouped product
 // ---------------------------------------------------------------------------
-constexpr int MXP_THREADS = 192;   // warp 0: weights, warp 1: MMA, warps 2-5: activations, then the epilogue
+// Per chunk width NT (entries = MMA N): groups of 4 epilogue warps (behind warp
+// 0, copies, and warp 1, MMA)
+template <int NT> __host__ __device__ constexpr int mxp_epi() { return NT >= 64 ? 2 : 1; }
+template <int NT> __host__ __device__ constexpr int mxp_threads() { return 64 + 128 * mxp_epi<NT>(); }
+constexpr int MXP_TPS = 2;   // K tiles per ring stage: halves what a stage costs the two issuing warps
+constexpr int MXP_WIDE = 96; // the widest chunk: two matrices' accumulators, twice, in 384 TMEM columns
 
 // Instruction descriptor of kind::mxf4: e2m1 A and B (K-major), UE8M0 scales,
 // M = 128, N; `half` picks the pair of scale bytes of the tile's K = 64 half.
@@ -285,31 +262,57 @@ __device__ __forceinline__ uint32_t mx_idesc(int N, int half) {
            (1u << 23) | (static_cast<uint32_t>(MX_M >> 4) << 24) | (static_cast<uint32_t>(2 * half) << 29);
 }
 
-__device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+// Shared-memory descriptors (K-major, no swizzle, 8-row groups 128 bytes apart)
+// as their two words: the low one holds the address and the distance of the
+// 16-byte chunks along K, the high one is the same for every operand here.
+constexpr uint32_t MX_DESC_HI = (128u >> 4) | (1u << 14);
+__device__ __forceinline__ uint32_t mx_desc_lo(uint32_t saddr, uint32_t lbo) {
+    return ((saddr >> 4) & 0x3FFFu) | ((lbo >> 4) << 16);   // (in a cluster the address also holds the CTA's rank)
+}
+
+// The tcgen05 instructions below are issued by the lane whose `on` is set, all
+// lanes of the warp calling: with a predicate instead of a branch the control
+// flow stays uniform, and the operands -- which the hardware takes from uniform
+// registers -- are computed there instead of being moved one by one.
+__device__ __forceinline__ void umma_mxf4(uint32_t on, uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,
                                           uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 q, %8, 0;\n\t"
+        "mov.b64 da, {%1, %7};\n\tmov.b64 db, {%2, %7};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], da, db, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(MX_DESC_HI), "r"(on)
         : "memory");
 }
 
 // 512 scale bytes (32 rows of 16) from shared memory to 4 TMEM columns of all four lane quarters
-__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint32_t saddr) {
-    const uint64_t desc = umma_desc(saddr, 0u, 128u);
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+__device__ __forceinline__ void tmem_cp_scales(uint32_t on, uint32_t taddr, uint32_t lo) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t.reg .b64 d;\n\tsetp.ne.b32 q, %3, 0;\n\tmov.b64 d, {%1, %2};\n\t"
+        "@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], d;\n\t}" ::"r"(taddr), "r"(lo), "r"(MX_DESC_HI), "r"(on)
+        : "memory");
 }
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// bulk copy global -> shared, and the barrier's arrival that announces its bytes
+__device__ __forceinline__ void bulk_g2s_if(uint32_t on, uint32_t dst, const void *src, uint32_t bytes, uint32_t bar,
+                                            uint64_t policy) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;\n\t}"
+        ::"r"(dst), "l"(src), "r"(bytes), "r"(bar), "l"(policy), "r"(on)
+        : "memory");
 }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ void mbar_expect_if(uint32_t on, uint32_t bar, uint32_t bytes) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+        "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes), "r"(on)
+        : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void umma_commit_if(uint32_t on, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(on)
+        : "memory");
+}
 
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -327,21 +330,274 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t saddr, uint32_t rank) {
     return v;
 }
 
+// ---------------------------------------------------------------------------
+// What the product needs first: its entries grouped into chunks (up to NT
+// entries of one expert), and per chunk the entries' quantised rows as the MMA
+// reads them -- an image: per K tile and plane, with N = the chunk's entries
+// rounded up to 16, 16-byte chunk c of entry j at c * 16 N + j * 16, then 512
+// bytes of scales (block c of entry j at (j % 32) * 16 + (j / 32) * 4 + c). A
+// tile's planes are contiguous, so the product fetches them with one bulk
+// copy; a row that k experts picked is quantised once and written k times.
+// (Gathering rows inside the product, 16 bytes at a time by four warps, cost
+// about 1,000 cycles per tile against the 250 that its MMAs take.)
+//
+// Up to MX_DIRECT entries nothing is grouped beforehand: an entry that is number
+// 0, NT, 2 NT, ... of its expert's entries leads a chunk, whose index is the
+// entry's own, and every CTA works that out for itself.
+// ---------------------------------------------------------------------------
+constexpr int MXG_CTAS = 8;         // CTAs (one cluster) that group
+constexpr int MXG_THREADS = 1024;   // at most
+constexpr int MXG_MAX_EXPERTS = 4096;
+
+__host__ __device__ constexpr int mx_round16(int n) { return (n + 15) / 16 * 16; }
+__host__ __device__ constexpr uint32_t mx_image_plane(int N) { return 64u * N + MX_SF; }          // bytes of one tile's plane
+__host__ __device__ constexpr uint64_t mx_image_bytes(int NT, int KT, int planes) {               // between chunks
+    return static_cast<uint64_t>(KT) * planes * mx_image_plane(NT);
+}
+
+struct MxPrep {
+    const void *x;
+    int64_t stride, n_rows;
+    int32_t nb, KT, planes, per_pick;
+    uint8_t *images;
+    const int32_t *ids;
+    int64_t ids_stride;
+    int32_t n_entries, k, n_experts, NT;
+    int32_t *entries, *n_chunks, *where;   // chunked form: mx_where of each entry, -1: left out
+    int4 *chunks;
+    int *err;
+};
+
+// an entry's chunk, its place there and the chunk's N, in one word (chunks < 2^19, N <= 256)
+__device__ __forceinline__ int mx_where(int chunk, int place, int N) { return (chunk << 12) | ((N / 16 - 1) << 8) | place; }
+
+// Grouping by one cluster of MXG_CTAS: each CTA counts its share of the entries
+// per expert in shared memory, reads the other CTAs' counts, and places its
+// entries behind theirs. Chunks of an expert are consecutive. Order inside an
+// expert changes no result. Id -1: left out.
+__global__ void __cluster_dims__(MXG_CTAS, 1, 1) __launch_bounds__(MXG_THREADS) mx_group_kernel(const MxPrep a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    extern __shared__ int group_smem[];
+    __shared__ int scratch[64];
+    int *cnt = group_smem, *cur = cnt + a.n_experts, *ch0 = cur + a.n_experts, *ex0 = ch0 + a.n_experts,
+        *tot = ex0 + a.n_experts;
+    const int tid = threadIdx.x, nth = blockDim.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = blockIdx.x, E = a.n_experts, N = a.n_entries;
+    for (int e = tid; e < E; e += nth) cnt[e] = 0;
+    __syncthreads();
+    auto id_of = [&](int i) {
+        if (i >= N) return -1;
+        const int t = i / a.k;
+        const int x = a.ids[static_cast<int64_t>(t) * a.ids_stride + (i - t * a.k)];
+        if (x >= 0 && x < E) return x;
+        if (x != -1) set_error(a.err, DERR_BAD_ID);
+        return -1;
+    };
+    // shared-memory atomics; one per warp where all its entries are of one expert (a token's picks
+    // differ, so otherwise at most 32 / k lanes meet)
+    auto add = [&](int *c, int x) {
+        const int x0 = __shfl_sync(0xffffffffu, x, 0);
+        if (__all_sync(0xffffffffu, x == x0)) {
+            int base = 0;
+            if (x0 >= 0 && lane == 0) base = atomicAdd(&c[x0], 32);
+            return __shfl_sync(0xffffffffu, base, 0) + lane;
+        }
+        return x >= 0 ? atomicAdd(&c[x], 1) : 0;
+    };
+    constexpr int KEEP = 4;   // ids kept in registers
+    int x[KEEP];
+#pragma unroll
+    for (int m = 0; m < KEEP; ++m) x[m] = id_of((m * MXG_CTAS + rank) * nth + tid);
+#pragma unroll
+    for (int m = 0; m < KEEP; ++m)
+        if ((m * MXG_CTAS + rank) * nth < N) add(cnt, x[m]);
+    for (int64_t i0 = static_cast<int64_t>(KEEP * MXG_CTAS + rank) * nth; i0 < N; i0 += MXG_CTAS * nth)
+        add(cnt, id_of(static_cast<int>(i0) + tid));
+    __syncthreads();
+    cluster_sync();
+    int carry_e = 0, carry_c = 0;
+    for (int base = 0; base < E; base += nth) {
+        const int e = base + tid;
+        int total = 0, before = 0;
+        if (e < E)
+#pragma unroll
+            for (int c = 0; c < MXG_CTAS; ++c) {
+                const int v = __float_as_int(ld_cluster_f32(smem_u32(&cnt[e]), c));
+                if (c < rank) before += v;
+                total += v;
+            }
+        const int nc = (total + a.NT - 1) / a.NT;
+        int se = total, sc = nc;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int oe = __shfl_up_sync(0xffffffffu, se, off), oc = __shfl_up_sync(0xffffffffu, sc, off);
+            if (lane >= off) { se += oe; sc += oc; }
+        }
+        if (lane == 31) { scratch[warp] = se; scratch[32 + warp] = sc; }
+        __syncthreads();
+        // every warp scans the warps' sums
+        int we = lane < nth / 32 ? scratch[lane] : 0, wc = lane < nth / 32 ? scratch[32 + lane] : 0;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int oe = __shfl_up_sync(0xffffffffu, we, off), oc = __shfl_up_sync(0xffffffffu, wc, off);
+            if (lane >= off) { we += oe; wc += oc; }
+        }
+        const int pe = carry_e + (warp ? __shfl_sync(0xffffffffu, we, (warp - 1) & 31) : 0);
+        const int pc = carry_c + (warp ? __shfl_sync(0xffffffffu, wc, (warp - 1) & 31) : 0);
+        carry_e += __shfl_sync(0xffffffffu, we, 31);
+        carry_c += __shfl_sync(0xffffffffu, wc, 31);
+        __syncthreads();
+        if (e < E) {
+            const int first = pe + se - total, c0 = pc + sc - nc;
+            ex0[e] = first;
+            tot[e] = total;
+            ch0[e] = c0;
+            cur[e] = first + before;
+            for (int q = rank; q < nc; q += MXG_CTAS)
+                a.chunks[c0 + q] = make_int4(e, first + q * a.NT, min(a.NT, total - q * a.NT), 0);
+        }
+    }
+    if (rank == 0 && tid == 0) *a.n_chunks = carry_c;
+    __syncthreads();
+    auto place = [&](int i, int xi) {
+        const int at = add(cur, xi);
+        if (xi >= 0) {
+            a.entries[at] = i;
+            const int pos = at - ex0[xi], q = pos / a.NT;
+            a.where[i] = mx_where(ch0[xi] + q, pos - q * a.NT, mx_round16(min(a.NT, tot[xi] - q * a.NT)));
+        } else if (i < N) {
+            a.where[i] = -1;
+        }
+    };
+#pragma unroll
+    for (int m = 0; m < KEEP; ++m) {
+        const int i0 = (m * MXG_CTAS + rank) * nth;
+        if (i0 < N) place(i0 + tid, x[m]);
+    }
+    for (int64_t i0 = static_cast<int64_t>(KEEP * MXG_CTAS + rank) * nth; i0 < N; i0 += MXG_CTAS * nth)
+        place(static_cast<int>(i0) + tid, id_of(static_cast<int>(i0) + tid));
+    cluster_sync();   // the counts stay until every CTA has read them
+}
+
+// The direct form's chunk of entry i: the entries of its expert among all
+// (bits of `same`), its place in the chunk and the chunk's size. A whole warp
+// calls with entries i and i + 32 of lane i's ids x0, x1.
+__device__ __forceinline__ uint64_t mx_same(int x0, int x1, int e) {
+    return __ballot_sync(0xffffffffu, x0 == e) | (static_cast<uint64_t>(__ballot_sync(0xffffffffu, x1 == e)) << 32);
+}
+__device__ __forceinline__ int mx_before(uint64_t same, int i) { return __popcll(same & ((1ull << i) - 1ull)); }
+__device__ __forceinline__ int mx_id(const int32_t *ids, int64_t stride, int n_entries, int k, int i) {
+    return i < n_entries ? ids[(i / k) * stride + i % k] : -2;
+}
+
+// Quantise x and write the images: 4 lanes per block, 16 per K tile of a row.
+template <int XT, bool VEC, bool DIRECT>
+__global__ void __launch_bounds__(256) mx_images_kernel(const MxPrep a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __shared__ int where_s[MX_DIRECT];
+    __shared__ __align__(16) int id_s[MX_DIRECT];
+    const int lane = threadIdx.x & 31;
+    if (DIRECT) {
+        const int t = threadIdx.x;
+        if (t < MX_DIRECT) id_s[t] = mx_id(a.ids, a.ids_stride, a.n_entries, a.k, t);
+        __syncthreads();
+        if (t < a.n_entries) {   // entry t's expert among all entries
+            const int e = id_s[t];
+            uint64_t same = 0;
+#pragma unroll
+            for (int j = 0; j < MX_DIRECT; j += 4) {
+                const int4 v = *reinterpret_cast<const int4 *>(id_s + j);
+                same |= static_cast<uint64_t>((v.x == e ? 1u : 0u) | (v.y == e ? 2u : 0u) | (v.z == e ? 4u : 0u) |
+                                              (v.w == e ? 8u : 0u)) << j;
+            }
+            const int pos = mx_before(same, t), lead = pos / a.NT * a.NT;
+            uint64_t rest = same;                     // the lead: the set bit that `lead` set bits precede
+            for (int j = 0; j < lead; ++j) rest &= rest - 1;
+            where_s[t] = e >= 0 && e < a.n_experts
+                             ? mx_where(__ffsll(static_cast<long long>(rest)) - 1, pos - lead,
+                                        mx_round16(min(__popcll(same) - lead, a.NT)))
+                             : -1;
+        }
+        __syncthreads();
+    }
+    const int64_t g = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 2;   // (row, block), K padded
+    const int i = threadIdx.x & 3;
+    const int64_t row = g / (a.KT * 4);
+    const int b = static_cast<int>(g - row * (a.KT * 4)), tile = b >> 2;
+    const bool row_ok = row < a.n_rows;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (row_ok && b < a.nb) {
+        const typename MxElem<XT>::T *p = static_cast<const typename MxElem<XT>::T *>(a.x) + row * a.stride +
+                                          static_cast<int64_t>(b) * 32 + 4 * i;
+        mx_load4<XT, VEC>(p, v);
+        mx_load4<XT, VEC>(p + 16, v + 4);
+    }
+    uint32_t w[MX_MAX_PLANES][4], sc[MX_MAX_PLANES];
+#pragma unroll
+    for (int pl = 0; pl < MX_MAX_PLANES; ++pl) {
+        if (pl >= a.planes) break;
+        uint32_t byte;
+        const uint32_t mine = mx_quant_block(v, byte);
+        if (pl + 1 < a.planes) mx_residual(v, mine, byte);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[pl][j] = __shfl_sync(0xffffffffu, mine, (lane & ~3) + j);   // the block's 16 bytes
+        uint32_t word = byte << (8 * ((lane >> 2) & 3));                                          // the tile's 4 scales
+        word |= __shfl_xor_sync(0xffffffffu, word, 4);
+        word |= __shfl_xor_sync(0xffffffffu, word, 8);
+        sc[pl] = word;
+    }
+    if (!DIRECT) asm volatile("griddepcontrol.wait;" ::: "memory");   // the grouping
+    if (!row_ok) return;
+    const int n_dst = a.per_pick ? 1 : a.k;
+    const int64_t en0 = row * n_dst;
+    const uint64_t image = mx_image_bytes(a.NT, a.KT, a.planes);
+    // lane i of the 4 serves destinations i, i + 4, ..., lane l of the tile's 16 the scales of l, l + 16, ...
+    auto plane_at = [&](int64_t en, int &j, int &N) -> uint8_t * {
+        const int at = DIRECT ? where_s[en] : a.where[en];
+        if (at < 0) return nullptr;
+        j = at & 255;
+        N = (((at >> 8) & 15) + 1) * 16;
+        return a.images + static_cast<uint64_t>(at >> 12) * image + static_cast<uint64_t>(tile) * a.planes * mx_image_plane(N);
+    };
+    for (int q = i; q < n_dst; q += 4) {
+        int j, N;
+        uint8_t *t = plane_at(en0 + q, j, N);
+        if (!t) continue;
+#pragma unroll
+        for (int pl = 0; pl < MX_MAX_PLANES; ++pl)
+            if (pl < a.planes)
+                *reinterpret_cast<uint4 *>(t + pl * mx_image_plane(N) + (b & 3) * 16 * N + j * 16) =
+                    make_uint4(w[pl][0], w[pl][1], w[pl][2], w[pl][3]);
+    }
+    for (int q = lane & 15; q < n_dst; q += 16) {
+        int j, N;
+        uint8_t *t = plane_at(en0 + q, j, N);
+        if (!t) continue;
+#pragma unroll
+        for (int pl = 0; pl < MX_MAX_PLANES; ++pl)
+            if (pl < a.planes)
+                *reinterpret_cast<uint32_t *>(t + pl * mx_image_plane(N) + 64 * N + (j & 31) * 16 + (j >> 5) * 4) = sc[pl];
+    }
+}
+
+// One lane of the converged warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 template <int NT>
 struct MxCtl {
-    uint64_t a_full[MX_MAX_STAGES], b_full[MX_MAX_STAGES], empty[MX_MAX_STAGES], done;
+    uint64_t full[MX_MAX_STAGES], empty[MX_MAX_STAGES], acc_full[2], acc_empty[2], drain;
     uint32_t tmem;
     int32_t abort, expert, count;
     int32_t entry[NT];
 };
 
 template <int NT>
-__host__ __device__ constexpr uint32_t mx_lbo() { return 16u * NT + 16u; }   // 16 bytes past a power of two: no bank conflicts
-template <int NT>
-__host__ __device__ constexpr uint32_t mx_b_bytes() { return (4u * mx_lbo<NT>() + MX_SF + 127u) / 128u * 128u; }
-template <int NT>
 __host__ __device__ constexpr uint32_t mx_stage_bytes(int mats, int planes) {
-    return mats * MX_TILE + planes * mx_b_bytes<NT>();
+    return MXP_TPS * (mats * MX_TILE + planes * mx_image_plane(NT));
 }
 
 template <int NT>
@@ -358,71 +614,95 @@ __device__ __forceinline__ bool mx_wait(MxCtl<NT> &C, uint64_t *bar, uint32_t pa
         }
     }
 }
+// the same for a whole warp: the lanes agree
+template <int NT>
+__device__ __forceinline__ bool mx_wait_warp(MxCtl<NT> &C, uint64_t *bar, uint32_t parity, const MxArgs &a) {
+    return __all_sync(0xffffffffu, mx_wait(C, bar, parity, a)) != 0;
+}
 
-// One CTA: 128 weight rows (of w, and of gate with GLU) x the up to NT entries
-// of one chunk x this cluster rank's share of K.
-//   warp 0    one lane streams the weight tiles, one bulk copy each (a tile is
-//             contiguous and already in the MMA's layout);
-//   warp 1    one lane copies each tile's scales to tensor memory and issues
-//             the MMAs, D += A B_plane over the planes;
-//   warps 2-5 bring the entries' quantised rows (cp.async, 16-byte chunks),
-//             then read the accumulators (thread = weight row) and store.
-// With split > 1 the ranks' partial sums meet in shared memory and are added
-// in rank order, so results do not depend on timing.
-template <int NT, bool GLU, bool DIRECT>
-__global__ void __launch_bounds__(MXP_THREADS) mx_product_kernel(const MxArgs a) {
+// The GLU ops of glu_apply for the epilogue, which is issue bound: exp and the
+// quotient by the approximate units, 2 + |1.2 g| and 2 units in the last place.
+__device__ __forceinline__ float mx_sigmoid_times(float x, float t) { return __fdividef(x, 1.0f + __expf(-t)); }
+template <int OP>
+__device__ __forceinline__ float mx_glu(float g, float up, float limit) {
+    if constexpr (OP == 0) return up * mx_sigmoid_times(g, g);
+    else if constexpr (OP == 2) {
+        const float x = fminf(g, 7.0f);
+        return mx_sigmoid_times(x, 1.702f * x) * (fmaxf(fminf(up, 7.0f), -7.0f) + 1.0f);
+    } else if constexpr (OP == 3) {
+        const float x = fminf(g, limit);
+        return mx_sigmoid_times(x, x) * fmaxf(fminf(up, limit), -limit);
+    } else return glu_apply(OP, g, up, limit);
+}
+
+// Work item: 128 weight rows (of w, and of gate with GLU) x the up to NT
+// entries of one chunk x this cluster rank's share of K. A CTA walks items
+// blockIdx / split, + gridDim / split, ... with its roles running ahead of one
+// another through the ring and the accumulators:
+//   warp 0    streams tiles by bulk copies: the weights' (contiguous and already
+//             in the MMA's layout, as is the chunk's image);
+//   warp 1    copies each tile's scales to tensor memory and issues the MMAs,
+//             D += A B_plane over the planes;
+//   the rest  in groups of 4 warps that take 16 columns in turn, read the
+//             accumulators (thread = weight row), add biases, apply the GLU and
+//             store, while the next item multiplies.
+// With split > 1 a cluster's CTAs have one item each; their partial sums meet in
+// shared memory and are added in rank order, so results do not depend on timing.
+// PAIR (the widest chunks, no GLU): an item is two row tiles of w, so that the
+// image is fetched once for both.
+template <int NT, bool GLU, bool DIRECT, int PLANES>
+__global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxArgs a) {
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ MxCtl<NT> C;
-    constexpr int MATS = GLU ? 2 : 1;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    constexpr bool PAIR = !GLU && NT == MXP_WIDE;
+    constexpr int MATS = GLU || PAIR ? 2 : 1, MXP_EPI = mxp_epi<NT>();
+    const int RI = PAIR ? (a.RT + 1) / 2 : a.RT;   // items of a chunk
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int rank = a.split > 1 ? static_cast<int>(cluster_rank()) : 0;
-    const int unit = blockIdx.x / a.split;
-    const int rt = unit % a.RT, chunk = unit / a.RT;
+    const int item0 = blockIdx.x / a.split, item_step = gridDim.x / a.split;
 
-    // ids and the chunk table are complete before the launch of the quantiser
-    // that this one overlaps with; only the quantised rows wait for its end
-    if (!DIRECT) {
-        const bool have = chunk < *a.n_chunks;   // (the grid covers the largest possible table)
-        if (tid < NT) {
-            const int4 ch = have ? a.chunks[chunk] : make_int4(0, 0, 0, 0);
-            if (tid == 0) { C.expert = ch.x; C.count = ch.z; }
-            if (tid < ch.z) C.entry[tid] = a.entries[ch.y + tid];
-        }
-    } else if (warp == 0) {
-        // entry `chunk` leads a chunk when it is number 0, NT, 2 NT, ... of its expert's entries
-        auto id_of = [&](int i) {
-            return i < a.n_entries ? a.ids[(i / a.k) * a.ids_stride + i % a.k] : -2;
-        };
-        const int x0 = id_of(lane), x1 = id_of(lane + 32);
-        const int e = __shfl_sync(0xffffffffu, chunk < 32 ? x0 : x1, chunk & 31);
-        const uint64_t same = __ballot_sync(0xffffffffu, x0 == e) |
-                              (static_cast<uint64_t>(__ballot_sync(0xffffffffu, x1 == e)) << 32);
-        const auto before = [&](int i) { return __popcll(same & ((1ull << i) - 1ull)); };
-        const int pos = before(chunk);
+    if (DIRECT && warp == 0) {
+        // (ids are complete before the launch that this one overlaps with; the images are not)
+        const int lead = item0 / RI;
+        const int x0 = mx_id(a.ids, a.ids_stride, a.n_entries, a.k, lane);
+        const int x1 = mx_id(a.ids, a.ids_stride, a.n_entries, a.k, lane + 32);
+        const int e = __shfl_sync(0xffffffffu, lead < 32 ? x0 : x1, lead & 31);
+        const uint64_t same = mx_same(x0, x1, e);
+        const int pos = mx_before(same, lead);
         const bool ok = e >= 0 && e < a.n_experts;
         const int count = ok && pos % NT == 0 ? min(__popcll(same) - pos, NT) : 0;
         if (!ok && e != -1 && lane == 0) set_error(a.err, DERR_BAD_ID);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int i = lane + 32 * h, n = before(i) - pos;
+            const int i = lane + 32 * h, n = mx_before(same, i) - pos;
             if (((same >> i) & 1ull) && n >= 0 && n < count) C.entry[n] = i;
         }
         if (lane == 0) { C.expert = e; C.count = count; }
     }
-    if (tid == 0) {
+    if (tid == 32) {
         for (int s = 0; s < a.stages; ++s) {
-            mbar_init(&C.a_full[s], 1);
-            mbar_init(&C.b_full[s], 4);
+            mbar_init(&C.full[s], 1);
             mbar_init(&C.empty[s], 1);
         }
-        mbar_init(&C.done, 1);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&C.acc_full[s], 1);
+            mbar_init(&C.acc_empty[s], 4 * MXP_EPI);
+        }
+        mbar_init(&C.drain, 1);
         C.abort = 0;
         fence_mbar_init();
     }
     __syncthreads();
-    const int count = C.count, expert = C.expert;
-    if (count == 0) {   // the same for every rank of the cluster
+    int n_items = 0;
+    if (DIRECT) {
+        n_items = C.count > 0 ? item0 + 1 : 0;   // one item per CTA
+    } else {
         asm volatile("griddepcontrol.wait;" ::: "memory");
+        n_items = *a.n_chunks * RI;
+    }
+    if (item0 >= n_items) {   // nothing here; the same for every rank of the cluster
+        if (DIRECT) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
     if (warp == 1) {
@@ -431,163 +711,292 @@ __global__ void __launch_bounds__(MXP_THREADS) mx_product_kernel(const MxArgs a)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    const int kt0 = a.KT * rank / a.split, n_it = a.KT * (rank + 1) / a.split - kt0;
-    const int planes = a.planes, stages = a.stages;
-    const uint32_t stage_bytes = mx_stage_bytes<NT>(MATS, planes);
+    const int kt0 = a.KT * rank / a.split, n_kt = a.KT * (rank + 1) / a.split - kt0;   // this rank's K tiles,
+    const int n_it = (n_kt + MXP_TPS - 1) / MXP_TPS;                                   // MXP_TPS to a stage
+    constexpr int planes = PLANES;
+    const int stages = a.stages, acc = a.acc;
+    constexpr uint32_t stage_bytes = mx_stage_bytes<NT>(MATS, planes);
     const uint32_t ring0 = smem_u32(ring);
-
-    int fills = 0;   // weight copies issued by this thread
-    auto fill = [&](int until) {
-        // weights depend on nothing that the launches before write: stream at once
-        const uint64_t pol = l2_evict_first_policy();
-        const uint64_t at = static_cast<uint64_t>(expert) * a.expert_bytes +
-                            (static_cast<uint64_t>(rt) * a.KT + kt0) * MX_TILE;
-        for (; fills < until; ++fills) {
-            const int i = fills, s = i % stages;
-            if (i >= stages && !mx_wait(C, &C.empty[s], ((i / stages) - 1) & 1, a)) return;
-            mbar_arrive_expect_tx(&C.a_full[s], MATS * MX_TILE);
-            uint8_t *dst = ring + s * stage_bytes;
-            bulk_g2s(dst, a.w + at + static_cast<uint64_t>(i) * MX_TILE, MX_TILE, &C.a_full[s], pol);
-            if (GLU) bulk_g2s(dst + MX_TILE, a.gate + at + static_cast<uint64_t>(i) * MX_TILE, MX_TILE, &C.a_full[s], pol);
+    struct Item { int rt, chunk, expert, count, first, mats; };
+    auto item_at = [&](int item) {
+        Item I;
+        I.chunk = item / RI;
+        I.rt = item - I.chunk * RI;
+        I.mats = MATS;
+        if (PAIR) {
+            I.rt *= 2;
+            if (I.rt + 1 >= a.RT) I.mats = 1;
         }
+        if (DIRECT) {
+            I.expert = C.expert; I.count = C.count; I.first = 0;
+        } else {
+            const int4 ch = a.chunks[I.chunk];
+            I.expert = ch.x; I.first = ch.y; I.count = ch.z;
+        }
+        return I;
     };
-    if (warp == 0 && lane == 0) fill(n_it < stages ? n_it : stages);   // what the ring holds, before anything else
+    auto entry_of = [&](const Item &I, int j) { return DIRECT ? C.entry[j] : a.entries[I.first + j]; };
+
+    // warp 0: stages issued so far, and the ring's next stage
+    int fills = 0;
+    uint32_t w_stage = 0, w_phase = 0;
+    const uint32_t full0 = smem_u32(C.full);
+    auto tiles_of = [&](int i) { return min(MXP_TPS, n_kt - i * MXP_TPS); };
+    // stage: the weight tiles, the gate's, then the image's
+    auto fill_weights = [&](uint32_t on, uint64_t at, int mats, int i, uint32_t image_tile, uint64_t pol) {
+        const uint32_t n = tiles_of(i), dst = ring0 + w_stage * stage_bytes, bar = full0 + 8 * w_stage;
+        at += static_cast<uint64_t>(i) * (MXP_TPS * MX_TILE);
+        mbar_expect_if(on, bar, n * (mats * MX_TILE + image_tile));
+        bulk_g2s_if(on, dst, a.w + at, n * MX_TILE, bar, pol);
+        if (MATS == 2 && mats == 2)
+            bulk_g2s_if(on, dst + MXP_TPS * MX_TILE, GLU ? a.gate + at : a.w + at + static_cast<uint64_t>(a.KT) * MX_TILE,
+                        n * MX_TILE, bar, pol);
+    };
+    auto weights_at = [&](const Item &I) {
+        return static_cast<uint64_t>(I.expert) * a.expert_bytes + (static_cast<uint64_t>(I.rt) * a.KT + kt0) * MX_TILE;
+    };
+    const uint32_t on = elect_one() ? 1u : 0u;   // the lane that issues for its warp
+    int early = 0;
+    if (DIRECT && warp == 0) {   // weights depend on nothing that the launch before writes: what the ring holds, at once
+        const Item I = item_at(item0);
+        early = n_it < stages ? n_it : stages;
+        const uint64_t pol = l2_evict_first_policy();
+        for (w_stage = 0; static_cast<int>(w_stage) < early; ++w_stage)
+            fill_weights(on, weights_at(I), I.mats, w_stage, planes * mx_image_plane(mx_round16(I.count)), pol);
+        w_stage = 0;
+        __syncwarp();
+    }
     tc_fence_before();
     __syncthreads();   // the tensor memory's address
     tc_fence_after();
-    const uint32_t tmem = C.tmem;
-    const int N = (count + 15) / 16 * 16;
-    const uint32_t sf0 = tmem + MATS * NT;                                     // scale columns, a slot per stage
-    const uint32_t sf_slot = 4u * (MATS + planes);
+    const uint32_t tmem = __shfl_sync(0xffffffffu, C.tmem, 0);
 
-    if (warp == 0 && lane == 0) {
-        fill(n_it);
-    } else if (warp == 1 && lane == 0) {
+    if (warp == 0) {
+        if (DIRECT) asm volatile("griddepcontrol.wait;" ::: "memory");
+        const uint64_t pol_w = l2_evict_first_policy(), pol_x = l2_evict_last_policy();
         bool ok = true;
-        for (int i = 0; i < n_it && ok; ++i) {
-            const int s = i % stages;
-            const uint32_t ph = (i / stages) & 1;
-            ok = mx_wait(C, &C.a_full[s], ph, a) && mx_wait(C, &C.b_full[s], ph, a);
-            if (!ok) break;
+        for (int item = item0; item < n_items && ok; item += item_step) {
+            const Item I = item_at(item);
+            const uint32_t tile = __shfl_sync(0xffffffffu, planes * mx_image_plane(mx_round16(I.count)), 0);
+            const uint64_t wat = weights_at(I);
+            const int mats = __shfl_sync(0xffffffffu, I.mats, 0);
+            const uint8_t *image = a.images + static_cast<uint64_t>(I.chunk) * mx_image_bytes(NT, a.KT, planes) +
+                                   static_cast<uint64_t>(kt0) * tile;
+            for (int i = 0; i < n_it; ++i) {
+                if (fills >= stages) {
+                    ok = mx_wait_warp(C, &C.empty[w_stage], w_phase ^ 1u, a);
+                    if (!ok) break;
+                }
+                if (i >= early) fill_weights(on, wat, mats, i, tile, pol_w);
+                bulk_g2s_if(on, ring0 + w_stage * stage_bytes + MXP_TPS * MATS * MX_TILE, image, tiles_of(i) * tile,
+                            full0 + 8 * w_stage, pol_x);
+                image += MXP_TPS * tile;
+                ++fills;
+                if (++w_stage == static_cast<uint32_t>(stages)) { w_stage = 0; w_phase ^= 1u; }
+            }
+        }
+    } else if (warp == 1) {
+        const uint32_t sf0 = tmem + static_cast<uint32_t>(acc * MATS * NT);   // scale columns, a slot per stage
+        constexpr uint32_t SFB = 4;                                             // columns of a plane's scales
+        constexpr uint32_t sf_tile = 4u * MATS + SFB * planes, sf_slot = MXP_TPS * sf_tile;
+        const uint32_t empty0 = smem_u32(C.empty), acc0 = smem_u32(C.acc_full);
+        uint32_t s = 0, ph = 0, n = 0;
+        bool ok = true;
+        Item next = item_at(item0);
+        for (int item = item0; item < n_items && ok; item += item_step, ++n) {
+            const uint32_t ab = acc == 2 ? n & 1u : 0u, aph = acc == 2 ? (n >> 1) & 1u : n & 1u;
+            const Item I = next;
+            if (item + item_step < n_items) next = item_at(item + item_step);      // asked for one item ahead
+            const int N = __shfl_sync(0xffffffffu, mx_round16(I.count), 0);
+            const int mats = __shfl_sync(0xffffffffu, I.mats, 0);
+            if (n >= static_cast<uint32_t>(acc)) ok = mx_wait_warp(C, &C.acc_empty[ab], aph ^ 1u, a);
+            const uint32_t id0 = mx_idesc(N, 0), id1 = mx_idesc(N, 1);
+            const uint32_t d0 = tmem + ab * (MATS * NT);
+            const uint32_t bp = mx_image_plane(N) >> 4, bh = 2u * N;   // next plane, next K = 64 (descriptor units)
+            bool ready = false;
+            for (int i = 0; i < n_it && ok; ++i) {
+                if (!ready) ok = mx_wait_warp(C, &C.full[s], ph, a);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t A = ring0 + s * stage_bytes, B = A + MXP_TPS * MATS * MX_TILE, sf = sf0 + s * sf_slot;
+                const uint32_t al = mx_desc_lo(A, 16 * MX_M), bl = mx_desc_lo(B, 16 * N);
+                const uint32_t asf = mx_desc_lo(A + MX_CODES, 0u), bsf = mx_desc_lo(B + 64 * N, 0u);
+                // in descriptor units: next tile, next matrix, next K = 64
+                constexpr uint32_t AT = MX_TILE >> 4, AM = MXP_TPS * AT, AH = (2 * 16 * MX_M) >> 4;
+                const int n = tiles_of(i);
+                const uint32_t free_bar = empty0 + 8 * s;
+                if (++s == static_cast<uint32_t>(stages)) { s = 0; ph ^= 1u; }
+#pragma unroll
+                for (int t = 0; t < MXP_TPS; ++t) {
+                    // the next stage's barrier is looked at while this one's first MMAs run
+                    if (t == MXP_TPS - 1) ready = i + 1 < n_it && __all_sync(0xffffffffu, mbar_test_wait(&C.full[s], ph));
+                    if (t >= n) break;
+                    const uint32_t sft = sf + t * sf_tile, bt = t * planes * bp;
+#pragma unroll
+                    for (int m = 0; m < MATS; ++m)
+                        if (m < mats) tmem_cp_scales(on, sft + 4 * m, asf + t * AT + m * AM);
+#pragma unroll
+                    for (int p = 0; p < planes; ++p) {
+                        tmem_cp_scales(on, sft + 4 * MATS + SFB * p, bsf + bt + p * bp);
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int p = 0; p < planes; ++p)
+#pragma unroll
+                            for (int m = 0; m < MATS; ++m)
+                                if (m < mats)
+                                    umma_mxf4(on, d0 + m * NT, al + t * AT + m * AM + h * AH, bl + bt + p * bp + h * bh,
+                                              h ? id1 : id0, sft + 4 * m, sft + 4 * MATS + SFB * p,
+                                              t + h + p > 0 || i > 0 ? 1u : 0u);
+                }
+                umma_commit_if(on, free_bar);
+            }
+            if (ok) umma_commit_if(on, acc0 + 8 * ab);
+        }
+        if (!ok) {   // a wait ran out: the MMAs in flight end before the memory they use goes
+            if (elect_one()) {
+                umma_commit(&C.drain);
+                if (!mbar_wait_bounded(&C.drain, 0, drain_limit_ns(a.timeout_ns))) set_error(a.err, DERR_DRAIN);
+            }
+            __syncwarp();
+        }
+    } else {
+        // ---- epilogue -------------------------------------------------------
+        // Thread = weight row. Group g takes columns 16 (g + EPI q), round q. All of them go to
+        // registers first: the accumulators are free for the next item but one at once.
+        const int grp = (warp - 2) >> 2;
+        const int quarter = warp & 3;                 // TMEM lanes this warp may read
+        const int r = 32 * quarter + lane;            // weight row of the tile
+        constexpr int ROUNDS = (NT + 16 * MXP_EPI - 1) / (16 * MXP_EPI);
+        uint32_t n = 0;
+        Item next = item_at(item0);
+        for (int item = item0; item < n_items; item += item_step, ++n) {
+            const uint32_t ab = acc == 2 ? n & 1u : 0u, aph = acc == 2 ? (n >> 1) & 1u : n & 1u;
+            const Item I = next;
+            if (item + item_step < n_items) next = item_at(item + item_step);
+            const int row = I.rt * MX_M + r;
+            const bool row_ok = row < a.rows, row2_ok = PAIR && row + MX_M < a.rows;
+            auto bias_of = [&](const float *b, int at) { return b[static_cast<int64_t>(I.expert) * a.rows + at]; };
+            const float bu = a.bias && row_ok ? bias_of(a.bias, row) : 0.f;
+            const float bg = GLU ? (a.gate_bias && row_ok ? bias_of(a.gate_bias, row) : 0.f)
+                                 : (PAIR && a.bias && row2_ok ? bias_of(a.bias, row + MX_M) : 0.f);
+            float *out = a.dst + row;
+            // lane j: entry of column j of each round, asked for before the wait
+            int ens[ROUNDS];
+#pragma unroll
+            for (int q = 0; q < ROUNDS; ++q) {
+                const int c = 16 * (grp + MXP_EPI * q) + (lane & 15);
+                ens[q] = c < I.count ? entry_of(I, c) : 0;
+            }
+            if (!mx_wait_warp(C, &C.acc_full[ab], aph, a)) break;
             tc_fence_after();
-            const uint32_t A = ring0 + s * stage_bytes, B = A + MATS * MX_TILE, sf = sf0 + s * sf_slot;
+            const uint32_t cols = tmem + ab * (MATS * NT) + (static_cast<uint32_t>(32 * quarter) << 16);
+            auto column0 = [&](int q) { return 16 * (grp + MXP_EPI * q); };
+            auto load = [&](int q, uint32_t (&u)[16], uint32_t (&gt)[16]) {
+                if (column0(q) < I.count) {
+                    tmem_ld16(cols + column0(q), u);
+                    if (GLU || (PAIR && I.mats == 2)) tmem_ld16(cols + NT + column0(q), gt);
+                }
+            };
+            auto release = [&]() {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&C.acc_empty[ab]);
+            };
+            // one round's results in place of its accumulators
+            auto finish = [&](uint32_t (&u)[16], uint32_t (&gt)[16]) {
+                auto apply = [&](auto op) {
 #pragma unroll
-            for (int m = 0; m < MATS; ++m) tmem_cp_scales(sf + 4 * m, A + m * MX_TILE + MX_CODES);
-            for (int p = 0; p < planes; ++p) tmem_cp_scales(sf + 4 * (MATS + p), B + p * mx_b_bytes<NT>() + 4 * mx_lbo<NT>());
+                    for (int j = 0; j < 16; ++j)
+                        u[j] = __float_as_uint(mx_glu<decltype(op)::value>(__uint_as_float(gt[j]) + bg, __uint_as_float(u[j]) + bu,
+                                                                         a.glu_limit));
+                };
+                if (GLU) {
+                    switch (a.glu_op) {
+                        case 0: apply(std::integral_constant<int, 0>{}); break;
+                        case 1: apply(std::integral_constant<int, 1>{}); break;
+                        case 2: apply(std::integral_constant<int, 2>{}); break;
+                        case 3: apply(std::integral_constant<int, 3>{}); break;
+                        default: apply(std::integral_constant<int, 4>{}); break;
+                    }
+                } else {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t idesc = mx_idesc(N, h);
-                for (int p = 0; p < planes; ++p) {
-                    const uint64_t bd = umma_desc(B + p * mx_b_bytes<NT>() + 2 * h * mx_lbo<NT>(), mx_lbo<NT>(), 128u);
-#pragma unroll
-                    for (int m = 0; m < MATS; ++m) {
-                        const uint64_t ad = umma_desc(A + m * MX_TILE + 2 * h * (16 * MX_M), 16 * MX_M, 128u);
-                        umma_mxf4(tmem + m * NT, ad, bd, idesc, sf + 4 * m, sf + 4 * (MATS + p),
-                                  (i | h | p) != 0 ? 1u : 0u);
+                    for (int j = 0; j < 16; ++j) {
+                        u[j] = __float_as_uint(__uint_as_float(u[j]) + bu);
+                        if (PAIR) gt[j] = __float_as_uint(__uint_as_float(gt[j]) + bg);
                     }
                 }
-            }
-            umma_commit(&C.empty[s]);
-        }
-        umma_commit(&C.done);
-    } else if (warp >= 2) {
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-        // the rows' quantised tiles: piece = 16 bytes of codes, planes * 4 pieces per row, then the scale words
-        constexpr int LAG = 2;
-        const int t = tid - 64, per = 4 * planes;
-        auto arrive = [&](int i) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&C.b_full[i % stages]);
-        };
-        bool ok = true;
-        int issued = 0;
-        for (int i = 0; i < n_it; ++i) {
-            const int s = i % stages;
-            if (i >= stages) ok = mx_wait(C, &C.empty[s], ((i / stages) - 1) & 1, a);
-            if (!__all_sync(0xffffffffu, ok)) break;
-            const uint32_t B = ring0 + s * stage_bytes + MATS * MX_TILE;
-            for (int q = t; q < count * per; q += 128) {
-                const int j = q / per, c = q - j * per, p = c >> 2;
-                const int64_t row = a.per_pick ? C.entry[j] : C.entry[j] / a.k;
-                const uint8_t *src = a.xq + ((row * a.KT + kt0 + i) * planes) * 64 + c * 16;
-                cp_async16(B + p * mx_b_bytes<NT>() + (c & 3) * mx_lbo<NT>() + (j >> 3) * 128 + (j & 7) * 16, src);
-            }
-            for (int q = t; q < count * planes; q += 128) {
-                const int j = q / planes, p = q - j * planes;
-                const int64_t row = a.per_pick ? C.entry[j] : C.entry[j] / a.k;
-                cp_async4(B + p * mx_b_bytes<NT>() + 4 * mx_lbo<NT>() + (j & 31) * 16 + (j >> 5) * 4,
-                          a.xs + (row * a.KT + kt0 + i) * planes + p);
-            }
-            cp_async_commit();
-            ++issued;
-            if (i >= LAG) {
-                cp_async_wait<LAG>();
-                arrive(i - LAG);
-            }
-        }
-        cp_async_wait<0>();
-        for (int i = issued > LAG ? issued - LAG : 0; i < issued; ++i) arrive(i);
-    }
-
-    // ---- epilogue ----------------------------------------------------------
-    __syncwarp();   // (the lanes that had no role wait here, not at the barrier)
-    const bool fine = __all_sync(0xffffffffu, mx_wait(C, &C.done, 0, a) &&
-                                                  *reinterpret_cast<volatile int32_t *>(&C.abort) == 0);
-    tc_fence_after();
-    const int quarter = warp & 3;                 // TMEM lanes this warp may read
-    const int r = 32 * quarter + lane;            // weight row of the tile
-    const int row = rt * MX_M + r;
-    const bool row_ok = row < a.rows;
-    const float bu = a.bias && row_ok ? a.bias[static_cast<int64_t>(expert) * a.rows + row] : 0.f;
-    const float bg = GLU && a.gate_bias && row_ok ? a.gate_bias[static_cast<int64_t>(expert) * a.rows + row] : 0.f;
-    auto finish = [&](int j, float u, float gt) {
-        u += bu;
-        if (GLU) u = glu_apply(a.glu_op, gt + bg, u, a.glu_limit);
-        if (row_ok) a.dst[static_cast<int64_t>(C.entry[j]) * a.rows + row] = u;
-    };
-    if (warp >= 2 && fine) {
-        const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
-        for (int n0 = 0; n0 < N; n0 += 16) {
-            uint32_t u[16], gt[16];
-            tmem_ld16(lanes + n0, u);
-            if (GLU) tmem_ld16(lanes + NT + n0, gt);
-            tmem_wait_ld();
-            if (a.split == 1) {
+            };
+            auto store = [&](int q, const uint32_t (&u)[16], const uint32_t (&gt)[16]) {
+                // every address first: a shuffle between the stores would hold each store back
+                float *at[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
-                    if (n0 + j < count) finish(n0 + j, __uint_as_float(u[j]), GLU ? __uint_as_float(gt[j]) : 0.f);
-            } else {
-                float *part = reinterpret_cast<float *>(ring);
+                    at[j] = out + static_cast<int64_t>(__shfl_sync(0xffffffffu, ens[q], j)) * a.rows;
+                const int left = I.count - column0(q), live = row_ok ? left : 0, live2 = row2_ok ? left : 0;
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    part[(n0 + j) * MX_M + r] = __uint_as_float(u[j]);
-                    if (GLU) part[(NT + n0 + j) * MX_M + r] = __uint_as_float(gt[j]);
+                    if (j < live) *at[j] = __uint_as_float(u[j]);
+                    if (PAIR && j < live2) at[j][MX_M] = __uint_as_float(gt[j]);
                 }
+            };
+            if (a.split > 1) {   // this rank's partial sums, for the cluster
+                float *part = reinterpret_cast<float *>(ring);
+                for (int q = 0; q < ROUNDS && column0(q) < I.count; ++q) {
+                    uint32_t u[16], gt[16];
+                    load(q, u, gt);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        part[(column0(q) + j) * MX_M + r] = __uint_as_float(u[j]);
+                        if (GLU) part[(NT + column0(q) + j) * MX_M + r] = __uint_as_float(gt[j]);
+                    }
+                }
+                release();
+            } else {
+                uint32_t us[ROUNDS][16], gs[MATS == 2 ? ROUNDS : 1][16];
+#pragma unroll
+                for (int q = 0; q < ROUNDS; ++q) load(q, us[q], gs[MATS == 2 ? q : 0]);
+                tmem_wait_ld();
+                release();
+#pragma unroll
+                for (int q = 0; q < ROUNDS; ++q)
+                    if (column0(q) < I.count) {
+                        finish(us[q], gs[MATS == 2 ? q : 0]);
+                        store(q, us[q], gs[MATS == 2 ? q : 0]);
+                    }
             }
         }
     }
+    __syncwarp();
     if (a.split > 1) {
         cluster_sync();
-        if (warp >= 2 && fine) {
-            for (int j = rank; j < count; j += a.split) {
-                float u = 0.f, gt = 0.f;
-                for (int q = 0; q < a.split; ++q) {
-                    u += ld_cluster_f32(ring0 + 4 * (j * MX_M + r), q);
-                    if (GLU) gt += ld_cluster_f32(ring0 + 4 * ((NT + j) * MX_M + r), q);
+        if (warp >= 2 && *reinterpret_cast<volatile int32_t *>(&C.abort) == 0) {
+            const Item I = item_at(item0);
+            const int r = (tid - 64) & (MX_M - 1), row = I.rt * MX_M + r;
+            if (row < a.rows) {
+                const float bu = a.bias ? a.bias[static_cast<int64_t>(I.expert) * a.rows + row] : 0.f;
+                const float bg = GLU && a.gate_bias ? a.gate_bias[static_cast<int64_t>(I.expert) * a.rows + row] : 0.f;
+                for (int j = rank + a.split * ((tid - 64) / MX_M); j < I.count; j += a.split * MXP_EPI) {
+                    float u = 0.f, gt = 0.f;
+                    for (int q = 0; q < a.split; ++q) {
+                        u += ld_cluster_f32(ring0 + 4 * (j * MX_M + r), q);
+                        if (GLU) gt += ld_cluster_f32(ring0 + 4 * ((NT + j) * MX_M + r), q);
+                    }
+                    u += bu;
+                    if (GLU) u = glu_apply(a.glu_op, gt + bg, u, a.glu_limit);
+                    a.dst[static_cast<int64_t>(entry_of(I, j)) * a.rows + row] = u;
                 }
-                finish(j, u, gt);
             }
         }
         cluster_sync();   // the partial sums stay until every rank has read them
     }
-    if (!fine && lane == 0) {
-        // a wait ran out: let the weight copies and MMAs in flight end before the memory they use goes
+    if (*reinterpret_cast<volatile int32_t *>(&C.abort) != 0 && warp == 0 && lane == 0) {
+        // a wait ran out: let the copies in flight land before the shared memory goes
         const uint64_t lim = drain_limit_ns(a.timeout_ns);
-        if (warp == 0)
-            for (int i = fills > stages ? fills - stages : 0; i < fills; ++i)
-                if (!mbar_wait_bounded(&C.a_full[i % stages], (i / stages) & 1, lim)) set_error(a.err, DERR_DRAIN);
-        if (warp == 1 && !mbar_wait_bounded(&C.done, 0, lim)) set_error(a.err, DERR_DRAIN);
+        for (int i = fills > stages ? fills - stages : 0; i < fills; ++i)
+            if (!mbar_wait_bounded(&C.full[i % stages], (i / stages) & 1, lim)) set_error(a.err, DERR_DRAIN);
     }
     tc_fence_before();
     __syncthreads();
@@ -595,7 +1004,6 @@ __global__ void __launch_bounds__(MXP_THREADS) mx_product_kernel(const MxArgs a)
     if (warp == 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
 }
-
 
 template <int XT>
 bool mx_vec_ok(const void *p, int64_t stride) {
@@ -623,64 +1031,73 @@ void dequantize_t(const uint8_t *y, int64_t n_blocks, int nb, int planes, void *
         mx_dequantize_kernel<OT, false><<<grid, 4 * MXQ_BLK, 0, st>>>(y, n_blocks, nb, planes, stride, static_cast<T *>(out));
 }
 
+template <int XT, bool VEC, bool DIRECT>
+cudaError_t images_t(const MxPrep &a, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>((a.n_rows * a.KT * 16 + 255) / 256));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // overlaps the grouping
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = DIRECT ? 0 : 1;
+    return cudaLaunchKernelEx(&cfg, mx_images_kernel<XT, VEC, DIRECT>, a);
+}
+
 template <int XT>
-void quantize_x_t(const void *x, int64_t stride, int64_t n_rows, int nb, int KT, int planes, uint8_t *xq, uint8_t *xs,
-                  cudaStream_t st) {
-    using T = typename MxElem<XT>::T;
-    const unsigned grid = static_cast<unsigned>((n_rows * KT * 16 + 255) / 256);
-    if (mx_vec_ok<XT>(x, stride))
-        mx_quantize_x_kernel<XT, true><<<grid, 256, 0, st>>>(static_cast<const T *>(x), stride, n_rows, nb, KT, planes, xq, xs);
-    else
-        mx_quantize_x_kernel<XT, false><<<grid, 256, 0, st>>>(static_cast<const T *>(x), stride, n_rows, nb, KT, planes, xq, xs);
+cudaError_t images_x(const MxPrep &a, cudaStream_t st) {
+    if (mx_vec_ok<XT>(a.x, a.stride)) return a.entries ? images_t<XT, true, false>(a, st) : images_t<XT, true, true>(a, st);
+    return a.entries ? images_t<XT, false, false>(a, st) : images_t<XT, false, true>(a, st);
 }
 
 constexpr uint32_t kSmemMax = 227u * 1024u;
 
-template <int NT, bool GLU, bool DIRECT>
-cudaError_t product_t(MxArgs &a, int64_t units, cudaStream_t st) {
-    constexpr int MATS = GLU ? 2 : 1;
-    auto kern = mx_product_kernel<NT, GLU, DIRECT>;
+template <int NT, bool GLU, bool DIRECT, int PLANES>
+cudaError_t product_p(MxArgs &a, int64_t units, cudaStream_t st) {
+    constexpr bool PAIR = !GLU && NT == MXP_WIDE;
+    constexpr int MATS = GLU || PAIR ? 2 : 1;
+    const int RI = PAIR ? (a.RT + 1) / 2 : a.RT;
+    auto kern = mx_product_kernel<NT, GLU, DIRECT, PLANES>;
     constexpr uint32_t fixed = (sizeof(MxCtl<NT>) + 127u) / 128u * 128u + 1024u;   // static part and the system's 1 KB
-    const uint32_t sb = mx_stage_bytes<NT>(MATS, a.planes);
-    const int per = (a.KT + a.split - 1) / a.split;
+    const uint32_t sb = mx_stage_bytes<NT>(MATS, PLANES), sf = MXP_TPS * 4u * (MATS + PLANES);
+    const bool single = DIRECT || a.split > 1;       // one item per CTA
+    a.acc = single ? 1 : 2;
+    const int tiles = (a.KT + a.split - 1) / a.split;
+    const int most = single ? (tiles + MXP_TPS - 1) / MXP_TPS : MX_MAX_STAGES;   // stages that would be used
     const uint32_t part = a.split > 1 ? MATS * NT * MX_M * 4u : 0u;
-    // two CTAs per SM where their accumulators and scales fit in half the tensor memory each
-    uint32_t budget = kSmemMax / 2 - fixed;
-    auto cols_of = [&](int stages) {
-        const uint32_t need = MATS * NT + stages * 4u * (MATS + a.planes);
-        uint32_t c = 32;
-        while (c < need) c *= 2;
-        return c;
-    };
-    int stages = static_cast<int>(budget / sb);
-    if (stages > per) stages = per;
-    if (stages < 2 || cols_of(stages) > 256u) {
-        budget = kSmemMax - fixed;
-        stages = static_cast<int>(budget / sb);
-        if (stages > per) stages = per;
-    }
-    if (stages > MX_MAX_STAGES) stages = MX_MAX_STAGES;
-    while (stages > 1 && cols_of(stages) > 512u) --stages;
+    const uint32_t acc_cols = a.acc * MATS * NT;
+    // two CTAs per SM where their accumulators fit in half the tensor memory each, else one
+    const uint32_t least = std::min(most, 2);
+    const int per_sm = acc_cols + least * sf <= 256u && least * sb <= kSmemMax / 2 - fixed ? 2 : 1;
+    int stages = static_cast<int>((kSmemMax / per_sm - fixed) / sb);
+    stages = std::min(stages, static_cast<int>((512u / per_sm - acc_cols) / sf));
+    stages = std::min(std::min(stages, most), MX_MAX_STAGES);
     a.stages = stages;
-    a.tmem_cols = cols_of(stages);
+    a.tmem_cols = 32;
+    while (a.tmem_cols < acc_cols + stages * sf) a.tmem_cols *= 2;
     // shared memory in proportion to the tensor memory: CTAs that fit an SM together never wait for
     // columns, so ranks of a cluster cannot wait for one another through them
-    uint32_t smem = stages * sb > part ? stages * sb : part;
+    uint32_t smem = std::max(stages * sb, part);
     const uint32_t fair = static_cast<uint32_t>((static_cast<uint64_t>(kSmemMax) * a.tmem_cols + 511) / 512);
     if (smem + fixed < fair) smem = (fair - fixed + 127u) / 128u * 128u;
-    static bool configured[64] = {};
-    int dev = 0;
+    int dev = 0, n_sm = 148;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    static int configured[64] = {};   // SMs of a device that knows the kernel's limit
     if (!configured[dev]) {
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                    static_cast<int>(kSmemMax - fixed + 1024u));
         if (e != cudaSuccess) return e;
-        configured[dev] = true;
+        cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, dev);
+        configured[dev] = n_sm;
     }
+    n_sm = configured[dev];
+    int64_t grid = units * RI * a.split;
+    if (!single) grid = std::min<int64_t>(grid, static_cast<int64_t>(n_sm) * per_sm);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(units * a.RT * a.split));
-    cfg.blockDim = dim3(MXP_THREADS);
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(mxp_threads<NT>());
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
@@ -694,10 +1111,9 @@ cudaError_t product_t(MxArgs &a, int64_t units, cudaStream_t st) {
     return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
-template <int NT>
-cudaError_t product_n(MxArgs &a, bool glu, bool direct, int64_t units, cudaStream_t st) {
-    if (glu) return direct ? product_t<NT, true, true>(a, units, st) : product_t<NT, true, false>(a, units, st);
-    return direct ? product_t<NT, false, true>(a, units, st) : product_t<NT, false, false>(a, units, st);
+template <int NT, bool GLU, bool DIRECT>
+cudaError_t product_t(MxArgs &a, int64_t units, cudaStream_t st) {
+    return a.planes == 1 ? product_p<NT, GLU, DIRECT, 1>(a, units, st) : product_p<NT, GLU, DIRECT, 2>(a, units, st);
 }
 
 }  // namespace
@@ -733,34 +1149,83 @@ cudaError_t launch_mx_pack(const uint8_t *src, int64_t E, int64_t rows, int64_t 
     return cudaGetLastError();
 }
 
-cudaError_t launch_mx_quantize_x(const void *x, int xt, int64_t stride, int64_t n_rows, int64_t K, int planes,
-                                 uint8_t *xq, uint32_t *xs, cudaStream_t st) {
-    const int nb = static_cast<int>(K / 32), KT = static_cast<int>((K + MX_KT - 1) / MX_KT);
-    uint8_t *s = reinterpret_cast<uint8_t *>(xs);
-    if (xt == MX_F32) quantize_x_t<MX_F32>(x, stride, n_rows, nb, KT, planes, xq, s, st);
-    else if (xt == MX_F16) quantize_x_t<MX_F16>(x, stride, n_rows, nb, KT, planes, xq, s, st);
-    else quantize_x_t<MX_BF16>(x, stride, n_rows, nb, KT, planes, xq, s, st);
-    return cudaGetLastError();
-}
-
+// Entries per chunk: 64 at most in the direct form; else by the entries an
+// expert has on average.
 int mx_chunk_tokens(int64_t n_tok, int64_t k, int64_t n_experts) {
     const int64_t n = n_tok * k;
     if (n <= MX_DIRECT) return n_tok <= 16 ? 16 : 64;
-    const int64_t per = n / (n < n_experts ? n : n_experts);   // entries of an expert, on average
-    return per <= 12 ? 16 : per <= 48 ? 64 : 128;
+    const int64_t per = n / (n < n_experts ? n : n_experts);
+    return per <= 12 ? 16 : per <= 48 ? 64 : MXP_WIDE;
 }
 
 bool mx_direct(int64_t n_tok, int64_t k) { return n_tok * k <= MX_DIRECT; }
 
+int64_t mx_max_experts() { return MXG_MAX_EXPERTS; }
+
+uint64_t mx_images_bytes(int64_t chunks, int NT, int64_t K, int planes) {
+    return static_cast<uint64_t>(chunks) * mx_image_bytes(NT, static_cast<int>((K + MX_KT - 1) / MX_KT), planes);
+}
+
+cudaError_t launch_mx_prep(const void *x, int xt, int64_t stride, int64_t n_rows, int64_t K, const MxArgs &a, int NT,
+                           cudaStream_t st) {
+    MxPrep p{};
+    p.x = x;
+    p.stride = stride;
+    p.n_rows = n_rows;
+    p.nb = static_cast<int32_t>(K / 32);
+    p.KT = a.KT;
+    p.planes = a.planes;
+    p.per_pick = a.per_pick;
+    p.images = const_cast<uint8_t *>(a.images);
+    p.ids = a.ids;
+    p.ids_stride = a.ids_stride;
+    p.n_entries = a.n_entries;
+    p.k = a.k;
+    p.n_experts = a.n_experts;
+    p.NT = NT;
+    p.err = a.err;
+    if (a.chunks) {
+        p.entries = const_cast<int32_t *>(a.entries);
+        p.n_chunks = const_cast<int32_t *>(a.n_chunks);
+        p.chunks = const_cast<int4 *>(a.chunks);
+        p.where = a.where;
+        const size_t smem = 5 * static_cast<size_t>(a.n_experts) * sizeof(int);   // 80 KB at most
+        static bool configured[64] = {};
+        int dev = 0;
+        cudaGetDevice(&dev);
+        if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+        if (!configured[dev]) {
+            const cudaError_t e = cudaFuncSetAttribute(mx_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                       5 * MXG_MAX_EXPERTS * static_cast<int>(sizeof(int)));
+            if (e != cudaSuccess) return e;
+            configured[dev] = true;
+        }
+        const int threads = a.n_entries <= 2048 * MXG_CTAS / 8 ? 256 : a.n_entries <= 1024 * MXG_CTAS ? 512 : MXG_THREADS;
+        mx_group_kernel<<<MXG_CTAS, threads, smem, st>>>(p);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+    }
+    if (xt == MX_F32) return images_x<MX_F32>(p, st);
+    if (xt == MX_F16) return images_x<MX_F16>(p, st);
+    return images_x<MX_BF16>(p, st);
+}
+
 cudaError_t launch_mx_product(MxArgs &a, int NT, int64_t units, cudaStream_t st) {
     const bool glu = a.gate != nullptr, direct = a.chunks == nullptr;
+    // few tiles: a cluster of 2, 4 or 8 CTAs shares a tile's K
     int split = 1;
     if (NT <= 64)
         while (split < 8 && units * a.RT * split < 296 && a.KT / (2 * split) >= 2) split *= 2;
     a.split = split;
-    if (NT == 16) return product_n<16>(a, glu, direct, units, st);
-    if (NT == 64) return product_n<64>(a, glu, direct, units, st);
-    return glu ? product_t<128, true, false>(a, units, st) : product_t<128, false, false>(a, units, st);
+    if (NT == 16) {
+        if (glu) return direct ? product_t<16, true, true>(a, units, st) : product_t<16, true, false>(a, units, st);
+        return direct ? product_t<16, false, true>(a, units, st) : product_t<16, false, false>(a, units, st);
+    }
+    if (NT == 64) {
+        if (glu) return direct ? product_t<64, true, true>(a, units, st) : product_t<64, true, false>(a, units, st);
+        return direct ? product_t<64, false, true>(a, units, st) : product_t<64, false, false>(a, units, st);
+    }
+    return glu ? product_t<MXP_WIDE, true, false>(a, units, st) : product_t<MXP_WIDE, false, false>(a, units, st);
 }
 
 }  // namespace moe

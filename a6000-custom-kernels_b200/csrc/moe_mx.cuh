@@ -36,16 +36,16 @@ struct MxArgs {
     int32_t n_experts, rows, RT, KT;
     int32_t glu_op;
     float glu_limit;
-    const uint8_t *xq;               // [x row][KT][planes][64] codes
-    const uint32_t *xs;              // [x row][KT][planes] scales of the tile's 4 blocks
+    const uint8_t *images;           // quantised rows, per chunk (mx_images_kernel)
     int32_t planes, k, n_entries, per_pick;
     const int32_t *ids;              // direct form: [tok * ids_stride + pick]
     int64_t ids_stride;
     const int32_t *entries;          // chunked form: entries grouped by expert,
+    int32_t *where;                  // each entry's place (moe_mx.cu), -1: left out;
     const int4 *chunks;              // {expert, first entry, count, -},
     const int32_t *n_chunks;         // and their number on the device
     float *dst;                      // [entry][rows]
-    int32_t split, stages;           // CTAs of a cluster that share K; ring stages
+    int32_t split, stages, acc;      // CTAs of a cluster that share K; ring stages; accumulator sets
     uint32_t tmem_cols;
     int *err;
     uint64_t timeout_ns;

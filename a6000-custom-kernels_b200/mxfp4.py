@@ -81,9 +81,9 @@ class MXFP4Weights:
         self.ref = ctypes.byref(self.desc)
 
 
-def mxfp4_workspace_size(w, n_tok, k, x_per_pick=False, planes=2):
+def mxfp4_workspace_size(w, n_tok, k, planes=2):
     """Bytes of device workspace mxfp4_mul_mat_id needs (moe_b200_mxfp4_workspace_size)."""
-    return lib().moe_b200_mxfp4_workspace_size(w.ref, n_tok, k, int(x_per_pick), planes)
+    return lib().moe_b200_mxfp4_workspace_size(w.ref, n_tok, k, planes)
 
 
 def mxfp4_mul_mat_id(w, x, ids, gate=None, bias=None, gate_bias=None, glu_op=GLU_SWIGLU, glu_limit=0.0, planes=2,
@@ -118,7 +118,7 @@ def mxfp4_mul_mat_id(w, x, ids, gate=None, bias=None, gate_bias=None, glu_op=GLU
             need(dst.dtype == torch.float32 and dst.device == w.device and dst.is_contiguous() and
                   tuple(dst.shape) == (n_tok, k, rows), "dst must be contiguous f32 [n_tok, k, rows]")
         if workspace is None:
-            workspace = torch.empty(L.moe_b200_mxfp4_workspace_size(w.ref, n_tok, k, int(per_pick), planes) or 1,
+            workspace = torch.empty(L.moe_b200_mxfp4_workspace_size(w.ref, n_tok, k, planes) or 1,
                                     dtype=torch.uint8, device=w.device)
         else:
             need(workspace.dtype == torch.uint8 and workspace.device == w.device and workspace.is_contiguous(),

@@ -547,7 +547,7 @@ int moe_b200_mxfp4_pack(const moe_tensor *src0, void *dst, size_t dst_bytes, moe
  * share one, captured graphs included. Allocates nothing, except that the
  * first call of a process makes the device error word: not during stream
  * capture (MOE_ERR_STATE). */
-size_t moe_b200_mxfp4_workspace_size(const moe_mxfp4 *w, int64_t n_tok, int64_t k, int32_t x_per_pick, int32_t planes);
+size_t moe_b200_mxfp4_workspace_size(const moe_mxfp4 *w, int64_t n_tok, int64_t k, int32_t planes);
 int moe_b200_mxfp4_mul_mat_id(const moe_mxfp4 *w, const moe_mxfp4 *gate, const float *bias, const float *gate_bias,
                               int32_t glu_op, float glu_limit, const void *x, int32_t x_type, int64_t x_row_stride,
                               int32_t x_per_pick, int64_t n_tok, const int32_t *ids, int64_t k, int64_t ids_stride,
