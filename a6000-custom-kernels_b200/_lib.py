@@ -159,6 +159,8 @@ def _declare(L):
 def lib():
     """The loaded C library (built on first use if missing or stale)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             build()

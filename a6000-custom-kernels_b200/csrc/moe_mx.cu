@@ -14,14 +14,100 @@ namespace moe {
 namespace {
 
 // ---------------------------------------------------------------------------
-// One block of 32 values by 4 lanes: lane i holds values 4 i .. 4 i + 3 (v[0..3])
-// and 16 + 4 i .. 16 + 4 i + 3 (v[4..7]), so its 4 code bytes pair them as the
-// format does. scale byte = max(floor(log2 amax) - 2, -127) + 127, read off
-// amax's exponent field; codes are the nearest magnitudes of v 2^-e, ties to the
-// even code, saturating at 6 (the scaled values lie below 8). An infinity or a
-// NaN makes the block's scale NaN.
+// One block of 32 values by 4 lanes: lane i holds values 4 i .. 4 i + 3 and
+// 16 + 4 i .. 16 + 4 i + 3, the pairs that share its 4 code bytes.
+// scale byte = max(floor(log2 amax) - 2, -127) + 127, read off amax's exponent
+// field; codes are the nearest magnitudes of v 2^-e, ties to the even code,
+// saturating at 6 (the scaled values lie below 8). An infinity or a NaN makes
+// the block's scale NaN.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t mx_codes(const float (&v)[8], float inv) {
+template <int XT> struct MxElem;
+template <> struct MxElem<MX_F32> { using T = float; };
+template <> struct MxElem<MX_F16> { using T = __half; };
+template <> struct MxElem<MX_BF16> { using T = __nv_bfloat16; };
+
+// a lane's 8 values of the block at p (VEC: groups of 4 aligned to their size), as loaded
+template <int XT> struct MxRaw { uint32_t w[XT == MX_F32 ? 8 : 4]; };
+template <int XT, bool VEC>
+__device__ __forceinline__ MxRaw<XT> mx_load(const typename MxElem<XT>::T *p, int i) {
+    MxRaw<XT> r;
+    p += 4 * i;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if constexpr (XT == MX_F32 && VEC) {
+            const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p + 16 * h));
+            r.w[4 * h] = a.x; r.w[4 * h + 1] = a.y; r.w[4 * h + 2] = a.z; r.w[4 * h + 3] = a.w;
+        } else if constexpr (XT == MX_F32) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r.w[4 * h + j] = reinterpret_cast<const uint32_t *>(p + 16 * h)[j];
+        } else if constexpr (VEC) {
+            const uint2 a = __ldg(reinterpret_cast<const uint2 *>(p + 16 * h));
+            r.w[2 * h] = a.x; r.w[2 * h + 1] = a.y;
+        } else {
+            const uint16_t *q = reinterpret_cast<const uint16_t *>(p + 16 * h);
+            r.w[2 * h] = q[0] | static_cast<uint32_t>(q[1]) << 16;
+            r.w[2 * h + 1] = q[2] | static_cast<uint32_t>(q[3]) << 16;
+        }
+    }
+    return r;
+}
+template <int XT>
+__device__ __forceinline__ MxRaw<XT> mx_zero() {
+    MxRaw<XT> r;
+#pragma unroll
+    for (uint32_t &w : r.w) w = 0u;
+    return r;
+}
+template <int XT> struct MxPair;
+template <> struct MxPair<MX_F16> {
+    using T = __half2;
+    static __device__ __forceinline__ T abs(uint32_t w) { w &= 0x7FFF7FFFu; return *reinterpret_cast<T *>(&w); }
+};
+template <> struct MxPair<MX_BF16> {
+    using T = __nv_bfloat162;
+    static __device__ __forceinline__ T abs(uint32_t w) { w &= 0x7FFF7FFFu; return *reinterpret_cast<T *>(&w); }
+};
+// the values, and the largest magnitude's f32 bits (magnitudes compare as integers, a NaN above
+// infinity above every number)
+template <int XT>
+__device__ __forceinline__ uint32_t mx_floats(const MxRaw<XT> &r, float (&v)[8]) {
+    if constexpr (XT == MX_F32) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j] = __uint_as_float(r.w[j]);
+            top = max(top, r.w[j] & 0x7FFFFFFFu);
+        }
+        return top;
+    } else {
+        // two at a time; the .NaN maximum keeps a NaN
+        typename MxPair<XT>::T two = MxPair<XT>::abs(r.w[0]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j > 0) two = __hmax2_nan(two, MxPair<XT>::abs(r.w[j]));
+            if constexpr (XT == MX_BF16) {
+                v[2 * j] = __uint_as_float(r.w[j] << 16);
+                v[2 * j + 1] = __uint_as_float(r.w[j] & 0xFFFF0000u);
+            } else {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r.w[j]));
+                v[2 * j] = f.x;
+                v[2 * j + 1] = f.y;
+            }
+        }
+        const uint32_t both = *reinterpret_cast<const uint32_t *>(&two), one = max(both & 0xFFFFu, both >> 16);
+        if constexpr (XT == MX_BF16) return one << 16;
+        else return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(one)))) & 0x7FFFFFFFu;
+    }
+}
+__device__ __forceinline__ uint32_t mx_top(const float (&v)[8]) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+    return top;
+}
+
+// byte j: the code of a[j] in its low nibble, of b[j] in its high one (scaled by inv first)
+__device__ __forceinline__ uint32_t mx_codes(const float (&a)[4], const float (&b)[4], float inv) {
     uint32_t w;
     asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 b0, %5, %1;\n\t"
@@ -30,14 +116,13 @@ __device__ __forceinline__ uint32_t mx_codes(const float (&v)[8], float inv) {
         "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %4;\n\t"
         "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
         : "=r"(w)
-        : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv),
-          "f"(v[6] * inv), "f"(v[7] * inv));
+        : "f"(a[0] * inv), "f"(a[1] * inv), "f"(a[2] * inv), "f"(a[3] * inv), "f"(b[0] * inv), "f"(b[1] * inv),
+          "f"(b[2] * inv), "f"(b[3] * inv));
     return w;
 }
 
-// the 8 magnitudes with signs that 4 code bytes hold: v[0..3] their low
-// nibbles, v[4..7] their high ones (unscaled)
-__device__ __forceinline__ void mx_values(uint32_t w, float (&v)[8]) {
+// the signed magnitudes (unscaled) that 4 code bytes hold, of the low nibbles and the high ones
+__device__ __forceinline__ void mx_values(uint32_t w, float (&lo)[4], float (&hi)[4]) {
     uint32_t h[4];
     asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
         "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
@@ -50,8 +135,8 @@ __device__ __forceinline__ void mx_values(uint32_t w, float (&v)[8]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[j]));
-        v[j] = f.x;
-        v[4 + j] = f.y;
+        lo[j] = f.x;
+        hi[j] = f.y;
     }
 }
 
@@ -59,161 +144,224 @@ __device__ __forceinline__ float mx_scale(uint32_t byte) {   // 2^(byte - 127); 
     return __uint_as_float(byte == 255u ? 0x7FFFFFFFu : byte == 0u ? 0x00400000u : byte << 23);
 }
 
-__device__ __forceinline__ uint32_t mx_quant_block(const float (&v)[8], uint32_t &byte) {
-    uint32_t top = 0;   // magnitudes compare as integers; a NaN above infinity above every number
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+// The block's scale byte and this lane's 4 code bytes, from its values and the
+// lane's largest magnitude
+__device__ __forceinline__ uint32_t mx_quant_block(const float (&v)[8], uint32_t top, uint32_t &byte) {
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const uint32_t ex = top >> 23;
-    if (ex == 255u) {
-        byte = 255u;
-        return 0u;
-    }
-    byte = ex > 2u ? ex - 2u : 0u;
-    return mx_codes(v, __uint_as_float((254u - byte) << 23));   // 2^(127 - byte), exact
+    byte = ex == 255u ? 255u : ex > 2u ? ex - 2u : 0u;
+    const float inv = __uint_as_float((254u - min(byte, 252u)) << 23);   // 2^(127 - byte), exact
+    const float a[4] = {v[0], v[1], v[2], v[3]}, b[4] = {v[4], v[5], v[6], v[7]};
+    return byte == 255u ? 0u : mx_codes(a, b, inv);
 }
-
-// what the block's codes leave of v (exact: a multiple of v's last place, no larger than v's block)
+// what the codes leave of v (exact: a multiple of v's last place, no larger than the block's largest value)
 __device__ __forceinline__ void mx_residual(float (&v)[8], uint32_t codes, uint32_t byte) {
-    float q[8];
-    mx_values(codes, q);
+    float a[4], b[4];
+    mx_values(codes, a, b);
     const float s = mx_scale(byte);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] -= q[j] * s;
+    for (int j = 0; j < 4; ++j) { v[j] -= a[j] * s; v[4 + j] -= b[j] * s; }
 }
 
-template <int XT> struct MxElem;
-template <> struct MxElem<MX_F32> { using T = float; };
-template <> struct MxElem<MX_F16> { using T = __half; };
-template <> struct MxElem<MX_BF16> { using T = __nv_bfloat16; };
-
-__device__ __forceinline__ float to_f32(float x) { return x; }
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-
-// 4 consecutive elements at p (VEC: aligned to their total size)
-template <int XT, bool VEC>
-__device__ __forceinline__ void mx_load4(const typename MxElem<XT>::T *p, float *v) {
-    if constexpr (!VEC) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = to_f32(p[j]);
-    } else if constexpr (XT == MX_F32) {
-        const float4 a = __ldg(reinterpret_cast<const float4 *>(p));
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+// ---------------------------------------------------------------------------
+// The 17-byte blocks as a stream of words: 4 consecutive blocks are 17 words.
+// 16 lanes hold them, lane 4 q + i code bytes 4 i .. 4 i + 3 of block q, which
+// begin q + 1 bytes past a word; so lane l's word l is its own code word and
+// the bytes before it (the lane before's, and the scale where i = 0) shifted
+// together, and word 16 is lane 15's code word as it is. Reading goes the other
+// way. Words leave and arrive straight from registers; y may have any
+// alignment (bytes then), and past `end` nothing is touched.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void mx_put(uint8_t *y, int64_t at, int64_t end, bool words, uint32_t w) {
+    if (words && at + 4 <= end) {
+        *reinterpret_cast<uint32_t *>(y + at) = w;
     } else {
-        const uint2 a = __ldg(reinterpret_cast<const uint2 *>(p));
-        const typename MxElem<XT>::T *e = reinterpret_cast<const typename MxElem<XT>::T *>(&a);
+        for (int j = 0; j < 4; ++j)
+            if (at + j < end) y[at + j] = static_cast<uint8_t>(w >> (8 * j));
+    }
+}
+__device__ __forceinline__ uint32_t mx_get(const uint8_t *y, int64_t at, int64_t end, bool words) {
+    if (words && at + 4 <= end) return __ldg(reinterpret_cast<const uint32_t *>(y + at));
+    uint32_t w = 0;
+    for (int j = 0; j < 4; ++j)
+        if (at + j < end) w |= static_cast<uint32_t>(y[at + j]) << (8 * j);
+    return w;
+}
+// the stream word that a lane writes (lane 15 of 16 also writes its codes behind it)
+__device__ __forceinline__ uint32_t mx_stream_word(uint32_t codes, uint32_t byte, int lane) {
+    const uint32_t before = __shfl_up_sync(0xffffffffu, codes, 1);
+    const uint32_t pre = (lane & 3) == 0 ? before >> 8 | byte << 24 : before;
+    return __funnelshift_lc(pre, codes, 8 * (((lane >> 2) & 3) + 1));
+}
+struct MxWords { uint32_t own, extra; };   // word l, and lane 15's word 16
+__device__ __forceinline__ MxWords mx_get_words(const uint8_t *y, int64_t group, int64_t n_blocks, bool words, int lane) {
+    const int l = lane & 15;
+    const int64_t at = group * 17, end = n_blocks * 17;
+    return {mx_get(y, at + 4 * l, end, words), l == 15 ? mx_get(y, at + 64, end, words) : 0u};
+}
+__device__ __forceinline__ uint32_t mx_take_block(const MxWords &m, int lane, uint32_t &byte) {
+    const int q = (lane >> 2) & 3;
+    const uint32_t next = __shfl_down_sync(0xffffffffu, m.own, 1);
+    byte = __shfl_sync(0xffffffffu, m.own, lane & ~3) >> (8 * q) & 255u;
+    return __funnelshift_rc(m.own, (lane & 15) == 15 ? m.extra : next, 8 * (q + 1));
+}
+
+// ---------------------------------------------------------------------------
+// quantise into ggml blocks, y [planes][rows][nb], and read back: out [rows][K]
+// = the planes' values added, rounded once to OT. 4 blocks per lane quad with
+// all their loads in flight at once (one per quad left the memory waiting:
+// 2.4 TB/s); byte stores through shared memory cost a quarter of the time.
+// ---------------------------------------------------------------------------
+constexpr int MXQ_THREADS = 256;
+constexpr int MXQ_PER = 4;                                // blocks per lane quad
+constexpr int MXQ_STEP = MXQ_THREADS / 4;
+constexpr int MXQ_BLK = MXQ_STEP * MXQ_PER;               // blocks per CTA
+
+// a CTA whose blocks are all there, in dense rows, every plane's stream on word boundaries
+__device__ __forceinline__ bool mx_whole(const void *y, int64_t stride, int64_t n_blocks, int nb, int planes) {
+    return (static_cast<int64_t>(blockIdx.x) + 1) * MXQ_BLK <= n_blocks && stride == static_cast<int64_t>(nb) * 32 &&
+           (reinterpret_cast<uintptr_t>(y) & 3u) == 0 && (planes == 1 || n_blocks % 4 == 0);
+}
+// row of block g: 32-bit division where the number of blocks allows
+__device__ __forceinline__ int64_t mx_row_of(int64_t g, int nb, bool small) {
+    return small ? static_cast<int64_t>(static_cast<uint32_t>(g) / static_cast<uint32_t>(nb)) : g / nb;
+}
+// element offset of block g; dense rows follow one another
+__device__ __forceinline__ int64_t mx_block_at(int64_t g, int nb, int64_t stride, bool dense, bool small) {
+    if (dense) return g * 32;
+    const int64_t row = mx_row_of(g, nb, small);
+    return row * stride + (g - row * nb) * 32;
+}
+
+// FAST: dense rows, aligned words and a whole CTA of blocks -- addresses are one
+// base and constants (with 64-bit offsets and tests per word the kernel was
+// bound by its 140 instructions per 8 values)
+template <int XT, bool VEC, bool FAST>
+__device__ __forceinline__ void mx_quantize_blocks(const typename MxElem<XT>::T *__restrict__ x, int64_t stride,
+                                                   int64_t n_blocks, int nb, int planes, uint8_t *__restrict__ y) {
+    const int lane = threadIdx.x & 31, quad = threadIdx.x >> 2, i = threadIdx.x & 3;
+    const int64_t b0 = static_cast<int64_t>(blockIdx.x) * MXQ_BLK;
+    const bool dense = stride == static_cast<int64_t>(nb) * 32, small = n_blocks < (int64_t{1} << 31);
+    const typename MxElem<XT>::T *const x0 = x + (b0 + quad) * 32;
+    uint8_t *const y0 = y + (b0 + (quad & ~3)) * 17 + 4 * (lane & 15);
+    MxRaw<XT> raw[MXQ_PER];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = to_f32(e[j]);
+    for (int u = 0; u < MXQ_PER; ++u) {
+        if constexpr (FAST) {
+            raw[u] = mx_load<XT, VEC>(x0 + u * (MXQ_STEP * 32), i);
+        } else {
+            const int64_t g = b0 + u * MXQ_STEP + quad;
+            raw[u] = mx_zero<XT>();
+            if (g < n_blocks) raw[u] = mx_load<XT, VEC>(x + mx_block_at(g, nb, stride, dense, small), i);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < MXQ_PER; ++u) {
+        float v[8];
+        uint32_t top = mx_floats<XT>(raw[u], v);
+        for (int pl = 0;; ++pl) {
+            uint32_t byte;
+            const uint32_t w = mx_quant_block(v, top, byte);
+            const int64_t plane = pl * n_blocks * 17;
+            if constexpr (FAST) {
+                uint8_t *o = y0 + plane + u * (MXQ_STEP * 17);
+                *reinterpret_cast<uint32_t *>(o) = mx_stream_word(w, byte, lane);
+                if ((lane & 15) == 15) *reinterpret_cast<uint32_t *>(o + 4) = w;
+            } else {
+                uint8_t *o = y + plane;
+                const int64_t at = (b0 + u * MXQ_STEP + (quad & ~3)) * 17, end = n_blocks * 17;
+                const bool words = (reinterpret_cast<uintptr_t>(o) & 3u) == 0;
+                mx_put(o, at + 4 * (lane & 15), end, words, mx_stream_word(w, byte, lane));
+                if ((lane & 15) == 15) mx_put(o, at + 64, end, words, w);
+            }
+            if (pl + 1 == planes) break;
+            mx_residual(v, w, byte);
+            top = mx_top(v);
+        }
     }
 }
 
-// ---------------------------------------------------------------------------
-// quantise into ggml blocks: y [planes][rows][nb] blocks. A CTA makes MXQ_BLK
-// consecutive blocks of the rows' concatenation; the 17-byte blocks are put
-// together in shared memory and leave as whole words.
-// ---------------------------------------------------------------------------
-constexpr int MXQ_BLK = 128;                    // blocks per CTA (512 threads, 4 lanes each)
-constexpr int MXQ_BYTES = MXQ_BLK * 17;         // a multiple of 16
-
 template <int XT, bool VEC>
-__global__ void __launch_bounds__(4 * MXQ_BLK) mx_quantize_kernel(const typename MxElem<XT>::T *__restrict__ x,
+__global__ void __launch_bounds__(MXQ_THREADS) mx_quantize_kernel(const typename MxElem<XT>::T *__restrict__ x,
                                                                   int64_t stride, int64_t n_blocks, int nb, int planes,
                                                                   uint8_t *__restrict__ y) {
-    __shared__ __align__(16) uint8_t buf[MX_MAX_PLANES][MXQ_BYTES];
-    const int lb = threadIdx.x >> 2, i = threadIdx.x & 3;
+    if (VEC && mx_whole(y, stride, n_blocks, nb, planes)) mx_quantize_blocks<XT, VEC, VEC>(x, stride, n_blocks, nb, planes, y);
+    else mx_quantize_blocks<XT, VEC, false>(x, stride, n_blocks, nb, planes, y);
+}
+
+template <int OT, bool VEC, bool FAST>
+__device__ __forceinline__ void mx_dequantize_blocks(const uint8_t *__restrict__ y, int64_t n_blocks, int nb, int planes,
+                                                     int64_t stride, typename MxElem<OT>::T *__restrict__ out) {
+    using T = typename MxElem<OT>::T;
+    const int lane = threadIdx.x & 31, quad = threadIdx.x >> 2, i = threadIdx.x & 3;
     const int64_t b0 = static_cast<int64_t>(blockIdx.x) * MXQ_BLK;
-    const int64_t g = b0 + lb;
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (g < n_blocks) {
-        const int64_t row = g / nb;
-        const typename MxElem<XT>::T *p = x + row * stride + (g - row * nb) * 32 + 4 * i;
-        mx_load4<XT, VEC>(p, v);
-        mx_load4<XT, VEC>(p + 16, v + 4);
-    }
-    for (int pl = 0; pl < planes; ++pl) {
-        uint32_t byte;
-        const uint32_t w = mx_quant_block(v, byte);
-        uint8_t *o = buf[pl] + lb * 17;
-        if (i == 0) o[0] = static_cast<uint8_t>(byte);
+    const bool dense = stride == static_cast<int64_t>(nb) * 32, small = n_blocks < (int64_t{1} << 31);
+    const uint8_t *const y0 = y + (b0 + (quad & ~3)) * 17 + 4 * (lane & 15);
+    T *const out0 = out + (b0 + quad) * 32 + 4 * i;
+    MxWords m[MX_MAX_PLANES][MXQ_PER];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[1 + 4 * i + j] = static_cast<uint8_t>(w >> (8 * j));
-        if (pl + 1 < planes) mx_residual(v, w, byte);
+    for (int pl = 0; pl < MX_MAX_PLANES; ++pl) {
+        if (pl >= planes) break;
+        const int64_t plane = pl * n_blocks * 17;
+#pragma unroll
+        for (int u = 0; u < MXQ_PER; ++u) {
+            if constexpr (FAST) {
+                const uint32_t *o = reinterpret_cast<const uint32_t *>(y0 + plane + u * (MXQ_STEP * 17));
+                m[pl][u].own = __ldg(o);
+                m[pl][u].extra = (lane & 15) == 15 ? __ldg(o + 1) : 0u;
+            } else {
+                const uint8_t *o = y + plane;
+                m[pl][u] = mx_get_words(o, b0 + u * MXQ_STEP + (quad & ~3), n_blocks, (reinterpret_cast<uintptr_t>(o) & 3u) == 0, lane);
+            }
+        }
     }
-    __syncthreads();
-    const int64_t left = (n_blocks - b0) * 17;
-    const int bytes = left < MXQ_BYTES ? static_cast<int>(left) : MXQ_BYTES;
-    for (int pl = 0; pl < planes; ++pl) {
-        uint8_t *o = y + pl * n_blocks * 17 + b0 * 17;
-        if ((reinterpret_cast<uintptr_t>(o) & 15u) == 0) {
-            for (int t = threadIdx.x; t < bytes / 16; t += blockDim.x)
-                reinterpret_cast<uint4 *>(o)[t] = reinterpret_cast<const uint4 *>(buf[pl])[t];
-            for (int t = (bytes & ~15) + threadIdx.x; t < bytes; t += blockDim.x) o[t] = buf[pl][t];
-        } else {
-            for (int t = threadIdx.x; t < bytes; t += blockDim.x) o[t] = buf[pl][t];
+#pragma unroll
+    for (int u = 0; u < MXQ_PER; ++u) {
+        const int64_t g = b0 + u * MXQ_STEP + quad;
+        float v[8];
+#pragma unroll
+        for (int pl = 0; pl < MX_MAX_PLANES; ++pl) {
+            if (pl >= planes) break;
+            uint32_t byte;
+            float lo[4], hi[4];
+            mx_values(mx_take_block(m[pl][u], lane, byte), lo, hi);
+            const float s = mx_scale(byte);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[j] = pl == 0 ? lo[j] * s : v[j] + lo[j] * s;
+                v[4 + j] = pl == 0 ? hi[j] * s : v[4 + j] + hi[j] * s;
+            }
+        }
+        if (!FAST && g >= n_blocks) continue;
+        T *p = FAST ? out0 + u * (MXQ_STEP * 32) : out + mx_block_at(g, nb, stride, dense, small) + 4 * i;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            __align__(16) T e[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (OT == MX_F32) e[j] = v[4 * h + j];
+                else if constexpr (OT == MX_F16) e[j] = __float2half_rn(v[4 * h + j]);
+                else e[j] = __float2bfloat16_rn(v[4 * h + j]);
+            }
+            if constexpr (!VEC) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) p[16 * h + j] = e[j];
+            } else if constexpr (OT == MX_F32) {
+                *reinterpret_cast<float4 *>(p + 16 * h) = make_float4(e[0], e[1], e[2], e[3]);
+            } else {
+                *reinterpret_cast<uint2 *>(p + 16 * h) = *reinterpret_cast<const uint2 *>(e);
+            }
         }
     }
 }
 
-// ---------------------------------------------------------------------------
-// read back: out [rows][K] = the planes' values added, rounded once to OT
-// ---------------------------------------------------------------------------
 template <int OT, bool VEC>
-__global__ void __launch_bounds__(4 * MXQ_BLK) mx_dequantize_kernel(const uint8_t *__restrict__ y, int64_t n_blocks,
+__global__ void __launch_bounds__(MXQ_THREADS) mx_dequantize_kernel(const uint8_t *__restrict__ y, int64_t n_blocks,
                                                                     int nb, int planes, int64_t stride,
                                                                     typename MxElem<OT>::T *__restrict__ out) {
-    using T = typename MxElem<OT>::T;
-    __shared__ __align__(16) uint8_t buf[MX_MAX_PLANES][MXQ_BYTES];
-    const int lb = threadIdx.x >> 2, i = threadIdx.x & 3;
-    const int64_t b0 = static_cast<int64_t>(blockIdx.x) * MXQ_BLK;
-    const int64_t left = (n_blocks - b0) * 17;
-    const int bytes = left < MXQ_BYTES ? static_cast<int>(left) : MXQ_BYTES;
-    for (int pl = 0; pl < planes; ++pl) {
-        const uint8_t *o = y + pl * n_blocks * 17 + b0 * 17;
-        if ((reinterpret_cast<uintptr_t>(o) & 15u) == 0) {
-            for (int t = threadIdx.x; t < bytes / 16; t += blockDim.x)
-                reinterpret_cast<uint4 *>(buf[pl])[t] = __ldg(reinterpret_cast<const uint4 *>(o) + t);
-            for (int t = (bytes & ~15) + threadIdx.x; t < bytes; t += blockDim.x) buf[pl][t] = o[t];
-        } else {
-            for (int t = threadIdx.x; t < bytes; t += blockDim.x) buf[pl][t] = o[t];
-        }
-    }
-    __syncthreads();
-    const int64_t g = b0 + lb;
-    if (g >= n_blocks) return;
-    float v[8];
-    for (int pl = 0; pl < planes; ++pl) {
-        const uint8_t *o = buf[pl] + lb * 17;
-        uint32_t w = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w |= static_cast<uint32_t>(o[1 + 4 * i + j]) << (8 * j);
-        const float s = mx_scale(o[0]);
-        float q[8];
-        mx_values(w, q);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = pl == 0 ? q[j] * s : v[j] + q[j] * s;
-    }
-    const int64_t row = g / nb;
-    T *p = out + row * stride + (g - row * nb) * 32 + 4 * i;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        T e[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if constexpr (OT == MX_F32) e[j] = v[4 * h + j];
-            else if constexpr (OT == MX_F16) e[j] = __float2half_rn(v[4 * h + j]);
-            else e[j] = __float2bfloat16_rn(v[4 * h + j]);
-        }
-        if constexpr (!VEC) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) p[16 * h + j] = e[j];
-        } else if constexpr (OT == MX_F32) {
-            *reinterpret_cast<float4 *>(p + 16 * h) = make_float4(e[0], e[1], e[2], e[3]);
-        } else {
-            *reinterpret_cast<uint2 *>(p + 16 * h) = *reinterpret_cast<const uint2 *>(e);
-        }
-    }
+    if (VEC && mx_whole(y, stride, n_blocks, nb, planes)) mx_dequantize_blocks<OT, VEC, VEC>(y, n_blocks, nb, planes, stride, out);
+    else mx_dequantize_blocks<OT, VEC, false>(y, n_blocks, nb, planes, stride, out);
 }
 
 // ---------------------------------------------------------------------------
@@ -522,23 +670,24 @@ __global__ void __launch_bounds__(256) mx_images_kernel(const MxPrep a) {
     }
     const int64_t g = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 2;   // (row, block), K padded
     const int i = threadIdx.x & 3;
-    const int64_t row = g / (a.KT * 4);
+    const int64_t row = mx_row_of(g, a.KT * 4, a.n_rows * a.KT < (int64_t{1} << 28));
     const int b = static_cast<int>(g - row * (a.KT * 4)), tile = b >> 2;
     const bool row_ok = row < a.n_rows;
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (row_ok && b < a.nb) {
-        const typename MxElem<XT>::T *p = static_cast<const typename MxElem<XT>::T *>(a.x) + row * a.stride +
-                                          static_cast<int64_t>(b) * 32 + 4 * i;
-        mx_load4<XT, VEC>(p, v);
-        mx_load4<XT, VEC>(p + 16, v + 4);
-    }
+    MxRaw<XT> raw = mx_zero<XT>();
+    if (row_ok && b < a.nb)
+        raw = mx_load<XT, VEC>(static_cast<const typename MxElem<XT>::T *>(a.x) + row * a.stride + static_cast<int64_t>(b) * 32, i);
+    float v[8];
+    uint32_t top = mx_floats<XT>(raw, v);
     uint32_t w[MX_MAX_PLANES][4], sc[MX_MAX_PLANES];
 #pragma unroll
     for (int pl = 0; pl < MX_MAX_PLANES; ++pl) {
         if (pl >= a.planes) break;
         uint32_t byte;
-        const uint32_t mine = mx_quant_block(v, byte);
-        if (pl + 1 < a.planes) mx_residual(v, mine, byte);
+        const uint32_t mine = mx_quant_block(v, top, byte);
+        if (pl + 1 < a.planes) {
+            mx_residual(v, mine, byte);
+            top = mx_top(v);
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[pl][j] = __shfl_sync(0xffffffffu, mine, (lane & ~3) + j);   // the block's 16 bytes
         uint32_t word = byte << (8 * ((lane >> 2) & 3));                                          // the tile's 4 scales
@@ -1016,9 +1165,9 @@ void quantize_t(const void *x, int64_t stride, int64_t n_blocks, int nb, int pla
     using T = typename MxElem<XT>::T;
     const unsigned grid = static_cast<unsigned>((n_blocks + MXQ_BLK - 1) / MXQ_BLK);
     if (mx_vec_ok<XT>(x, stride))
-        mx_quantize_kernel<XT, true><<<grid, 4 * MXQ_BLK, 0, st>>>(static_cast<const T *>(x), stride, n_blocks, nb, planes, y);
+        mx_quantize_kernel<XT, true><<<grid, MXQ_THREADS, 0, st>>>(static_cast<const T *>(x), stride, n_blocks, nb, planes, y);
     else
-        mx_quantize_kernel<XT, false><<<grid, 4 * MXQ_BLK, 0, st>>>(static_cast<const T *>(x), stride, n_blocks, nb, planes, y);
+        mx_quantize_kernel<XT, false><<<grid, MXQ_THREADS, 0, st>>>(static_cast<const T *>(x), stride, n_blocks, nb, planes, y);
 }
 
 template <int OT>
@@ -1026,9 +1175,9 @@ void dequantize_t(const uint8_t *y, int64_t n_blocks, int nb, int planes, void *
     using T = typename MxElem<OT>::T;
     const unsigned grid = static_cast<unsigned>((n_blocks + MXQ_BLK - 1) / MXQ_BLK);
     if (mx_vec_ok<OT>(out, stride))
-        mx_dequantize_kernel<OT, true><<<grid, 4 * MXQ_BLK, 0, st>>>(y, n_blocks, nb, planes, stride, static_cast<T *>(out));
+        mx_dequantize_kernel<OT, true><<<grid, MXQ_THREADS, 0, st>>>(y, n_blocks, nb, planes, stride, static_cast<T *>(out));
     else
-        mx_dequantize_kernel<OT, false><<<grid, 4 * MXQ_BLK, 0, st>>>(y, n_blocks, nb, planes, stride, static_cast<T *>(out));
+        mx_dequantize_kernel<OT, false><<<grid, MXQ_THREADS, 0, st>>>(y, n_blocks, nb, planes, stride, static_cast<T *>(out));
 }
 
 template <int XT, bool VEC, bool DIRECT>

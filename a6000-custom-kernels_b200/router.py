@@ -4,7 +4,7 @@ import ctypes
 
 import torch
 
-from ._call import ELEM, On, dense_rows, need
+from ._call import ELEM, bad, dense_rows, given, on
 from ._lib import MoeRouter, check, lib
 
 SCORES = {"softmax": 0, "sigmoid": 1, "softmax_topk": 2}
@@ -20,31 +20,34 @@ class Router:
     multiplies them."""
 
     def __init__(self, k, score="softmax", bias=None, n_group=1, topk_group=1, group_score="top2", norm_w=False, scale=1.0):
-        need(score in SCORES, f"score must be one of {sorted(SCORES)}")
-        need(group_score in GROUP_SCORES, f"group_score must be one of {sorted(GROUP_SCORES)}")
-        need(bias is None or (isinstance(bias, torch.Tensor) and bias.is_cuda and bias.dtype == torch.float32 and
-                              bias.dim() == 1 and bias.is_contiguous()), "bias must be a contiguous f32 CUDA vector")
+        if score not in SCORES:
+            raise bad(f"score must be one of {sorted(SCORES)}")
+        if group_score not in GROUP_SCORES:
+            raise bad(f"group_score must be one of {sorted(GROUP_SCORES)}")
+        if bias is not None and not (isinstance(bias, torch.Tensor) and bias.is_cuda and bias.dtype == torch.float32 and
+                                     bias.dim() == 1 and bias.is_contiguous()):
+            raise bad("bias must be a contiguous f32 CUDA vector")
         self.k, self.bias = k, bias
-        self.desc = MoeRouter(SCORES[score], n_group, topk_group, GROUP_SCORES[group_score], int(norm_w), scale)
+        self.desc = MoeRouter(SCORES[score], n_group, topk_group, GROUP_SCORES[group_score], norm_w, scale)
         self.ref = ctypes.byref(self.desc)
 
     def __call__(self, logits, ids=None, weights=None, stream=None):
         """logits f32 / f16 / bf16 [n_tok, E] -> (ids i32 [n_tok, k], weights f32 [n_tok, k])."""
-        stride, _ = dense_rows(logits, "logits", ELEM)
-        need(logits.dim() == 2, "logits must be [n_tok, n_experts]")
+        stride = dense_rows(logits, "logits")
+        if logits.dim() != 2:
+            raise bad("logits must be [n_tok, n_experts]")
         n_tok, E = logits.shape
-        dev = logits.device
-        need(self.bias is None or (self.bias.device == dev and self.bias.numel() == E), "bias must be f32 [n_experts] on the logits' device")
-        with On(dev, stream) as st:
-            if ids is None:
-                ids = torch.empty((n_tok, self.k), dtype=torch.int32, device=dev)
-            if weights is None:
-                weights = torch.empty((n_tok, self.k), dtype=torch.float32, device=dev)
-            for name, t, dt in (("ids", ids, torch.int32), ("weights", weights, torch.float32)):
-                need(t.dtype == dt and t.device == dev and t.is_contiguous() and tuple(t.shape) == (n_tok, self.k),
-                     f"{name} must be contiguous {dt} [n_tok, k] on the logits' device")
-            check(lib().moe_b200_route_experts(self.ref, logits.data_ptr(), ELEM[logits.dtype], max(stride, E),
-                                               None if self.bias is None else self.bias.data_ptr(), n_tok, E, self.k,
+        k, dev, bias = self.k, logits.device, self.bias
+        if bias is not None and (bias.device != dev or bias.shape[0] != E):
+            raise bad("bias must be f32 [n_experts] on the logits' device")
+        ctx, st = on(dev, stream)
+        with ctx:
+            ids = logits.new_empty((n_tok, k), dtype=torch.int32) if ids is None else \
+                given(ids, "ids", torch.int32, (n_tok, k), dev)
+            weights = logits.new_empty((n_tok, k), dtype=torch.float32) if weights is None else \
+                given(weights, "weights", torch.float32, (n_tok, k), dev)
+            check(lib().moe_b200_route_experts(self.ref, logits.data_ptr(), ELEM[logits.dtype], stride,
+                                               None if bias is None else bias.data_ptr(), n_tok, E, k,
                                                ids.data_ptr(), weights.data_ptr(), st))
         return ids, weights
 
