@@ -111,10 +111,11 @@ struct RouteArgs {
     const float *bias;       // [n_experts] or null
     int32_t n_experts, k, score, n_group, topk_group, group_score, norm_w;
     float scale;
+    uint32_t group_magic;    // set by the launcher
     int32_t *ids;            // [tok][k]
     float *weights;          // [tok][k]
 };
-cudaError_t launch_route(const RouteArgs &a, int logits_type, cudaStream_t st);
+cudaError_t launch_route(RouteArgs a, int logits_type, cudaStream_t st);
 
 // MXFP4 (moe_mx.cu). Element types: MX_F32, MX_F16, MX_BF16; strides in elements.
 cudaError_t launch_mx_quantize(const void *x, int xt, int64_t stride, int64_t n_rows, int64_t n_cols, int planes,
