@@ -69,6 +69,14 @@ class MoeMxfp4(ctypes.Structure):
     _fields_ = [("data", ctypes.c_void_p), ("n_experts", ctypes.c_int64), ("rows", ctypes.c_int64), ("K", ctypes.c_int64)]
 
 
+class MoeMxfp4Layer(ctypes.Structure):
+    _fields_ = [("gate", MoeMxfp4), ("up", MoeMxfp4), ("down", MoeMxfp4), ("gate_bias", ctypes.c_void_p),
+                ("up_bias", ctypes.c_void_p), ("down_bias", ctypes.c_void_p), ("shared_gate", MoeMxfp4),
+                ("shared_up", MoeMxfp4), ("shared_down", MoeMxfp4), ("k", ctypes.c_int64), ("glu_op", ctypes.c_int32),
+                ("glu_limit", ctypes.c_float), ("planes", ctypes.c_int32), ("router", MoeRouter),
+                ("router_bias", ctypes.c_void_p)]
+
+
 def _sources():
     out = []
     for d in (CSRC, os.path.join(REPO, "include")):
@@ -143,6 +151,8 @@ def _declare(L):
         "moe_b200_route_experts": (i32, [ctypes.POINTER(MoeRouter), vp, i32, i64, vp, i64, i64, i64, vp, vp, vp]),
         "moe_b200_quantize_mxfp4": (i32, [vp, i32, i64, i64, i64, i32, vp, vp]),
         "moe_b200_dequantize_mxfp4": (i32, [vp, i64, i64, i32, vp, i32, i64, vp]),
+        "moe_b200_mxfp4_layer_workspace_size": (sz, [ctypes.POINTER(MoeMxfp4Layer), i64]),
+        "moe_b200_mxfp4_layer_run": (i32, [ctypes.POINTER(MoeMxfp4Layer), vp, i32, i64, vp, i32, i64, vp, i64, vp, sz, vp]),
         "moe_b200_mxfp4_packed_size": (sz, [i64, i64, i64]),
         "moe_b200_mxfp4_pack": (i32, [PT, vp, sz, vp]),
         "moe_b200_mxfp4_workspace_size": (sz, [ctypes.POINTER(MoeMxfp4), i64, i64, i32]),

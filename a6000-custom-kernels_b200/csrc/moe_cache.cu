@@ -2243,3 +2243,112 @@ int moe_b200_mxfp4_mul_mat_id(const moe_mxfp4 *w, const moe_mxfp4 *gate, const f
 }
 
 }  // extern "C"
+
+// ---- MXFP4 layer --------------------------------------------------------------
+namespace {
+
+struct MxLayerWs {
+    int32_t *ids, *zero_ids;
+    float *w, *h, *y, *hs, *ys;
+    char *scratch;
+    size_t scratch_bytes, bytes;
+};
+
+MxLayerWs mx_layer_ws(const moe_mxfp4_layer *L, int64_t n, char *base) {
+    MxLayerWs w{};
+    size_t off = 0;
+    auto take = [&](size_t bytes) { char *p = base ? base + off : nullptr; off += align256(bytes); return p; };
+    const size_t nk = static_cast<size_t>(n * L->k), F = static_cast<size_t>(L->up.rows), H = static_cast<size_t>(L->up.K);
+    w.ids = reinterpret_cast<int32_t *>(take(4 * nk));
+    w.w = reinterpret_cast<float *>(take(4 * nk));
+    w.h = reinterpret_cast<float *>(take(4 * nk * F));
+    w.y = reinterpret_cast<float *>(take(4 * nk * H));
+    const bool shared = L->shared_up.data != nullptr;
+    if (shared) {
+        w.zero_ids = reinterpret_cast<int32_t *>(take(4 * static_cast<size_t>(n)));
+        w.hs = reinterpret_cast<float *>(take(4 * static_cast<size_t>(n) * static_cast<size_t>(L->shared_up.rows)));
+        w.ys = reinterpret_cast<float *>(take(4 * static_cast<size_t>(n) * H));
+    }
+    auto need = [&](const moe_mxfp4 &m, int64_t k) {
+        w.scratch_bytes = std::max(w.scratch_bytes, mx_ws(m.n_experts, m.K, n, k, L->planes, nullptr).bytes);
+    };
+    need(L->up, L->k);
+    need(L->down, L->k);
+    if (shared) {
+        need(L->shared_up, 1);
+        need(L->shared_down, 1);
+    }
+    w.scratch = take(w.scratch_bytes);
+    w.bytes = off;
+    return w;
+}
+
+int mx_layer_check(const moe_mxfp4_layer *L) {
+    if (!L) return fail(MOE_ERR_INVALID, "null argument");
+    int rc = mx_shape_check(L->up.n_experts, L->up.rows, L->up.K);
+    if (!rc) rc = mx_shape_check(L->down.n_experts, L->down.rows, L->down.K);
+    if (rc) return rc;
+    auto same = [](const moe_mxfp4 &a, const moe_mxfp4 &b) { return a.n_experts == b.n_experts && a.rows == b.rows && a.K == b.K; };
+    if (!same(L->gate, L->up)) return fail(MOE_ERR_INVALID, "gate and up must have one shape");
+    if (L->down.n_experts != L->up.n_experts || L->down.K != L->up.rows || L->down.rows != L->up.K)
+        return fail(MOE_ERR_INVALID, "down must be [n_experts][H][F] for gate and up [n_experts][F][H]");
+    if (L->k < 1 || L->k > 32 || L->k > L->up.n_experts) return fail(MOE_ERR_INVALID, "need 1 <= k <= min(32, n_experts)");
+    if (L->planes < 1 || L->planes > moe::MX_MAX_PLANES) return fail(MOE_ERR_INVALID, "planes must be 1 or 2");
+    if (L->shared_up.data) {
+        rc = mx_shape_check(L->shared_up.n_experts, L->shared_up.rows, L->shared_up.K);
+        if (rc) return rc;
+        if (!L->shared_gate.data || !L->shared_down.data || !same(L->shared_gate, L->shared_up) || L->shared_up.n_experts != 1 ||
+            L->shared_up.K != L->up.K || L->shared_down.n_experts != 1 || L->shared_down.K != L->shared_up.rows ||
+            L->shared_down.rows != L->up.K)
+            return fail(MOE_ERR_INVALID, "the shared expert must be gate, up [1][Fs][H] and down [1][H][Fs]");
+    }
+    return MOE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t moe_b200_mxfp4_layer_workspace_size(const moe_mxfp4_layer *layer, int64_t n_tok) {
+    std::lock_guard<std::recursive_mutex> lock(g_mu);
+    if (mx_layer_check(layer) || n_tok < 1 || n_tok > (int64_t{1} << 30) / layer->k) return 0;
+    return mx_layer_ws(layer, n_tok, nullptr).bytes;
+}
+
+int moe_b200_mxfp4_layer_run(const moe_mxfp4_layer *layer, const void *x, int32_t x_type, int64_t x_row_stride,
+                             const void *logits, int32_t logits_type, int64_t logits_row_stride, float *out, int64_t n_tok,
+                             void *workspace, size_t workspace_bytes, moe_stream_t stream) {
+    std::lock_guard<std::recursive_mutex> lock(g_mu);
+    int rc = mx_layer_check(layer);
+    if (rc) return rc;
+    const moe_mxfp4_layer &L = *layer;
+    if (n_tok < 0 || n_tok > (int64_t{1} << 30) / L.k) return fail(MOE_ERR_INVALID, "need 0 <= n_tok, n_tok * k <= 2^30");
+    if (n_tok == 0) return MOE_OK;
+    if (!x || !logits || !out) return fail(MOE_ERR_INVALID, "null argument");
+    const MxLayerWs w = mx_layer_ws(layer, n_tok, static_cast<char *>(workspace));
+    if (!workspace || workspace_bytes < w.bytes)
+        return fail(MOE_ERR_INVALID, "workspace too small (%zu < %zu bytes)", workspace_bytes, w.bytes);
+    if (!aligned16(workspace)) return fail(MOE_ERR_INVALID, "workspace must be 16-byte aligned");
+    const int64_t k = L.k, F = L.up.rows, H = L.up.K;
+    rc = moe_b200_route_experts(&L.router, logits, logits_type, logits_row_stride, L.router_bias, n_tok, L.up.n_experts, k,
+                                w.ids, w.w, stream);
+    if (!rc)
+        rc = moe_b200_mxfp4_mul_mat_id(&L.up, &L.gate, L.up_bias, L.gate_bias, L.glu_op, L.glu_limit, x, x_type, x_row_stride, 0,
+                                       n_tok, w.ids, k, k, L.planes, w.h, w.scratch, w.scratch_bytes, stream);
+    if (!rc)
+        rc = moe_b200_mxfp4_mul_mat_id(&L.down, nullptr, L.down_bias, nullptr, 0, 0.f, w.h, MOE_TYPE_F32, F, 1, n_tok, w.ids, k, k,
+                                       L.planes, w.y, w.scratch, w.scratch_bytes, stream);
+    if (!rc && L.shared_up.data) {
+        CK(cudaMemsetAsync(w.zero_ids, 0, 4 * static_cast<size_t>(n_tok), reinterpret_cast<cudaStream_t>(stream)));
+        rc = moe_b200_mxfp4_mul_mat_id(&L.shared_up, &L.shared_gate, nullptr, nullptr, L.glu_op, L.glu_limit, x, x_type,
+                                       x_row_stride, 0, n_tok, w.zero_ids, 1, 1, L.planes, w.hs, w.scratch, w.scratch_bytes, stream);
+        if (!rc)
+            rc = moe_b200_mxfp4_mul_mat_id(&L.shared_down, nullptr, nullptr, nullptr, 0, 0.f, w.hs, MOE_TYPE_F32, L.shared_up.rows, 0,
+                                           n_tok, w.zero_ids, 1, 1, L.planes, w.ys, w.scratch, w.scratch_bytes, stream);
+    }
+    if (rc) return rc;
+    CK(moe::launch_combine(w.y, w.w, L.shared_up.data ? w.ys : nullptr, out, n_tok, H, k, reinterpret_cast<cudaStream_t>(stream)));
+    return MOE_OK;
+}
+
+}  // extern "C"

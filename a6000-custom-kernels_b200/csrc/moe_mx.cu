@@ -329,8 +329,8 @@ __device__ __forceinline__ void mx_dequantize_blocks(const uint8_t *__restrict__
             const float s = mx_scale(byte);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                v[j] = pl == 0 ? lo[j] * s : v[j] + lo[j] * s;
-                v[4 + j] = pl == 0 ? hi[j] * s : v[4 + j] + hi[j] * s;
+                v[j] = pl == 0 ? lo[j] * s : __fadd_rn(v[j], __fmul_rn(lo[j], s));   // (each value as it stands in 32 bits)
+                v[4 + j] = pl == 0 ? hi[j] * s : __fadd_rn(v[4 + j], __fmul_rn(hi[j], s));
             }
         }
         if (!FAST && g >= n_blocks) continue;
@@ -751,10 +751,12 @@ __host__ __device__ constexpr uint32_t mx_stage_bytes(int mats, int planes) {
 
 template <int NT>
 __device__ __forceinline__ bool mx_wait(MxCtl<NT> &C, uint64_t *bar, uint32_t parity, const MxArgs &a) {
-    if (mbar_try_wait(bar, parity)) return true;
+    // limits below 20 us poll (try_wait may suspend for longer), so that a tiny limit gives up at once
+    const bool poll = a.timeout_ns < 20000u;
+    if (poll ? mbar_test_wait(bar, parity) : mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = clock64(), lim = timeout_cycles(a.timeout_ns);
     for (;;) {
-        if (mbar_try_wait_hint(bar, parity, 2000u)) return true;
+        if (poll ? mbar_test_wait(bar, parity) : mbar_try_wait_hint(bar, parity, 2000u)) return true;
         if (*reinterpret_cast<volatile int32_t *>(&C.abort)) return false;
         if (static_cast<uint64_t>(clock64()) - t0 > lim) {
             *reinterpret_cast<volatile int32_t *>(&C.abort) = 1;

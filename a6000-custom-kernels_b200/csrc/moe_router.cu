@@ -108,8 +108,8 @@ __device__ __forceinline__ T group_score_of(const T *s, int gsz, int n_group, in
         m2 = lo > hi ? lo : hi;
         m1 = m1 > o1 ? m1 : o1;
     }
-    if (group_score == ROUTE_GROUP_MAX || gsz == 1) return m1;
-    return m1 > 0 && m1 * static_cast<T>(0.5) == m1 ? m1 : m1 + m2;   // (infinity whatever the second is)
+    // (one expert left in the group counts alone)
+    return group_score == ROUTE_GROUP_MAX || !(m2 > -INFINITY) ? m1 : m1 + m2;
 }
 __device__ __forceinline__ int lanes_per_group(int n_group) {
     int per = 1;

@@ -7,20 +7,36 @@ around the reference's intercepted MUL_MAT_ID calls (build_moe_ffn order:
 route, gate/up, GLU, down, weight, sum over picks, add the shared expert).
 """
 import ctypes
+import math
 
 import torch
 
-from ._lib import MoeLayerDesc, check, lib
-from .moe_cache import GLU_SWIGLU, _ptr, _stream, expert_tensor, fill_quantized, row_size
+from ._call import ELEM, bad, dense_rows, given, on
+from ._lib import MoeLayerDesc, MoeMxfp4Layer, check, lib
+from .moe_cache import GLU_SWIGLU, MXFP4, _ptr, _stream, expert_tensor, fill_quantized, row_size
+from .mxfp4 import MXFP4Weights, quantize_mxfp4
+from .router import Router
 
 
 class MoELayer:
     """Expert weights live in `device` memory (HBM-resident) unless `host=True`,
-    in which case they live in pinned host memory behind the tiered cache."""
+    in which case they live in pinned host memory behind the tiered cache.
+
+    `router` (a Router) makes tokens pick their experts as it says, through
+    decode and prefill alike; None is softmax over all experts, top-k.
+    MoELayer(..., types with MXFP4 for gate, up and down) makes an MXFP4Layer."""
+
+    def __new__(cls, H=None, F=None, n_experts=None, k=None, types=None, **kw):
+        if cls is MoELayer and types is not None and MXFP4 in dict(types).values():
+            return super().__new__(MXFP4Layer)
+        return super().__new__(cls)
 
     def __init__(self, H, F, n_experts, k, types, shared=True, glu_op=GLU_SWIGLU, glu_limit=0.0, norm_w=False,
-                 device="cuda", host=False, name="blk.0", seed=0, weights=None, sigma=0.02):
+                 device="cuda", host=False, name="blk.0", seed=0, weights=None, sigma=0.02, router=None):
         self.H, self.F, self.E, self.k = H, F, n_experts, k
+        if router is not None and router.k != k:
+            raise bad("the router picks another number of experts than the layer has")
+        self.router = router
         self.types = dict(types)          # {"gate": t, "up": t, "down": t}
         self.glu_op, self.glu_limit, self.norm_w = glu_op, glu_limit, norm_w
         self.device = torch.device(device)
@@ -88,6 +104,8 @@ class MoELayer:
         record per expert tensor, as the reference's trace hook writes it for
         each MUL_MAT_ID (this reads the ids back to the host)."""
         n_tok = x.shape[0]
+        if self.router is not None:
+            return self._routed(x, logits, out, stream, trace)
         if out is None:
             out = torch.empty((n_tok, self.H), dtype=torch.float32, device=self.device)
         ws = self.workspace(n_tok)
@@ -103,6 +121,8 @@ class MoELayer:
         """x f32 [n_tok, H], logits f32 [n_tok, E] (device) -> out f32 [n_tok, H] for any
         n_tok: the tensor-core prefill path (moe_b200_layer_prefill)."""
         n_tok = x.shape[0]
+        if self.router is not None:
+            return self._routed(x, logits, out, stream)
         if out is None:
             out = torch.empty((n_tok, self.H), dtype=torch.float32, device=self.device)
         key = ("prefill", n_tok)
@@ -113,6 +133,36 @@ class MoELayer:
             self._ws[key] = ws
         check(lib().moe_b200_layer_prefill(ctypes.byref(self.desc), _ptr(x), _ptr(logits), _ptr(out), n_tok,
                                            _ptr(ws), ws.numel(), _stream(stream)))
+        return out
+
+    def _routed(self, x, logits, out, stream, trace=None):
+        """The layer with its own router: route, the experts of the picks, the
+        shared expert, combine (any n_tok >= 1; x contiguous f32)."""
+        n_tok, dev = x.shape[0], self.device
+        if x.dtype != torch.float32 or not x.is_contiguous() or tuple(x.shape) != (n_tok, self.H) or n_tok < 1 or \
+                tuple(logits.shape) != (n_tok, self.E):
+            raise bad("x must be contiguous f32 [n_tok, H] with n_tok >= 1, logits [n_tok, n_experts]")
+        ctx, st = on(x.device, stream)
+        with ctx:
+            ids, w = self.router(logits)
+            if out is None:
+                out = torch.empty((n_tok, self.H), dtype=torch.float32, device=dev)
+            kept = self._ws.get(("routed", n_tok))
+            if kept is None:
+                nbytes = lib().moe_b200_experts_prefill_workspace_size(ctypes.byref(self.desc), n_tok, self.k)
+                kept = self._ws[("routed", n_tok)] = (
+                    torch.empty(nbytes, dtype=torch.uint8, device=dev),
+                    torch.empty((n_tok, self.k, self.H), dtype=torch.float32, device=dev),
+                    torch.empty((n_tok, self.H), dtype=torch.float32, device=dev) if self.shared else None)
+            ws, y, ys = kept
+            check(lib().moe_b200_experts_prefill(ctypes.byref(self.desc), _ptr(x), 0, _ptr(ids), n_tok, self.k, _ptr(y),
+                                                 _ptr(ws), ws.numel(), st))
+            if ys is not None:
+                check(lib().moe_b200_shared_prefill(ctypes.byref(self.desc), _ptr(x), n_tok, _ptr(ys), _ptr(ws), ws.numel(), st))
+            check(lib().moe_b200_combine(_ptr(y), _ptr(w), _ptr(ys), _ptr(out), n_tok, self.H, self.k, st))
+        if trace is not None:
+            for r in ("gate", "up", "down"):
+                trace.record(self.desc_t[r].name.decode(), ids.cpu().numpy(), self.E)
         return out
 
     def prefill_intermediates(self, n_tok):
@@ -154,6 +204,120 @@ class MoELayer:
         """(ids, weights) views of the last decode's routing in the workspace."""
         ids, w = self.intermediates(n_tok)[:2]
         return ids, w
+
+
+class MXFP4Layer(MoELayer):
+    """One MoE FFN layer whose experts are MXFP4 (gate, up and down alike), in
+    device memory, laid out for the 4-bit tensor cores
+    (moe_b200_mxfp4_layer_run). `router` (a Router) says how tokens pick their
+    experts, None as MoELayer does: softmax, top-k. `biases` may hold f32
+    "gate", "up" [E, F] and "down" [E, H]; `planes` MXFP4 planes hold every
+    activation. `weights` as MoELayer's: ggml blocks, uint8 [E, rows, bytes] per
+    role and [rows, bytes] for "shared_<role>" (whose F may be its own); None
+    draws N(0, sigma)."""
+
+    def __init__(self, H, F, n_experts, k, types, shared=True, glu_op=GLU_SWIGLU, glu_limit=0.0, norm_w=False, device="cuda",
+                 host=False, name="blk.0", seed=0, weights=None, sigma=0.02, router=None, biases=None, planes=2):
+        self.types = dict(types)
+        if set(self.types.values()) != {MXFP4}:
+            raise bad("an MXFP4 layer has gate, up and down of type MXFP4")
+        if host:
+            raise bad("MXFP4 experts live in device memory")
+        device = torch.device(device)
+        if device.index is None:
+            device = torch.device(device.type, torch.cuda.current_device())
+        self.H, self.F, self.E, self.k, self.device = H, F, n_experts, k, device
+        self.glu_op, self.glu_limit, self.norm_w, self.planes = glu_op, glu_limit, norm_w, planes
+        self.router = Router(k, norm_w=norm_w) if router is None else router
+        if self.router.k != k:
+            raise bad("the router picks another number of experts than the layer has")
+        rb = self.router.bias
+        if rb is not None and (rb.device != device or rb.shape[0] != n_experts):
+            raise bad("the router's bias must be f32 [n_experts] on the layer's device")
+        shapes = {"gate": (F, H), "up": (F, H), "down": (H, F)}
+        gen = torch.Generator(device=device).manual_seed(seed)
+
+        def blocks(key, n, rows, K):
+            if weights is not None:
+                b = torch.as_tensor(weights[key]).to(device)
+                return b.reshape(n, *b.shape[-2:]).contiguous()
+            return quantize_mxfp4(sigma * torch.randn((n, rows, K), generator=gen, device=device))
+        self.w, self.shared, self.biases = {}, {}, {}
+        for role, (rows, K) in shapes.items():
+            self.w[role] = MXFP4Weights(blocks(role, n_experts, rows, K), K, rows)
+        if shared and (weights is None or weights.get("shared_up") is not None):
+            Fs = F if weights is None else torch.as_tensor(weights["shared_up"]).shape[-2]
+            for role, (rows, K) in (("gate", (Fs, H)), ("up", (Fs, H)), ("down", (H, Fs))):
+                self.shared[role] = MXFP4Weights(blocks(f"shared_{role}", 1, rows, K), K, rows)
+        d = MoeMxfp4Layer()
+        for role in shapes:
+            setattr(d, role, self.w[role].desc)
+            if self.shared:
+                setattr(d, f"shared_{role}", self.shared[role].desc)
+            b = (biases or {}).get(role)
+            if b is not None:
+                given(b, f"{role} bias", torch.float32, (n_experts, shapes[role][0]), device)
+                self.biases[role] = b
+                setattr(d, f"{role}_bias", b.data_ptr())
+        d.k, d.glu_op, d.glu_limit, d.planes, d.router = k, glu_op, glu_limit, planes, self.router.desc
+        d.router_bias = None if rb is None else rb.data_ptr()
+        self.desc, self.ref, self._ws = d, ctypes.byref(d), {}
+
+    def weight_bytes_per_token(self):
+        """Expert bytes one batch-1 token streams: k routed + shared experts x 3 matrices."""
+        per = sum(self.w[r].data.numel() // self.E for r in ("gate", "up", "down"))
+        return per * self.k + sum(m.data.numel() for m in self.shared.values())
+
+    def workspace(self, n_tok):
+        ws = self._ws.get(n_tok)
+        if ws is None:
+            nbytes = lib().moe_b200_mxfp4_layer_workspace_size(self.ref, n_tok)
+            ws = self._ws[n_tok] = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        return ws
+
+    def fused(self, n_tok):
+        return False
+
+    def decode(self, x, logits, out=None, stream=None, trace=None):
+        """x f32 / f16 / bf16 [n_tok, H], logits f32 / f16 / bf16 [n_tok, E] -> out f32
+        [n_tok, H], for one token or a prompt. Uses the layer's workspace for
+        n_tok: calls for the same n_tok must not overlap on the GPU. `trace` as
+        MoELayer.decode."""
+        xs, ls = dense_rows(x, "x"), dense_rows(logits, "logits")
+        n_tok, dev = x.shape[0], self.device
+        if tuple(x.shape) != (n_tok, self.H) or tuple(logits.shape) != (n_tok, self.E) or x.device != dev or logits.device != dev:
+            raise bad("x must be [n_tok, H] and logits [n_tok, n_experts] on the layer's device")
+        ctx, st = on(dev, stream)
+        with ctx:
+            out = x.new_empty((n_tok, self.H), dtype=torch.float32) if out is None else \
+                given(out, "out", torch.float32, (n_tok, self.H), dev)
+            if n_tok:
+                ws = self.workspace(n_tok)
+                check(lib().moe_b200_mxfp4_layer_run(self.ref, x.data_ptr(), ELEM[x.dtype], xs, logits.data_ptr(),
+                                                     ELEM[logits.dtype], ls, out.data_ptr(), n_tok, ws.data_ptr(), ws.numel(), st))
+        if trace is not None and n_tok:
+            ids = self.routing_of(n_tok)[0].cpu().numpy()
+            for r in ("gate", "up", "down"):
+                trace.record(f"ffn_{r}_exps.weight", ids, self.E)
+        return out
+
+    prefill = decode
+
+    def intermediates(self, n_tok):
+        """Views of the last call's workspace: ids [n][k], weights [n][k], h [n][k][F]
+        (GLU output), y [n][k][H] (down outputs)."""
+        ws, n, k = self._ws[n_tok], n_tok, self.k
+        out, off = [], 0
+        for dt, shape in ((torch.int32, (n, k)), (torch.float32, (n, k)), (torch.float32, (n, k, self.F)),
+                          (torch.float32, (n, k, self.H))):
+            nbytes = 4 * math.prod(shape)
+            out.append(ws[off: off + nbytes].view(dt).view(shape))
+            off += (nbytes + 255) // 256 * 256
+        return tuple(out)
+
+    def routing_of(self, n_tok):
+        """(ids, weights) views of the last call's routing in the workspace."""
+        return self.intermediates(n_tok)[:2]
 
 
 class Stack:

@@ -464,7 +464,7 @@ enum { MOE_ROUTE_SOFTMAX = 0,        /* s = softmax over all experts */
        MOE_ROUTE_SIGMOID = 1,        /* s = 1 / (1 + exp(-l)) */
        MOE_ROUTE_SOFTMAX_TOPK = 2 }; /* s = l; weights = softmax over the picks' logits */
 enum { MOE_ROUTE_GROUP_MAX = 0,      /* a group's score: its largest c */
-       MOE_ROUTE_GROUP_TOP2 = 1 };   /* the sum of its two largest c */
+       MOE_ROUTE_GROUP_TOP2 = 1 };   /* the sum of its two largest c (of the one, where one is above -inf) */
 typedef struct {
     int32_t score;                 /* MOE_ROUTE_* */
     int32_t n_group, topk_group;   /* n_group groups of consecutive experts, the topk_group best stay (1, 1: no groups) */
@@ -552,6 +552,33 @@ int moe_b200_mxfp4_mul_mat_id(const moe_mxfp4 *w, const moe_mxfp4 *gate, const f
                               int32_t glu_op, float glu_limit, const void *x, int32_t x_type, int64_t x_row_stride,
                               int32_t x_per_pick, int64_t n_tok, const int32_t *ids, int64_t k, int64_t ids_stride,
                               int32_t planes, float *dst, void *workspace, size_t workspace_bytes, moe_stream_t stream);
+
+/* One MoE FFN layer of MXFP4 experts: matrices laid out by moe_b200_mxfp4_pack,
+ * gate and up [n_experts][F][H], down [n_experts][H][F]. */
+typedef struct {
+    moe_mxfp4    gate, up, down;
+    const float *gate_bias, *up_bias, *down_bias;        /* f32 [n_experts][rows] or NULL */
+    moe_mxfp4    shared_gate, shared_up, shared_down;    /* one expert each, [1][Fs][H] and [1][H][Fs]; data NULL: none */
+    int64_t      k;                                      /* picks per token */
+    int32_t      glu_op;
+    float        glu_limit;
+    int32_t      planes;                                 /* MXFP4 planes of every activation */
+    moe_router   router;
+    const float *router_bias;                            /* f32 [n_experts] or NULL */
+} moe_mxfp4_layer;
+
+/* The layer for n_tok tokens, one or a prompt: out[t] = sum over the picks p of
+ * weight[t][p] * down(GLU(gate . x, up . x)), plus the shared expert, from
+ * moe_b200_route_experts, moe_b200_mxfp4_mul_mat_id (gate and up with the GLU,
+ * then down with a row per pick) and moe_b200_combine, on one stream. x and
+ * logits F32, F16 or BF16 with row strides in elements, out f32 [n_tok][H].
+ * Workspace as moe_b200_mxfp4_mul_mat_id; its start holds, each part 256-byte
+ * aligned, ids int32 [n_tok][k], weights f32 [n_tok][k], h f32 [n_tok][k][F] and
+ * the down outputs y f32 [n_tok][k][H]. n_tok may be 0. */
+size_t moe_b200_mxfp4_layer_workspace_size(const moe_mxfp4_layer *layer, int64_t n_tok);
+int moe_b200_mxfp4_layer_run(const moe_mxfp4_layer *layer, const void *x, int32_t x_type, int64_t x_row_stride,
+                             const void *logits, int32_t logits_type, int64_t logits_row_stride, float *out, int64_t n_tok,
+                             void *workspace, size_t workspace_bytes, moe_stream_t stream);
 
 #ifdef __cplusplus
 }
