@@ -2060,14 +2060,19 @@ struct MxWs {
     size_t bytes;
 };
 
+// sized for the call with and without a gate (their widest chunks differ)
 MxWs mx_ws(int64_t E, int64_t K, int64_t n_tok, int64_t k, int planes, char *base) {
     MxWs w{};
     size_t off = 0;
     auto take = [&](size_t bytes) { char *p = base ? base + off : nullptr; off += align256(bytes); return p; };
     const bool direct = moe::mx_direct(n_tok, k);
-    const int NT = moe::mx_chunk_tokens(n_tok, k, E);
-    w.max_chunks = direct ? n_tok * k : moe::mmq_max_chunks(n_tok * k, E, NT);
-    const size_t images = static_cast<size_t>(moe::mx_images_bytes(w.max_chunks, NT, K, planes));
+    size_t images = 0;
+    for (const bool glu : {false, true}) {
+        const int NT = moe::mx_chunk_tokens(n_tok, k, E, glu);
+        const int64_t chunks = direct ? n_tok * k : moe::mmq_max_chunks(n_tok * k, E, NT);
+        w.max_chunks = std::max(w.max_chunks, chunks);
+        images = std::max(images, static_cast<size_t>(moe::mx_images_bytes(chunks, NT, K, planes)));
+    }
     w.images = reinterpret_cast<uint8_t *>(take(images));
     if (!direct) {
         w.entries = reinterpret_cast<int32_t *>(take(4 * static_cast<size_t>(n_tok * k)));
@@ -2207,9 +2212,9 @@ int moe_b200_mxfp4_mul_mat_id(const moe_mxfp4 *w, const moe_mxfp4 *gate, const f
     }
     rc = ensure_device();
     if (rc) return rc;
-    const int NT = moe::mx_chunk_tokens(n_tok, k, w->n_experts);
+    const int NT = moe::mx_chunk_tokens(n_tok, k, w->n_experts, gate != nullptr);
     const bool direct = moe::mx_direct(n_tok, k);
-    const int64_t units = s.max_chunks;
+    const int64_t units = direct ? n_tok * k : moe::mmq_max_chunks(n_tok * k, w->n_experts, NT);
     moe::MxArgs a{};
     a.RT = static_cast<int32_t>(mx_row_tiles(w->rows));
     a.KT = static_cast<int32_t>(mx_k_tiles(w->K));

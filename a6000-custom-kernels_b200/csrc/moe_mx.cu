@@ -400,8 +400,14 @@ __global__ void mx_pack_kernel(const uint8_t *__restrict__ src, int rows, int nb
 // 0, copies, and warp 1, MMA)
 template <int NT> __host__ __device__ constexpr int mxp_epi() { return NT >= 64 ? 2 : 1; }
 template <int NT> __host__ __device__ constexpr int mxp_threads() { return 64 + 128 * mxp_epi<NT>(); }
-constexpr int MXP_TPS = 2;   // K tiles per ring stage: halves what a stage costs the two issuing warps
-constexpr int MXP_WIDE = 96; // the widest chunk: two matrices' accumulators, twice, in 384 TMEM columns
+// K tiles per ring stage: two halve what a stage costs the two issuing warps; a
+// tile of the widest chunk keeps the tensor cores busy long enough by itself
+template <int NT> __host__ __device__ constexpr int mxp_tps() { return NT >= 192 ? 1 : 2; }
+// The widest chunks: 384 TMEM columns hold one matrix's accumulators, or gate's
+// and up's, twice. Shared memory bounds them (the MMAs' operand reads and the
+// copies' writes share its 128 bytes a cycle), so the product is fastest where
+// an operand byte meets the most others: 128 x 192, and 256 x 96 with the gate.
+constexpr int MXP_WIDE = 192, MXP_WIDE_GLU = 96;
 
 // Instruction descriptor of kind::mxf4: e2m1 A and B (K-major), UE8M0 scales,
 // M = 128, N; `half` picks the pair of scale bytes of the tile's K = 64 half.
@@ -482,8 +488,9 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t saddr, uint32_t rank) {
 // What the product needs first: its entries grouped into chunks (up to NT
 // entries of one expert), and per chunk the entries' quantised rows as the MMA
 // reads them -- an image: per K tile and plane, with N = the chunk's entries
-// rounded up to 16, 16-byte chunk c of entry j at c * 16 N + j * 16, then 512
-// bytes of scales (block c of entry j at (j % 32) * 16 + (j / 32) * 4 + c). A
+// rounded up to 16, 16-byte chunk c of entry j at c * 16 N + j * 16, then per 128
+// entries 512 bytes of scales (block c of entry j at j / 128 * 512 + (j % 32) * 16
+// + j % 128 / 32 * 4 + c). A
 // tile's planes are contiguous, so the product fetches them with one bulk
 // copy; a row that k experts picked is quantised once and written k times.
 // (Gathering rows inside the product, 16 bytes at a time by four warps, cost
@@ -498,7 +505,8 @@ constexpr int MXG_THREADS = 1024;   // at most
 constexpr int MXG_MAX_EXPERTS = 4096;
 
 __host__ __device__ constexpr int mx_round16(int n) { return (n + 15) / 16 * 16; }
-__host__ __device__ constexpr uint32_t mx_image_plane(int N) { return 64u * N + MX_SF; }          // bytes of one tile's plane
+// bytes of one tile's plane: codes, then 512 bytes of scales for every 128 entries begun
+__host__ __device__ constexpr uint32_t mx_image_plane(int N) { return 64u * N + (N > 128 ? 2u : 1u) * MX_SF; }
 __host__ __device__ constexpr uint64_t mx_image_bytes(int NT, int KT, int planes) {               // between chunks
     return static_cast<uint64_t>(KT) * planes * mx_image_plane(NT);
 }
@@ -725,7 +733,7 @@ __global__ void __launch_bounds__(256) mx_images_kernel(const MxPrep a) {
 #pragma unroll
         for (int pl = 0; pl < MX_MAX_PLANES; ++pl)
             if (pl < a.planes)
-                *reinterpret_cast<uint32_t *>(t + pl * mx_image_plane(N) + 64 * N + (j & 31) * 16 + (j >> 5) * 4) = sc[pl];
+                *reinterpret_cast<uint32_t *>(t + pl * mx_image_plane(N) + 64 * N + (j >> 7) * MX_SF + (j & 31) * 16 + ((j >> 5) & 3) * 4) = sc[pl];
     }
 }
 
@@ -746,7 +754,7 @@ struct MxCtl {
 
 template <int NT>
 __host__ __device__ constexpr uint32_t mx_stage_bytes(int mats, int planes) {
-    return MXP_TPS * (mats * MX_TILE + planes * mx_image_plane(NT));
+    return mxp_tps<NT>() * (mats * MX_TILE + planes * mx_image_plane(NT));
 }
 
 template <int NT>
@@ -799,15 +807,11 @@ __device__ __forceinline__ float mx_glu(float g, float up, float limit) {
 //             store, while the next item multiplies.
 // With split > 1 a cluster's CTAs have one item each; their partial sums meet in
 // shared memory and are added in rank order, so results do not depend on timing.
-// PAIR (the widest chunks, no GLU): an item is two row tiles of w, so that the
-// image is fetched once for both.
 template <int NT, bool GLU, bool DIRECT, int PLANES>
 __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxArgs a) {
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ MxCtl<NT> C;
-    constexpr bool PAIR = !GLU && NT == MXP_WIDE;
-    constexpr int MATS = GLU || PAIR ? 2 : 1, MXP_EPI = mxp_epi<NT>();
-    const int RI = PAIR ? (a.RT + 1) / 2 : a.RT;   // items of a chunk
+    constexpr int MATS = GLU ? 2 : 1, MXP_EPI = mxp_epi<NT>(), MXP_TPS = mxp_tps<NT>();
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int rank = a.split > 1 ? static_cast<int>(cluster_rank()) : 0;
@@ -815,7 +819,7 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
 
     if (DIRECT && warp == 0) {
         // (ids are complete before the launch that this one overlaps with; the images are not)
-        const int lead = item0 / RI;
+        const int lead = item0 / a.RT;
         const int x0 = mx_id(a.ids, a.ids_stride, a.n_entries, a.k, lane);
         const int x1 = mx_id(a.ids, a.ids_stride, a.n_entries, a.k, lane + 32);
         const int e = __shfl_sync(0xffffffffu, lead < 32 ? x0 : x1, lead & 31);
@@ -850,7 +854,7 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
         n_items = C.count > 0 ? item0 + 1 : 0;   // one item per CTA
     } else {
         asm volatile("griddepcontrol.wait;" ::: "memory");
-        n_items = *a.n_chunks * RI;
+        n_items = *a.n_chunks * a.RT;
     }
     if (item0 >= n_items) {   // nothing here; the same for every rank of the cluster
         if (DIRECT) asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -868,16 +872,11 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
     const int stages = a.stages, acc = a.acc;
     constexpr uint32_t stage_bytes = mx_stage_bytes<NT>(MATS, planes);
     const uint32_t ring0 = smem_u32(ring);
-    struct Item { int rt, chunk, expert, count, first, mats; };
+    struct Item { int rt, chunk, expert, count, first; };
     auto item_at = [&](int item) {
         Item I;
-        I.chunk = item / RI;
-        I.rt = item - I.chunk * RI;
-        I.mats = MATS;
-        if (PAIR) {
-            I.rt *= 2;
-            if (I.rt + 1 >= a.RT) I.mats = 1;
-        }
+        I.chunk = item / a.RT;
+        I.rt = item - I.chunk * a.RT;
         if (DIRECT) {
             I.expert = C.expert; I.count = C.count; I.first = 0;
         } else {
@@ -894,14 +893,12 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
     const uint32_t full0 = smem_u32(C.full);
     auto tiles_of = [&](int i) { return min(MXP_TPS, n_kt - i * MXP_TPS); };
     // stage: the weight tiles, the gate's, then the image's
-    auto fill_weights = [&](uint32_t on, uint64_t at, int mats, int i, uint32_t image_tile, uint64_t pol) {
+    auto fill_weights = [&](uint32_t on, uint64_t at, int i, uint32_t image_tile, uint64_t pol) {
         const uint32_t n = tiles_of(i), dst = ring0 + w_stage * stage_bytes, bar = full0 + 8 * w_stage;
         at += static_cast<uint64_t>(i) * (MXP_TPS * MX_TILE);
-        mbar_expect_if(on, bar, n * (mats * MX_TILE + image_tile));
+        mbar_expect_if(on, bar, n * (MATS * MX_TILE + image_tile));
         bulk_g2s_if(on, dst, a.w + at, n * MX_TILE, bar, pol);
-        if (MATS == 2 && mats == 2)
-            bulk_g2s_if(on, dst + MXP_TPS * MX_TILE, GLU ? a.gate + at : a.w + at + static_cast<uint64_t>(a.KT) * MX_TILE,
-                        n * MX_TILE, bar, pol);
+        if (GLU) bulk_g2s_if(on, dst + MXP_TPS * MX_TILE, a.gate + at, n * MX_TILE, bar, pol);
     };
     auto weights_at = [&](const Item &I) {
         return static_cast<uint64_t>(I.expert) * a.expert_bytes + (static_cast<uint64_t>(I.rt) * a.KT + kt0) * MX_TILE;
@@ -913,7 +910,7 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
         early = n_it < stages ? n_it : stages;
         const uint64_t pol = l2_evict_first_policy();
         for (w_stage = 0; static_cast<int>(w_stage) < early; ++w_stage)
-            fill_weights(on, weights_at(I), I.mats, w_stage, planes * mx_image_plane(mx_round16(I.count)), pol);
+            fill_weights(on, weights_at(I), w_stage, planes * mx_image_plane(mx_round16(I.count)), pol);
         w_stage = 0;
         __syncwarp();
     }
@@ -930,7 +927,6 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
             const Item I = item_at(item);
             const uint32_t tile = __shfl_sync(0xffffffffu, planes * mx_image_plane(mx_round16(I.count)), 0);
             const uint64_t wat = weights_at(I);
-            const int mats = __shfl_sync(0xffffffffu, I.mats, 0);
             const uint8_t *image = a.images + static_cast<uint64_t>(I.chunk) * mx_image_bytes(NT, a.KT, planes) +
                                    static_cast<uint64_t>(kt0) * tile;
             for (int i = 0; i < n_it; ++i) {
@@ -938,7 +934,7 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
                     ok = mx_wait_warp(C, &C.empty[w_stage], w_phase ^ 1u, a);
                     if (!ok) break;
                 }
-                if (i >= early) fill_weights(on, wat, mats, i, tile, pol_w);
+                if (i >= early) fill_weights(on, wat, i, tile, pol_w);
                 bulk_g2s_if(on, ring0 + w_stage * stage_bytes + MXP_TPS * MATS * MX_TILE, image, tiles_of(i) * tile,
                             full0 + 8 * w_stage, pol_x);
                 image += MXP_TPS * tile;
@@ -948,7 +944,7 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
         }
     } else if (warp == 1) {
         const uint32_t sf0 = tmem + static_cast<uint32_t>(acc * MATS * NT);   // scale columns, a slot per stage
-        constexpr uint32_t SFB = 4;                                             // columns of a plane's scales
+        constexpr uint32_t SFB = NT > 128 ? 8 : 4;                              // columns of a plane's scales
         constexpr uint32_t sf_tile = 4u * MATS + SFB * planes, sf_slot = MXP_TPS * sf_tile;
         const uint32_t empty0 = smem_u32(C.empty), acc0 = smem_u32(C.acc_full);
         uint32_t s = 0, ph = 0, n = 0;
@@ -959,7 +955,6 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
             const Item I = next;
             if (item + item_step < n_items) next = item_at(item + item_step);      // asked for one item ahead
             const int N = __shfl_sync(0xffffffffu, mx_round16(I.count), 0);
-            const int mats = __shfl_sync(0xffffffffu, I.mats, 0);
             if (n >= static_cast<uint32_t>(acc)) ok = mx_wait_warp(C, &C.acc_empty[ab], aph ^ 1u, a);
             const uint32_t id0 = mx_idesc(N, 0), id1 = mx_idesc(N, 1);
             const uint32_t d0 = tmem + ab * (MATS * NT);
@@ -985,10 +980,11 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
                     const uint32_t sft = sf + t * sf_tile, bt = t * planes * bp;
 #pragma unroll
                     for (int m = 0; m < MATS; ++m)
-                        if (m < mats) tmem_cp_scales(on, sft + 4 * m, asf + t * AT + m * AM);
+                        tmem_cp_scales(on, sft + 4 * m, asf + t * AT + m * AM);
 #pragma unroll
                     for (int p = 0; p < planes; ++p) {
                         tmem_cp_scales(on, sft + 4 * MATS + SFB * p, bsf + bt + p * bp);
+                        if (NT > 128 && N > 128) tmem_cp_scales(on, sft + 4 * MATS + SFB * p + 4, bsf + bt + p * bp + (MX_SF >> 4));
                     }
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
@@ -996,10 +992,9 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
                         for (int p = 0; p < planes; ++p)
 #pragma unroll
                             for (int m = 0; m < MATS; ++m)
-                                if (m < mats)
-                                    umma_mxf4(on, d0 + m * NT, al + t * AT + m * AM + h * AH, bl + bt + p * bp + h * bh,
-                                              h ? id1 : id0, sft + 4 * m, sft + 4 * MATS + SFB * p,
-                                              t + h + p > 0 || i > 0 ? 1u : 0u);
+                                umma_mxf4(on, d0 + m * NT, al + t * AT + m * AM + h * AH, bl + bt + p * bp + h * bh,
+                                          h ? id1 : id0, sft + 4 * m, sft + 4 * MATS + SFB * p,
+                                          t + h + p > 0 || i > 0 ? 1u : 0u);
                 }
                 umma_commit_if(on, free_bar);
             }
@@ -1027,11 +1022,10 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
             const Item I = next;
             if (item + item_step < n_items) next = item_at(item + item_step);
             const int row = I.rt * MX_M + r;
-            const bool row_ok = row < a.rows, row2_ok = PAIR && row + MX_M < a.rows;
+            const bool row_ok = row < a.rows;
             auto bias_of = [&](const float *b, int at) { return b[static_cast<int64_t>(I.expert) * a.rows + at]; };
             const float bu = a.bias && row_ok ? bias_of(a.bias, row) : 0.f;
-            const float bg = GLU ? (a.gate_bias && row_ok ? bias_of(a.gate_bias, row) : 0.f)
-                                 : (PAIR && a.bias && row2_ok ? bias_of(a.bias, row + MX_M) : 0.f);
+            const float bg = GLU && a.gate_bias && row_ok ? bias_of(a.gate_bias, row) : 0.f;
             float *out = a.dst + row;
             // lane j: entry of column j of each round, asked for before the wait
             int ens[ROUNDS];
@@ -1047,7 +1041,7 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
             auto load = [&](int q, uint32_t (&u)[16], uint32_t (&gt)[16]) {
                 if (column0(q) < I.count) {
                     tmem_ld16(cols + column0(q), u);
-                    if (GLU || (PAIR && I.mats == 2)) tmem_ld16(cols + NT + column0(q), gt);
+                    if (GLU) tmem_ld16(cols + NT + column0(q), gt);
                 }
             };
             auto release = [&]() {
@@ -1073,24 +1067,19 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
                     }
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        u[j] = __float_as_uint(__uint_as_float(u[j]) + bu);
-                        if (PAIR) gt[j] = __float_as_uint(__uint_as_float(gt[j]) + bg);
-                    }
+                    for (int j = 0; j < 16; ++j) u[j] = __float_as_uint(__uint_as_float(u[j]) + bu);
                 }
             };
-            auto store = [&](int q, const uint32_t (&u)[16], const uint32_t (&gt)[16]) {
+            auto store = [&](int q, const uint32_t (&u)[16]) {
                 // every address first: a shuffle between the stores would hold each store back
                 float *at[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
                     at[j] = out + static_cast<int64_t>(__shfl_sync(0xffffffffu, ens[q], j)) * a.rows;
-                const int left = I.count - column0(q), live = row_ok ? left : 0, live2 = row2_ok ? left : 0;
+                const int live = row_ok ? I.count - column0(q) : 0;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
+                for (int j = 0; j < 16; ++j)
                     if (j < live) *at[j] = __uint_as_float(u[j]);
-                    if (PAIR && j < live2) at[j][MX_M] = __uint_as_float(gt[j]);
-                }
             };
             if (a.split > 1) {   // this rank's partial sums, for the cluster
                 float *part = reinterpret_cast<float *>(ring);
@@ -1115,7 +1104,7 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
                 for (int q = 0; q < ROUNDS; ++q)
                     if (column0(q) < I.count) {
                         finish(us[q], gs[MATS == 2 ? q : 0]);
-                        store(q, us[q], gs[MATS == 2 ? q : 0]);
+                        store(q, us[q]);
                     }
             }
         }
@@ -1206,12 +1195,10 @@ constexpr uint32_t kSmemMax = 227u * 1024u;
 
 template <int NT, bool GLU, bool DIRECT, int PLANES>
 cudaError_t product_p(MxArgs &a, int64_t units, cudaStream_t st) {
-    constexpr bool PAIR = !GLU && NT == MXP_WIDE;
-    constexpr int MATS = GLU || PAIR ? 2 : 1;
-    const int RI = PAIR ? (a.RT + 1) / 2 : a.RT;
+    constexpr int MATS = GLU ? 2 : 1, MXP_TPS = mxp_tps<NT>();
     auto kern = mx_product_kernel<NT, GLU, DIRECT, PLANES>;
     constexpr uint32_t fixed = (sizeof(MxCtl<NT>) + 127u) / 128u * 128u + 1024u;   // static part and the system's 1 KB
-    const uint32_t sb = mx_stage_bytes<NT>(MATS, PLANES), sf = MXP_TPS * 4u * (MATS + PLANES);
+    const uint32_t sb = mx_stage_bytes<NT>(MATS, PLANES), sf = MXP_TPS * (4u * MATS + (NT > 128 ? 8u : 4u) * PLANES);
     const bool single = DIRECT || a.split > 1;       // one item per CTA
     a.acc = single ? 1 : 2;
     const int tiles = (a.KT + a.split - 1) / a.split;
@@ -1244,7 +1231,7 @@ cudaError_t product_p(MxArgs &a, int64_t units, cudaStream_t st) {
         configured[dev] = n_sm;
     }
     n_sm = configured[dev];
-    int64_t grid = units * RI * a.split;
+    int64_t grid = units * a.RT * a.split;
     if (!single) grid = std::min<int64_t>(grid, static_cast<int64_t>(n_sm) * per_sm);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(grid));
@@ -1302,11 +1289,11 @@ cudaError_t launch_mx_pack(const uint8_t *src, int64_t E, int64_t rows, int64_t 
 
 // Entries per chunk: 64 at most in the direct form; else by the entries an
 // expert has on average.
-int mx_chunk_tokens(int64_t n_tok, int64_t k, int64_t n_experts) {
+int mx_chunk_tokens(int64_t n_tok, int64_t k, int64_t n_experts, bool glu) {
     const int64_t n = n_tok * k;
     if (n <= MX_DIRECT) return n_tok <= 16 ? 16 : 64;
     const int64_t per = n / (n < n_experts ? n : n_experts);
-    return per <= 12 ? 16 : per <= 48 ? 64 : MXP_WIDE;
+    return per <= 12 ? 16 : per <= 48 ? 64 : glu ? MXP_WIDE_GLU : MXP_WIDE;
 }
 
 bool mx_direct(int64_t n_tok, int64_t k) { return n_tok * k <= MX_DIRECT; }
@@ -1376,7 +1363,7 @@ cudaError_t launch_mx_product(MxArgs &a, int NT, int64_t units, cudaStream_t st)
         if (glu) return direct ? product_t<64, true, true>(a, units, st) : product_t<64, true, false>(a, units, st);
         return direct ? product_t<64, false, true>(a, units, st) : product_t<64, false, false>(a, units, st);
     }
-    return glu ? product_t<MXP_WIDE, true, false>(a, units, st) : product_t<MXP_WIDE, false, false>(a, units, st);
+    return glu ? product_t<MXP_WIDE_GLU, true, false>(a, units, st) : product_t<MXP_WIDE, false, false>(a, units, st);
 }
 
 }  // namespace moe
