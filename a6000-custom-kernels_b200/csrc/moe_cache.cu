@@ -2054,8 +2054,9 @@ int mx_shape_check(int64_t E, int64_t rows, int64_t K) {
 
 struct MxWs {
     uint8_t *images;
-    int32_t *entries, *n_chunks, *where;
-    int4 *chunks;
+    int32_t *entries, *n_chunks;
+    int2 *where;
+    int4 *experts, *chunks;
     int64_t max_chunks;
     size_t bytes;
 };
@@ -2076,7 +2077,8 @@ MxWs mx_ws(int64_t E, int64_t K, int64_t n_tok, int64_t k, int planes, char *bas
     w.images = reinterpret_cast<uint8_t *>(take(images));
     if (!direct) {
         w.entries = reinterpret_cast<int32_t *>(take(4 * static_cast<size_t>(n_tok * k)));
-        w.where = reinterpret_cast<int32_t *>(take(4 * static_cast<size_t>(n_tok * k)));
+        w.where = reinterpret_cast<int2 *>(take(8 * static_cast<size_t>(n_tok * k)));
+        w.experts = reinterpret_cast<int4 *>(take(16 * static_cast<size_t>(E)));
         w.chunks = reinterpret_cast<int4 *>(take(16 * static_cast<size_t>(w.max_chunks)));
         w.n_chunks = reinterpret_cast<int32_t *>(take(4));
     }
@@ -2230,6 +2232,7 @@ int moe_b200_mxfp4_mul_mat_id(const moe_mxfp4 *w, const moe_mxfp4 *gate, const f
     a.glu_limit = glu_limit;
     a.images = s.images;
     a.where = s.where;
+    a.experts = s.experts;
     a.planes = planes;
     a.k = static_cast<int32_t>(k);
     a.n_entries = static_cast<int32_t>(n_tok * k);

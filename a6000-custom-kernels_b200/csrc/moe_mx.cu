@@ -67,18 +67,23 @@ template <> struct MxPair<MX_BF16> {
     using T = __nv_bfloat162;
     static __device__ __forceinline__ T abs(uint32_t w) { w &= 0x7FFF7FFFu; return *reinterpret_cast<T *>(&w); }
 };
-// the values, and the largest magnitude's f32 bits (magnitudes compare as integers, a NaN above
-// infinity above every number)
+// the largest magnitude's f32 bits, a NaN's where there is one
+__device__ __forceinline__ float mx_max_nan(float a, float b) {
+    float c;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return c;
+}
+__device__ __forceinline__ uint32_t mx_top(const float (&v)[8]) {
+    const float a = mx_max_nan(v[0], v[1]), b = mx_max_nan(v[2], v[3]), c = mx_max_nan(v[4], v[5]), d = mx_max_nan(v[6], v[7]);
+    return __float_as_uint(mx_max_nan(mx_max_nan(a, b), mx_max_nan(c, d)));
+}
+// the values, and their largest magnitude's bits
 template <int XT>
 __device__ __forceinline__ uint32_t mx_floats(const MxRaw<XT> &r, float (&v)[8]) {
     if constexpr (XT == MX_F32) {
-        uint32_t top = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[j] = __uint_as_float(r.w[j]);
-            top = max(top, r.w[j] & 0x7FFFFFFFu);
-        }
-        return top;
+        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r.w[j]);
+        return mx_top(v);
     } else {
         // two at a time; the .NaN maximum keeps a NaN
         typename MxPair<XT>::T two = MxPair<XT>::abs(r.w[0]);
@@ -99,13 +104,6 @@ __device__ __forceinline__ uint32_t mx_floats(const MxRaw<XT> &r, float (&v)[8])
         else return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(one)))) & 0x7FFFFFFFu;
     }
 }
-__device__ __forceinline__ uint32_t mx_top(const float (&v)[8]) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-    return top;
-}
-
 // byte j: the code of a[j] in its low nibble, of b[j] in its high one (scaled by inv first)
 __device__ __forceinline__ uint32_t mx_codes(const float (&a)[4], const float (&b)[4], float inv) {
     uint32_t w;
@@ -519,27 +517,36 @@ struct MxPrep {
     const int32_t *ids;
     int64_t ids_stride;
     int32_t n_entries, k, n_experts, NT;
-    int32_t *entries, *n_chunks, *where;   // chunked form: mx_where of each entry, -1: left out
-    int4 *chunks;
+    // chunked form: of each entry its expert (-1: left out) and its number among the expert's entries; of
+    // each expert {first chunk, entries, first entry, -}
+    int32_t *entries, *n_chunks;
+    int2 *where;
+    int4 *experts, *chunks;
     int *err;
 };
 
-// an entry's chunk, its place there and the chunk's N, in one word (chunks < 2^19, N <= 256)
+// direct form: an entry's chunk, its place there and the chunk's N, in one word
 __device__ __forceinline__ int mx_where(int chunk, int place, int N) { return (chunk << 12) | ((N / 16 - 1) << 8) | place; }
+
+__host__ __device__ constexpr int mx_group_sets(int E) { return E <= 512 ? 8 : 1; }
 
 // Grouping by one cluster of MXG_CTAS: each CTA counts its share of the entries
 // per expert in shared memory, reads the other CTAs' counts, and places its
 // entries behind theirs. Chunks of an expert are consecutive. Order inside an
-// expert changes no result. Id -1: left out.
+// expert changes no result. Id -1: left out. What an entry's number means -- its
+// chunk, its place in the image -- is worked out by the kernel behind this one,
+// on every SM: done here, on 8 of them, it took twice as long.
 __global__ void __cluster_dims__(MXG_CTAS, 1, 1) __launch_bounds__(MXG_THREADS) mx_group_kernel(const MxPrep a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ int group_smem[];
     __shared__ int scratch[64];
-    int *cnt = group_smem, *cur = cnt + a.n_experts, *ch0 = cur + a.n_experts, *ex0 = ch0 + a.n_experts,
-        *tot = ex0 + a.n_experts;
+    // counts of several sets of warps: a popular expert's counter, one for all, took 20 cycles an entry
+    const int sets = mx_group_sets(a.n_experts);
+    int *sum = group_smem, *cur = sum + a.n_experts, *kept = cur + a.n_experts, *cnt = kept + a.n_experts;   // cnt: [sets][n_experts]
     const int tid = threadIdx.x, nth = blockDim.x, lane = tid & 31, warp = tid >> 5;
     const int rank = blockIdx.x, E = a.n_experts, N = a.n_entries;
-    for (int e = tid; e < E; e += nth) cnt[e] = 0;
+    int *const mine = cnt + warp % sets * E;
+    for (int e = tid; e < sets * E; e += nth) cnt[e] = 0;
     __syncthreads();
     auto id_of = [&](int i) {
         if (i >= N) return -1;
@@ -560,15 +567,30 @@ __global__ void __cluster_dims__(MXG_CTAS, 1, 1) __launch_bounds__(MXG_THREADS) 
         }
         return x >= 0 ? atomicAdd(&c[x], 1) : 0;
     };
-    constexpr int KEEP = 4;   // ids kept in registers
-    int x[KEEP];
+    constexpr int KEEP = 4;   // ids kept in registers, and their places among the CTA's
+    int x[KEEP], at_cta[KEEP];
 #pragma unroll
     for (int m = 0; m < KEEP; ++m) x[m] = id_of((m * MXG_CTAS + rank) * nth + tid);
 #pragma unroll
-    for (int m = 0; m < KEEP; ++m)
-        if ((m * MXG_CTAS + rank) * nth < N) add(cnt, x[m]);
-    for (int64_t i0 = static_cast<int64_t>(KEEP * MXG_CTAS + rank) * nth; i0 < N; i0 += MXG_CTAS * nth)
-        add(cnt, id_of(static_cast<int>(i0) + tid));
+    for (int m = 0; m < KEEP; ++m) {
+        at_cta[m] = 0;
+        if ((m * MXG_CTAS + rank) * nth < N) at_cta[m] = add(mine, x[m]);
+    }
+    __syncthreads();
+    for (int e = tid; e < E; e += nth) {   // each set's first place
+        int run = 0;
+        for (int c = 0; c < sets; ++c) {
+            const int n = cnt[c * E + e];
+            cnt[c * E + e] = run;
+            run += n;
+        }
+        sum[e] = kept[e] = run;
+    }
+    __syncthreads();
+    const bool more = static_cast<int64_t>(KEEP * MXG_CTAS) * nth < N;   // entries past the registers: counted here, placed below
+    if (more)
+        for (int64_t i0 = static_cast<int64_t>(KEEP * MXG_CTAS + rank) * nth; i0 < N; i0 += MXG_CTAS * nth)
+            add(sum, id_of(static_cast<int>(i0) + tid));
     __syncthreads();
     cluster_sync();
     int carry_e = 0, carry_c = 0;
@@ -578,7 +600,7 @@ __global__ void __cluster_dims__(MXG_CTAS, 1, 1) __launch_bounds__(MXG_THREADS) 
         if (e < E)
 #pragma unroll
             for (int c = 0; c < MXG_CTAS; ++c) {
-                const int v = __float_as_int(ld_cluster_f32(smem_u32(&cnt[e]), c));
+                const int v = __float_as_int(ld_cluster_f32(smem_u32(&sum[e]), c));
                 if (c < rank) before += v;
                 total += v;
             }
@@ -605,33 +627,28 @@ __global__ void __cluster_dims__(MXG_CTAS, 1, 1) __launch_bounds__(MXG_THREADS) 
         __syncthreads();
         if (e < E) {
             const int first = pe + se - total, c0 = pc + sc - nc;
-            ex0[e] = first;
-            tot[e] = total;
-            ch0[e] = c0;
-            cur[e] = first + before;
+            cur[e] = before;
+            if (rank == 0) a.experts[e] = make_int4(c0, total, first, 0);
             for (int q = rank; q < nc; q += MXG_CTAS)
                 a.chunks[c0 + q] = make_int4(e, first + q * a.NT, min(a.NT, total - q * a.NT), 0);
         }
     }
     if (rank == 0 && tid == 0) *a.n_chunks = carry_c;
     __syncthreads();
-    auto place = [&](int i, int xi) {
-        const int at = add(cur, xi);
-        if (xi >= 0) {
-            a.entries[at] = i;
-            const int pos = at - ex0[xi], q = pos / a.NT;
-            a.where[i] = mx_where(ch0[xi] + q, pos - q * a.NT, mx_round16(min(a.NT, tot[xi] - q * a.NT)));
-        } else if (i < N) {
-            a.where[i] = -1;
-        }
-    };
 #pragma unroll
     for (int m = 0; m < KEEP; ++m) {
-        const int i0 = (m * MXG_CTAS + rank) * nth;
-        if (i0 < N) place(i0 + tid, x[m]);
+        const int i = (m * MXG_CTAS + rank) * nth + tid;
+        if (i < N) a.where[i] = make_int2(x[m], x[m] >= 0 ? cur[x[m]] + mine[x[m]] + at_cta[m] : 0);
     }
-    for (int64_t i0 = static_cast<int64_t>(KEEP * MXG_CTAS + rank) * nth; i0 < N; i0 += MXG_CTAS * nth)
-        place(static_cast<int>(i0) + tid, id_of(static_cast<int>(i0) + tid));
+    if (more) {
+        __syncthreads();
+        for (int e = tid; e < E; e += nth) cur[e] += kept[e];
+        __syncthreads();
+        for (int64_t i0 = static_cast<int64_t>(KEEP * MXG_CTAS + rank) * nth; i0 < N; i0 += MXG_CTAS * nth) {
+            const int i = static_cast<int>(i0) + tid, xi = id_of(i), at = add(cur, xi);
+            if (i < N) a.where[i] = make_int2(xi, at);
+        }
+    }
     cluster_sync();   // the counts stay until every CTA has read them
 }
 
@@ -646,9 +663,11 @@ __device__ __forceinline__ int mx_id(const int32_t *ids, int64_t stride, int n_e
     return i < n_entries ? ids[(i / k) * stride + i % k] : -2;
 }
 
-// Quantise x and write the images: 4 lanes per block, 16 per K tile of a row.
-template <int XT, bool VEC, bool DIRECT>
-__global__ void __launch_bounds__(256) mx_images_kernel(const MxPrep a) {
+// Quantise x and write the images: 4 lanes per block, 16 per K tile of a row, RUN
+// tiles in turn: what finds a row's places serves them all, and their loads are
+// in flight together.
+template <int XT, bool VEC, bool DIRECT, int RUN>
+__global__ void __launch_bounds__(256, 4) mx_images_kernel(const MxPrep a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __shared__ int where_s[MX_DIRECT];
     __shared__ __align__(16) int id_s[MX_DIRECT];
@@ -676,64 +695,104 @@ __global__ void __launch_bounds__(256) mx_images_kernel(const MxPrep a) {
         }
         __syncthreads();
     }
-    const int64_t g = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 2;   // (row, block), K padded
-    const int i = threadIdx.x & 3;
-    const int64_t row = mx_row_of(g, a.KT * 4, a.n_rows * a.KT < (int64_t{1} << 28));
-    const int b = static_cast<int>(g - row * (a.KT * 4)), tile = b >> 2;
+    const int64_t g = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 4;   // (row, run of RUN tiles)
+    const int i = threadIdx.x & 3, b = (threadIdx.x >> 2) & 3;                           // block b of a tile
+    const int runs = (a.KT + RUN - 1) / RUN;
+    const int64_t row = mx_row_of(g, runs, a.n_rows * runs < (int64_t{1} << 31));
+    const int t0 = static_cast<int>(g - row * runs) * RUN;
     const bool row_ok = row < a.n_rows;
-    MxRaw<XT> raw = mx_zero<XT>();
-    if (row_ok && b < a.nb)
-        raw = mx_load<XT, VEC>(static_cast<const typename MxElem<XT>::T *>(a.x) + row * a.stride + static_cast<int64_t>(b) * 32, i);
-    float v[8];
-    uint32_t top = mx_floats<XT>(raw, v);
-    uint32_t w[MX_MAX_PLANES][4], sc[MX_MAX_PLANES];
+    const typename MxElem<XT>::T *x = static_cast<const typename MxElem<XT>::T *>(a.x) + row * a.stride + (t0 * 4 + b) * 32;
+    MxRaw<XT> raw[RUN];
 #pragma unroll
-    for (int pl = 0; pl < MX_MAX_PLANES; ++pl) {
-        if (pl >= a.planes) break;
-        uint32_t byte;
-        const uint32_t mine = mx_quant_block(v, top, byte);
-        if (pl + 1 < a.planes) {
-            mx_residual(v, mine, byte);
-            top = mx_top(v);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[pl][j] = __shfl_sync(0xffffffffu, mine, (lane & ~3) + j);   // the block's 16 bytes
-        uint32_t word = byte << (8 * ((lane >> 2) & 3));                                          // the tile's 4 scales
-        word |= __shfl_xor_sync(0xffffffffu, word, 4);
-        word |= __shfl_xor_sync(0xffffffffu, word, 8);
-        sc[pl] = word;
+    for (int u = 0; u < RUN; ++u) {   // K padded to whole tiles with zeros
+        raw[u] = mx_zero<XT>();
+        if (row_ok && (t0 + u) * 4 + b < a.nb) raw[u] = mx_load<XT, VEC>(x + 128 * u, i);
     }
     if (!DIRECT) asm volatile("griddepcontrol.wait;" ::: "memory");   // the grouping
-    if (!row_ok) return;
-    const int n_dst = a.per_pick ? 1 : a.k;
-    const int64_t en0 = row * n_dst;
-    const uint64_t image = mx_image_bytes(a.NT, a.KT, a.planes);
-    // lane i of the 4 serves destinations i, i + 4, ..., lane l of the tile's 16 the scales of l, l + 16, ...
-    auto plane_at = [&](int64_t en, int &j, int &N) -> uint8_t * {
-        const int at = DIRECT ? where_s[en] : a.where[en];
-        if (at < 0) return nullptr;
-        j = at & 255;
-        N = (((at >> 8) & 15) + 1) * 16;
-        return a.images + static_cast<uint64_t>(at >> 12) * image + static_cast<uint64_t>(tile) * a.planes * mx_image_plane(N);
+    // The row's destinations: lane i of the 4 serves number i, i + 4, ... Two of them are looked up
+    // here, while x is on its way: behind the arithmetic the look-ups were most of the kernel's time.
+    const int n_dst = row_ok ? (a.per_pick ? 1 : a.k) : 0;
+    const int64_t en0 = row * (a.per_pick ? 1 : a.k);
+    struct Place { int chunk, j, N; };
+    auto place_of = [&](int64_t en) {
+        Place d;
+        if (DIRECT) {
+            const int at = where_s[en];
+            d.chunk = at < 0 ? -1 : at >> 12;
+            d.j = at & 255;
+            d.N = (((at >> 8) & 15) + 1) * 16;
+        } else {
+            const int2 w = a.where[en];
+            const int4 ex = a.experts[max(w.x, 0)];
+            const int c = w.y / a.NT;
+            d.chunk = w.x < 0 ? -1 : ex.x + c;
+            d.j = w.y - c * a.NT;
+            d.N = mx_round16(min(a.NT, ex.y - c * a.NT));
+            if (t0 == 0 && b == 0 && w.x >= 0) a.entries[ex.z + w.y] = static_cast<int32_t>(en);
+        }
+        return d;
     };
-    for (int q = i; q < n_dst; q += 4) {
-        int j, N;
-        uint8_t *t = plane_at(en0 + q, j, N);
-        if (!t) continue;
+    const uint64_t image = mx_image_bytes(a.NT, a.KT, a.planes);
+    // where tile t0 of a destination's image keeps this block's codes and the tile's scales, and the step to the next tile
+    struct Spot { uint8_t *codes; uint32_t scales, plane; };
+    auto spot_of = [&](const Place &d) {
+        Spot o;
+        o.plane = mx_image_plane(d.N);
+        uint8_t *t = a.images + static_cast<uint64_t>(d.chunk) * image + static_cast<uint64_t>(t0 * a.planes) * o.plane;
+        o.codes = d.chunk < 0 ? nullptr : t + b * 16 * d.N + d.j * 16;
+        o.scales = 64 * d.N + (d.j >> 7) * MX_SF + (d.j & 31) * 16 + ((d.j >> 5) & 3) * 4 - (b * 16 * d.N + d.j * 16);
+        return o;
+    };
+    constexpr int AHEAD = 2;
+    Spot ahead[AHEAD];
 #pragma unroll
-        for (int pl = 0; pl < MX_MAX_PLANES; ++pl)
-            if (pl < a.planes)
-                *reinterpret_cast<uint4 *>(t + pl * mx_image_plane(N) + (b & 3) * 16 * N + j * 16) =
-                    make_uint4(w[pl][0], w[pl][1], w[pl][2], w[pl][3]);
+    for (int p = 0; p < AHEAD; ++p) {
+        ahead[p].codes = nullptr;
+        ahead[p].plane = ahead[p].scales = 0;
+        if (i + 4 * p < n_dst) ahead[p] = spot_of(place_of(en0 + i + 4 * p));
     }
-    for (int q = lane & 15; q < n_dst; q += 16) {
-        int j, N;
-        uint8_t *t = plane_at(en0 + q, j, N);
-        if (!t) continue;
+
 #pragma unroll
-        for (int pl = 0; pl < MX_MAX_PLANES; ++pl)
-            if (pl < a.planes)
-                *reinterpret_cast<uint32_t *>(t + pl * mx_image_plane(N) + 64 * N + (j >> 7) * MX_SF + (j & 31) * 16 + ((j >> 5) & 3) * 4) = sc[pl];
+    for (int u = 0; u < RUN; ++u) {
+        if (t0 + u >= a.KT) break;
+        float v[8];
+        uint32_t top = mx_floats<XT>(raw[u], v);
+        uint32_t w[MX_MAX_PLANES][4], sc[MX_MAX_PLANES];
+#pragma unroll
+        for (int pl = 0; pl < MX_MAX_PLANES; ++pl) {
+            if (pl >= a.planes) break;
+            uint32_t byte;
+            const uint32_t mine = mx_quant_block(v, top, byte);
+            if (pl + 1 < a.planes) {
+                mx_residual(v, mine, byte);
+                top = mx_top(v);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[pl][j] = __shfl_sync(0xffffffffu, mine, (lane & ~3) + j);   // the block's 16 bytes
+            uint32_t word = byte << (8 * b);                                                          // the tile's 4 scales
+            word |= __shfl_xor_sync(0xffffffffu, word, 4);
+            word |= __shfl_xor_sync(0xffffffffu, word, 8);
+            sc[pl] = word;
+        }
+        auto put = [&](uint8_t *codes, const Spot &o) {
+#pragma unroll
+            for (int pl = 0; pl < MX_MAX_PLANES; ++pl)
+                if (pl < a.planes) {
+                    uint8_t *c = codes + pl * o.plane;
+                    *reinterpret_cast<uint4 *>(c) = make_uint4(w[pl][0], w[pl][1], w[pl][2], w[pl][3]);
+                    if (b == 0) *reinterpret_cast<uint32_t *>(c + static_cast<int32_t>(o.scales)) = sc[pl];
+                }
+        };
+#pragma unroll
+        for (int p = 0; p < AHEAD; ++p)
+            if (ahead[p].codes) {
+                put(ahead[p].codes, ahead[p]);
+                ahead[p].codes += a.planes * ahead[p].plane;
+            }
+        for (int q = i + 4 * AHEAD; q < n_dst; q += 4) {
+            const Spot o = spot_of(place_of(en0 + q));
+            if (o.codes) put(o.codes + static_cast<uint64_t>(u * a.planes) * o.plane, o);
+        }
     }
 }
 
@@ -1079,7 +1138,7 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
                 const int live = row_ok ? I.count - column0(q) : 0;
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
-                    if (j < live) *at[j] = __uint_as_float(u[j]);
+                    if (j < live) __stcs(at[j], __uint_as_float(u[j]));   // the weights keep the L2
             };
             if (a.split > 1) {   // this rank's partial sums, for the cluster
                 float *part = reinterpret_cast<float *>(ring);
@@ -1171,10 +1230,10 @@ void dequantize_t(const uint8_t *y, int64_t n_blocks, int nb, int planes, void *
         mx_dequantize_kernel<OT, false><<<grid, MXQ_THREADS, 0, st>>>(y, n_blocks, nb, planes, stride, static_cast<T *>(out));
 }
 
-template <int XT, bool VEC, bool DIRECT>
-cudaError_t images_t(const MxPrep &a, cudaStream_t st) {
+template <int XT, bool VEC, bool DIRECT, int RUN>
+cudaError_t images_run(const MxPrep &a, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>((a.n_rows * a.KT * 16 + 255) / 256));
+    cfg.gridDim = dim3(static_cast<unsigned>((a.n_rows * ((a.KT + RUN - 1) / RUN) * 16 + 255) / 256));
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
@@ -1182,7 +1241,14 @@ cudaError_t images_t(const MxPrep &a, cudaStream_t st) {
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = DIRECT ? 0 : 1;
-    return cudaLaunchKernelEx(&cfg, mx_images_kernel<XT, VEC, DIRECT>, a);
+    return cudaLaunchKernelEx(&cfg, mx_images_kernel<XT, VEC, DIRECT, RUN>, a);
+}
+
+template <int XT, bool VEC, bool DIRECT>
+cudaError_t images_t(const MxPrep &a, cudaStream_t st) {
+    // a small call spreads over the SMs (the direct form is one always)
+    if constexpr (DIRECT) return images_run<XT, VEC, true, 1>(a, st);
+    else return a.n_rows * a.KT < 16384 ? images_run<XT, VEC, false, 1>(a, st) : images_run<XT, VEC, false, 2>(a, st);
 }
 
 template <int XT>
@@ -1327,14 +1393,15 @@ cudaError_t launch_mx_prep(const void *x, int xt, int64_t stride, int64_t n_rows
         p.n_chunks = const_cast<int32_t *>(a.n_chunks);
         p.chunks = const_cast<int4 *>(a.chunks);
         p.where = a.where;
-        const size_t smem = 5 * static_cast<size_t>(a.n_experts) * sizeof(int);   // 80 KB at most
+        p.experts = a.experts;
+        const size_t smem = (3 + static_cast<size_t>(mx_group_sets(a.n_experts))) * a.n_experts * sizeof(int);   // 64 KB at most
         static bool configured[64] = {};
         int dev = 0;
         cudaGetDevice(&dev);
         if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
         if (!configured[dev]) {
             const cudaError_t e = cudaFuncSetAttribute(mx_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                       5 * MXG_MAX_EXPERTS * static_cast<int>(sizeof(int)));
+                                                       4 * MXG_MAX_EXPERTS * static_cast<int>(sizeof(int)));
             if (e != cudaSuccess) return e;
             configured[dev] = true;
         }

@@ -41,7 +41,8 @@ struct MxArgs {
     const int32_t *ids;              // direct form: [tok * ids_stride + pick]
     int64_t ids_stride;
     const int32_t *entries;          // chunked form: entries grouped by expert,
-    int32_t *where;                  // each entry's place (moe_mx.cu), -1: left out;
+    int2 *where;                     // scratch of the grouping: per entry,
+    int4 *experts;                   // and per expert;
     const int4 *chunks;              // {expert, first entry, count, -},
     const int32_t *n_chunks;         // and their number on the device
     float *dst;                      // [entry][rows]
