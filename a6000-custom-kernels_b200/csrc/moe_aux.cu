@@ -183,10 +183,15 @@ cudaError_t launch_combine_local(const float *y, const float *w, const float *ys
 
 cudaError_t launch_combine(const float *y, const float *w, const float *ys, float *out, int64_t n_tok, int64_t H,
                            int64_t k, cudaStream_t st) {
-    if (n_tok == 0) return cudaSuccess;
-    dim3 grid(static_cast<unsigned>((H + 255) / 256), static_cast<unsigned>(n_tok));
-    combine_kernel<<<grid, 256, 0, st>>>(y, w, ys, out, static_cast<int>(H), static_cast<int>(k));
-    return cudaGetLastError();
+    constexpr int64_t most = 65535;   // tokens of a launch
+    for (int64_t t = 0; t < n_tok; t += most) {
+        dim3 grid(static_cast<unsigned>((H + 255) / 256), static_cast<unsigned>(n_tok - t < most ? n_tok - t : most));
+        combine_kernel<<<grid, 256, 0, st>>>(y + t * k * H, w + t * k, ys ? ys + t * H : nullptr, out + t * H,
+                                             static_cast<int>(H), static_cast<int>(k));
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 // ---------------------------------------------------------------------------

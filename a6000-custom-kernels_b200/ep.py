@@ -23,6 +23,7 @@ import ctypes
 
 import torch
 
+from ._call import bad
 from ._lib import MoeLayerDesc, check, lib
 from .moe_cache import _ptr, _stream, expert_tensor, topk_softmax
 
@@ -36,9 +37,12 @@ class EPMoELayer:
     """This rank's share of one MoE layer. Built from a full MoELayer (same
     weights as the single-GPU layer) by slicing its expert tensors (the full
     tensors are not kept), or with local=True from a MoELayer that already
-    holds only this rank's experts [lo, hi) of n_experts."""
+    holds only this rank's experts [lo, hi) of n_experts. Layers with a router of
+    their own, MXFP4 ones among them, are refused."""
 
     def __init__(self, full, rank, world, group=None, local=False, n_experts=None):
+        if getattr(full, "router", None) is not None:
+            raise bad("expert parallelism routes by softmax, top-k: it takes no layer with a router of its own")
         self.H, self.F, self.k = full.H, full.F, full.k
         self.E = n_experts if local else full.E
         self.rank, self.world, self.group = rank, world, group

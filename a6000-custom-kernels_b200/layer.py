@@ -26,7 +26,7 @@ class MoELayer:
     decode and prefill alike; None is softmax over all experts, top-k.
     MoELayer(..., types with MXFP4 for gate, up and down) makes an MXFP4Layer."""
 
-    def __new__(cls, H=None, F=None, n_experts=None, k=None, types=None, **kw):
+    def __new__(cls, H=None, F=None, n_experts=None, k=None, types=None, *args, **kw):
         if cls is MoELayer and types is not None and MXFP4 in dict(types).values():
             return super().__new__(MXFP4Layer)
         return super().__new__(cls)
@@ -138,15 +138,15 @@ class MoELayer:
     def _routed(self, x, logits, out, stream, trace=None):
         """The layer with its own router: route, the experts of the picks, the
         shared expert, combine (any n_tok >= 1; x contiguous f32)."""
-        n_tok, dev = x.shape[0], self.device
-        if x.dtype != torch.float32 or not x.is_contiguous() or tuple(x.shape) != (n_tok, self.H) or n_tok < 1 or \
-                tuple(logits.shape) != (n_tok, self.E):
-            raise bad("x must be contiguous f32 [n_tok, H] with n_tok >= 1, logits [n_tok, n_experts]")
-        ctx, st = on(x.device, stream)
+        n_tok, dev = x.shape[0], x.device
+        if x.dtype != torch.float32 or not x.is_cuda or not x.is_contiguous() or tuple(x.shape) != (n_tok, self.H) or \
+                n_tok < 1 or tuple(logits.shape) != (n_tok, self.E) or logits.device != dev:
+            raise bad("x must be contiguous f32 [n_tok, H] with n_tok >= 1, logits [n_tok, n_experts] on its device")
+        ctx, st = on(dev, stream)
         with ctx:
+            out = torch.empty((n_tok, self.H), dtype=torch.float32, device=dev) if out is None else \
+                given(out, "out", torch.float32, (n_tok, self.H), dev)
             ids, w = self.router(logits)
-            if out is None:
-                out = torch.empty((n_tok, self.H), dtype=torch.float32, device=dev)
             kept = self._ws.get(("routed", n_tok))
             if kept is None:
                 nbytes = lib().moe_b200_experts_prefill_workspace_size(ctypes.byref(self.desc), n_tok, self.k)
@@ -160,9 +160,10 @@ class MoELayer:
             if ys is not None:
                 check(lib().moe_b200_shared_prefill(ctypes.byref(self.desc), _ptr(x), n_tok, _ptr(ys), _ptr(ws), ws.numel(), st))
             check(lib().moe_b200_combine(_ptr(y), _ptr(w), _ptr(ys), _ptr(out), n_tok, self.H, self.k, st))
+            picks = None if trace is None else ids.cpu().numpy()   # (waits for the stream that wrote them)
         if trace is not None:
             for r in ("gate", "up", "down"):
-                trace.record(self.desc_t[r].name.decode(), ids.cpu().numpy(), self.E)
+                trace.record(self.desc_t[r].name.decode(), picks, self.E)
         return out
 
     def prefill_intermediates(self, n_tok):
@@ -226,12 +227,12 @@ class MXFP4Layer(MoELayer):
         device = torch.device(device)
         if device.index is None:
             device = torch.device(device.type, torch.cuda.current_device())
-        self.H, self.F, self.E, self.k, self.device = H, F, n_experts, k, device
+        self.H, self.F, self.E, self.k, self.device, self.name = H, F, n_experts, k, device, name
         self.glu_op, self.glu_limit, self.norm_w, self.planes = glu_op, glu_limit, norm_w, planes
         self.router = Router(k, norm_w=norm_w) if router is None else router
         if self.router.k != k:
             raise bad("the router picks another number of experts than the layer has")
-        rb = self.router.bias
+        rb = self._router_bias = self.router.bias   # (kept: the descriptor points at it)
         if rb is not None and (rb.device != device or rb.shape[0] != n_experts):
             raise bad("the router's bias must be f32 [n_experts] on the layer's device")
         shapes = {"gate": (F, H), "up": (F, H), "down": (H, F)}
@@ -295,10 +296,10 @@ class MXFP4Layer(MoELayer):
                 ws = self.workspace(n_tok)
                 check(lib().moe_b200_mxfp4_layer_run(self.ref, x.data_ptr(), ELEM[x.dtype], xs, logits.data_ptr(),
                                                      ELEM[logits.dtype], ls, out.data_ptr(), n_tok, ws.data_ptr(), ws.numel(), st))
-        if trace is not None and n_tok:
-            ids = self.routing_of(n_tok)[0].cpu().numpy()
+            picks = self.routing_of(n_tok)[0].cpu().numpy() if trace is not None and n_tok else None
+        if picks is not None:
             for r in ("gate", "up", "down"):
-                trace.record(f"ffn_{r}_exps.weight", ids, self.E)
+                trace.record(f"{self.name}.ffn_{r}_exps.weight", picks, self.E)
         return out
 
     prefill = decode
@@ -327,11 +328,14 @@ class Stack:
     x_nexts, x_nexts[l] = xs[l] + outs[l] (a residual chain when xs[l + 1]
     is x_nexts[l]). The layers share one shape; their types are either one
     type for every tensor or, per layer, gate = up with the gate/up and down
-    types among Q2_K, Q3_K, Q4_K, Q6_K (the mixed-type kernel). run() may be
+    types among Q2_K, Q3_K, Q4_K, Q6_K (the mixed-type kernel); layers with a
+    router of their own, MXFP4 ones among them, are refused. run() may be
     repeated; every tensor must stay alive."""
 
     def __init__(self, layers, xs, logits, outs, x_nexts=None, stream=None):
         n = len(layers)
+        if any(getattr(L, "router", None) is not None for L in layers):
+            raise bad("the stack kernel routes by softmax, top-k: it takes no layer with a router of its own")
         self.layers, self.n = layers, n
         self.desc0 = layers[0].desc
         arr = (MoeLayerDesc * n)(*[L.desc for L in layers])

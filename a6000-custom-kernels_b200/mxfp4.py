@@ -68,7 +68,8 @@ def dequantize_mxfp4(blocks, K, planes=None, dtype=torch.float32, out=None, stre
 class MXFP4Weights:
     """The matrices of a layer's experts, laid out once for the 4-bit tensor
     cores from ggml MXFP4 blocks (uint8 [E, rows, 17 K / 32], on the device).
-    `blocks` may be dropped afterwards."""
+    `blocks` may be dropped afterwards; calls on other streams than `stream` wait
+    for it as for any tensor made there."""
 
     def __init__(self, blocks, K, rows, stream=None):
         if not (isinstance(blocks, torch.Tensor) and blocks.is_cuda and blocks.dtype == torch.uint8 and
@@ -84,6 +85,8 @@ class MXFP4Weights:
         t.nb[0], t.nb[1], t.nb[2], t.nb[3] = TSIZE[MXFP4], rb, rb * rows, rb * rows * self.E
         ctx, st = on(self.device, stream)
         with ctx:
+            if stream is not None:
+                blocks.record_stream(torch.cuda.current_stream())
             self.data = blocks.new_empty(max(1, lib().moe_b200_mxfp4_packed_size(self.E, rows, K)))
             check(lib().moe_b200_mxfp4_pack(ctypes.byref(t), self.data.data_ptr(), self.data.numel(), st))
         self.shape = (self.E, rows, K, self.device)

@@ -27,9 +27,14 @@ class Router:
         if bias is not None and not (isinstance(bias, torch.Tensor) and bias.is_cuda and bias.dtype == torch.float32 and
                                      bias.dim() == 1 and bias.is_contiguous()):
             raise bad("bias must be a contiguous f32 CUDA vector")
-        self.k, self.bias = k, bias
+        self.k, self._bias = k, bias
         self.desc = MoeRouter(SCORES[score], n_group, topk_group, GROUP_SCORES[group_score], norm_w, scale)
         self.ref = ctypes.byref(self.desc)
+
+    @property
+    def bias(self):
+        """The bias (written in place, it takes effect from the next call on)."""
+        return self._bias
 
     def __call__(self, logits, ids=None, weights=None, stream=None):
         """logits f32 / f16 / bf16 [n_tok, E] -> (ids i32 [n_tok, k], weights f32 [n_tok, k])."""
@@ -37,7 +42,7 @@ class Router:
         if logits.dim() != 2:
             raise bad("logits must be [n_tok, n_experts]")
         n_tok, E = logits.shape
-        k, dev, bias = self.k, logits.device, self.bias
+        k, dev, bias = self.k, logits.device, self._bias
         if bias is not None and (bias.device != dev or bias.shape[0] != E):
             raise bad("bias must be f32 [n_experts] on the logits' device")
         ctx, st = on(dev, stream)

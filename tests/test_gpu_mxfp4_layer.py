@@ -149,3 +149,52 @@ def test_ggml_layer_behind_a_router(pkg, cuda, t, n):
         assert (one - y[:, 0]).abs().max() <= 1e-6 * y.abs().max()
     finally:
         pkg.moe_cache.reset()
+
+
+def test_trace_names_and_streams(pkg, cuda, tmp_path):
+    """The trace has the layer's name and the picks of the stream that the call ran on; a router's bias written
+    in place takes effect."""
+    from importlib import import_module
+    seed = import_module("a6000-custom-kernels_b200.seed")
+    bias = torch.zeros(8, device=cuda)
+    t = {r: pkg.moe_cache.MXFP4 for r in ("gate", "up", "down")}
+    L = pkg.MoELayer(64, 64, 8, 2, t, False, device=cuda, name="blk.7", router=pkg.Router(2, "sigmoid", bias=bias))
+    x, lg = torch.randn((4, 64), device=cuda), torch.randn((4, 8), device=cuda)
+    path = tmp_path / "t.bin"
+    with seed.TraceWriter(str(path)) as tw:
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        L.decode(x, lg, stream=s, trace=tw)
+        torch.cuda.synchronize()
+        bias[5] = 10.0
+        L.decode(x, lg, trace=tw)
+    rec = list(seed.read_trace(str(path)))
+    assert [r[0] for r in rec] == 2 * [f"blk.7.ffn_{r}_exps.weight" for r in ("gate", "up", "down")]
+    ids = pkg.route_experts(lg, 2, "sigmoid")[0].cpu().numpy()
+    np.testing.assert_array_equal(np.asarray(rec[0][-1]).reshape(4, 2), ids)
+    assert (np.asarray(rec[3][-1]).reshape(4, 2)[:, 0] == 5).all()
+
+
+def test_router_layer_refusals(pkg, cuda):
+    pkg.moe_cache.configure(enabled=True)
+    try:
+        types = {r: pkg.moe_cache.Q4_0 for r in ("gate", "up", "down")}
+        L = pkg.MoELayer(256, 128, 8, 2, types, False, device=cuda, router=pkg.Router(2, "sigmoid"))
+        x, lg = torch.randn((3, 256), device=cuda), torch.randn((3, 8), device=cuda)
+        for kw in (dict(x=x.half()), dict(x=x[:, :128]), dict(x=x.cpu()), dict(logits=lg.cpu()), dict(logits=lg[:2]),
+                   dict(out=torch.empty((3, 255), device=cuda)), dict(out=torch.empty((3, 256), device=cuda).half())):
+            with pytest.raises(pkg.MoeError):
+                L.decode(**{**dict(x=x, logits=lg), **kw})
+        assert torch.isfinite(L.decode(x, lg)).all()
+    finally:
+        pkg.moe_cache.reset()
+
+
+def test_more_tokens_than_a_grid_has_rows(pkg, cuda):
+    t = {r: pkg.moe_cache.MXFP4 for r in ("gate", "up", "down")}
+    L = pkg.MoELayer(32, 32, 2, 1, t, device=cuda, planes=1)
+    n = 65535 + 70
+    x, lg = torch.randn((n, 32), device=cuda), torch.randn((n, 2), device=cuda)
+    out = L.prefill(x, lg)
+    part = L.prefill(x[-100:], lg[-100:])
+    assert torch.equal(out[-100:], part) and torch.equal(out[:100], L.prefill(x[:100], lg[:100]))

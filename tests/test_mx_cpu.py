@@ -157,3 +157,22 @@ def test_python_refusals_without_a_gpu(pkg):
                  lambda: pkg.MoELayer(64, 64, 4, 2, {r: pkg.moe_cache.MXFP4 for r in ("gate", "up", "down")}, host=True)):
         with pytest.raises(pkg.MoeError):
             call()
+
+
+def test_a_layer_with_its_own_router_stays_off_paths_that_route_themselves(pkg):
+    from importlib import import_module
+    from types import SimpleNamespace
+    ep = import_module("a6000-custom-kernels_b200.ep")
+    layer = SimpleNamespace(router=object())
+    with pytest.raises(pkg.MoeError, match="router"):
+        pkg.Stack([SimpleNamespace(router=None), layer], [], [], [])
+    with pytest.raises(pkg.MoeError, match="router"):
+        ep.EPMoELayer(layer, 0, 2)
+
+
+def test_layer_arguments_by_position(pkg):
+    """`shared` and what follows may be given by position, for every type."""
+    mc = pkg.moe_cache
+    assert type(pkg.MoELayer.__new__(pkg.MoELayer, 64, 64, 4, 2, {r: mc.Q4_0 for r in ("gate", "up", "down")}, False)) is pkg.MoELayer
+    with pytest.raises(pkg.MoeError, match="device memory"):
+        pkg.MoELayer(64, 64, 4, 2, {r: mc.MXFP4 for r in ("gate", "up", "down")}, False, host=True)
