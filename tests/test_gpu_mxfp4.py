@@ -384,3 +384,52 @@ def test_waits_give_up(pkg, cuda, n):
     assert code == mc.DERR_TIMEOUT_FULL
     assert torch.equal(pkg.mxfp4_mul_mat_id(w, x, ids, gate=w), good)
     assert mc.device_error() == 0
+
+
+@pytest.mark.parametrize("n,k,E,K,rows,per_pick", [
+    (3, 20, 40, 64, 33, False),        # more picks than a row's lanes look up at once, direct
+    (40, 12, 700, 96, 70, False),      # and grouped, with one set of counters
+    (30, 4, 4096, 32, 17, False),      # the most experts
+    (16, 3, 4096, 64, 20, True),       # and direct
+    (4500, 8, 16, 32, 20, False),      # entries past those whose ids stay in registers
+    (33000, 1, 3, 32, 16, True),
+    (2100, 16, 24, 96, 40, False),     # both
+])
+def test_product_of_many(pkg, cuda, n, k, E, K, rows, per_pick):
+    rng = np.random.default_rng(n + E)
+    W = _experts(rng, E, rows, K)
+    x = rng.normal(size=(n, k, K) if per_pick else (n, K))
+    ids = _ids(rng, n, k, E)
+    ids[rng.random(ids.shape) < 0.05] = -1
+    dst = torch.full((n, k, rows), 7.0, device=cuda)
+    y, xv = _run(pkg, cuda, W, x, ids, K, 2, torch.float32, None, dst)
+    assert pkg.moe_cache.device_error() == 0 and (y[ids < 0] == 7.0).all()
+    ref, mag = R.product(W, xv, np.maximum(ids, 0), 2, None)
+    assert (np.abs(y - ref) <= R.product_tol(mag, K, 2))[ids >= 0].all()
+
+
+def test_offsets_past_32_bits(pkg, cuda):
+    """Rows of x and of dst more than 2^31 elements from their tensors' first."""
+    rng = np.random.default_rng(1)
+    E, K, rows = 2, 64, 40
+    W = _experts(rng, E, rows, K)
+    w = _weights(pkg, cuda, W, K)
+    n, wide = 70000, 32768
+    big = torch.empty((n, wide), dtype=torch.bfloat16, device=cuda)          # 4.6 GB, 2.3e9 elements
+    x = big[:, 8:8 + K]
+    x.copy_(torch.randn((n, K), device=cuda))
+    ids = torch.randint(0, E, (n, 1), dtype=torch.int32, device=cuda)
+    tail = x[-64:].contiguous()
+    assert torch.equal(pkg.mxfp4_mul_mat_id(w, x, ids)[-64:], pkg.mxfp4_mul_mat_id(w, tail, ids[-64:].contiguous()))
+    assert torch.equal(pkg.quantize_mxfp4(x)[-64:], pkg.quantize_mxfp4(tail))
+    assert torch.equal(pkg.route_experts(x, 4)[0][-64:], pkg.route_experts(tail, 4)[0])
+    pkg.dequantize_mxfp4(pkg.quantize_mxfp4(tail), K, dtype=torch.bfloat16, out=x[-64:])
+    assert torch.equal(x[-64:], pkg.dequantize_mxfp4(pkg.quantize_mxfp4(tail), K, dtype=torch.bfloat16))
+    del big, x
+    n, rows = 4200, 65536                                                    # dst: 8.8 GB, 2.2e9 elements
+    W = _experts(rng, E, rows, 32)
+    w = _weights(pkg, cuda, W, 32)
+    x = torch.randn((n, 32), device=cuda)
+    ids = torch.randint(0, E, (n, 8), dtype=torch.int32, device=cuda)
+    y = pkg.mxfp4_mul_mat_id(w, x, ids)
+    assert torch.equal(y[-8:], pkg.mxfp4_mul_mat_id(w, x[-8:].contiguous(), ids[-8:].contiguous()))
