@@ -2072,7 +2072,8 @@ MxWs mx_ws(int64_t E, int64_t K, int64_t n_tok, int64_t k, int planes, char *bas
         const int NT = moe::mx_chunk_tokens(n_tok, k, E, glu);
         const int64_t chunks = direct ? n_tok * k : moe::mmq_max_chunks(n_tok * k, E, NT);
         w.max_chunks = std::max(w.max_chunks, chunks);
-        images = std::max(images, static_cast<size_t>(moe::mx_images_bytes(chunks, NT, K, planes)));
+        if (!moe::mx_rows_direct(n_tok, k))
+            images = std::max(images, static_cast<size_t>(moe::mx_images_bytes(chunks, NT, K, planes)));
     }
     w.images = reinterpret_cast<uint8_t *>(take(images));
     if (!direct) {
@@ -2202,7 +2203,7 @@ int moe_b200_mxfp4_mul_mat_id(const moe_mxfp4 *w, const moe_mxfp4 *gate, const f
     if (!x || !ids || !dst || !aligned_elem(x, x_type)) return fail(MOE_ERR_INVALID, "null or misaligned argument");
     const bool per_pick = x_per_pick != 0;
     const MxWs s = mx_ws(w->n_experts, w->K, n_tok, k, planes, static_cast<char *>(workspace));
-    if (!workspace || workspace_bytes < s.bytes)
+    if (s.bytes && (!workspace || workspace_bytes < s.bytes))
         return fail(MOE_ERR_INVALID, "workspace too small (%zu < %zu bytes)", workspace_bytes, s.bytes);
     if (!aligned16(workspace)) return fail(MOE_ERR_INVALID, "workspace must be 16-byte aligned");
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -2245,7 +2246,15 @@ int moe_b200_mxfp4_mul_mat_id(const moe_mxfp4 *w, const moe_mxfp4 *gate, const f
     a.dst = dst;
     a.err = g.d_err;
     a.timeout_ns = g.timeout_ns_kernel;
-    CK(moe::launch_mx_prep(x, mx_elem(x_type), x_row_stride, per_pick ? n_tok * k : n_tok, w->K, a, NT, st));
+    if (moe::mx_rows_direct(n_tok, k)) {
+        a.images = nullptr;
+        a.x = x;
+        a.x_stride = x_row_stride;
+        a.x_type = mx_elem(x_type);
+        a.nb = static_cast<int32_t>(w->K / 32);
+    } else {
+        CK(moe::launch_mx_prep(x, mx_elem(x_type), x_row_stride, per_pick ? n_tok * k : n_tok, w->K, a, NT, st));
+    }
     CK(moe::launch_mx_product(a, NT, units, st));
     return MOE_OK;
 }

@@ -58,6 +58,12 @@ __device__ __forceinline__ MxRaw<XT> mx_zero() {
     for (uint32_t &w : r.w) w = 0u;
     return r;
 }
+// rows whose groups of 4 values are aligned to their size
+template <int XT>
+__host__ __device__ __forceinline__ bool mx_vec_ok(const void *p, int64_t stride) {
+    constexpr int64_t need = 4 * sizeof(typename MxElem<XT>::T);
+    return reinterpret_cast<uintptr_t>(p) % need == 0 && (stride * static_cast<int64_t>(sizeof(typename MxElem<XT>::T))) % need == 0;
+}
 template <int XT> struct MxPair;
 template <> struct MxPair<MX_F16> {
     using T = __half2;
@@ -652,12 +658,7 @@ __global__ void __cluster_dims__(MXG_CTAS, 1, 1) __launch_bounds__(MXG_THREADS) 
     cluster_sync();   // the counts stay until every CTA has read them
 }
 
-// The direct form's chunk of entry i: the entries of its expert among all
-// (bits of `same`), its place in the chunk and the chunk's size. A whole warp
-// calls with entries i and i + 32 of lane i's ids x0, x1.
-__device__ __forceinline__ uint64_t mx_same(int x0, int x1, int e) {
-    return __ballot_sync(0xffffffffu, x0 == e) | (static_cast<uint64_t>(__ballot_sync(0xffffffffu, x1 == e)) << 32);
-}
+// The direct form groups its entries by itself: bit j of `same` says that entry j has an entry's expert.
 __device__ __forceinline__ int mx_before(uint64_t same, int i) { return __popcll(same & ((1ull << i) - 1ull)); }
 __device__ __forceinline__ int mx_id(const int32_t *ids, int64_t stride, int n_entries, int k, int i) {
     return i < n_entries ? ids[(i / k) * stride + i % k] : -2;
@@ -803,12 +804,14 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 
-template <int NT>
+template <int ENTRIES>
 struct MxCtl {
     uint64_t full[MX_MAX_STAGES], empty[MX_MAX_STAGES], acc_full[2], acc_empty[2], drain;
+    uint64_t rows[MX_MAX_STAGES];   // a stage's image, where the CTA quantises it
     uint32_t tmem;
-    int32_t abort, expert, count;
-    int32_t entry[NT];
+    int32_t abort, n_chunks;
+    int32_t entry[ENTRIES];     // direct form: the entries grouped by expert
+    int4 chunk[ENTRIES];        // {expert, first entry, count, number of its image}
 };
 
 template <int NT>
@@ -816,8 +819,8 @@ __host__ __device__ constexpr uint32_t mx_stage_bytes(int mats, int planes) {
     return mxp_tps<NT>() * (mats * MX_TILE + planes * mx_image_plane(NT));
 }
 
-template <int NT>
-__device__ __forceinline__ bool mx_wait(MxCtl<NT> &C, uint64_t *bar, uint32_t parity, const MxArgs &a) {
+template <int ENTRIES>
+__device__ __forceinline__ bool mx_wait(MxCtl<ENTRIES> &C, uint64_t *bar, uint32_t parity, const MxArgs &a) {
     // limits below 20 us poll (try_wait may suspend for longer), so that a tiny limit gives up at once
     const bool poll = a.timeout_ns < 20000u;
     if (poll ? mbar_test_wait(bar, parity) : mbar_try_wait(bar, parity)) return true;
@@ -853,6 +856,113 @@ __device__ __forceinline__ float mx_glu(float g, float up, float limit) {
     } else return glu_apply(OP, g, up, limit);
 }
 
+// The direct form's chunks, by one warp from the ids of up to 64 entries: lane l
+// looks at entries l and l + 32. Experts follow one another as they first appear.
+template <int NT>
+__device__ __forceinline__ void mx_direct_table(MxCtl<MX_DIRECT> &C, const MxArgs &a, int lane) {
+    int x[2];
+    uint64_t same[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        x[h] = mx_id(a.ids, a.ids_stride, a.n_entries, a.k, lane + 32 * h);
+        if (lane + 32 * h < a.n_entries && x[h] != -1 && (x[h] < 0 || x[h] >= a.n_experts)) {
+            set_error(a.err, DERR_BAD_ID);
+            x[h] = -1;
+        }
+    }
+    if (a.n_entries <= 32) {
+        same[0] = __match_any_sync(0xffffffffu, x[0]);
+        same[1] = 0;
+    } else {
+        same[0] = same[1] = 0;
+#pragma unroll 8
+        for (int j = 0; j < MX_DIRECT; ++j) {
+            const int y = __shfl_sync(0xffffffffu, x[j >> 5], j & 31);
+            same[0] |= static_cast<uint64_t>(x[0] == y) << j;
+            same[1] |= static_cast<uint64_t>(x[1] == y) << j;
+        }
+    }
+    // (entries, chunks) of the experts that appear before: a scan over each expert's first entry
+    int before[2], carry = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int cnt = __popcll(same[h]);
+        const bool leads = x[h] >= 0 && mx_before(same[h], lane + 32 * h) == 0;
+        const int mine = leads ? cnt | ((cnt + NT - 1) / NT) << 16 : 0;
+        int sum = mine;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, sum, off);
+            if (lane >= off) sum += o;
+        }
+        before[h] = carry + sum - mine;
+        carry += __shfl_sync(0xffffffffu, sum, 31);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int i = lane + 32 * h, pos = mx_before(same[h], i), lead = same[h] ? __ffsll(static_cast<long long>(same[h])) - 1 : 0;
+        const int lo = __shfl_sync(0xffffffffu, before[0], lead & 31), hi = __shfl_sync(0xffffffffu, before[1], lead & 31);
+        const int at = lead < 32 ? lo : hi, first = at & 0xFFFF;
+        if (x[h] >= 0) {
+            C.entry[first + pos] = i;
+            if (pos % NT == 0)
+                C.chunk[(at >> 16) + pos / NT] = make_int4(x[h], first + pos, min(NT, __popcll(same[h]) - pos), i);
+        }
+    }
+    if (lane == 0) C.n_chunks = carry >> 16;
+}
+
+// A chunk's rows into the ring's images, by the warps behind the first two: one
+// row of one stage (8 blocks, 4 lanes each) per warp and step, the next step's
+// values on their way meanwhile.
+struct MxRing { int s, ph, fills; };   // the ring's next stage, the parity of its use, stages used so far
+template <int NT, int XT, int PLANES, int MATS>
+__device__ __forceinline__ void mx_rows(MxCtl<MX_DIRECT> &C, const MxArgs &a, int first, int count, int kt0, int n_it,
+                                        MxRing &at, int warp, int lane, uint8_t *ring) {
+    static_assert(mxp_tps<NT>() * MX_KT == 8 * 32, "a warp takes a row of a stage");
+    constexpr int WARPS = 4 * mxp_epi<NT>(), TPS = mxp_tps<NT>();
+    constexpr uint32_t PLANE = mx_image_plane(NT);
+    using T = typename MxElem<XT>::T;
+    const int i4 = lane & 3, b = (lane >> 2) & 3, t = lane >> 4;   // block b of tile t
+    const bool vec = mx_vec_ok<XT>(a.x, a.x_stride);
+    const int steps = n_it * count;
+    auto load = [&](int p) {
+        const int i = p / count, en = C.entry[first + p - i * count], blk = (kt0 + i * TPS) * 4 + (lane >> 2);
+        const T *x = static_cast<const T *>(a.x) + static_cast<int64_t>(a.per_pick ? en : en / a.k) * a.x_stride + blk * 32;
+        if (p >= steps || blk >= a.nb) return mx_zero<XT>();       // K padded to whole tiles with zeros
+        return vec ? mx_load<XT, true>(x, i4) : mx_load<XT, false>(x, i4);
+    };
+    int p = warp;
+    MxRaw<XT> next = load(p);
+    for (int i = 0; i < n_it; ++i) {
+        if (at.fills >= a.stages && !mx_wait_warp(C, &C.empty[at.s], at.ph ^ 1, a)) return;
+        uint8_t *const image = ring + at.s * mx_stage_bytes<NT>(MATS, PLANES) + TPS * MATS * MX_TILE + t * (PLANES * PLANE);
+        for (; p < (i + 1) * count; p += WARPS) {
+            const int j = p - i * count;
+            float v[8];
+            uint32_t top = mx_floats<XT>(next, v);
+            next = load(p + WARPS);
+#pragma unroll
+            for (int pl = 0; pl < PLANES; ++pl) {
+                uint32_t byte;
+                const uint32_t w = mx_quant_block(v, top, byte);
+                uint8_t *const o = image + pl * PLANE;
+                *reinterpret_cast<uint32_t *>(o + b * (16 * NT) + j * 16 + 4 * i4) = w;
+                if (i4 == 0) o[64 * NT + j * 16 + b] = static_cast<uint8_t>(byte);
+                if (pl + 1 < PLANES) {
+                    mx_residual(v, w, byte);
+                    top = mx_top(v);
+                }
+            }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&C.rows[at.s]);
+        ++at.fills;
+        if (++at.s == a.stages) { at.s = 0; at.ph ^= 1; }
+    }
+}
+
 // Work item: 128 weight rows (of w, and of gate with GLU) x the up to NT
 // entries of one chunk x this cluster rank's share of K. A CTA walks items
 // blockIdx / split, + gridDim / split, ... with its roles running ahead of one
@@ -864,40 +974,30 @@ __device__ __forceinline__ float mx_glu(float g, float up, float limit) {
 //   the rest  in groups of 4 warps that take 16 columns in turn, read the
 //             accumulators (thread = weight row), add biases, apply the GLU and
 //             store, while the next item multiplies.
+// Up to 16 tokens (NT = 16, direct) the last warps first quantise the chunk's
+// rows straight into the ring: every tile of weight rows does it again, but a
+// few rows are done before their weights arrive, and the call is one launch
+// without a workspace (a launch more cost 3 us of 17 for one token).
 // With split > 1 a cluster's CTAs have one item each; their partial sums meet in
 // shared memory and are added in rank order, so results do not depend on timing.
 template <int NT, bool GLU, bool DIRECT, int PLANES>
 __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxArgs a) {
     extern __shared__ __align__(128) uint8_t ring[];
-    __shared__ MxCtl<NT> C;
     constexpr int MATS = GLU ? 2 : 1, MXP_EPI = mxp_epi<NT>(), MXP_TPS = mxp_tps<NT>();
+    constexpr bool ROWS = DIRECT && NT == MX_ROWS_TOKENS;   // quantises x itself
+    __shared__ MxCtl<DIRECT ? MX_DIRECT : 1> C;
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int rank = a.split > 1 ? static_cast<int>(cluster_rank()) : 0;
     const int item0 = blockIdx.x / a.split, item_step = gridDim.x / a.split;
 
-    if (DIRECT && warp == 0) {
-        // (ids are complete before the launch that this one overlaps with; the images are not)
-        const int lead = item0 / a.RT;
-        const int x0 = mx_id(a.ids, a.ids_stride, a.n_entries, a.k, lane);
-        const int x1 = mx_id(a.ids, a.ids_stride, a.n_entries, a.k, lane + 32);
-        const int e = __shfl_sync(0xffffffffu, lead < 32 ? x0 : x1, lead & 31);
-        const uint64_t same = mx_same(x0, x1, e);
-        const int pos = mx_before(same, lead);
-        const bool ok = e >= 0 && e < a.n_experts;
-        const int count = ok && pos % NT == 0 ? min(__popcll(same) - pos, NT) : 0;
-        if (!ok && e != -1 && lane == 0) set_error(a.err, DERR_BAD_ID);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int i = lane + 32 * h, n = mx_before(same, i) - pos;
-            if (((same >> i) & 1ull) && n >= 0 && n < count) C.entry[n] = i;
-        }
-        if (lane == 0) { C.expert = e; C.count = count; }
-    }
+    if constexpr (DIRECT)   // (ids are complete before the launch that this one overlaps with; the images are not)
+        if (warp == 0) mx_direct_table<NT>(C, a, lane);
     if (tid == 32) {
         for (int s = 0; s < a.stages; ++s) {
             mbar_init(&C.full[s], 1);
             mbar_init(&C.empty[s], 1);
+            if (ROWS) mbar_init(&C.rows[s], 4 * MXP_EPI);
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(&C.acc_full[s], 1);
@@ -910,13 +1010,13 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
     __syncthreads();
     int n_items = 0;
     if (DIRECT) {
-        n_items = C.count > 0 ? item0 + 1 : 0;   // one item per CTA
+        n_items = C.n_chunks * a.RT;
     } else {
         asm volatile("griddepcontrol.wait;" ::: "memory");
         n_items = *a.n_chunks * a.RT;
     }
     if (item0 >= n_items) {   // nothing here; the same for every rank of the cluster
-        if (DIRECT) asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (DIRECT && !ROWS) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
     if (warp == 1) {
@@ -931,20 +1031,17 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
     const int stages = a.stages, acc = a.acc;
     constexpr uint32_t stage_bytes = mx_stage_bytes<NT>(MATS, planes);
     const uint32_t ring0 = smem_u32(ring);
-    struct Item { int rt, chunk, expert, count, first; };
+    struct Item { int rt, chunk, expert, count, first; };   // chunk: the number of its image
     auto item_at = [&](int item) {
         Item I;
         I.chunk = item / a.RT;
         I.rt = item - I.chunk * a.RT;
-        if (DIRECT) {
-            I.expert = C.expert; I.count = C.count; I.first = 0;
-        } else {
-            const int4 ch = a.chunks[I.chunk];
-            I.expert = ch.x; I.first = ch.y; I.count = ch.z;
-        }
+        const int4 ch = DIRECT ? C.chunk[I.chunk] : a.chunks[I.chunk];
+        I.expert = ch.x; I.first = ch.y; I.count = ch.z;
+        if (DIRECT) I.chunk = ch.w;
         return I;
     };
-    auto entry_of = [&](const Item &I, int j) { return DIRECT ? C.entry[j] : a.entries[I.first + j]; };
+    auto entry_of = [&](const Item &I, int j) { return DIRECT ? C.entry[I.first + j] : a.entries[I.first + j]; };
 
     // warp 0: stages issued so far, and the ring's next stage
     int fills = 0;
@@ -969,7 +1066,7 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
         early = n_it < stages ? n_it : stages;
         const uint64_t pol = l2_evict_first_policy();
         for (w_stage = 0; static_cast<int>(w_stage) < early; ++w_stage)
-            fill_weights(on, weights_at(I), w_stage, planes * mx_image_plane(mx_round16(I.count)), pol);
+            fill_weights(on, weights_at(I), w_stage, ROWS ? 0u : planes * mx_image_plane(mx_round16(I.count)), pol);
         w_stage = 0;
         __syncwarp();
     }
@@ -979,12 +1076,12 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
     const uint32_t tmem = __shfl_sync(0xffffffffu, C.tmem, 0);
 
     if (warp == 0) {
-        if (DIRECT) asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (DIRECT && !ROWS) asm volatile("griddepcontrol.wait;" ::: "memory");
         const uint64_t pol_w = l2_evict_first_policy(), pol_x = l2_evict_last_policy();
         bool ok = true;
         for (int item = item0; item < n_items && ok; item += item_step) {
             const Item I = item_at(item);
-            const uint32_t tile = __shfl_sync(0xffffffffu, planes * mx_image_plane(mx_round16(I.count)), 0);
+            const uint32_t tile = ROWS ? 0u : __shfl_sync(0xffffffffu, planes * mx_image_plane(mx_round16(I.count)), 0);
             const uint64_t wat = weights_at(I);
             const uint8_t *image = a.images + static_cast<uint64_t>(I.chunk) * mx_image_bytes(NT, a.KT, planes) +
                                    static_cast<uint64_t>(kt0) * tile;
@@ -993,9 +1090,10 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
                     ok = mx_wait_warp(C, &C.empty[w_stage], w_phase ^ 1u, a);
                     if (!ok) break;
                 }
-                if (i >= early) fill_weights(on, wat, i, tile, pol_w);
-                bulk_g2s_if(on, ring0 + w_stage * stage_bytes + MXP_TPS * MATS * MX_TILE, image, tiles_of(i) * tile,
-                            full0 + 8 * w_stage, pol_x);
+                if (i >= early || item != item0) fill_weights(on, wat, i, tile, pol_w);
+                if (!ROWS)
+                    bulk_g2s_if(on, ring0 + w_stage * stage_bytes + MXP_TPS * MATS * MX_TILE, image, tiles_of(i) * tile,
+                                full0 + 8 * w_stage, pol_x);
                 image += MXP_TPS * tile;
                 ++fills;
                 if (++w_stage == static_cast<uint32_t>(stages)) { w_stage = 0; w_phase ^= 1u; }
@@ -1021,6 +1119,7 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
             bool ready = false;
             for (int i = 0; i < n_it && ok; ++i) {
                 if (!ready) ok = mx_wait_warp(C, &C.full[s], ph, a);
+                if (ROWS && ok) ok = mx_wait_warp(C, &C.rows[s], ph, a);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t A = ring0 + s * stage_bytes, B = A + MXP_TPS * MATS * MX_TILE, sf = sf0 + s * sf_slot;
@@ -1073,13 +1172,25 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
         const int grp = (warp - 2) >> 2;
         const int quarter = warp & 3;                 // TMEM lanes this warp may read
         const int r = 32 * quarter + lane;            // weight row of the tile
+        MxRing at{0, 0, 0};
+        auto rows_of = [&](const Item &I) {   // (a wait that gives up: the epilogue's gives up with it)
+            if constexpr (ROWS) {
+                if (a.x_type == MX_F32) mx_rows<NT, MX_F32, PLANES, MATS>(C, a, I.first, I.count, kt0, n_it, at, warp - 2, lane, ring);
+                else if (a.x_type == MX_F16) mx_rows<NT, MX_F16, PLANES, MATS>(C, a, I.first, I.count, kt0, n_it, at, warp - 2, lane, ring);
+                else mx_rows<NT, MX_BF16, PLANES, MATS>(C, a, I.first, I.count, kt0, n_it, at, warp - 2, lane, ring);
+            }
+        };
         constexpr int ROUNDS = (NT + 16 * MXP_EPI - 1) / (16 * MXP_EPI);
         uint32_t n = 0;
         Item next = item_at(item0);
+        if constexpr (ROWS) rows_of(next);
         for (int item = item0; item < n_items; item += item_step, ++n) {
             const uint32_t ab = acc == 2 ? n & 1u : 0u, aph = acc == 2 ? (n >> 1) & 1u : n & 1u;
             const Item I = next;
-            if (item + item_step < n_items) next = item_at(item + item_step);
+            if (item + item_step < n_items) {
+                next = item_at(item + item_step);
+                if constexpr (ROWS) rows_of(next);   // while this one multiplies
+            }
             const int row = I.rt * MX_M + r;
             const bool row_ok = row < a.rows;
             auto bias_of = [&](const float *b, int at) { return b[static_cast<int64_t>(I.expert) * a.rows + at]; };
@@ -1205,12 +1316,6 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
 }
 
 template <int XT>
-bool mx_vec_ok(const void *p, int64_t stride) {
-    constexpr int64_t need = 4 * sizeof(typename MxElem<XT>::T);
-    return reinterpret_cast<uintptr_t>(p) % need == 0 && (stride * static_cast<int64_t>(sizeof(typename MxElem<XT>::T))) % need == 0;
-}
-
-template <int XT>
 void quantize_t(const void *x, int64_t stride, int64_t n_blocks, int nb, int planes, uint8_t *y, cudaStream_t st) {
     using T = typename MxElem<XT>::T;
     const unsigned grid = static_cast<unsigned>((n_blocks + MXQ_BLK - 1) / MXQ_BLK);
@@ -1263,9 +1368,9 @@ template <int NT, bool GLU, bool DIRECT, int PLANES>
 cudaError_t product_p(MxArgs &a, int64_t units, cudaStream_t st) {
     constexpr int MATS = GLU ? 2 : 1, MXP_TPS = mxp_tps<NT>();
     auto kern = mx_product_kernel<NT, GLU, DIRECT, PLANES>;
-    constexpr uint32_t fixed = (sizeof(MxCtl<NT>) + 127u) / 128u * 128u + 1024u;   // static part and the system's 1 KB
+    constexpr uint32_t fixed = (sizeof(MxCtl<DIRECT ? MX_DIRECT : 1>) + 127u) / 128u * 128u + 1024u;   // static part and the system's 1 KB
     const uint32_t sb = mx_stage_bytes<NT>(MATS, PLANES), sf = MXP_TPS * (4u * MATS + (NT > 128 ? 8u : 4u) * PLANES);
-    const bool single = DIRECT || a.split > 1;       // one item per CTA
+    const bool single = a.split > 1;                 // one item per CTA
     a.acc = single ? 1 : 2;
     const int tiles = (a.KT + a.split - 1) / a.split;
     const int most = single ? (tiles + MXP_TPS - 1) / MXP_TPS : MX_MAX_STAGES;   // stages that would be used
@@ -1311,7 +1416,7 @@ cudaError_t product_p(MxArgs &a, int64_t units, cudaStream_t st) {
     at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = DIRECT && NT == MX_ROWS_TOKENS ? 1 : 2;
     return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
@@ -1357,12 +1462,13 @@ cudaError_t launch_mx_pack(const uint8_t *src, int64_t E, int64_t rows, int64_t 
 // expert has on average.
 int mx_chunk_tokens(int64_t n_tok, int64_t k, int64_t n_experts, bool glu) {
     const int64_t n = n_tok * k;
-    if (n <= MX_DIRECT) return n_tok <= 16 ? 16 : 64;
+    if (n <= MX_DIRECT) return n_tok <= MX_ROWS_TOKENS ? MX_ROWS_TOKENS : 64;
     const int64_t per = n / (n < n_experts ? n : n_experts);
     return per <= 12 ? 16 : per <= 48 ? 64 : glu ? MXP_WIDE_GLU : MXP_WIDE;
 }
 
 bool mx_direct(int64_t n_tok, int64_t k) { return n_tok * k <= MX_DIRECT; }
+bool mx_rows_direct(int64_t n_tok, int64_t k) { return mx_direct(n_tok, k) && n_tok <= MX_ROWS_TOKENS; }
 
 int64_t mx_max_experts() { return MXG_MAX_EXPERTS; }
 
@@ -1420,11 +1526,11 @@ cudaError_t launch_mx_product(MxArgs &a, int NT, int64_t units, cudaStream_t st)
     // few tiles: a cluster of 2, 4 or 8 CTAs shares a tile's K
     int split = 1;
     if (NT <= 64)
-        while (split < 8 && units * a.RT * split < 296 && a.KT / (2 * split) >= 2) split *= 2;
+        while (split < 8 && units * a.RT * split < 148 && a.KT / (2 * split) >= 2) split *= 2;
     a.split = split;
-    if (NT == 16) {
-        if (glu) return direct ? product_t<16, true, true>(a, units, st) : product_t<16, true, false>(a, units, st);
-        return direct ? product_t<16, false, true>(a, units, st) : product_t<16, false, false>(a, units, st);
+    if (NT == MX_ROWS_TOKENS) {
+        if (glu) return direct ? product_t<MX_ROWS_TOKENS, true, true>(a, units, st) : product_t<MX_ROWS_TOKENS, true, false>(a, units, st);
+        return direct ? product_t<MX_ROWS_TOKENS, false, true>(a, units, st) : product_t<MX_ROWS_TOKENS, false, false>(a, units, st);
     }
     if (NT == 64) {
         if (glu) return direct ? product_t<64, true, true>(a, units, st) : product_t<64, true, false>(a, units, st);

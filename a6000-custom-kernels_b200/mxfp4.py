@@ -95,7 +95,7 @@ class MXFP4Weights:
 
 
 def mxfp4_workspace_size(w, n_tok, k, planes=2):
-    """Bytes of device workspace mxfp4_mul_mat_id needs (moe_b200_mxfp4_workspace_size)."""
+    """Bytes of device workspace mxfp4_mul_mat_id needs (moe_b200_mxfp4_workspace_size): 0 for a few tokens."""
     return lib().moe_b200_mxfp4_workspace_size(w.ref, n_tok, k, planes)
 
 
@@ -139,14 +139,20 @@ def mxfp4_mul_mat_id(w, x, ids, gate=None, bias=None, gate_bias=None, glu_op=GLU
     with ctx:
         dst = x.new_empty((n_tok, k, rows), dtype=torch.float32) if dst is None else \
             given(dst, "dst", torch.float32, (n_tok, k, rows), dev)
+        ws_ptr, ws_bytes = None, 0
         if workspace is None:
-            workspace = x.new_empty(L.moe_b200_mxfp4_workspace_size(w.ref, n_tok, k, planes) or 1, dtype=torch.uint8)
+            ws_bytes = L.moe_b200_mxfp4_workspace_size(w.ref, n_tok, k, planes)
+            if ws_bytes:
+                workspace = x.new_empty(ws_bytes, dtype=torch.uint8)
+                ws_ptr = workspace.data_ptr()
         elif workspace.dtype != torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
             raise bad("workspace must be contiguous uint8 on the weights' device")
+        else:
+            ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel()
         check(L.moe_b200_mxfp4_mul_mat_id(
             w.ref, None if gate is None else gate.ref, _bias(bias, "bias", w), _bias(gate_bias, "gate_bias", w),
             glu_op, glu_limit, x.data_ptr(), ELEM[x.dtype], stride, per_pick, n_tok, ids.data_ptr(), k, ids_stride, planes,
-            dst.data_ptr(), workspace.data_ptr(), workspace.numel(), st))
+            dst.data_ptr(), ws_ptr, ws_bytes, st))
     return dst
 
 
