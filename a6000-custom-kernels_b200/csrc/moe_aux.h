@@ -124,9 +124,8 @@ cudaError_t launch_mx_dequantize(const uint8_t *y, int64_t n_rows, int64_t n_col
                                  int64_t stride, cudaStream_t st);
 cudaError_t launch_mx_pack(const uint8_t *src, int64_t E, int64_t rows, int64_t K, uint8_t *dst, cudaStream_t st);
 // entries per chunk, and whether the product groups the entries itself (no chunk table)
-int mx_chunk_tokens(int64_t n_tok, int64_t k, int64_t n_experts, bool glu);
-bool mx_direct(int64_t n_tok, int64_t k);
-bool mx_rows_direct(int64_t n_tok, int64_t k);   // the product alone: no preparation, no images
+int mx_chunk_tokens(int64_t n_tok, int64_t k, int64_t n_experts, int64_t K, bool glu);
+bool mx_direct(int64_t n_tok, int64_t k, int64_t n_experts, int64_t K);
 int64_t mx_max_experts();
 uint64_t mx_images_bytes(int64_t chunks, int NT, int64_t K, int planes);
 // with a.chunks, group a.ids into chunks of up to NT entries; quantise x into a.images

@@ -2066,17 +2066,16 @@ MxWs mx_ws(int64_t E, int64_t K, int64_t n_tok, int64_t k, int planes, char *bas
     MxWs w{};
     size_t off = 0;
     auto take = [&](size_t bytes) { char *p = base ? base + off : nullptr; off += align256(bytes); return p; };
-    const bool direct = moe::mx_direct(n_tok, k);
+    const bool direct = moe::mx_direct(n_tok, k, E, K);
     size_t images = 0;
     for (const bool glu : {false, true}) {
-        const int NT = moe::mx_chunk_tokens(n_tok, k, E, glu);
-        const int64_t chunks = direct ? n_tok * k : moe::mmq_max_chunks(n_tok * k, E, NT);
+        const int NT = moe::mx_chunk_tokens(n_tok, k, E, K, glu);
+        const int64_t chunks = moe::mmq_max_chunks(n_tok * k, E, NT);
         w.max_chunks = std::max(w.max_chunks, chunks);
-        if (!moe::mx_rows_direct(n_tok, k))
-            images = std::max(images, static_cast<size_t>(moe::mx_images_bytes(chunks, NT, K, planes)));
+        images = std::max(images, static_cast<size_t>(moe::mx_images_bytes(chunks, NT, K, planes)));
     }
-    w.images = reinterpret_cast<uint8_t *>(take(images));
     if (!direct) {
+        w.images = reinterpret_cast<uint8_t *>(take(images));
         w.entries = reinterpret_cast<int32_t *>(take(4 * static_cast<size_t>(n_tok * k)));
         w.where = reinterpret_cast<int2 *>(take(8 * static_cast<size_t>(n_tok * k)));
         w.experts = reinterpret_cast<int4 *>(take(16 * static_cast<size_t>(E)));
@@ -2215,9 +2214,9 @@ int moe_b200_mxfp4_mul_mat_id(const moe_mxfp4 *w, const moe_mxfp4 *gate, const f
     }
     rc = ensure_device();
     if (rc) return rc;
-    const int NT = moe::mx_chunk_tokens(n_tok, k, w->n_experts, gate != nullptr);
-    const bool direct = moe::mx_direct(n_tok, k);
-    const int64_t units = direct ? n_tok * k : moe::mmq_max_chunks(n_tok * k, w->n_experts, NT);
+    const int NT = moe::mx_chunk_tokens(n_tok, k, w->n_experts, w->K, gate != nullptr);
+    const bool direct = moe::mx_direct(n_tok, k, w->n_experts, w->K);
+    const int64_t units = std::min(n_tok * k, moe::mmq_max_chunks(n_tok * k, w->n_experts, NT));   // chunks at most
     moe::MxArgs a{};
     a.RT = static_cast<int32_t>(mx_row_tiles(w->rows));
     a.KT = static_cast<int32_t>(mx_k_tiles(w->K));
@@ -2246,12 +2245,14 @@ int moe_b200_mxfp4_mul_mat_id(const moe_mxfp4 *w, const moe_mxfp4 *gate, const f
     a.dst = dst;
     a.err = g.d_err;
     a.timeout_ns = g.timeout_ns_kernel;
-    if (moe::mx_rows_direct(n_tok, k)) {
+    if (direct) {
         a.images = nullptr;
         a.x = x;
         a.x_stride = x_row_stride;
         a.x_type = mx_elem(x_type);
         a.nb = static_cast<int32_t>(w->K / 32);
+        const uint64_t four = mx_elem(x_type) == moe::MX_F32 ? 16 : 8;
+        a.x_vec = reinterpret_cast<uintptr_t>(x) % four == 0 && static_cast<uint64_t>(x_row_stride) % 4 == 0;
     } else {
         CK(moe::launch_mx_prep(x, mx_elem(x_type), x_row_stride, per_pick ? n_tok * k : n_tok, w->K, a, NT, st));
     }

@@ -500,9 +500,8 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t saddr, uint32_t rank) {
 // (Gathering rows inside the product, 16 bytes at a time by four warps, cost
 // about 1,000 cycles per tile against the 250 that its MMAs take.)
 //
-// Up to MX_DIRECT entries nothing is grouped beforehand: an entry that is number
-// 0, NT, 2 NT, ... of its expert's entries leads a chunk, whose index is the
-// entry's own, and every CTA works that out for itself.
+// Up to MX_DIRECT entries nothing is grouped beforehand: every CTA works the
+// chunks out for itself and quantises their rows: there are no images.
 // ---------------------------------------------------------------------------
 constexpr int MXG_CTAS = 8;         // CTAs (one cluster) that group
 constexpr int MXG_THREADS = 1024;   // at most
@@ -530,9 +529,6 @@ struct MxPrep {
     int4 *experts, *chunks;
     int *err;
 };
-
-// direct form: an entry's chunk, its place there and the chunk's N, in one word
-__device__ __forceinline__ int mx_where(int chunk, int place, int N) { return (chunk << 12) | ((N / 16 - 1) << 8) | place; }
 
 __host__ __device__ constexpr int mx_group_sets(int E) { return E <= 512 ? 8 : 1; }
 
@@ -667,35 +663,10 @@ __device__ __forceinline__ int mx_id(const int32_t *ids, int64_t stride, int n_e
 // Quantise x and write the images: 4 lanes per block, 16 per K tile of a row, RUN
 // tiles in turn: what finds a row's places serves them all, and their loads are
 // in flight together.
-template <int XT, bool VEC, bool DIRECT, int RUN>
+template <int XT, bool VEC, int RUN>
 __global__ void __launch_bounds__(256, 4) mx_images_kernel(const MxPrep a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    __shared__ int where_s[MX_DIRECT];
-    __shared__ __align__(16) int id_s[MX_DIRECT];
     const int lane = threadIdx.x & 31;
-    if (DIRECT) {
-        const int t = threadIdx.x;
-        if (t < MX_DIRECT) id_s[t] = mx_id(a.ids, a.ids_stride, a.n_entries, a.k, t);
-        __syncthreads();
-        if (t < a.n_entries) {   // entry t's expert among all entries
-            const int e = id_s[t];
-            uint64_t same = 0;
-#pragma unroll
-            for (int j = 0; j < MX_DIRECT; j += 4) {
-                const int4 v = *reinterpret_cast<const int4 *>(id_s + j);
-                same |= static_cast<uint64_t>((v.x == e ? 1u : 0u) | (v.y == e ? 2u : 0u) | (v.z == e ? 4u : 0u) |
-                                              (v.w == e ? 8u : 0u)) << j;
-            }
-            const int pos = mx_before(same, t), lead = pos / a.NT * a.NT;
-            uint64_t rest = same;                     // the lead: the set bit that `lead` set bits precede
-            for (int j = 0; j < lead; ++j) rest &= rest - 1;
-            where_s[t] = e >= 0 && e < a.n_experts
-                             ? mx_where(__ffsll(static_cast<long long>(rest)) - 1, pos - lead,
-                                        mx_round16(min(__popcll(same) - lead, a.NT)))
-                             : -1;
-        }
-        __syncthreads();
-    }
     const int64_t g = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 4;   // (row, run of RUN tiles)
     const int i = threadIdx.x & 3, b = (threadIdx.x >> 2) & 3;                           // block b of a tile
     const int runs = (a.KT + RUN - 1) / RUN;
@@ -709,7 +680,7 @@ __global__ void __launch_bounds__(256, 4) mx_images_kernel(const MxPrep a) {
         raw[u] = mx_zero<XT>();
         if (row_ok && (t0 + u) * 4 + b < a.nb) raw[u] = mx_load<XT, VEC>(x + 128 * u, i);
     }
-    if (!DIRECT) asm volatile("griddepcontrol.wait;" ::: "memory");   // the grouping
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // the grouping
     // The row's destinations: lane i of the 4 serves number i, i + 4, ... Two of them are looked up
     // here, while x is on its way: behind the arithmetic the look-ups were most of the kernel's time.
     const int n_dst = row_ok ? (a.per_pick ? 1 : a.k) : 0;
@@ -717,20 +688,13 @@ __global__ void __launch_bounds__(256, 4) mx_images_kernel(const MxPrep a) {
     struct Place { int chunk, j, N; };
     auto place_of = [&](int64_t en) {
         Place d;
-        if (DIRECT) {
-            const int at = where_s[en];
-            d.chunk = at < 0 ? -1 : at >> 12;
-            d.j = at & 255;
-            d.N = (((at >> 8) & 15) + 1) * 16;
-        } else {
-            const int2 w = a.where[en];
-            const int4 ex = a.experts[max(w.x, 0)];
-            const int c = w.y / a.NT;
-            d.chunk = w.x < 0 ? -1 : ex.x + c;
-            d.j = w.y - c * a.NT;
-            d.N = mx_round16(min(a.NT, ex.y - c * a.NT));
-            if (t0 == 0 && b == 0 && w.x >= 0) a.entries[ex.z + w.y] = static_cast<int32_t>(en);
-        }
+        const int2 w = a.where[en];
+        const int4 ex = a.experts[max(w.x, 0)];
+        const int c = w.y / a.NT;
+        d.chunk = w.x < 0 ? -1 : ex.x + c;
+        d.j = w.y - c * a.NT;
+        d.N = mx_round16(min(a.NT, ex.y - c * a.NT));
+        if (t0 == 0 && b == 0 && w.x >= 0) a.entries[ex.z + w.y] = static_cast<int32_t>(en);
         return d;
     };
     const uint64_t image = mx_image_bytes(a.NT, a.KT, a.planes);
@@ -811,7 +775,7 @@ struct MxCtl {
     uint32_t tmem;
     int32_t abort, n_chunks;
     int32_t entry[ENTRIES];     // direct form: the entries grouped by expert
-    int4 chunk[ENTRIES];        // {expert, first entry, count, number of its image}
+    int4 chunk[ENTRIES];        // {expert, first entry, count, -}
 };
 
 template <int NT>
@@ -906,7 +870,7 @@ __device__ __forceinline__ void mx_direct_table(MxCtl<MX_DIRECT> &C, const MxArg
         if (x[h] >= 0) {
             C.entry[first + pos] = i;
             if (pos % NT == 0)
-                C.chunk[(at >> 16) + pos / NT] = make_int4(x[h], first + pos, min(NT, __popcll(same[h]) - pos), i);
+                C.chunk[(at >> 16) + pos / NT] = make_int4(x[h], first + pos, min(NT, __popcll(same[h]) - pos), 0);
         }
     }
     if (lane == 0) C.n_chunks = carry >> 16;
@@ -916,31 +880,46 @@ __device__ __forceinline__ void mx_direct_table(MxCtl<MX_DIRECT> &C, const MxArg
 // row of one stage (8 blocks, 4 lanes each) per warp and step, the next step's
 // values on their way meanwhile.
 struct MxRing { int s, ph, fills; };   // the ring's next stage, the parity of its use, stages used so far
-template <int NT, int XT, int PLANES, int MATS>
+template <int NT, int PLANES, int MATS>
 __device__ __forceinline__ void mx_rows(MxCtl<MX_DIRECT> &C, const MxArgs &a, int first, int count, int kt0, int n_it,
                                         MxRing &at, int warp, int lane, uint8_t *ring) {
     static_assert(mxp_tps<NT>() * MX_KT == 8 * 32, "a warp takes a row of a stage");
     constexpr int WARPS = 4 * mxp_epi<NT>(), TPS = mxp_tps<NT>();
     constexpr uint32_t PLANE = mx_image_plane(NT);
-    using T = typename MxElem<XT>::T;
+    using Raw = MxRaw<MX_F32>;                                     // of any type: f16 and bf16 fill half of it
     const int i4 = lane & 3, b = (lane >> 2) & 3, t = lane >> 4;   // block b of tile t
-    const bool vec = mx_vec_ok<XT>(a.x, a.x_stride);
     const int steps = n_it * count;
     auto load = [&](int p) {
         const int i = p / count, en = C.entry[first + p - i * count], blk = (kt0 + i * TPS) * 4 + (lane >> 2);
-        const T *x = static_cast<const T *>(a.x) + static_cast<int64_t>(a.per_pick ? en : en / a.k) * a.x_stride + blk * 32;
-        if (p >= steps || blk >= a.nb) return mx_zero<XT>();       // K padded to whole tiles with zeros
-        return vec ? mx_load<XT, true>(x, i4) : mx_load<XT, false>(x, i4);
+        const int64_t from = static_cast<int64_t>(a.per_pick ? en : en / a.k) * a.x_stride + blk * 32;
+        Raw r = mx_zero<MX_F32>();
+        if (p >= steps || blk >= a.nb) return r;                   // K padded to whole tiles with zeros
+        if (a.x_type == MX_F32) {
+            const float *x = static_cast<const float *>(a.x) + from;
+            r = a.x_vec ? mx_load<MX_F32, true>(x, i4) : mx_load<MX_F32, false>(x, i4);
+        } else {
+            const __half *x = static_cast<const __half *>(a.x) + from;   // (16 bits each; what they mean comes later)
+            const MxRaw<MX_F16> h = a.x_vec ? mx_load<MX_F16, true>(x, i4) : mx_load<MX_F16, false>(x, i4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r.w[j] = h.w[j];
+        }
+        return r;
+    };
+    auto floats = [&](const Raw &r, float (&v)[8]) {
+        if (a.x_type == MX_F32) return mx_floats<MX_F32>(r, v);
+        const MxRaw<MX_F16> f{{r.w[0], r.w[1], r.w[2], r.w[3]}};
+        const MxRaw<MX_BF16> g{{r.w[0], r.w[1], r.w[2], r.w[3]}};
+        return a.x_type == MX_F16 ? mx_floats<MX_F16>(f, v) : mx_floats<MX_BF16>(g, v);
     };
     int p = warp;
-    MxRaw<XT> next = load(p);
+    Raw next = load(p);
     for (int i = 0; i < n_it; ++i) {
         if (at.fills >= a.stages && !mx_wait_warp(C, &C.empty[at.s], at.ph ^ 1, a)) return;
         uint8_t *const image = ring + at.s * mx_stage_bytes<NT>(MATS, PLANES) + TPS * MATS * MX_TILE + t * (PLANES * PLANE);
         for (; p < (i + 1) * count; p += WARPS) {
             const int j = p - i * count;
             float v[8];
-            uint32_t top = mx_floats<XT>(next, v);
+            uint32_t top = floats(next, v);
             next = load(p + WARPS);
 #pragma unroll
             for (int pl = 0; pl < PLANES; ++pl) {
@@ -974,30 +953,31 @@ __device__ __forceinline__ void mx_rows(MxCtl<MX_DIRECT> &C, const MxArgs &a, in
 //   the rest  in groups of 4 warps that take 16 columns in turn, read the
 //             accumulators (thread = weight row), add biases, apply the GLU and
 //             store, while the next item multiplies.
-// Up to 16 tokens (NT = 16, direct) the last warps first quantise the chunk's
-// rows straight into the ring: every tile of weight rows does it again, but a
+// In the direct form (NT = 16) the last warps first quantise the chunk's rows
+// straight into the ring: every tile of weight rows does it again, but a
 // few rows are done before their weights arrive, and the call is one launch
 // without a workspace (a launch more cost 3 us of 17 for one token).
+// The direct form keeps its chunks in shared memory (a CTA for each possible
+// chunk instead, most of them empty, took 10 us for 1024 CTAs by itself).
 // With split > 1 a cluster's CTAs have one item each; their partial sums meet in
 // shared memory and are added in rank order, so results do not depend on timing.
 template <int NT, bool GLU, bool DIRECT, int PLANES>
 __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxArgs a) {
     extern __shared__ __align__(128) uint8_t ring[];
     constexpr int MATS = GLU ? 2 : 1, MXP_EPI = mxp_epi<NT>(), MXP_TPS = mxp_tps<NT>();
-    constexpr bool ROWS = DIRECT && NT == MX_ROWS_TOKENS;   // quantises x itself
     __shared__ MxCtl<DIRECT ? MX_DIRECT : 1> C;
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int rank = a.split > 1 ? static_cast<int>(cluster_rank()) : 0;
     const int item0 = blockIdx.x / a.split, item_step = gridDim.x / a.split;
 
-    if constexpr (DIRECT)   // (ids are complete before the launch that this one overlaps with; the images are not)
+    if constexpr (DIRECT)
         if (warp == 0) mx_direct_table<NT>(C, a, lane);
     if (tid == 32) {
         for (int s = 0; s < a.stages; ++s) {
             mbar_init(&C.full[s], 1);
             mbar_init(&C.empty[s], 1);
-            if (ROWS) mbar_init(&C.rows[s], 4 * MXP_EPI);
+            if (DIRECT) mbar_init(&C.rows[s], 4 * MXP_EPI);
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(&C.acc_full[s], 1);
@@ -1015,10 +995,7 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
         asm volatile("griddepcontrol.wait;" ::: "memory");
         n_items = *a.n_chunks * a.RT;
     }
-    if (item0 >= n_items) {   // nothing here; the same for every rank of the cluster
-        if (DIRECT && !ROWS) asm volatile("griddepcontrol.wait;" ::: "memory");
-        return;
-    }
+    if (item0 >= n_items) return;   // nothing here; the same for every rank of the cluster
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&C.tmem)),
                      "r"(a.tmem_cols)
@@ -1031,14 +1008,13 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
     const int stages = a.stages, acc = a.acc;
     constexpr uint32_t stage_bytes = mx_stage_bytes<NT>(MATS, planes);
     const uint32_t ring0 = smem_u32(ring);
-    struct Item { int rt, chunk, expert, count, first; };   // chunk: the number of its image
+    struct Item { int rt, chunk, expert, count, first; };
     auto item_at = [&](int item) {
         Item I;
         I.chunk = item / a.RT;
         I.rt = item - I.chunk * a.RT;
         const int4 ch = DIRECT ? C.chunk[I.chunk] : a.chunks[I.chunk];
         I.expert = ch.x; I.first = ch.y; I.count = ch.z;
-        if (DIRECT) I.chunk = ch.w;
         return I;
     };
     auto entry_of = [&](const Item &I, int j) { return DIRECT ? C.entry[I.first + j] : a.entries[I.first + j]; };
@@ -1061,12 +1037,12 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
     };
     const uint32_t on = elect_one() ? 1u : 0u;   // the lane that issues for its warp
     int early = 0;
-    if (DIRECT && warp == 0) {   // weights depend on nothing that the launch before writes: what the ring holds, at once
+    if (DIRECT && warp == 0) {   // what the ring holds, at once
         const Item I = item_at(item0);
         early = n_it < stages ? n_it : stages;
         const uint64_t pol = l2_evict_first_policy();
         for (w_stage = 0; static_cast<int>(w_stage) < early; ++w_stage)
-            fill_weights(on, weights_at(I), w_stage, ROWS ? 0u : planes * mx_image_plane(mx_round16(I.count)), pol);
+            fill_weights(on, weights_at(I), w_stage, 0u, pol);
         w_stage = 0;
         __syncwarp();
     }
@@ -1076,12 +1052,11 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
     const uint32_t tmem = __shfl_sync(0xffffffffu, C.tmem, 0);
 
     if (warp == 0) {
-        if (DIRECT && !ROWS) asm volatile("griddepcontrol.wait;" ::: "memory");
         const uint64_t pol_w = l2_evict_first_policy(), pol_x = l2_evict_last_policy();
         bool ok = true;
         for (int item = item0; item < n_items && ok; item += item_step) {
             const Item I = item_at(item);
-            const uint32_t tile = ROWS ? 0u : __shfl_sync(0xffffffffu, planes * mx_image_plane(mx_round16(I.count)), 0);
+            const uint32_t tile = DIRECT ? 0u : __shfl_sync(0xffffffffu, planes * mx_image_plane(mx_round16(I.count)), 0);
             const uint64_t wat = weights_at(I);
             const uint8_t *image = a.images + static_cast<uint64_t>(I.chunk) * mx_image_bytes(NT, a.KT, planes) +
                                    static_cast<uint64_t>(kt0) * tile;
@@ -1091,7 +1066,7 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
                     if (!ok) break;
                 }
                 if (i >= early || item != item0) fill_weights(on, wat, i, tile, pol_w);
-                if (!ROWS)
+                if (!DIRECT)
                     bulk_g2s_if(on, ring0 + w_stage * stage_bytes + MXP_TPS * MATS * MX_TILE, image, tiles_of(i) * tile,
                                 full0 + 8 * w_stage, pol_x);
                 image += MXP_TPS * tile;
@@ -1119,7 +1094,7 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
             bool ready = false;
             for (int i = 0; i < n_it && ok; ++i) {
                 if (!ready) ok = mx_wait_warp(C, &C.full[s], ph, a);
-                if (ROWS && ok) ok = mx_wait_warp(C, &C.rows[s], ph, a);
+                if (DIRECT && ok) ok = mx_wait_warp(C, &C.rows[s], ph, a);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t A = ring0 + s * stage_bytes, B = A + MXP_TPS * MATS * MX_TILE, sf = sf0 + s * sf_slot;
@@ -1172,25 +1147,23 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
         const int grp = (warp - 2) >> 2;
         const int quarter = warp & 3;                 // TMEM lanes this warp may read
         const int r = 32 * quarter + lane;            // weight row of the tile
-        MxRing at{0, 0, 0};
-        auto rows_of = [&](const Item &I) {   // (a wait that gives up: the epilogue's gives up with it)
-            if constexpr (ROWS) {
-                if (a.x_type == MX_F32) mx_rows<NT, MX_F32, PLANES, MATS>(C, a, I.first, I.count, kt0, n_it, at, warp - 2, lane, ring);
-                else if (a.x_type == MX_F16) mx_rows<NT, MX_F16, PLANES, MATS>(C, a, I.first, I.count, kt0, n_it, at, warp - 2, lane, ring);
-                else mx_rows<NT, MX_BF16, PLANES, MATS>(C, a, I.first, I.count, kt0, n_it, at, warp - 2, lane, ring);
-            }
-        };
+        MxRing at{0, 0, 0};                           // (direct form)
         constexpr int ROUNDS = (NT + 16 * MXP_EPI - 1) / (16 * MXP_EPI);
         uint32_t n = 0;
         Item next = item_at(item0);
-        if constexpr (ROWS) rows_of(next);
-        for (int item = item0; item < n_items; item += item_step, ++n) {
-            const uint32_t ab = acc == 2 ? n & 1u : 0u, aph = acc == 2 ? (n >> 1) & 1u : n & 1u;
+        // the direct form enters one item early, with the first one's rows (one place in the code:
+        // fetching a second copy took longer than what it does)
+        for (int item = DIRECT ? item0 - item_step : item0; item < n_items; item += item_step) {
             const Item I = next;
             if (item + item_step < n_items) {
                 next = item_at(item + item_step);
-                if constexpr (ROWS) rows_of(next);   // while this one multiplies
+                if constexpr (DIRECT) {   // while this one multiplies (a wait that gives up: the epilogue's gives up with it)
+                    mx_rows<NT, PLANES, MATS>(C, a, next.first, next.count, kt0, n_it, at, warp - 2, lane, ring);
+                    if (item < item0) continue;
+                }
             }
+            const uint32_t ab = acc == 2 ? n & 1u : 0u, aph = acc == 2 ? (n >> 1) & 1u : n & 1u;
+            ++n;
             const int row = I.rt * MX_M + r;
             const bool row_ok = row < a.rows;
             auto bias_of = [&](const float *b, int at) { return b[static_cast<int64_t>(I.expert) * a.rows + at]; };
@@ -1335,7 +1308,7 @@ void dequantize_t(const uint8_t *y, int64_t n_blocks, int nb, int planes, void *
         mx_dequantize_kernel<OT, false><<<grid, MXQ_THREADS, 0, st>>>(y, n_blocks, nb, planes, stride, static_cast<T *>(out));
 }
 
-template <int XT, bool VEC, bool DIRECT, int RUN>
+template <int XT, bool VEC, int RUN>
 cudaError_t images_run(const MxPrep &a, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>((a.n_rows * ((a.KT + RUN - 1) / RUN) * 16 + 255) / 256));
@@ -1345,21 +1318,19 @@ cudaError_t images_run(const MxPrep &a, cudaStream_t st) {
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // overlaps the grouping
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = DIRECT ? 0 : 1;
-    return cudaLaunchKernelEx(&cfg, mx_images_kernel<XT, VEC, DIRECT, RUN>, a);
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, mx_images_kernel<XT, VEC, RUN>, a);
 }
 
-template <int XT, bool VEC, bool DIRECT>
+template <int XT, bool VEC>
 cudaError_t images_t(const MxPrep &a, cudaStream_t st) {
-    // a small call spreads over the SMs (the direct form is one always)
-    if constexpr (DIRECT) return images_run<XT, VEC, true, 1>(a, st);
-    else return a.n_rows * a.KT < 16384 ? images_run<XT, VEC, false, 1>(a, st) : images_run<XT, VEC, false, 2>(a, st);
+    // a small call spreads over the SMs
+    return a.n_rows * a.KT < 16384 ? images_run<XT, VEC, 1>(a, st) : images_run<XT, VEC, 2>(a, st);
 }
 
 template <int XT>
 cudaError_t images_x(const MxPrep &a, cudaStream_t st) {
-    if (mx_vec_ok<XT>(a.x, a.stride)) return a.entries ? images_t<XT, true, false>(a, st) : images_t<XT, true, true>(a, st);
-    return a.entries ? images_t<XT, false, false>(a, st) : images_t<XT, false, true>(a, st);
+    return mx_vec_ok<XT>(a.x, a.stride) ? images_t<XT, true>(a, st) : images_t<XT, false>(a, st);
 }
 
 constexpr uint32_t kSmemMax = 227u * 1024u;
@@ -1416,7 +1387,7 @@ cudaError_t product_p(MxArgs &a, int64_t units, cudaStream_t st) {
     at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = DIRECT && NT == MX_ROWS_TOKENS ? 1 : 2;
+    cfg.numAttrs = DIRECT ? 1 : 2;
     return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
@@ -1458,17 +1429,22 @@ cudaError_t launch_mx_pack(const uint8_t *src, int64_t E, int64_t rows, int64_t 
     return cudaGetLastError();
 }
 
-// Entries per chunk: 64 at most in the direct form; else by the entries an
-// expert has on average.
-int mx_chunk_tokens(int64_t n_tok, int64_t k, int64_t n_experts, bool glu) {
+// The direct form, while its four quantising warps keep up with the weights. Kernel times of it and of the other
+// form's three: one token's 8 experts (K = 2048, 768 rows, GLU) 9.1 and 15.6 us, 64 tokens' one of 8 experts 13.8
+// and 15.7, 21 tokens' 3 of 8 (K = 4096, 1536 rows) 28.3 and 23.2, 16 tokens' 4 of 4 29.7 and 25.0.
+bool mx_direct(int64_t n_tok, int64_t k, int64_t n_experts, int64_t K) {
+    const int64_t n = n_tok * k, most = n < n_experts ? n : n_experts;
+    return n <= MX_DIRECT && (n == 0 || std::min<int64_t>((n + most - 1) / most, 16) * K <= MX_DIRECT_VALUES);
+}
+
+// Entries per chunk: by the entries an expert has on average.
+int mx_chunk_tokens(int64_t n_tok, int64_t k, int64_t n_experts, int64_t K, bool glu) {
     const int64_t n = n_tok * k;
-    if (n <= MX_DIRECT) return n_tok <= MX_ROWS_TOKENS ? MX_ROWS_TOKENS : 64;
+    if (mx_direct(n_tok, k, n_experts, K)) return 16;
     const int64_t per = n / (n < n_experts ? n : n_experts);
     return per <= 12 ? 16 : per <= 48 ? 64 : glu ? MXP_WIDE_GLU : MXP_WIDE;
 }
 
-bool mx_direct(int64_t n_tok, int64_t k) { return n_tok * k <= MX_DIRECT; }
-bool mx_rows_direct(int64_t n_tok, int64_t k) { return mx_direct(n_tok, k) && n_tok <= MX_ROWS_TOKENS; }
 
 int64_t mx_max_experts() { return MXG_MAX_EXPERTS; }
 
@@ -1523,18 +1499,18 @@ cudaError_t launch_mx_prep(const void *x, int xt, int64_t stride, int64_t n_rows
 
 cudaError_t launch_mx_product(MxArgs &a, int NT, int64_t units, cudaStream_t st) {
     const bool glu = a.gate != nullptr, direct = a.chunks == nullptr;
-    // few tiles: a cluster of 2, 4 or 8 CTAs shares a tile's K
+    // few tiles: a cluster of 2, 4 or 8 CTAs shares a tile's K, until every SM has work (one token's gate
+    // and up, K = 2048 and 48 tiles: 9.9 us without, 8.4, 7.9 and 10.2 by clusters of 2, 4 and 8)
     int split = 1;
     if (NT <= 64)
         while (split < 8 && units * a.RT * split < 148 && a.KT / (2 * split) >= 2) split *= 2;
     a.split = split;
-    if (NT == MX_ROWS_TOKENS) {
-        if (glu) return direct ? product_t<MX_ROWS_TOKENS, true, true>(a, units, st) : product_t<MX_ROWS_TOKENS, true, false>(a, units, st);
-        return direct ? product_t<MX_ROWS_TOKENS, false, true>(a, units, st) : product_t<MX_ROWS_TOKENS, false, false>(a, units, st);
+    if (NT == 16) {
+        if (glu) return direct ? product_t<16, true, true>(a, units, st) : product_t<16, true, false>(a, units, st);
+        return direct ? product_t<16, false, true>(a, units, st) : product_t<16, false, false>(a, units, st);
     }
     if (NT == 64) {
-        if (glu) return direct ? product_t<64, true, true>(a, units, st) : product_t<64, true, false>(a, units, st);
-        return direct ? product_t<64, false, true>(a, units, st) : product_t<64, false, false>(a, units, st);
+        return glu ? product_t<64, true, false>(a, units, st) : product_t<64, false, false>(a, units, st);
     }
     return glu ? product_t<MXP_WIDE_GLU, true, false>(a, units, st) : product_t<MXP_WIDE, false, false>(a, units, st);
 }

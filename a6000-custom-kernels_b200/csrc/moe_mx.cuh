@@ -25,8 +25,8 @@ constexpr uint32_t MX_SF = MX_M * MX_KT / 32;      // scale bytes of a tile
 constexpr uint32_t MX_TILE = MX_CODES + MX_SF;
 constexpr int MX_MAX_PLANES = 2;
 constexpr int MX_MAX_STAGES = 16;
-constexpr int MX_ROWS_TOKENS = 16;                 // tokens of a direct call whose rows the product quantises itself
-constexpr int MX_DIRECT = 64;                      // entries the product groups by itself, without a chunk table
+constexpr int64_t MX_DIRECT_VALUES = 24 * 1024;    // of a chunk's rows, in the direct form
+constexpr int MX_DIRECT = 64;                      // entries up to which the product groups and quantises by itself
 
 enum : int { MX_F32 = 0, MX_F16 = 1, MX_BF16 = 2 };   // element types of x and of the read-back
 
@@ -37,10 +37,10 @@ struct MxArgs {
     int32_t n_experts, rows, RT, KT;
     int32_t glu_op;
     float glu_limit;
-    const uint8_t *images;           // quantised rows, per chunk (mx_images_kernel); few tokens: null, and
-    const void *x;                   // the rows themselves, quantised by the product
+    const uint8_t *images;           // quantised rows, per chunk (mx_images_kernel); direct form:
+    const void *x;                   // the rows themselves
     int64_t x_stride;
-    int32_t x_type, nb;              // MX_*, blocks of a row
+    int32_t x_type, x_vec, nb;       // MX_*, whether groups of 4 values are aligned, blocks of a row
     int32_t planes, k, n_entries, per_pick;
     const int32_t *ids;              // direct form: [tok * ids_stride + pick]
     int64_t ids_stride;

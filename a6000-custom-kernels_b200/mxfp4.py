@@ -92,11 +92,21 @@ class MXFP4Weights:
         self.shape = (self.E, rows, K, self.device)
         self.desc = MoeMxfp4(self.data.data_ptr(), self.E, rows, K)
         self.ref = ctypes.byref(self.desc)
+        self._ws_bytes = {}      # workspace sizes by (n_tok, k, planes)
+
+
+def _workspace_bytes(w, *call):
+    n = w._ws_bytes.get(call)
+    if n is None:
+        if len(w._ws_bytes) >= 1024:
+            w._ws_bytes.clear()
+        n = w._ws_bytes[call] = lib().moe_b200_mxfp4_workspace_size(w.ref, *call)
+    return n
 
 
 def mxfp4_workspace_size(w, n_tok, k, planes=2):
     """Bytes of device workspace mxfp4_mul_mat_id needs (moe_b200_mxfp4_workspace_size): 0 for a few tokens."""
-    return lib().moe_b200_mxfp4_workspace_size(w.ref, n_tok, k, planes)
+    return _workspace_bytes(w, n_tok, k, planes)
 
 
 def _bias(b, name, w):
@@ -141,7 +151,7 @@ def mxfp4_mul_mat_id(w, x, ids, gate=None, bias=None, gate_bias=None, glu_op=GLU
             given(dst, "dst", torch.float32, (n_tok, k, rows), dev)
         ws_ptr, ws_bytes = None, 0
         if workspace is None:
-            ws_bytes = L.moe_b200_mxfp4_workspace_size(w.ref, n_tok, k, planes)
+            ws_bytes = _workspace_bytes(w, n_tok, k, planes)
             if ws_bytes:
                 workspace = x.new_empty(ws_bytes, dtype=torch.uint8)
                 ws_ptr = workspace.data_ptr()

@@ -543,8 +543,8 @@ int moe_b200_mxfp4_pack(const moe_tensor *src0, void *dst, size_t dst_bytes, moe
  * (MOE_DERR_BAD_ID). A NaN or an infinity in a block of x makes that row's
  * outputs NaN and no other's. n_tok may be 0.
  * Workspace: moe_b200_mxfp4_workspace_size bytes of device memory, 16-byte
- * aligned, no initialisation needed (0, and NULL does, for up to 16 tokens with
- * up to 64 picks; 0 also for arguments that the call refuses); calls that overlap on the GPU must not
+ * aligned, no initialisation needed (0, and NULL does, for a few picks; 0 also
+ * for arguments that the call refuses); calls that overlap on the GPU must not
  * share one, captured graphs included. Allocates nothing, except that the
  * first call of a process makes the device error word: not during stream
  * capture (MOE_ERR_STATE). */

@@ -148,8 +148,11 @@ def _run(pkg, cuda, W, x, ids, K, planes, dtype=torch.float32, bias=None, dst=No
     (13, 5, 16, 256, 128, False, True, torch.float32),    # 65: grouped
     (40, 1, 2, 512, 200, False, False, torch.float32),    # one pick each: more than a chunk of one expert
     (16, 4, 4, 160, 384, False, False, torch.bfloat16),   # every token picks every expert
-    (16, 2, 2, 8224, 128, False, True, torch.float16),    # a ring that is used several times over
-    (17, 3, 8, 416, 130, False, False, torch.float32),    # past the tokens whose rows the product quantises itself
+    (1, 1, 2, 24544, 128, False, True, torch.float16),    # a ring that is used several times over
+    (16, 4, 64, 8224, 128, False, True, torch.float16),   # and by several chunks
+    (16, 2, 2, 2048, 128, False, False, torch.float32),   # more rows to a chunk than the product quantises
+    (17, 3, 8, 416, 130, False, False, torch.float32),    # some experts in several chunks
+    (64, 1, 1, 352, 128, False, True, torch.bfloat16),    # one expert, four full chunks
     (100, 4, 8, 384, 250, True, True, torch.float32),     # chunks of 64
     (300, 4, 4, 256, 256, False, False, torch.float32),   # the widest chunks, an even number of row tiles
     (500, 2, 3, 640, 390, True, True, torch.bfloat16),    # and an odd one
@@ -319,7 +322,7 @@ def test_no_tokens_and_refusals(pkg, cuda):
                dict(ids=ids[:1].expand(3, 2)), dict(gate=other), dict(gate_bias=torch.zeros((4, 64), device=cuda)),
                dict(bias=torch.zeros((4, 63), device=cuda)), dict(bias=torch.zeros((4, 64), device=cuda).half()), dict(planes=3),
                dict(dst=torch.empty((3, 2, 63), device=cuda)), dict(workspace=torch.empty(16, device=cuda)),
-               dict(x=x.repeat(9, 1), ids=ids.repeat(9, 1), workspace=torch.empty(16, dtype=torch.uint8, device=cuda)),
+               dict(x=x.repeat(11, 1), ids=ids.repeat(11, 1), workspace=torch.empty(16, dtype=torch.uint8, device=cuda)),
                dict(x=torch.randn((3, 3, 64), device=cuda)), dict(gate=w, glu_op=7)):
         with pytest.raises(pkg.MoeError):
             pkg.mxfp4_mul_mat_id(**{**good, **kw})

@@ -101,7 +101,7 @@ def test_route_and_product_of_no_tokens(pkg):
     (dict(E=4097), "UNSUPPORTED"), (dict(gate=(0x1000, 4, 128, 64)), "INVALID"), (dict(gate_bias=0x1000), "INVALID"),
     (dict(gate=(0x1000, 4, 128, 128), glu=9), "INVALID"), (dict(x_type=10), "UNSUPPORTED"), (dict(planes=3), "INVALID"),
     (dict(k=0), "INVALID"), (dict(ids_stride=1), "INVALID"), (dict(x_stride=96), "INVALID"), (dict(n_tok=1 << 40), "UNSUPPORTED"),
-    (dict(x=None), "INVALID"), (dict(n_tok=17, ws_bytes=100), "INVALID"), (dict(n_tok=40, k=2, ws=None), "INVALID"),
+    (dict(x=None), "INVALID"), (dict(n_tok=33, ws_bytes=100), "INVALID"), (dict(n_tok=40, k=2, ws=None), "INVALID"),
     (dict(ws=0x1004), "INVALID"),
 ])
 def test_product_refusals(pkg, kw, code):
@@ -121,7 +121,7 @@ def test_workspace_grows_with_the_call(pkg):
     lm = _lm()
     w = lm.MoeMxfp4(0x1000, 16, 256, 512)
     size = pkg.lib().moe_b200_mxfp4_workspace_size
-    assert 0 < size(ctypes.byref(w), 17, 3, 1) < size(ctypes.byref(w), 17, 3, 2) < size(ctypes.byref(w), 300, 4, 2)
+    assert 0 < size(ctypes.byref(w), 17, 4, 1) < size(ctypes.byref(w), 17, 4, 2) < size(ctypes.byref(w), 300, 4, 2)
     assert size(ctypes.byref(w), 16, 4, 2) == 0 < size(ctypes.byref(w), 13, 5, 2)     # a few tokens need none
     assert size(ctypes.byref(w), 1, 0, 1) == 0 and size(ctypes.byref(w), 1, 4, 3) == 0 and size(None, 1, 4, 1) == 0
 
