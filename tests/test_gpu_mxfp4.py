@@ -439,3 +439,31 @@ def test_offsets_past_32_bits(pkg, cuda):
     ids = torch.randint(0, E, (n, 8), dtype=torch.int32, device=cuda)
     y = pkg.mxfp4_mul_mat_id(w, x, ids)
     assert torch.equal(y[-8:], pkg.mxfp4_mul_mat_id(w, x[-8:].contiguous(), ids[-8:].contiguous()))
+
+
+@pytest.mark.parametrize("n", [3, 120])
+def test_two_graphs_at_once(pkg, cuda, n):
+    """Two captured calls with workspaces of their own (a few tokens: none), replayed on two streams at once."""
+    rng = np.random.default_rng(n)
+    w = _weights(pkg, cuda, _experts(rng, 16, 384, 512), 512)
+    xs = [torch.randn((n, 512), device=cuda) for _ in range(2)]
+    ids = [torch.from_numpy(_ids(rng, n, 4, 16)).to(cuda) for _ in range(2)]
+    alone = [pkg.mxfp4_mul_mat_id(w, x, i, gate=w) for x, i in zip(xs, ids)]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for x, i in zip(xs, ids):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(pkg.mxfp4_mul_mat_id(w, x, i, gate=w))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(10):
+        for y in outs:
+            y.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, alone))
+    assert pkg.moe_cache.device_error() == 0
