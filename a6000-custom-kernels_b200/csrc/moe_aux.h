@@ -123,7 +123,7 @@ cudaError_t launch_mx_quantize(const void *x, int xt, int64_t stride, int64_t n_
 cudaError_t launch_mx_dequantize(const uint8_t *y, int64_t n_rows, int64_t n_cols, int planes, void *out, int ot,
                                  int64_t stride, cudaStream_t st);
 cudaError_t launch_mx_pack(const uint8_t *src, int64_t E, int64_t rows, int64_t K, uint8_t *dst, cudaStream_t st);
-// entries per chunk, and whether the product groups the entries itself (no chunk table)
+// entries per chunk, and whether the product groups and quantises by itself (no launch_mx_prep, no workspace)
 int mx_chunk_tokens(int64_t n_tok, int64_t k, int64_t n_experts, int64_t K, bool glu);
 bool mx_direct(int64_t n_tok, int64_t k, int64_t n_experts, int64_t K);
 int64_t mx_max_experts();
@@ -131,8 +131,8 @@ uint64_t mx_images_bytes(int64_t chunks, int NT, int64_t K, int planes);
 // with a.chunks, group a.ids into chunks of up to NT entries; quantise x into a.images
 cudaError_t launch_mx_prep(const void *x, int xt, int64_t stride, int64_t n_rows, int64_t K, const MxArgs &a, int NT,
                            cudaStream_t st);
-// right behind launch_mx_prep on the same stream (it overlaps its end);
-// units: entries (direct) or the largest possible number of chunks
+// right behind launch_mx_prep on the same stream (it overlaps its end), or alone with a.x;
+// units: the largest possible number of chunks
 cudaError_t launch_mx_product(MxArgs &a, int NT, int64_t units, cudaStream_t st);
 
 }  // namespace moe
