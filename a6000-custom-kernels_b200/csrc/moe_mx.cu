@@ -720,7 +720,9 @@ __global__ void __launch_bounds__(256, 4) mx_images_kernel(const MxPrep a) {
 
 #pragma unroll
     for (int u = 0; u < RUN; ++u) {
-        if (t0 + u >= a.KT) break;
+        // a tile past K is quantised too (zeros) and written nowhere: half a warp may be at its row's
+        // last, shorter run, and the shuffles below name all 32 lanes
+        const bool tile_ok = t0 + u < a.KT;
         float v[8];
         uint32_t top = mx_floats<XT>(raw[u], v);
         uint32_t w[MX_MAX_PLANES][4], sc[MX_MAX_PLANES];
@@ -751,11 +753,11 @@ __global__ void __launch_bounds__(256, 4) mx_images_kernel(const MxPrep a) {
         };
 #pragma unroll
         for (int p = 0; p < AHEAD; ++p)
-            if (ahead[p].codes) {
+            if (tile_ok && ahead[p].codes) {
                 put(ahead[p].codes, ahead[p]);
                 ahead[p].codes += a.planes * ahead[p].plane;
             }
-        for (int q = i + 4 * AHEAD; q < n_dst; q += 4) {
+        for (int q = i + 4 * AHEAD; tile_ok && q < n_dst; q += 4) {
             const Spot o = spot_of(place_of(en0 + q));
             if (o.codes) put(o.codes + static_cast<uint64_t>(u * a.planes) * o.plane, o);
         }
