@@ -1138,13 +1138,6 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
             }
             if (ok) umma_commit_if(on, acc0 + 8 * ab);
         }
-        if (!ok) {   // a wait ran out: the MMAs in flight end before the memory they use goes
-            if (elect_one()) {
-                umma_commit(&C.drain);
-                if (!mbar_wait_bounded(&C.drain, 0, drain_limit_ns(a.timeout_ns))) set_error(a.err, DERR_DRAIN);
-            }
-            __syncwarp();
-        }
     } else {
         // ---- epilogue -------------------------------------------------------
         // Thread = weight row. Group g takes columns 16 (g + EPI q), round q. All of them go to
@@ -1289,6 +1282,14 @@ __global__ void __launch_bounds__(mxp_threads<NT>()) mx_product_kernel(const MxA
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (*reinterpret_cast<volatile int32_t *>(&C.abort) != 0 && warp == 1) {
+        // whichever warp gave up, the MMAs in flight end before the memory they use goes
+        if (on) {
+            umma_commit(&C.drain);
+            if (!mbar_wait_bounded(&C.drain, 0, drain_limit_ns(a.timeout_ns))) set_error(a.err, DERR_DRAIN);
+        }
+        __syncwarp();
+    }
     if (warp == 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
 }

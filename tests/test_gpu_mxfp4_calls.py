@@ -36,3 +36,35 @@ def test_long_prompt_with_an_odd_number_of_tiles(pkg, cuda, n, K, planes):
     ref, mag = R.product(W, x, ids, planes)
     assert pkg.moe_cache.device_error() == 0
     assert (np.abs(y - ref) <= R.product_tol(mag, K, planes)).all()
+
+
+@pytest.mark.parametrize("glu", [False, True])
+@pytest.mark.parametrize("n,k,E,K,rows", [
+    (1, 4, 8, 2048, 256),      # K shared by a cluster
+    (8, 8, 64, 768, 1024),     # more tiles than CTAs
+    (40, 2, 8, 1024, 256),     # grouped: 16 columns,
+    (60, 4, 8, 512, 256),      # 64,
+    (300, 4, 8, 512, 256),     # and the widest
+])
+def test_whichever_warp_gives_up(pkg, cuda, n, k, E, K, rows, glu):
+    """Wait limits from nothing to a little less than the kernel's time, so that the copies', the MMAs' and the
+    epilogue's waits are the ones that run out: what is in flight ends before the CTA's memory goes, and the next call
+    is right."""
+    mc = pkg.moe_cache
+    rng = np.random.default_rng(n)
+    w = _weights(pkg, cuda, _experts(rng, E, rows, K), K)
+    x = torch.from_numpy(rng.normal(size=(n, K)).astype(np.float32)).to(cuda)
+    ids = torch.from_numpy(_ids(rng, n, k, E)).to(cuda)
+    kw = dict(gate=w) if glu else {}
+    good = pkg.mxfp4_mul_mat_id(w, x, ids, **kw)
+    assert mc.device_error() == 0
+    for limit in (1, 250, 500, 1000, 1500, 2000, 3000, 5000, 10000, 19000):
+        try:
+            mc.set_wait_limits(kernel_wait_ns=limit)
+            pkg.mxfp4_mul_mat_id(w, x, ids, **kw)
+            code = mc.device_error()
+        finally:
+            mc.set_wait_limits()
+        assert code in (0, mc.DERR_TIMEOUT_FULL)
+        assert torch.equal(pkg.mxfp4_mul_mat_id(w, x, ids, **kw), good)
+        assert mc.device_error() == 0
