@@ -93,7 +93,7 @@ struct Cache {
     moe::CacheTensorDev *d_reg = nullptr;   // registry array
     int reg_cap = 0;
     uint32_t *d_log = nullptr;              // [0] misses, [1] hits, [2..] miss log
-    int *d_err = nullptr;
+    int *d_err = nullptr;                   // error_word() of `device`
     uint64_t timeout_ns_ep = 2000000000ull;       // expert-parallel arrival waits
     uint64_t timeout_ns_kernel = 2000000000ull;   // waits inside the GEMV / layer / prefill kernels
     uint64_t idle_steps = 0;                // step calls with nothing tiered (no kernel launched)
@@ -205,6 +205,32 @@ uint32_t *clock_ptr() {
 }
 
 // The cache's device state on the current device, made on first use.
+// Error words by device, made on a device's first use and kept for the life of
+// the process: captured graphs hold their addresses, whatever reset() forgets.
+constexpr int kMaxDevices = 64;
+int *g_err_words[kMaxDevices] = {};
+
+// the current device's; not made while `st` is being captured
+int error_word(cudaStream_t st, int **out) {
+    int dev = 0;
+    CK(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= kMaxDevices) return fail(MOE_ERR_STATE, "device %d is past the last of %d", dev, kMaxDevices);
+    if (!g_err_words[dev]) {
+        if (st) {
+            cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+            CK(cudaStreamIsCapturing(st, &cap));
+            if (cap != cudaStreamCaptureStatusNone)
+                return fail(MOE_ERR_STATE, "the first call on a device allocates its error word: make it before capture");
+        }
+        int *word = nullptr;
+        CK(cudaMalloc(&word, sizeof(int)));
+        CK(cudaMemset(word, 0, sizeof(int)));
+        g_err_words[dev] = word;
+    }
+    *out = g_err_words[dev];
+    return MOE_OK;
+}
+
 int ensure_device() {
     int dev = 0;
     CK(cudaGetDevice(&dev));
@@ -216,10 +242,8 @@ int ensure_device() {
     CK(cudaMemset(g.dev, 0, sizeof(moe::CacheDev)));
     CK(cudaMalloc(&g.d_log, sizeof(uint32_t) * kLogWords));
     CK(cudaMemset(g.d_log, 0, sizeof(uint32_t) * kLogWords));
-    CK(cudaMalloc(&g.d_err, sizeof(int)));
-    CK(cudaMemset(g.d_err, 0, sizeof(int)));
     g.device = dev;
-    return MOE_OK;
+    return error_word(nullptr, &g.d_err);
 }
 
 // ---- seed lists -------------------------------------------------------------
@@ -477,7 +501,7 @@ void free_all() {
     cudaFree(g.dev);
     cudaFree(g.d_reg);
     cudaFree(g.d_log);
-    cudaFree(g.d_err);
+    if (g.d_err) cudaMemset(g.d_err, 0, sizeof(int));
     g.dev = nullptr;
     g.d_reg = nullptr;
     g.reg_cap = 0;
@@ -1242,11 +1266,17 @@ int moe_b200_device_error(moe_stream_t stream, int32_t *code) {
     std::lock_guard<std::recursive_mutex> lock(g_mu);
     if (code) *code = 0;
     CK(cudaStreamSynchronize(reinterpret_cast<cudaStream_t>(stream)));
-    if (!g.d_err) return MOE_OK;
-    int v = 0;
-    CK(cudaMemcpy(&v, g.d_err, sizeof(int), cudaMemcpyDeviceToHost));
-    CK(cudaMemset(g.d_err, 0, sizeof(int)));
-    if (code) *code = v;
+    // the current device's word, and that of the device which the cache's state belongs to
+    int dev = 0;
+    CK(cudaGetDevice(&dev));
+    int *const here = dev >= 0 && dev < kMaxDevices ? g_err_words[dev] : nullptr;
+    for (int *word : {here, g.d_err == here ? nullptr : g.d_err}) {
+        if (!word) continue;
+        int v = 0;
+        CK(cudaMemcpy(&v, word, sizeof(int), cudaMemcpyDeviceToHost));
+        CK(cudaMemset(word, 0, sizeof(int)));
+        if (code && !*code) *code = v;
+    }
     return MOE_OK;
 }
 
@@ -2206,13 +2236,8 @@ int moe_b200_mxfp4_mul_mat_id(const moe_mxfp4 *w, const moe_mxfp4 *gate, const f
         return fail(MOE_ERR_INVALID, "workspace too small (%zu < %zu bytes)", workspace_bytes, s.bytes);
     if (!aligned16(workspace)) return fail(MOE_ERR_INVALID, "workspace must be 16-byte aligned");
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (!g.d_err) {
-        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-        CK(cudaStreamIsCapturing(st, &cap));
-        if (cap != cudaStreamCaptureStatusNone)
-            return fail(MOE_ERR_STATE, "the first call on a device allocates the error word: make it before capture");
-    }
-    rc = ensure_device();
+    int *err = nullptr;
+    rc = error_word(st, &err);
     if (rc) return rc;
     const int NT = moe::mx_chunk_tokens(n_tok, k, w->n_experts, w->K, gate != nullptr);
     const bool direct = moe::mx_direct(n_tok, k, w->n_experts, w->K);
@@ -2243,7 +2268,7 @@ int moe_b200_mxfp4_mul_mat_id(const moe_mxfp4 *w, const moe_mxfp4 *gate, const f
     a.chunks = direct ? nullptr : s.chunks;
     a.n_chunks = s.n_chunks;
     a.dst = dst;
-    a.err = g.d_err;
+    a.err = err;
     a.timeout_ns = g.timeout_ns_kernel;
     if (direct) {
         a.images = nullptr;

@@ -166,7 +166,9 @@ int moe_b200_stats(moe_cache_stats *out);
 int moe_b200_table(const void *data, int32_t *slot_of, int32_t n_experts, int32_t *n_slots, int32_t *tensor_id);
 
 /* No counterpart in the reference: synchronise `stream`, then read and clear
- * the kernels' device-side error word (0 = none). */
+ * the kernels' device-side error word (0 = none). Every device has its own;
+ * this is the current device's and that of the cache's device. It stays where
+ * it is until the process ends: graphs captured before moe_b200_reset report there too. */
 int moe_b200_device_error(moe_stream_t stream, int32_t *code);
 
 /* No counterpart in the reference: limits of the bounded device-side waits,
@@ -545,9 +547,9 @@ int moe_b200_mxfp4_pack(const moe_tensor *src0, void *dst, size_t dst_bytes, moe
  * Workspace: moe_b200_mxfp4_workspace_size bytes of device memory, 16-byte
  * aligned, no initialisation needed (0, and NULL does, for a few picks; 0 also
  * for arguments that the call refuses); calls that overlap on the GPU must not
- * share one, captured graphs included. Allocates nothing, except that the
- * first call of a process makes the device error word: not during stream
- * capture (MOE_ERR_STATE). */
+ * share one, captured graphs included. Works on any device (the current one).
+ * Allocates nothing, except that the first call on a device makes its error
+ * word: not during stream capture (MOE_ERR_STATE). */
 size_t moe_b200_mxfp4_workspace_size(const moe_mxfp4 *w, int64_t n_tok, int64_t k, int32_t planes);
 int moe_b200_mxfp4_mul_mat_id(const moe_mxfp4 *w, const moe_mxfp4 *gate, const float *bias, const float *gate_bias,
                               int32_t glu_op, float glu_limit, const void *x, int32_t x_type, int64_t x_row_stride,

@@ -68,3 +68,32 @@ def test_whichever_warp_gives_up(pkg, cuda, n, k, E, K, rows, glu):
         assert code in (0, mc.DERR_TIMEOUT_FULL)
         assert torch.equal(pkg.mxfp4_mul_mat_id(w, x, ids, **kw), good)
         assert mc.device_error() == 0
+
+
+def test_a_graph_outlives_the_caches_reset(pkg, cuda):
+    """moe_b200_reset frees the cache's state; a captured product still reports a bad id, and a product captured
+    right after it needs no eager call first."""
+    mc = pkg.moe_cache
+    rng = np.random.default_rng(1)
+    w = _weights(pkg, cuda, _experts(rng, 4, 130, 96), 96)
+    x = torch.from_numpy(rng.normal(size=(6, 96)).astype(np.float32)).to(cuda)
+    ids = torch.zeros((6, 2), dtype=torch.int32, device=cuda)
+    mc.configure(enabled=True)
+    want = pkg.mxfp4_mul_mat_id(w, x, ids)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = pkg.mxfp4_mul_mat_id(w, x, ids)
+    mc.reset()
+    g.replay()
+    assert mc.device_error() == 0 and torch.equal(y, want)
+    ids[3, 1] = 9
+    g.replay()
+    assert mc.device_error() == mc.DERR_BAD_ID and mc.device_error() == 0
+    ids[3, 1] = 0
+    mc.reset()
+    g2 = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g2):
+        y2 = pkg.mxfp4_mul_mat_id(w, x, ids)
+    g2.replay()
+    assert mc.device_error() == 0 and torch.equal(y2, want)
