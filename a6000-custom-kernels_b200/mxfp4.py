@@ -15,6 +15,11 @@ from ._lib import MoeMxfp4, MoeTensor, check, lib
 from .moe_cache import GLU_SWIGLU, MXFP4, TSIZE, row_size
 
 
+def _version(t):
+    """What changes when something else writes t (inference tensors do not count)."""
+    return None if t.is_inference() else t._version
+
+
 def quantize_mxfp4(x, planes=1, out=None, stream=None):
     """f32 / f16 / bf16 [..., K] -> uint8 MXFP4 blocks [..., 17 K / 32], or
     [planes, ..., 17 K / 32] with planes = 2 (plane 1: what plane 0 leaves of
@@ -32,13 +37,17 @@ def quantize_mxfp4(x, planes=1, out=None, stream=None):
     with ctx:
         out = x.new_empty(shape, dtype=torch.uint8) if out is None else given(out, "out", torch.uint8, shape, x.device)
         check(lib().moe_b200_quantize_mxfp4(x.data_ptr(), ELEM[x.dtype], x.numel() // K, K, stride, planes, out.data_ptr(), st))
+    if len(shape) > 2 and shape[0] == 2:      # two planes or two matrices: only this call knows
+        out._mxfp4_planes = planes, _version(out)
     return out
 
 
 def dequantize_mxfp4(blocks, K, planes=None, dtype=torch.float32, out=None, stream=None):
-    """The values of quantize_mxfp4's blocks: [..., K] in `dtype`. `planes` says
-    whether the first dimension counts planes; None takes it for the planes
-    when `blocks` has three dimensions and the first is 2."""
+    """The values of quantize_mxfp4's blocks: [..., K] in `dtype`. `planes` = 2 says
+    that the first dimension counts planes. None reads a tensor as the call of
+    quantize_mxfp4 that returned it made it, and anything else as one plane --
+    unless it has a first dimension of 2 before the rows, which could be either:
+    that is refused."""
     if not (isinstance(blocks, torch.Tensor) and blocks.is_cuda and blocks.dtype == torch.uint8 and
             blocks.is_contiguous() and blocks.dim() >= 2):
         raise bad("blocks must be a contiguous uint8 CUDA tensor of two or more dimensions")
@@ -46,7 +55,11 @@ def dequantize_mxfp4(blocks, K, planes=None, dtype=torch.float32, out=None, stre
     if K <= 0 or K % 32 or shape[-1] != K // 32 * 17:
         raise bad("blocks' last dimension must hold K values, K a multiple of 32")
     if planes is None:
-        planes = 2 if len(shape) == 3 and shape[0] == 2 else 1
+        planes = 1
+        if len(shape) > 2 and shape[0] == 2:
+            planes, version = getattr(blocks, "_mxfp4_planes", (None, None))
+            if planes is None or version != _version(blocks):
+                raise bad("blocks with a first dimension of 2 may be two planes or two matrices: say planes=1 or planes=2")
     if planes != 1 and not (planes == 2 and len(shape) >= 3 and shape[0] == 2):
         raise bad("planes must be 1, or 2 with blocks [2, ..., bytes]")
     if dtype not in ELEM:

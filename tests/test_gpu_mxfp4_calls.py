@@ -97,3 +97,33 @@ def test_a_graph_outlives_the_caches_reset(pkg, cuda):
         y2 = pkg.mxfp4_mul_mat_id(w, x, ids)
     g2.replay()
     assert mc.device_error() == 0 and torch.equal(y2, want)
+
+
+@pytest.mark.parametrize("n", [1, 2, 3])
+def test_read_back_without_a_word_on_planes(pkg, cuda, n):
+    """What quantize_mxfp4 returned is read back as it was made, whatever its first dimension; blocks from
+    elsewhere whose first dimension could count planes are refused."""
+    x = torch.randn((n, 5, 64), device=cuda)
+    for planes in (1, 2):
+        q = pkg.quantize_mxfp4(x, planes=planes)
+        back = pkg.dequantize_mxfp4(q, 64)
+        assert back.shape == x.shape and torch.equal(back, pkg.dequantize_mxfp4(q, 64, planes=planes))
+        rows = pkg.quantize_mxfp4(x[:, 0], planes=planes)
+        assert torch.equal(pkg.dequantize_mxfp4(rows, 64), back[:, 0])
+        foreign = q.clone()
+        if foreign.shape[0] == 2:
+            with pytest.raises(pkg.MoeError, match="planes"):
+                pkg.dequantize_mxfp4(foreign, 64)
+        else:
+            assert torch.equal(pkg.dequantize_mxfp4(foreign, 64), back)
+        assert torch.equal(pkg.dequantize_mxfp4(foreign, 64, planes=planes), back)
+    buf = torch.empty((2, 5, 34), dtype=torch.uint8, device=cuda)
+    one, two = torch.randn((2, 5, 64), device=cuda), torch.randn((5, 64), device=cuda)
+    assert pkg.dequantize_mxfp4(pkg.quantize_mxfp4(one, out=buf), 64).shape == (2, 5, 64)      # one buffer, both ways
+    assert pkg.dequantize_mxfp4(pkg.quantize_mxfp4(two, planes=2, out=buf), 64).shape == (5, 64)
+    buf.copy_(pkg.quantize_mxfp4(one))                      # written by something else: says nothing any more
+    with pytest.raises(pkg.MoeError, match="planes"):
+        pkg.dequantize_mxfp4(buf, 64)
+    with torch.inference_mode():
+        assert pkg.dequantize_mxfp4(pkg.quantize_mxfp4(one), 64).shape == (2, 5, 64)
+        assert pkg.dequantize_mxfp4(pkg.quantize_mxfp4(two, planes=2), 64).shape == (5, 64)
