@@ -18,12 +18,22 @@ from .mxfp4 import MXFP4Weights, quantize_mxfp4
 from .router import Router
 
 
+def _checked_router(router, k, norm_w):
+    if router is not None:
+        if router.k != k:
+            raise bad("the router picks another number of experts than the layer has")
+        if norm_w and not router.desc.norm_w:
+            raise bad("norm_w with a router that does not normalise: the layer takes the router's weights (Router(norm_w=True))")
+    return router
+
+
 class MoELayer:
     """Expert weights live in `device` memory (HBM-resident) unless `host=True`,
     in which case they live in pinned host memory behind the tiered cache.
 
     `router` (a Router) makes tokens pick their experts as it says, through
-    decode and prefill alike; None is softmax over all experts, top-k.
+    decode and prefill alike; None is softmax over all experts, top-k. A router
+    brings its own norm_w: the layer's may repeat it, not contradict it.
     MoELayer(..., types with MXFP4 for gate, up and down) makes an MXFP4Layer."""
 
     def __new__(cls, H=None, F=None, n_experts=None, k=None, types=None, *args, **kw):
@@ -34,9 +44,7 @@ class MoELayer:
     def __init__(self, H, F, n_experts, k, types, shared=True, glu_op=GLU_SWIGLU, glu_limit=0.0, norm_w=False,
                  device="cuda", host=False, name="blk.0", seed=0, weights=None, sigma=0.02, router=None):
         self.H, self.F, self.E, self.k = H, F, n_experts, k
-        if router is not None and router.k != k:
-            raise bad("the router picks another number of experts than the layer has")
-        self.router = router
+        self.router = _checked_router(router, k, norm_w)
         self.types = dict(types)          # {"gate": t, "up": t, "down": t}
         self.glu_op, self.glu_limit, self.norm_w = glu_op, glu_limit, norm_w
         self.device = torch.device(device)
@@ -219,6 +227,7 @@ class MXFP4Layer(MoELayer):
 
     def __init__(self, H, F, n_experts, k, types, shared=True, glu_op=GLU_SWIGLU, glu_limit=0.0, norm_w=False, device="cuda",
                  host=False, name="blk.0", seed=0, weights=None, sigma=0.02, router=None, biases=None, planes=2):
+        router = _checked_router(router, k, norm_w)
         self.types = dict(types)
         if set(self.types.values()) != {MXFP4}:
             raise bad("an MXFP4 layer has gate, up and down of type MXFP4")
@@ -230,8 +239,6 @@ class MXFP4Layer(MoELayer):
         self.H, self.F, self.E, self.k, self.device, self.name = H, F, n_experts, k, device, name
         self.glu_op, self.glu_limit, self.norm_w, self.planes = glu_op, glu_limit, norm_w, planes
         self.router = Router(k, norm_w=norm_w) if router is None else router
-        if self.router.k != k:
-            raise bad("the router picks another number of experts than the layer has")
         rb = self._router_bias = self.router.bias   # (kept: the descriptor points at it)
         if rb is not None and (rb.device != device or rb.shape[0] != n_experts):
             raise bad("the router's bias must be f32 [n_experts] on the layer's device")
