@@ -33,6 +33,17 @@ def on(device, stream):
     return torch.cuda.stream(stream), stream.cuda_stream
 
 
+def keep(stream, *tensors):
+    """The memory of what a call on `stream` (a torch.cuda.Stream that the caller
+    named) uses is not handed out again before the stream has run the call.
+    Nothing for a raw handle: its owner may destroy the stream first, so the
+    caller keeps the tensors."""
+    if stream is not None and not isinstance(stream, int):
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+
+
 def dense_rows(x, name):
     """Row stride in elements of a device tensor of F32, F16 or BF16 whose last
     dimension is dense and whose rows step evenly in memory."""

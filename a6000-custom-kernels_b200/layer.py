@@ -11,7 +11,7 @@ import math
 
 import torch
 
-from ._call import ELEM, bad, dense_rows, given, on
+from ._call import ELEM, bad, dense_rows, given, keep, on
 from ._lib import MoeLayerDesc, MoeMxfp4Layer, check, lib
 from .moe_cache import GLU_SWIGLU, MXFP4, _ptr, _stream, expert_tensor, fill_quantized, row_size
 from .mxfp4 import MXFP4Weights, quantize_mxfp4
@@ -169,6 +169,8 @@ class MoELayer:
                 check(lib().moe_b200_shared_prefill(ctypes.byref(self.desc), _ptr(x), n_tok, _ptr(ys), _ptr(ws), ws.numel(), st))
             check(lib().moe_b200_combine(_ptr(y), _ptr(w), _ptr(ys), _ptr(out), n_tok, self.H, self.k, st))
             picks = None if trace is None else ids.cpu().numpy()   # (waits for the stream that wrote them)
+        if stream is not None:
+            keep(stream, x, logits, out, self.router.bias, *self.shared.values(), *(b for b in self.w.values() if b.is_cuda))
         if trace is not None:
             for r in ("gate", "up", "down"):
                 trace.record(self.desc_t[r].name.decode(), picks, self.E)
@@ -304,6 +306,9 @@ class MXFP4Layer(MoELayer):
                 check(lib().moe_b200_mxfp4_layer_run(self.ref, x.data_ptr(), ELEM[x.dtype], xs, logits.data_ptr(),
                                                      ELEM[logits.dtype], ls, out.data_ptr(), n_tok, ws.data_ptr(), ws.numel(), st))
             picks = self.routing_of(n_tok)[0].cpu().numpy() if trace is not None and n_tok else None
+        if stream is not None:
+            keep(stream, x, logits, out, self._router_bias, *self.biases.values(), *(m.data for m in self.w.values()),
+                 *(m.data for m in self.shared.values()))
         if picks is not None:
             for r in ("gate", "up", "down"):
                 trace.record(f"{self.name}.ffn_{r}_exps.weight", picks, self.E)

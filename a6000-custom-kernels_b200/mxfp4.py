@@ -4,13 +4,15 @@ the 4-bit tensor cores, and their MUL_MAT_ID (include/moe_cache_b200.h).
 Every call checks its tensors (device, type, layout; MoeError otherwise) and
 works on the tensors' device; `stream` is a torch.cuda.Stream, a raw handle, or
 None for the device's current stream. Outputs and workspaces that a call makes
-are allocated on that stream.
+are allocated on that stream. Inputs must be ready there; with a
+torch.cuda.Stream they may be dropped right behind the call, with a raw handle
+the caller keeps them until the stream has run it.
 """
 import ctypes
 
 import torch
 
-from ._call import ELEM, bad, dense_rows, given, on
+from ._call import ELEM, bad, dense_rows, given, keep, on
 from ._lib import MoeMxfp4, MoeTensor, check, lib
 from .moe_cache import GLU_SWIGLU, MXFP4, TSIZE, row_size
 
@@ -37,6 +39,7 @@ def quantize_mxfp4(x, planes=1, out=None, stream=None):
     with ctx:
         out = x.new_empty(shape, dtype=torch.uint8) if out is None else given(out, "out", torch.uint8, shape, x.device)
         check(lib().moe_b200_quantize_mxfp4(x.data_ptr(), ELEM[x.dtype], x.numel() // K, K, stride, planes, out.data_ptr(), st))
+    keep(stream, x, out)
     if len(shape) > 2 and shape[0] == 2:      # two planes or two matrices: only this call knows
         out._mxfp4_planes = planes, _version(out)
     return out
@@ -75,14 +78,15 @@ def dequantize_mxfp4(blocks, K, planes=None, dtype=torch.float32, out=None, stre
                 raise bad(f"out must be {dtype} {shape} on {blocks.device}")
         check(lib().moe_b200_dequantize_mxfp4(blocks.data_ptr(), out.numel() // K, K, planes, out.data_ptr(), ELEM[dtype],
                                               stride, st))
+    keep(stream, blocks, out)
     return out
 
 
 class MXFP4Weights:
     """The matrices of a layer's experts, laid out once for the 4-bit tensor
     cores from ggml MXFP4 blocks (uint8 [E, rows, 17 K / 32], on the device).
-    `blocks` may be dropped afterwards; calls on other streams than `stream` wait
-    for it as for any tensor made there."""
+    `blocks` may be dropped afterwards (as the inputs of every call here); calls on
+    other streams than `stream` wait for it as for any tensor made there."""
 
     def __init__(self, blocks, K, rows, stream=None):
         if not (isinstance(blocks, torch.Tensor) and blocks.is_cuda and blocks.dtype == torch.uint8 and
@@ -98,10 +102,9 @@ class MXFP4Weights:
         t.nb[0], t.nb[1], t.nb[2], t.nb[3] = TSIZE[MXFP4], rb, rb * rows, rb * rows * self.E
         ctx, st = on(self.device, stream)
         with ctx:
-            if stream is not None:
-                blocks.record_stream(torch.cuda.current_stream())
             self.data = blocks.new_empty(max(1, lib().moe_b200_mxfp4_packed_size(self.E, rows, K)))
             check(lib().moe_b200_mxfp4_pack(ctypes.byref(t), self.data.data_ptr(), self.data.numel(), st))
+        keep(stream, blocks)
         self.shape = (self.E, rows, K, self.device)
         self.desc = MoeMxfp4(self.data.data_ptr(), self.E, rows, K)
         self.ref = ctypes.byref(self.desc)
@@ -176,6 +179,8 @@ def mxfp4_mul_mat_id(w, x, ids, gate=None, bias=None, gate_bias=None, glu_op=GLU
             w.ref, None if gate is None else gate.ref, _bias(bias, "bias", w), _bias(gate_bias, "gate_bias", w),
             glu_op, glu_limit, x.data_ptr(), ELEM[x.dtype], stride, per_pick, n_tok, ids.data_ptr(), k, ids_stride, planes,
             dst.data_ptr(), ws_ptr, ws_bytes, st))
+    if stream is not None:
+        keep(stream, w.data, None if gate is None else gate.data, x, ids, bias, gate_bias, dst, workspace)
     return dst
 
 

@@ -4,7 +4,7 @@ import ctypes
 
 import torch
 
-from ._call import ELEM, bad, dense_rows, given, on
+from ._call import ELEM, bad, dense_rows, given, keep, on
 from ._lib import MoeRouter, check, lib
 
 SCORES = {"softmax": 0, "sigmoid": 1, "softmax_topk": 2}
@@ -37,7 +37,9 @@ class Router:
         return self._bias
 
     def __call__(self, logits, ids=None, weights=None, stream=None):
-        """logits f32 / f16 / bf16 [n_tok, E] -> (ids i32 [n_tok, k], weights f32 [n_tok, k])."""
+        """logits f32 / f16 / bf16 [n_tok, E] -> (ids i32 [n_tok, k], weights f32 [n_tok, k]).
+        With `stream` a torch.cuda.Stream the tensors may be dropped right behind the
+        call, with a raw handle the caller keeps them until the stream has run it."""
         stride = dense_rows(logits, "logits")
         if logits.dim() != 2:
             raise bad("logits must be [n_tok, n_experts]")
@@ -54,6 +56,7 @@ class Router:
             check(lib().moe_b200_route_experts(self.ref, logits.data_ptr(), ELEM[logits.dtype], stride,
                                                None if bias is None else bias.data_ptr(), n_tok, E, k,
                                                ids.data_ptr(), weights.data_ptr(), st))
+        keep(stream, logits, bias, ids, weights)
         return ids, weights
 
 

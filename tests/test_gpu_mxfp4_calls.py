@@ -127,3 +127,62 @@ def test_read_back_without_a_word_on_planes(pkg, cuda, n):
     with torch.inference_mode():
         assert pkg.dequantize_mxfp4(pkg.quantize_mxfp4(one), 64).shape == (2, 5, 64)
         assert pkg.dequantize_mxfp4(pkg.quantize_mxfp4(two, planes=2), 64).shape == (5, 64)
+
+
+def _behind_a_busy_stream(call, *inputs):
+    """call(stream, temporaries) on a stream that is busy; the temporaries go and their memory is taken again and
+    overwritten before the stream comes to the call."""
+    s = torch.cuda.Stream()
+    tmp = [t.clone() for t in inputs]
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(60_000_000)
+    out = call(s, tmp)
+    del tmp
+    junk = [torch.zeros_like(t) for t in inputs]
+    torch.cuda.synchronize()
+    assert all((j == 0).all() for j in junk)
+    return out
+
+
+def test_temporaries_on_another_stream(pkg, cuda):
+    """Inputs that the caller drops right behind a call on another stream keep their memory until it has run."""
+    rng = np.random.default_rng(2)
+    n, K, E, k = 2048, 1024, 8, 2
+    w = _weights(pkg, cuda, _experts(rng, E, 64, K), K)
+    x = torch.randn((n, K), device=cuda)
+    ids = torch.from_numpy(_ids(rng, n, k, E)).to(cuda)
+    bias = torch.randn((E, 64), device=cuda)
+    lg = torch.randn((n, 256), device=cuda)
+    rb = torch.randn(256, device=cuda)
+    blocks = pkg.quantize_mxfp4(x)
+    wide = torch.from_numpy(_experts(rng, 2, 512, K)).to(cuda)
+    layer = pkg.MoELayer(K, 64, E, k, {r: pkg.moe_cache.MXFP4 for r in ("gate", "up", "down")}, device=cuda)
+    l8 = torch.randn((n, E), device=cuda)
+    xs, i1 = torch.randn((4, K), device=cuda), torch.zeros((4, 1), dtype=torch.int32, device=cuda)
+    for call, inputs in (
+            (lambda s, t: pkg.quantize_mxfp4(t[0], stream=s), (x,)),
+            (lambda s, t: pkg.dequantize_mxfp4(t[0], K, stream=s), (blocks,)),
+            (lambda s, t: pkg.mxfp4_mul_mat_id(w, t[0], t[1], bias=t[2], stream=s), (x, ids, bias)),
+            (lambda s, t: pkg.mxfp4_mul_mat_id(w, t[0], t[1], gate=w, bias=t[2], gate_bias=t[2], stream=s), (x, ids, bias)),
+            (lambda s, t: pkg.route_experts(t[0], 4, bias=t[1], stream=s), (lg, rb)),
+            (lambda s, t: pkg.MXFP4Weights(t[0], K, 512, stream=s).data, (wide,)),
+            (lambda s, t: layer.decode(t[0], t[1], stream=s), (x, l8))):
+        here = call(None, inputs)
+        got = _behind_a_busy_stream(call, *inputs)
+        for a, b in zip(got, here) if isinstance(here, tuple) else ((got, here),):
+            assert torch.equal(a, b)
+    # matrices that go right behind the call that uses them
+    packed = lambda: pkg.MXFP4Weights(wide, K, 512)   # noqa: E731
+    here = pkg.mxfp4_mul_mat_id(packed(), xs, i1)
+    s = torch.cuda.Stream()
+    m = packed()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(60_000_000)
+    y = pkg.mxfp4_mul_mat_id(m, xs, i1, stream=s)
+    size = m.data.numel()
+    del m
+    junk = torch.zeros(size, dtype=torch.uint8, device=cuda)
+    torch.cuda.synchronize()
+    assert torch.equal(y, here) and not junk.any()
