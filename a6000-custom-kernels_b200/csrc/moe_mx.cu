@@ -813,15 +813,26 @@ __device__ __forceinline__ bool mx_wait_warp(MxCtl<NT> &C, uint64_t *bar, uint32
 // last place whatever g is (rounded to the nearest: 160 us instead of 137 for 32768 entries, K = 2048, 1024
 // rows); exp is expf, as __expf's error grows with |g| (135 us).
 __device__ __forceinline__ float mx_sigmoid_times(float x, float t) { return __fdividef(x, 1.0f + expf(-t)); }
+// (fminf and fmaxf would take the clamp's bound for a NaN)
+__device__ __forceinline__ float mx_min(float a, float b) {
+    float c;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+    return c;
+}
+__device__ __forceinline__ float mx_clamp(float a, float b) {   // to [-b, b]
+    float c;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(mx_min(a, b)), "f"(-b));
+    return c;
+}
 template <int OP>
 __device__ __forceinline__ float mx_glu(float g, float up, float limit) {
     if constexpr (OP == 0) return up * mx_sigmoid_times(g, g);
     else if constexpr (OP == 2) {
-        const float x = fminf(g, 7.0f);
-        return mx_sigmoid_times(x, 1.702f * x) * (fmaxf(fminf(up, 7.0f), -7.0f) + 1.0f);
+        const float x = mx_min(g, 7.0f);
+        return mx_sigmoid_times(x, 1.702f * x) * (mx_clamp(up, 7.0f) + 1.0f);
     } else if constexpr (OP == 3) {
-        const float x = fminf(g, limit);
-        return mx_sigmoid_times(x, x) * fmaxf(fminf(up, limit), -limit);
+        const float x = mx_min(g, limit);
+        return mx_sigmoid_times(x, x) * mx_clamp(up, limit);
     } else return glu_apply(OP, g, up, limit);
 }
 __device__ __forceinline__ float mx_glu_any(int op, float g, float up, float limit) {

@@ -67,3 +67,24 @@ def test_rounding_of_the_glu(pkg, cuda, op, n):
     ref = R.glu(op, g, u, LIMIT)
     units = 9 + (1 + 2 * 1.702 * np.abs(g) if op == 2 else 0)
     assert (np.abs(y - ref) <= units * 2.0 ** -24 * np.abs(ref) + (np.abs(g) + 7) * (np.abs(u) + 1) * 2.0 ** -126).all()
+
+
+@pytest.mark.parametrize("op", [0, 1, 2, 3, 4])
+@pytest.mark.parametrize("n", [1, 9, 40, 260])
+def test_nan_passes_the_clamps(pkg, cuda, op, n):
+    """A NaN of x, of a gate row or of an up row is a NaN of the outputs it enters, and of no other."""
+    rng = np.random.default_rng(n)
+    E, k, K, rows = 8, 4, 512, 130
+    x, W, ids = _exact_case(rng, n, k, E, K, rows, 4)
+    clean = _call(pkg, cuda, x, W, ids, op)
+    x[n // 2, 77] = np.nan
+    W[0][ids[0, 0], 3, 17] = 255          # a NaN scale in an up row,
+    W[1][ids[0, 0], 5, 34] = 255          # and in a gate row, of one expert
+    want = np.zeros((n, k, rows), bool)
+    want[n // 2] = True
+    hit = ids == ids[0, 0]
+    want[..., 3] |= hit
+    want[..., 5] |= hit
+    y = _call(pkg, cuda, x, W, ids, op)
+    assert np.isnan(y[want]).all()
+    np.testing.assert_array_equal(y[~want], clean[~want])
