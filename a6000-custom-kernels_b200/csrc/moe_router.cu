@@ -254,7 +254,8 @@ __global__ void __launch_bounds__(32 * RT_WARPS, NV == 8 ? 12 : 1) route_kernel(
         live = pk > logit_key(-INFINITY);
     } else {
         // Scores in 32 bits, and how far they may be off: exp and the quotient to 2 ulp, a
-        // rounding of 1 + e -- below 8e-7 of the largest score for sigmoid; for softmax also l - mx (|l - mx|
+        // rounding of 1 + e -- below 8e-7 of the largest score for sigmoid, and 2^-126 where the quotient
+        // of a denominator above 2^126 is 0; for softmax also l - mx (|l - mx|
         // e^(l - mx) <= 0.37) and up to 37 additions, below 4e-6; half an ulp of the sum with the bias.
         // Nothing where the logit is the score.
         float c[NV], big = 0.f, bigs = 0.f;
@@ -272,7 +273,7 @@ __global__ void __launch_bounds__(32 * RT_WARPS, NV == 8 ? 12 : 1) route_kernel(
         }
         big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
         bigs = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(bigs, 0.f))));
-        const float err = (a.score == ROUTE_SOFTMAX ? 4e-6f * bigs : a.score == ROUTE_SIGMOID ? 8e-7f * bigs : 0.f) +
+        const float err = (a.score == ROUTE_SOFTMAX ? 4e-6f * bigs : a.score == ROUTE_SIGMOID ? 8e-7f * bigs + 1.2e-38f : 0.f) +
                           (a.bias ? 1.2e-7f * big : 0.f);
         bool close_group = false;
         uint32_t kept = 0xffffffffu;
