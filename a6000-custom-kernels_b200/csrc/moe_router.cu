@@ -266,16 +266,17 @@ __global__ void __launch_bounds__(32 * RT_WARPS, NV == 8 ? 12 : 1) route_kernel(
             const bool has = l[j] > -INFINITY;
             c[j] = a.score == ROUTE_SOFTMAX ? (has ? expf(l[j] - mx) * rs : 0.f)
                  : a.score == ROUTE_SIGMOID ? __fdividef(1.0f, 1.0f + expf(-l[j])) : l[j];
-            if (has) bigs = fmaxf(bigs, c[j]);
+            if (has) bigs = fmaxf(bigs, fabsf(c[j]));
             if (a.bias && e < E) c[j] += a.bias[e];
             if (!has || c[j] != c[j]) c[j] = -INFINITY;
             if (fabsf(c[j]) < INFINITY) big = fmaxf(big, fabsf(c[j]));
         }
         big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
-        bigs = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(bigs, 0.f))));
+        bigs = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(bigs)));
         const float err = (a.score == ROUTE_SOFTMAX ? 4e-6f * bigs : a.score == ROUTE_SIGMOID ? 8e-7f * bigs + 1.2e-38f : 0.f) +
                           (a.bias ? 1.2e-7f * big : 0.f);
-        bool close_group = false;
+        // (sums of a bias with a score, and of two scores, that 32 bits do not hold: by 64 bits)
+        bool close_group = fmaxf(big, bigs) > 1.7e38f;
         uint32_t kept = 0xffffffffu;
         const int gsz = E / a.n_group;
         if (a.n_group > 1) {
@@ -293,7 +294,7 @@ __global__ void __launch_bounds__(32 * RT_WARPS, NV == 8 ? 12 : 1) route_kernel(
             const float worst = key_logit(__reduce_min_sync(0xffffffffu, in ? logit_key(gs) : 0xFFFFFFFFu));
             const uint32_t rest = __reduce_max_sync(0xffffffffu, mine && !in ? logit_key(gs) : 0u);
             // (a sum of two scores has twice the error and a rounding of its own)
-            if (rest > logit_key(-INFINITY)) close_group = !(worst - key_logit(rest) > 2.f * (2.f * err + 1.2e-7f * 2.f * big));
+            if (rest > logit_key(-INFINITY)) close_group |= !(worst - key_logit(rest) > 2.f * (2.f * err + 1.2e-7f * 2.f * big));
         }
         uint32_t key[NV], pk;
 #pragma unroll

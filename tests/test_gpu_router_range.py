@@ -31,3 +31,21 @@ def test_sigmoid_scores_that_underflow(pkg, cuda, dtype_step):
         _check(pkg, cuda, l, 6, score="sigmoid", n_group=8, topk_group=3, group_score=group_score)
     _check(pkg, cuda, l, 6, score="sigmoid", bias=np.zeros(64))
     _check(pkg, cuda, l, 6, score="sigmoid", bias=1e-38 * rng.random(64), n_group=4, topk_group=2)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax", "softmax_topk"])
+def test_biases_of_the_lowest_value(pkg, cuda, score):
+    """Two biases of the type's lowest value add up to less than 32 bits hold; such a group is still ahead of
+    one whose experts are all masked by -inf."""
+    low = np.finfo(np.float32).min
+    l = np.full((3, 8), -np.inf, np.float32)
+    l[0, 0], l[0, 6:] = 0.5, [0.25, 0.5]
+    l[1, 1], l[1, 4:6] = -0.5, [1.0, -1.0]
+    l[2, 0], l[2, 4:] = 0.25, 0.0
+    b = np.array([0, 0, 0, 0, low, low, low, low], np.float32)
+    for k in (1, 2, 3, 4):
+        _check(pkg, cuda, l, k, bias=b, score=score, n_group=4, topk_group=2, group_score="top2")
+    both = np.where(np.isneginf(l), np.float32(low), l)          # logits masked by the lowest value, biases too
+    for k in (2, 4):
+        _check(pkg, cuda, both, k, bias=b, score=score, n_group=4, topk_group=2, group_score="top2")
+        _check(pkg, cuda, both, k, bias=b, score=score)
