@@ -86,7 +86,7 @@ class MoELayer:
         d.H, d.F, d.n_experts, d.k = H, F, n_experts, k
         d.glu_op, d.glu_limit, d.norm_w = glu_op, glu_limit, int(norm_w)
         self.desc = d
-        self._ws = {}
+        self._ws, self._routed_key = {}, None
 
     def weight_bytes_per_token(self):
         """Expert bytes one batch-1 token streams: k routed + shared experts x 3 matrices."""
@@ -145,7 +145,8 @@ class MoELayer:
 
     def _routed(self, x, logits, out, stream, trace=None):
         """The layer with its own router: route, the experts of the picks, the
-        shared expert, combine (any n_tok >= 1; x contiguous f32)."""
+        shared expert, combine (any n_tok >= 1; x contiguous f32). Every call has buffers
+        of its own, allocated on its stream; the layer keeps the last call's."""
         n_tok, dev = x.shape[0], x.device
         if x.dtype != torch.float32 or not x.is_cuda or not x.is_contiguous() or tuple(x.shape) != (n_tok, self.H) or \
                 n_tok < 1 or tuple(logits.shape) != (n_tok, self.E) or logits.device != dev:
@@ -155,14 +156,13 @@ class MoELayer:
             out = torch.empty((n_tok, self.H), dtype=torch.float32, device=dev) if out is None else \
                 given(out, "out", torch.float32, (n_tok, self.H), dev)
             ids, w = self.router(logits)
-            kept = self._ws.get(("routed", n_tok))
-            if kept is None:
-                nbytes = lib().moe_b200_experts_prefill_workspace_size(ctypes.byref(self.desc), n_tok, self.k)
-                kept = self._ws[("routed", n_tok)] = (
-                    torch.empty(nbytes, dtype=torch.uint8, device=dev),
-                    torch.empty((n_tok, self.k, self.H), dtype=torch.float32, device=dev),
-                    torch.empty((n_tok, self.H), dtype=torch.float32, device=dev) if self.shared else None)
-            ws, y, ys = kept
+            self._ws.pop(self._routed_key, None)
+            nbytes = lib().moe_b200_experts_prefill_workspace_size(ctypes.byref(self.desc), n_tok, self.k)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            y = torch.empty((n_tok, self.k, self.H), dtype=torch.float32, device=dev)
+            ys = torch.empty((n_tok, self.H), dtype=torch.float32, device=dev) if self.shared else None
+            self._routed_key = ("routed", n_tok)
+            self._ws[self._routed_key] = ws, y, ys
             check(lib().moe_b200_experts_prefill(ctypes.byref(self.desc), _ptr(x), 0, _ptr(ids), n_tok, self.k, _ptr(y),
                                                  _ptr(ws), ws.numel(), st))
             if ys is not None:
@@ -271,7 +271,8 @@ class MXFP4Layer(MoELayer):
                 setattr(d, f"{role}_bias", b.data_ptr())
         d.k, d.glu_op, d.glu_limit, d.planes, d.router = k, glu_op, glu_limit, planes, self.router.desc
         d.router_bias = None if rb is None else rb.data_ptr()
-        self.desc, self.ref, self._ws = d, ctypes.byref(d), {}
+        self.desc, self.ref = d, ctypes.byref(d)
+        self._ws, self._ws_bytes = {}, {}       # the last call's workspace by its number of tokens; sizes
 
     def weight_bytes_per_token(self):
         """Expert bytes one batch-1 token streams: k routed + shared experts x 3 matrices."""
@@ -279,10 +280,16 @@ class MXFP4Layer(MoELayer):
         return per * self.k + sum(m.data.numel() for m in self.shared.values())
 
     def workspace(self, n_tok):
-        ws = self._ws.get(n_tok)
-        if ws is None:
-            nbytes = lib().moe_b200_mxfp4_layer_workspace_size(self.ref, n_tok)
-            ws = self._ws[n_tok] = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        """A call's workspace, from the current stream's memory (a capture's own within one): prompts come in
+        any length, so the layer keeps the last call's only."""
+        nbytes = self._ws_bytes.get(n_tok)
+        if nbytes is None:
+            if len(self._ws_bytes) >= 1024:
+                self._ws_bytes.clear()
+            nbytes = self._ws_bytes[n_tok] = lib().moe_b200_mxfp4_layer_workspace_size(self.ref, n_tok)
+        self._ws = {}
+        ws = self.w["up"].data.new_empty(nbytes)
+        self._ws = {n_tok: ws}
         return ws
 
     def fused(self, n_tok):
@@ -290,9 +297,8 @@ class MXFP4Layer(MoELayer):
 
     def decode(self, x, logits, out=None, stream=None, trace=None):
         """x f32 / f16 / bf16 [n_tok, H], logits f32 / f16 / bf16 [n_tok, E] -> out f32
-        [n_tok, H], for one token or a prompt. Uses the layer's workspace for
-        n_tok: calls for the same n_tok must not overlap on the GPU. `trace` as
-        MoELayer.decode."""
+        [n_tok, H], for one token or a prompt. Every call has a workspace of its own,
+        so calls may overlap on the GPU. `trace` as MoELayer.decode."""
         xs, ls = dense_rows(x, "x"), dense_rows(logits, "logits")
         n_tok, dev = x.shape[0], self.device
         if tuple(x.shape) != (n_tok, self.H) or tuple(logits.shape) != (n_tok, self.E) or x.device != dev or logits.device != dev:
@@ -319,7 +325,9 @@ class MXFP4Layer(MoELayer):
     def intermediates(self, n_tok):
         """Views of the last call's workspace: ids [n][k], weights [n][k], h [n][k][F]
         (GLU output), y [n][k][H] (down outputs)."""
-        ws, n, k = self._ws[n_tok], n_tok, self.k
+        ws, n, k = self._ws.get(n_tok), n_tok, self.k
+        if ws is None:
+            raise bad(f"the layer's last call was not one of {n_tok} tokens")
         out, off = [], 0
         for dt, shape in ((torch.int32, (n, k)), (torch.float32, (n, k)), (torch.float32, (n, k, self.F)),
                           (torch.float32, (n, k, self.H))):

@@ -1,0 +1,71 @@
+"""Layers with a router of their own: what they keep between calls, and what
+they answer about them."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+MX = 39
+
+
+@pytest.fixture(params=[MX, 2], ids=["mxfp4", "q4_0"])
+def layer(request, pkg, cuda):
+    pkg.moe_cache.configure(enabled=True)
+    types = {r: request.param for r in ("gate", "up", "down")}
+    yield pkg.MoELayer(256, 128, 8, 2, types, device=cuda, seed=3, router=pkg.Router(2, "sigmoid", norm_w=True))
+    pkg.moe_cache.reset()
+
+
+def _tokens(n, cuda, seed=0):
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    return torch.randn((n, 256), generator=g, device=cuda), torch.randn((n, 8), generator=g, device=cuda)
+
+
+def test_lengths_leave_no_memory_behind(pkg, cuda, layer):
+    """Prompts of many lengths: what the layer keeps is one call's, not one per length."""
+    x, lg = _tokens(512, cuda)
+    layer.prefill(x, lg)
+    torch.cuda.synchronize()
+    kept = torch.cuda.memory_allocated()
+    for n in range(100, 500, 40):
+        layer.prefill(x[:n], lg[:n])
+    layer.prefill(x, lg)
+    assert torch.cuda.memory_allocated() <= kept
+    small = torch.cuda.memory_allocated()
+    layer.decode(x[:1], lg[:1])
+    assert torch.cuda.memory_allocated() < small
+
+
+def test_calls_of_one_length_side_by_side(pkg, cuda, layer):
+    """Eager calls on two streams at once, and two captured ones replayed at once while eager calls of other
+    lengths come and go: each call has a workspace of its own."""
+    n = 96
+    data = [_tokens(n, cuda, seed) for seed in (1, 2)]
+    alone = [layer.prefill(x, lg).clone() for x, lg in data]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in data]
+    for _ in range(10):
+        got = [layer.prefill(x, lg, stream=s) for (x, lg), s in zip(data, streams)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, alone))
+    graphs, outs = [], []
+    for x, lg in data:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(layer.prefill(x, lg))
+        graphs.append(g)
+    big = _tokens(400, cuda, 3)
+    want = layer.prefill(*big).clone()
+    for i in range(10):
+        for y in outs:
+            y.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        assert torch.equal(layer.prefill(*big), want)
+        layer.prefill(big[0][: 97 + i], big[1][: 97 + i])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, alone))
+    assert pkg.moe_cache.device_error() == 0
