@@ -104,6 +104,8 @@ class MoELayer:
 
     def fused(self, n_tok):
         """True when decode() runs the layer as one fused kernel for n_tok tokens."""
+        if self.router is not None:      # decode() runs the prefill's calls
+            return False
         return bool(lib().moe_b200_layer_fused(ctypes.byref(self.desc), n_tok))
 
     def decode(self, x, logits, out=None, stream=None, trace=None):
@@ -162,7 +164,7 @@ class MoELayer:
             y = torch.empty((n_tok, self.k, self.H), dtype=torch.float32, device=dev)
             ys = torch.empty((n_tok, self.H), dtype=torch.float32, device=dev) if self.shared else None
             self._routed_key = ("routed", n_tok)
-            self._ws[self._routed_key] = ws, y, ys
+            self._ws[self._routed_key] = ws, y, ys, ids, w
             check(lib().moe_b200_experts_prefill(ctypes.byref(self.desc), _ptr(x), 0, _ptr(ids), n_tok, self.k, _ptr(y),
                                                  _ptr(ws), ws.numel(), st))
             if ys is not None:
@@ -180,7 +182,9 @@ class MoELayer:
         """Views of the last prefill's workspace (layout of moe_b200_layer_prefill):
         ids [n][k], weights [n][k], gate [n][k][F], h [n][k][F] (GLU output),
         y [n][k][H] (down outputs), then with a shared expert its gate [n][F],
-        hs [n][F] and ys [n][H]."""
+        hs [n][F] and ys [n][H]. Refused for a layer with a router, which lays its
+        calls out differently (routing_of)."""
+        self._routes_itself()
         ws = self._ws[("prefill", n_tok)]
         n, k, F, H = n_tok, self.k, self.F, self.H
         parts = [(n * k, torch.int32, (n, k)), (n * k, torch.float32, (n, k)), (n * k * F, torch.float32, (n, k, F)),
@@ -197,7 +201,9 @@ class MoELayer:
     def intermediates(self, n_tok):
         """Views of the last decode's workspace (layout of moe_b200_layer_decode):
         ids [n][k], weights [n][k], h [n][k][F] (GLU output), hs [n][F] (shared
-        GLU output), y [n][k][H] (down outputs), ys [n][H] (shared down)."""
+        GLU output), y [n][k][H] (down outputs), ys [n][H] (shared down). Refused for a
+        layer with a router, which lays its calls out differently (routing_of)."""
+        self._routes_itself()
         ws = self._ws[n_tok]
         n, k, F, H = n_tok, self.k, self.F, self.H
         # the first 256 bytes hold the fused kernels' launch epoch, then the
@@ -212,9 +218,22 @@ class MoELayer:
         return tuple(out)
 
     def routing_of(self, n_tok):
-        """(ids, weights) views of the last decode's routing in the workspace."""
+        """(ids, weights) views of the last decode's routing in the workspace; with a
+        router, the ids and weights of the last call (decode or prefill)."""
+        if self.router is not None:
+            return self._last(("routed", n_tok), n_tok)[3:]
         ids, w = self.intermediates(n_tok)[:2]
         return ids, w
+
+    def _routes_itself(self):
+        if self.router is not None:
+            raise bad("a layer with a router keeps no such workspace: routing_of has the last call's ids and weights")
+
+    def _last(self, key, n_tok):
+        kept = self._ws.get(key)
+        if kept is None:
+            raise bad(f"the layer's last call was not one of {n_tok} tokens")
+        return kept
 
 
 class MXFP4Layer(MoELayer):
@@ -325,9 +344,7 @@ class MXFP4Layer(MoELayer):
     def intermediates(self, n_tok):
         """Views of the last call's workspace: ids [n][k], weights [n][k], h [n][k][F]
         (GLU output), y [n][k][H] (down outputs)."""
-        ws, n, k = self._ws.get(n_tok), n_tok, self.k
-        if ws is None:
-            raise bad(f"the layer's last call was not one of {n_tok} tokens")
+        ws, n, k = self._last(n_tok, n_tok), n_tok, self.k
         out, off = [], 0
         for dt, shape in ((torch.int32, (n, k)), (torch.float32, (n, k)), (torch.float32, (n, k, self.F)),
                           (torch.float32, (n, k, self.H))):

@@ -69,3 +69,23 @@ def test_calls_of_one_length_side_by_side(pkg, cuda, layer):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, alone))
     assert pkg.moe_cache.device_error() == 0
+
+
+def test_what_a_routed_layer_says_of_its_last_call(pkg, cuda, layer):
+    """One launch is what the layer without a router makes; the last call's routing is its own; parts that the
+    call does not keep, or that another call has replaced, are refused."""
+    assert not layer.fused(1)
+    with pytest.raises(pkg.MoeError):
+        layer.routing_of(5)
+    x, lg = _tokens(5, cuda)
+    layer.decode(x, lg)
+    ids, w = layer.routing_of(5)
+    i, v = layer.router(lg)
+    assert torch.equal(ids, i) and torch.equal(w, v)
+    layer.prefill(*_tokens(7, cuda, 1))
+    assert layer.routing_of(7)[0].shape == (7, 2)
+    for call in (layer.routing_of, layer.intermediates, layer.prefill_intermediates):
+        with pytest.raises(pkg.MoeError):
+            call(5)
+    with pytest.raises(pkg.MoeError):
+        layer.prefill_intermediates(7)
