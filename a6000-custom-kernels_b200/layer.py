@@ -48,6 +48,8 @@ class MoELayer:
         self.types = dict(types)          # {"gate": t, "up": t, "down": t}
         self.glu_op, self.glu_limit, self.norm_w = glu_op, glu_limit, norm_w
         self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device(self.device.type, torch.cuda.current_device())
         shapes = {"gate": (F, H), "up": (F, H), "down": (H, F)}
         self.w = {}
         for i, role in enumerate(("gate", "up", "down")):
@@ -149,10 +151,10 @@ class MoELayer:
         """The layer with its own router: route, the experts of the picks, the
         shared expert, combine (any n_tok >= 1; x contiguous f32). Every call has buffers
         of its own, allocated on its stream; the layer keeps the last call's."""
-        n_tok, dev = x.shape[0], x.device
-        if x.dtype != torch.float32 or not x.is_cuda or not x.is_contiguous() or tuple(x.shape) != (n_tok, self.H) or \
+        n_tok, dev = x.shape[0], self.device
+        if x.dtype != torch.float32 or x.device != dev or not x.is_contiguous() or tuple(x.shape) != (n_tok, self.H) or \
                 n_tok < 1 or tuple(logits.shape) != (n_tok, self.E) or logits.device != dev:
-            raise bad("x must be contiguous f32 [n_tok, H] with n_tok >= 1, logits [n_tok, n_experts] on its device")
+            raise bad("x must be contiguous f32 [n_tok, H] with n_tok >= 1 and logits [n_tok, n_experts], on the layer's device")
         ctx, st = on(dev, stream)
         with ctx:
             out = torch.empty((n_tok, self.H), dtype=torch.float32, device=dev) if out is None else \

@@ -89,3 +89,13 @@ def test_what_a_routed_layer_says_of_its_last_call(pkg, cuda, layer):
             call(5)
     with pytest.raises(pkg.MoeError):
         layer.prefill_intermediates(7)
+
+
+def test_tensors_of_another_device_are_refused(pkg, cuda, layer):
+    """The experts lie on the layer's device: tokens of another one are refused (here the layer is told that it
+    lives elsewhere)."""
+    x, lg = _tokens(2, cuda)
+    layer.decode(x, lg)
+    layer.device = torch.device("cuda", 1)
+    with pytest.raises(pkg.MoeError, match="device"):
+        layer.decode(x, lg)
