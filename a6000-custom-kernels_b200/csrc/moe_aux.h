@@ -128,7 +128,7 @@ int mx_chunk_tokens(int64_t n_tok, int64_t k, int64_t n_experts, int64_t K, bool
 bool mx_direct(int64_t n_tok, int64_t k, int64_t n_experts, int64_t K);
 int64_t mx_max_experts();
 uint64_t mx_images_bytes(int64_t chunks, int NT, int64_t K, int planes);
-// with a.chunks, group a.ids into chunks of up to NT entries; quantise x into a.images
+// the form with images: group a.ids into chunks of up to NT entries, quantise x into a.images
 cudaError_t launch_mx_prep(const void *x, int xt, int64_t stride, int64_t n_rows, int64_t K, const MxArgs &a, int NT,
                            cudaStream_t st);
 // right behind launch_mx_prep on the same stream (it overlaps its end), or alone with a.x;

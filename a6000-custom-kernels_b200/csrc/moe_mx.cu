@@ -1498,28 +1498,26 @@ cudaError_t launch_mx_prep(const void *x, int xt, int64_t stride, int64_t n_rows
     p.n_experts = a.n_experts;
     p.NT = NT;
     p.err = a.err;
-    if (a.chunks) {
-        p.entries = const_cast<int32_t *>(a.entries);
-        p.n_chunks = const_cast<int32_t *>(a.n_chunks);
-        p.chunks = const_cast<int4 *>(a.chunks);
-        p.where = a.where;
-        p.experts = a.experts;
-        const size_t smem = (3 + static_cast<size_t>(mx_group_sets(a.n_experts))) * a.n_experts * sizeof(int);   // 64 KB at most
-        static bool configured[64] = {};
-        int dev = 0;
-        cudaGetDevice(&dev);
-        if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-        if (!configured[dev]) {
-            const cudaError_t e = cudaFuncSetAttribute(mx_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                       4 * MXG_MAX_EXPERTS * static_cast<int>(sizeof(int)));
-            if (e != cudaSuccess) return e;
-            configured[dev] = true;
-        }
-        const int threads = a.n_entries <= 2048 * MXG_CTAS / 8 ? 256 : a.n_entries <= 1024 * MXG_CTAS ? 512 : MXG_THREADS;
-        mx_group_kernel<<<MXG_CTAS, threads, smem, st>>>(p);
-        const cudaError_t e = cudaGetLastError();
+    p.entries = const_cast<int32_t *>(a.entries);
+    p.n_chunks = const_cast<int32_t *>(a.n_chunks);
+    p.chunks = const_cast<int4 *>(a.chunks);
+    p.where = a.where;
+    p.experts = a.experts;
+    const size_t smem = (3 + static_cast<size_t>(mx_group_sets(a.n_experts))) * a.n_experts * sizeof(int);   // 64 KB at most
+    static bool configured[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!configured[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(mx_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   4 * MXG_MAX_EXPERTS * static_cast<int>(sizeof(int)));
         if (e != cudaSuccess) return e;
+        configured[dev] = true;
     }
+    const int threads = a.n_entries <= 2048 * MXG_CTAS / 8 ? 256 : a.n_entries <= 1024 * MXG_CTAS ? 512 : MXG_THREADS;
+    mx_group_kernel<<<MXG_CTAS, threads, smem, st>>>(p);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
     if (xt == MX_F32) return images_x<MX_F32>(p, st);
     if (xt == MX_F16) return images_x<MX_F16>(p, st);
     return images_x<MX_BF16>(p, st);
