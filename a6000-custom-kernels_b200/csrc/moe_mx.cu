@@ -216,7 +216,7 @@ __device__ __forceinline__ uint32_t mx_take_block(const MxWords &m, int lane, ui
 // = the planes' values added, rounded once to OT. 4 blocks per lane quad with
 // all their loads in flight at once (one per quad left the memory waiting:
 // 2.4 TB/s); byte stores through shared memory cost a quarter of the time.
-// 16384 x 4096 bf16, one plane: 35.4 us (4.8 TB/s, bound by issue) and 28.2 us (6.0 TB/s, bound by HBM).
+// 16384 x 4096 bf16, one plane: 35.5 us (4.8 TB/s, bound by issue) and 28.1 us (6.0 TB/s, bound by HBM).
 // ---------------------------------------------------------------------------
 constexpr int MXQ_THREADS = 256;
 constexpr int MXQ_PER = 4;                                // blocks per lane quad
@@ -663,7 +663,7 @@ __device__ __forceinline__ int mx_id(const int32_t *ids, int64_t stride, int n_e
 // Quantise x and write the images: 4 lanes per block, 16 per K tile of a row, RUN
 // tiles in turn: what finds a row's places serves them all, and their loads are
 // in flight together (1 / 2 / 4 / 6 of them: 27.3, 24.3, 28.4 and 28.0 us). 16384 f32 rows of K = 768, two planes:
-// 22.5 us, bound by issue (68 % of the slots) and the last wave; 2.4 TB/s.
+// 22.2 to 24.2 us, bound by issue (69 % of the slots) and the last wave; 2.4 TB/s.
 template <int XT, bool VEC, int RUN>
 __global__ void __launch_bounds__(256, 4) mx_images_kernel(const MxPrep a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -810,8 +810,8 @@ __device__ __forceinline__ bool mx_wait_warp(MxCtl<NT> &C, uint64_t *bar, uint32
 
 // The GLU ops of glu_apply, for every form of the product: a token's results do not depend on how many
 // share its call. The epilogue is issue bound: the quotient is the approximate one, off by 2 units of its
-// last place whatever g is (rounded to the nearest: 160 us instead of 137 for 32768 entries, K = 2048, 1024
-// rows); exp is expf, as __expf's error grows with |g| (135 us).
+// last place whatever g is (rounded to the nearest: 161 us for a call of 32768 entries, K = 2048, 1024 rows,
+// instead of 138); exp is expf, as __expf's error grows with |g| (135 us).
 __device__ __forceinline__ float mx_sigmoid_times(float x, float t) { return __fdividef(x, 1.0f + expf(-t)); }
 // (fminf and fmaxf would take the clamp's bound for a NaN)
 __device__ __forceinline__ float mx_min(float a, float b) {
@@ -983,7 +983,7 @@ __device__ __forceinline__ void mx_rows(MxCtl<MX_DIRECT> &C, const MxArgs &a, in
 // few rows are done before their weights arrive, and the call is one launch
 // without a workspace (a launch more cost 3 us of 17 for one token).
 // 32768 entries of 64 experts (K = 2048, 1024 rows, gate and up, one plane): 99 us, 2.8 PFLOP/s; 16384 of 32
-// (K = 768, 2048 rows, two planes): 41 us. Bound by shared memory, then by the stores of the results.
+// (K = 768, 2048 rows, two planes): 40 us. Bound by shared memory, then by the stores of the results.
 // The direct form keeps its chunks in shared memory (a CTA for each possible
 // chunk instead, most of them empty, took 10 us for 1024 CTAs by itself).
 // With split > 1 a cluster's CTAs have one item each; their partial sums meet in
@@ -1458,21 +1458,27 @@ cudaError_t launch_mx_pack(const uint8_t *src, int64_t E, int64_t rows, int64_t 
 }
 
 // The direct form, while its four quantising warps keep up with the weights. Kernel times of it and of the other
-// form's three: one token's 8 experts (K = 2048, 768 rows, GLU) 9.1 and 15.6 us, 64 tokens' one of 8 experts 13.8
-// and 15.7, 21 tokens' 3 of 8 (K = 4096, 1536 rows) 28.3 and 23.2, 16 tokens' 4 of 4 29.7 and 25.0.
+// form's three, added up, GLU, two planes: one token's 8 of 64 experts (K = 2048, 768 rows) 8.6 and 14.9 us, 64 tokens'
+// one of 8 experts 14.5 and 15.2, 21 tokens' 3 of 8 (K = 4096, 1536 rows) 25.6 and 21.2, 16 tokens' 4 of 4 28.2 and
+// 22.9. (In a replayed graph the three overlap: 8.5 and 12.3, 14.3 and 12.6, 25.2 and 18.3, 27.8 and 19.6; a call
+// outside one pays the host for two launches more.)
 bool mx_direct(int64_t n_tok, int64_t k, int64_t n_experts, int64_t K) {
     const int64_t n = n_tok * k, most = n < n_experts ? n : n_experts;
     return n <= MX_DIRECT && (n == 0 || std::min<int64_t>((n + most - 1) / most, 16) * K <= MX_DIRECT_VALUES);
 }
 
-// Entries per chunk: by the entries an expert has on average.
+// Entries per chunk: by the entries an expert has on average. Replayed calls with 16, 64 and the widest chunks, two planes,
+// us: gate and up (64 experts, K = 2048, 768 rows) at 8 entries per expert 27.4, 26.0, 27.1, at 16 27.2, 26.9, 27.5, at 36 38.3,
+// 30.0, 31.0, at 48 45.3, 31.3, 32.2, at 64 53.1, 35.4, 34.6, at 96 72.4, 46.2, 42.0; down (32 experts, K = 768, 2048 rows) at 8
+// 11.3, 12.1, 14.2, at 12 11.9, 12.0, 14.2, at 16 13.6, 12.9, 14.8, at 48 20.0, 15.0, 16.8, at 64 23.5, 17.9, 18.6, at 96 29.2,
+// 20.0, 19.6. Picks as a skewed router makes them, at 8: 22.0, 18.7, 19.7 and 11.5, 12.1, 14.4; at 48: 47.2, 33.1, 35.1 and
+// 19.9, 15.8, 17.3.
 int mx_chunk_tokens(int64_t n_tok, int64_t k, int64_t n_experts, int64_t K, bool glu) {
     const int64_t n = n_tok * k;
     if (mx_direct(n_tok, k, n_experts, K)) return 16;
     const int64_t per = n / (n < n_experts ? n : n_experts);
     return per <= 12 ? 16 : per <= 48 ? 64 : glu ? MXP_WIDE_GLU : MXP_WIDE;
 }
-
 
 int64_t mx_max_experts() { return MXG_MAX_EXPERTS; }
 
@@ -1526,7 +1532,7 @@ cudaError_t launch_mx_prep(const void *x, int xt, int64_t stride, int64_t n_rows
 cudaError_t launch_mx_product(MxArgs &a, int NT, int64_t units, cudaStream_t st) {
     const bool glu = a.gate != nullptr, direct = a.chunks == nullptr;
     // few tiles: a cluster of 2, 4 or 8 CTAs shares a tile's K, until every SM has work (one token's gate
-    // and up, K = 2048 and 48 tiles: 9.9 us without, 8.4, 7.9 and 10.2 by clusters of 2, 4 and 8)
+    // and up, K = 2048 and 48 tiles: 10.7 us without, 8.5, 8.6 and 11.9 by clusters of 2, 4 and 8)
     int split = 1;
     if (NT <= 64)
         while (split < 8 && units * a.RT * split < 148 && a.KT / (2 * split) >= 2) split *= 2;

@@ -11,8 +11,8 @@
 // with a bound on their error: where all gaps that decide (between consecutive
 // picks, behind the last one, behind the last kept group) exceed it, the order
 // is the 64-bit one; a token with a closer pair is ranked again in 64 bits.
-// Weights are 32-bit throughout. 8192 tokens, 256 experts in 8 groups with a bias, top-8: 23.8 us with the call,
-// bound by issue; one token 12.9 us, of which the kernel is a third.
+// Weights are 32-bit throughout. 8192 tokens, 256 experts in 8 groups with a bias, top-8: 21.3 to
+// 23.5 us, bound by issue; one token 8.2 us, the latency of its serial steps (a call 12.8).
 #include "moe_aux.h"
 #include "moe_common.cuh"
 #include "moe_mx.cuh"
