@@ -238,12 +238,16 @@ int ensure_device() {
         if (dev != g.device) return fail(MOE_ERR_STATE, "moe-cache state belongs to device %d, called on %d", g.device, dev);
         return MOE_OK;
     }
+    int *err = nullptr;
+    const int rc = error_word(nullptr, &err);
+    if (rc) return rc;
     CK(cudaMalloc(&g.dev, sizeof(moe::CacheDev)));
     CK(cudaMemset(g.dev, 0, sizeof(moe::CacheDev)));
     CK(cudaMalloc(&g.d_log, sizeof(uint32_t) * kLogWords));
     CK(cudaMemset(g.d_log, 0, sizeof(uint32_t) * kLogWords));
+    g.d_err = err;
     g.device = dev;
-    return error_word(nullptr, &g.d_err);
+    return MOE_OK;
 }
 
 // ---- seed lists -------------------------------------------------------------
