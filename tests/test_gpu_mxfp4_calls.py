@@ -186,3 +186,37 @@ def test_temporaries_on_another_stream(pkg, cuda):
     junk = torch.zeros(size, dtype=torch.uint8, device=cuda)
     torch.cuda.synchronize()
     assert torch.equal(y, here) and not junk.any()
+
+
+def test_captured_with_a_forked_stream(pkg, cuda):
+    """A capture that forks: calls on another stream, on temporaries of the capturing one that go right behind them,
+    joined again; then eager calls, and the replays are right."""
+    rng = np.random.default_rng(6)
+    n, K, E, k = 300, 512, 8, 2
+    w = _weights(pkg, cuda, _experts(rng, E, 200, K), K)
+    layer = pkg.MoELayer(K, 64, E, k, {r: pkg.moe_cache.MXFP4 for r in ("gate", "up", "down")}, device=cuda)
+    x, lg = torch.randn((n, K), device=cuda), torch.randn((n, E), device=cuda)
+    ids = torch.from_numpy(_ids(rng, n, k, E)).to(cuda)
+
+    def calls(x, lg, s=None):
+        return (pkg.mxfp4_mul_mat_id(w, x, ids, gate=w, stream=s), layer.decode(x, lg, stream=s),
+                pkg.dequantize_mxfp4(pkg.quantize_mxfp4(x, planes=2, stream=s), K, stream=s))
+    want = calls(x * 2, lg * 2)
+    torch.cuda.synchronize()
+    fork = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        a, b = x * 2, lg * 2
+        fork.wait_stream(torch.cuda.current_stream())
+        out = calls(a, b, fork)
+        del a, b
+        junk = [torch.zeros((n, K), device=cuda) for _ in range(4)]
+        torch.cuda.current_stream().wait_stream(fork)
+    for _ in range(3):
+        for o in out:
+            o.zero_()
+        calls(torch.randn((n, K), device=cuda), lg)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        assert not any(j.any() for j in junk)
