@@ -37,11 +37,16 @@ def quantize_mxfp4(x, planes=1, out=None, stream=None):
         shape = (2, *shape)
     ctx, st = on(x.device, stream)
     with ctx:
-        out = x.new_empty(shape, dtype=torch.uint8) if out is None else given(out, "out", torch.uint8, shape, x.device)
+        if out is None:
+            out, known = x.new_empty(shape, dtype=torch.uint8), True
+        else:
+            known = not given(out, "out", torch.uint8, shape, x.device).is_inference()
+            if known:                          # other views of it see that it is written
+                torch.autograd.graph.increment_version(out)
         check(lib().moe_b200_quantize_mxfp4(x.data_ptr(), ELEM[x.dtype], x.numel() // K, K, stride, planes, out.data_ptr(), st))
     keep(stream, x, out)
     if len(shape) > 2 and shape[0] == 2:      # two planes or two matrices: only this call knows
-        out._mxfp4_planes = planes, _version(out)
+        out._mxfp4_planes = (planes, _version(out)) if known else (None, None)
     return out
 
 

@@ -124,6 +124,10 @@ def test_read_back_without_a_word_on_planes(pkg, cuda, n):
     buf.copy_(pkg.quantize_mxfp4(one))                      # written by something else: says nothing any more
     with pytest.raises(pkg.MoeError, match="planes"):
         pkg.dequantize_mxfp4(buf, 64)
+    pkg.quantize_mxfp4(two, planes=2, out=buf)
+    pkg.quantize_mxfp4(one, out=buf.view(2, 5, 34))         # so says a view of it
+    with pytest.raises(pkg.MoeError, match="planes"):
+        pkg.dequantize_mxfp4(buf, 64)
     with torch.inference_mode():
         assert pkg.dequantize_mxfp4(pkg.quantize_mxfp4(one), 64).shape == (2, 5, 64)
         assert pkg.dequantize_mxfp4(pkg.quantize_mxfp4(two, planes=2), 64).shape == (5, 64)
