@@ -10,4 +10,6 @@ from . import moe_cache  # noqa: F401
 from .moe_cache import *  # noqa: F401,F403
 from .router import *  # noqa: F401,F403
 from .mxfp4 import *  # noqa: F401,F403
+from .sorted import *  # noqa: F401,F403
+from .w4 import *  # noqa: F401,F403
 from .layer import MoELayer, MXFP4Layer, Stack  # noqa: F401

@@ -77,6 +77,11 @@ class MoeMxfp4Layer(ctypes.Structure):
                 ("router_bias", ctypes.c_void_p)]
 
 
+class MoeW4(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("n_experts", ctypes.c_int64), ("rows", ctypes.c_int64), ("K", ctypes.c_int64),
+                ("group", ctypes.c_int64), ("scale_type", ctypes.c_int32), ("has_zeros", ctypes.c_int32)]
+
+
 def _sources():
     out = []
     for d in (CSRC, os.path.join(REPO, "include")):
@@ -158,6 +163,15 @@ def _declare(L):
         "moe_b200_mxfp4_workspace_size": (sz, [ctypes.POINTER(MoeMxfp4), i64, i64, i32]),
         "moe_b200_mxfp4_mul_mat_id": (i32, [ctypes.POINTER(MoeMxfp4), ctypes.POINTER(MoeMxfp4), vp, vp, i32,
                                             ctypes.c_float, vp, i32, i64, i32, i64, vp, i64, i64, i32, vp, vp, sz, vp]),
+        "moe_b200_sort_by_expert": (i32, [vp, i64, i64, i64, i64, vp, vp, vp, vp, vp]),
+        "moe_b200_gather_sorted": (i32, [vp, i32, i64, i64, i64, i64, vp, vp, vp, vp]),
+        "moe_b200_combine_sorted": (i32, [vp, i32, i64, i64, i64, i64, vp, vp, vp, i64, vp, vp]),
+        "moe_b200_combine_sorted_grad": (i32, [vp, i32, i64, vp, i64, i64, i64, i64, vp, vp, vp, vp, vp, vp]),
+        "moe_b200_w4_packed_size": (sz, [ctypes.POINTER(MoeW4)]),
+        "moe_b200_w4_pack": (i32, [ctypes.POINTER(MoeW4), vp, vp, vp, vp, sz, vp]),
+        "moe_b200_w4_workspace_size": (sz, [ctypes.POINTER(MoeW4), i64, i64, i32]),
+        "moe_b200_w4_mul_mat_id": (i32, [ctypes.POINTER(MoeW4), ctypes.POINTER(MoeW4), vp, vp, i32, ctypes.c_float, vp, i32, i64,
+                                         i32, i64, vp, i64, i64, vp, vp, sz, vp]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(L, name)

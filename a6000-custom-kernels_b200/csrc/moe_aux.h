@@ -12,6 +12,7 @@ struct Layer2Args;
 struct StackArgs;
 struct MmqArgs;
 struct MxArgs;
+struct W4Args;
 
 cudaError_t launch_quantize_act(int act_type, const float *x, void *y, int64_t n_rows, int64_t n_cols,
                                 cudaStream_t st);
@@ -117,6 +118,36 @@ struct RouteArgs {
 };
 cudaError_t launch_route(RouteArgs a, int logits_type, cudaStream_t st);
 
+// Tokens sorted by expert and back (moe_sort.cu); n_entries = n_tok * k below 2^30
+constexpr int SORT_MAX_EXPERTS = 1024;
+struct SortArgs {
+    const int32_t *ids;      // [tok * ids_stride + pick]
+    int64_t ids_stride;
+    int32_t n_entries, k, n_experts;
+    int32_t *rows, *positions, *experts, *offsets;
+    int *err;
+};
+cudaError_t launch_sort(const SortArgs &a, cudaStream_t st);
+// Rows of one element type; strides in bytes; what is written is contiguous
+struct RowArgs {
+    const char *src;         // gather: x; combine: y; its gradient: d_out
+    int64_t src_stride;
+    const char *y;           // combine's gradient, with d_weights
+    int64_t y_stride;
+    const char *shared;      // combine: or null
+    int64_t shared_stride;
+    char *out;               // gradient: d_y, or null
+    int64_t row_bytes, n_tok;
+    int32_t k, n_entries;
+    const int32_t *positions, *live;   // [tok][k]; the number of sorted rows
+    const float *weights;    // [tok][k], null: 1
+    float *d_weights;        // gradient: [tok][k], or null
+    int32_t tpt, per_cta;    // set by the launchers: log2 of a token's threads, of a CTA's tokens
+};
+cudaError_t launch_gather_sorted(RowArgs a, int type, cudaStream_t st);
+cudaError_t launch_combine_sorted(RowArgs a, int type, cudaStream_t st);
+cudaError_t launch_combine_sorted_grad(const RowArgs &a, int type, cudaStream_t st);
+
 // MXFP4 (moe_mx.cu). Element types: MX_F32, MX_F16, MX_BF16; strides in elements.
 cudaError_t launch_mx_quantize(const void *x, int xt, int64_t stride, int64_t n_rows, int64_t n_cols, int planes,
                                uint8_t *y, cudaStream_t st);
@@ -134,5 +165,13 @@ cudaError_t launch_mx_prep(const void *x, int xt, int64_t stride, int64_t n_rows
 // right behind launch_mx_prep on the same stream (it overlaps its end), or alone with a.x;
 // units: the largest possible number of chunks
 cudaError_t launch_mx_product(MxArgs &a, int NT, int64_t units, cudaStream_t st);
+
+// 4-bit matrices with group scales (moe_w4.cu): their layout; the product of n_tok * k entries, after
+// launch_mmq_group into a.entries / a.chunks (chunks of w4_chunk_entries), or alone for up to W4_DIRECT of them.
+// max_chunks: the largest possible number of chunks; g32: groups of 32.
+cudaError_t launch_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, int64_t E, int64_t rows, int64_t K,
+                           int64_t groups, int64_t G, uint8_t *out, int *err, cudaStream_t st);
+int w4_chunk_entries(int64_t n_tok, int64_t k, int64_t n_experts, bool one_matrix, int x_type);
+cudaError_t launch_w4(W4Args &a, int64_t n_tok, int64_t max_chunks, bool g32, cudaStream_t st);
 
 }  // namespace moe

@@ -41,6 +41,7 @@
 #include "moe_stack.cuh"
 #include "moe_mmq.cuh"
 #include "moe_mx.cuh"
+#include "moe_w4.cuh"
 #include "moe_promote.cuh"
 
 namespace {
@@ -2395,6 +2396,295 @@ int moe_b200_mxfp4_layer_run(const moe_mxfp4_layer *layer, const void *x, int32_
     }
     if (rc) return rc;
     CK(moe::launch_combine(w.y, w.w, L.shared_up.data ? w.ys : nullptr, out, n_tok, H, k, reinterpret_cast<cudaStream_t>(stream)));
+    return MOE_OK;
+}
+
+}  // extern "C"
+
+// ---- tokens sorted by expert ----------------------------------------------------
+namespace {
+
+int sorted_check(int32_t type, int64_t n_tok, int64_t k, int64_t H) {
+    if (mx_elem(type) < 0) return fail(MOE_ERR_UNSUPPORTED, "element type must be F32, F16 or BF16");
+    if (n_tok < 0 || k < 1 || H < 1) return fail(MOE_ERR_INVALID, "need n_tok >= 0, k >= 1, H >= 1");
+    if (n_tok > (int64_t{1} << 30) / k || H > (int64_t{1} << 30)) return fail(MOE_ERR_UNSUPPORTED, "too many picks or values in one call");
+    return MOE_OK;
+}
+
+moe::RowArgs row_args(int32_t type, int64_t n_tok, int64_t k, int64_t H, const int32_t *positions) {
+    moe::RowArgs a{};
+    a.row_bytes = H * static_cast<int64_t>(elem_size(type));
+    a.n_tok = n_tok;
+    a.k = static_cast<int32_t>(k);
+    a.n_entries = static_cast<int32_t>(n_tok * k);
+    a.positions = positions;
+    return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+int moe_b200_sort_by_expert(const int32_t *ids, int64_t ids_stride, int64_t n_tok, int64_t k, int64_t n_experts,
+                            int32_t *rows, int32_t *positions, int32_t *experts, int32_t *offsets, moe_stream_t stream) {
+    std::lock_guard<std::recursive_mutex> lock(g_mu);
+    const int rc = sorted_check(MOE_TYPE_F32, n_tok, k, 1);
+    if (rc) return rc;
+    if (n_experts < 1 || n_experts > moe::SORT_MAX_EXPERTS)
+        return fail(MOE_ERR_UNSUPPORTED, "need 1 <= n_experts <= %d", moe::SORT_MAX_EXPERTS);
+    if (ids_stride < k) return fail(MOE_ERR_INVALID, "need ids_stride >= k");
+    if (!offsets || (n_tok && (!ids || !rows || !positions || !experts))) return fail(MOE_ERR_INVALID, "null argument");
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    moe::SortArgs a{};
+    const int erc = error_word(st, &a.err);
+    if (erc) return erc;
+    a.ids = ids;
+    a.ids_stride = ids_stride;
+    a.n_entries = static_cast<int32_t>(n_tok * k);
+    a.k = static_cast<int32_t>(k);
+    a.n_experts = static_cast<int32_t>(n_experts);
+    a.rows = rows;
+    a.positions = positions;
+    a.experts = experts;
+    a.offsets = offsets;
+    CK(moe::launch_sort(a, st));
+    return MOE_OK;
+}
+
+int moe_b200_gather_sorted(const void *x, int32_t type, int64_t x_row_stride, int64_t n_tok, int64_t k, int64_t H,
+                           const int32_t *positions, const int32_t *n_sorted, void *out, moe_stream_t stream) {
+    std::lock_guard<std::recursive_mutex> lock(g_mu);
+    const int rc = sorted_check(type, n_tok, k, H);
+    if (rc) return rc;
+    if (x_row_stride < H) return fail(MOE_ERR_INVALID, "row stride below H");
+    if (n_tok == 0) return MOE_OK;
+    if (!x || !positions || !n_sorted || !out || !aligned_elem(x, type) || !aligned_elem(out, type))
+        return fail(MOE_ERR_INVALID, "null or misaligned argument");
+    moe::RowArgs a = row_args(type, n_tok, k, H, positions);
+    a.src = static_cast<const char *>(x);
+    a.src_stride = x_row_stride * static_cast<int64_t>(elem_size(type));
+    a.out = static_cast<char *>(out);
+    a.live = n_sorted;
+    CK(moe::launch_gather_sorted(a, mx_elem(type), reinterpret_cast<cudaStream_t>(stream)));
+    return MOE_OK;
+}
+
+int moe_b200_combine_sorted(const void *y, int32_t type, int64_t y_row_stride, int64_t n_tok, int64_t k, int64_t H,
+                            const int32_t *positions, const float *weights, const void *shared, int64_t shared_row_stride,
+                            void *out, moe_stream_t stream) {
+    std::lock_guard<std::recursive_mutex> lock(g_mu);
+    const int rc = sorted_check(type, n_tok, k, H);
+    if (rc) return rc;
+    if (y_row_stride < H || (shared && shared_row_stride < H)) return fail(MOE_ERR_INVALID, "row stride below H");
+    if (n_tok == 0) return MOE_OK;
+    if (!y || !positions || !out || !aligned_elem(y, type) || !aligned_elem(shared, type) || !aligned_elem(out, type))
+        return fail(MOE_ERR_INVALID, "null or misaligned argument");
+    moe::RowArgs a = row_args(type, n_tok, k, H, positions);
+    a.src = static_cast<const char *>(y);
+    a.src_stride = y_row_stride * static_cast<int64_t>(elem_size(type));
+    a.weights = weights;
+    a.shared = static_cast<const char *>(shared);
+    a.shared_stride = shared_row_stride * static_cast<int64_t>(elem_size(type));
+    a.out = static_cast<char *>(out);
+    CK(moe::launch_combine_sorted(a, mx_elem(type), reinterpret_cast<cudaStream_t>(stream)));
+    return MOE_OK;
+}
+
+int moe_b200_combine_sorted_grad(const void *d_out, int32_t type, int64_t d_row_stride, const void *y, int64_t y_row_stride,
+                                 int64_t n_tok, int64_t k, int64_t H, const int32_t *positions, const int32_t *n_sorted,
+                                 const float *weights, void *d_y, float *d_weights, moe_stream_t stream) {
+    std::lock_guard<std::recursive_mutex> lock(g_mu);
+    const int rc = sorted_check(type, n_tok, k, H);
+    if (rc) return rc;
+    if (d_row_stride < H || (d_weights && y_row_stride < H)) return fail(MOE_ERR_INVALID, "row stride below H");
+    if (n_tok == 0) return MOE_OK;
+    if (!d_out || !positions || (d_y && !n_sorted) || (d_weights && !y) || !aligned_elem(d_out, type) || !aligned_elem(y, type) ||
+        !aligned_elem(d_y, type))
+        return fail(MOE_ERR_INVALID, "null or misaligned argument");
+    moe::RowArgs a = row_args(type, n_tok, k, H, positions);
+    a.src = static_cast<const char *>(d_out);
+    a.src_stride = d_row_stride * static_cast<int64_t>(elem_size(type));
+    a.y = d_weights ? static_cast<const char *>(y) : nullptr;
+    a.y_stride = y_row_stride * static_cast<int64_t>(elem_size(type));
+    a.live = n_sorted;
+    a.weights = weights;
+    a.out = static_cast<char *>(d_y);
+    a.d_weights = d_weights;
+    CK(moe::launch_combine_sorted_grad(a, mx_elem(type), reinterpret_cast<cudaStream_t>(stream)));
+    return MOE_OK;
+}
+
+}  // extern "C"
+
+// ---- 4-bit matrices with group scales ---------------------------------------------
+namespace {
+
+struct W4Shape {
+    int64_t RT, KS, groups, G;   // tiles of 16 rows, of 64 values; groups of a row, as the caller and as the layout has them
+    int gshift;
+    bool g32;
+    size_t codes, scales, zeros; // bytes of the parts
+};
+
+int w4_shape(const moe_w4 *w, W4Shape *out) {
+    if (!w) return fail(MOE_ERR_INVALID, "null argument");
+    if (w->n_experts < 1 || w->rows < 1 || w->K < 1 || w->group < 1)
+        return fail(MOE_ERR_INVALID, "need n_experts >= 1, rows >= 1, K >= 1, group >= 1");
+    if (w->n_experts > moe::SORT_MAX_EXPERTS || w->rows > (int64_t{1} << 24) || w->K > (int64_t{1} << 20))
+        return fail(MOE_ERR_UNSUPPORTED, "more than %d experts, rows above 2^24 or K above 2^20", moe::SORT_MAX_EXPERTS);
+    if (w->scale_type != MOE_TYPE_F16 && w->scale_type != MOE_TYPE_BF16)
+        return fail(MOE_ERR_UNSUPPORTED, "scales must be F16 or BF16");
+    W4Shape s{};
+    const bool row = w->group >= w->K;
+    if (!row && (w->group < 32 || (w->group & (w->group - 1))))
+        return fail(MOE_ERR_UNSUPPORTED, "group must be a power of two from 32 on, or at least K");
+    s.RT = (w->rows + moe::W4_M - 1) / moe::W4_M;
+    s.KS = (w->K + moe::W4_KT - 1) / moe::W4_KT;
+    s.groups = row ? 1 : (w->K + w->group - 1) / w->group;
+    s.g32 = !row && w->group == 32;
+    s.G = s.g32 ? 2 * s.KS : s.groups;
+    s.gshift = 31;
+    if (!row && !s.g32)
+        for (s.gshift = 0; (int64_t{moe::W4_KT} << s.gshift) < w->group;) ++s.gshift;
+    const int64_t tiles = w->n_experts * s.RT;
+    s.codes = static_cast<size_t>(tiles * s.KS) * moe::W4_TILE;
+    s.scales = static_cast<size_t>(tiles * s.G) * 32;
+    s.zeros = w->has_zeros ? static_cast<size_t>(tiles * s.G) * 16 : 0;
+    *out = s;
+    return MOE_OK;
+}
+
+moe::W4Matrix w4_matrix(const moe_w4 *w, const W4Shape &s) {
+    const uint8_t *p = static_cast<const uint8_t *>(w->data);
+    return {p, p + s.codes, w->has_zeros ? p + s.codes + s.scales : nullptr};
+}
+
+struct W4Ws {
+    int32_t *entries, *n_chunks;
+    int4 *chunks;
+    int64_t max_chunks;
+    size_t bytes;
+};
+
+W4Ws w4_ws(int64_t E, int64_t n_tok, int64_t k, int elem, bool one_matrix, char *base) {
+    W4Ws w{};
+    const int nc = moe::w4_chunk_entries(n_tok, k, E, one_matrix, elem);
+    const int64_t n = n_tok * k;
+    w.max_chunks = one_matrix ? (n + nc - 1) / nc : std::min(n, moe::mmq_max_chunks(n, E, nc));
+    if (one_matrix || n <= moe::W4_DIRECT) return w;
+    size_t off = 0;
+    auto take = [&](size_t bytes) { char *p = base ? base + off : nullptr; off += align256(bytes); return p; };
+    w.entries = reinterpret_cast<int32_t *>(take(4 * static_cast<size_t>(n)));
+    w.chunks = reinterpret_cast<int4 *>(take(16 * static_cast<size_t>(moe::mmq_max_chunks(n, E, nc))));
+    w.n_chunks = reinterpret_cast<int32_t *>(take(4));
+    w.bytes = off;
+    return w;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t moe_b200_w4_packed_size(const moe_w4 *w) {
+    W4Shape s{};
+    return w4_shape(w, &s) ? 0 : s.codes + s.scales + s.zeros;
+}
+
+int moe_b200_w4_pack(const moe_w4 *w, const void *codes, const void *scales, const void *zeros, void *dst, size_t dst_bytes,
+                     moe_stream_t stream) {
+    std::lock_guard<std::recursive_mutex> lock(g_mu);
+    W4Shape s{};
+    int rc = w4_shape(w, &s);
+    if (rc) return rc;
+    if (!codes || !scales || !dst || (w->has_zeros != 0) != (zeros != nullptr) || reinterpret_cast<uintptr_t>(scales) % 2)
+        return fail(MOE_ERR_INVALID, "null or misaligned argument, or zeros that do not go with has_zeros");
+    if (!aligned16(dst)) return fail(MOE_ERR_INVALID, "the packed matrices must be 16-byte aligned");
+    if (dst_bytes < s.codes + s.scales + s.zeros)
+        return fail(MOE_ERR_INVALID, "packed buffer too small (%zu < %zu bytes)", dst_bytes, s.codes + s.scales + s.zeros);
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    int *err = nullptr;
+    rc = error_word(st, &err);
+    if (rc) return rc;
+    CK(moe::launch_w4_pack(static_cast<const uint8_t *>(codes), scales, static_cast<const uint8_t *>(zeros), w->n_experts, w->rows,
+                           w->K, s.groups, s.G, static_cast<uint8_t *>(dst), err, st));
+    return MOE_OK;
+}
+
+size_t moe_b200_w4_workspace_size(const moe_w4 *w, int64_t n_tok, int64_t k, int32_t x_type) {
+    W4Shape s{};
+    if (w4_shape(w, &s) || n_tok < 1 || k < 1 || mx_elem(x_type) < 0 || n_tok > (int64_t{1} << 30) / k) return 0;
+    return w4_ws(w->n_experts, n_tok, k, mx_elem(x_type), false, nullptr).bytes;
+}
+
+int moe_b200_w4_mul_mat_id(const moe_w4 *w, const moe_w4 *gate, const float *bias, const float *gate_bias, int32_t glu_op,
+                           float glu_limit, const void *x, int32_t x_type, int64_t x_row_stride, int32_t x_per_pick,
+                           int64_t n_tok, const int32_t *ids, int64_t k, int64_t ids_stride, float *dst, void *workspace,
+                           size_t workspace_bytes, moe_stream_t stream) {
+    std::lock_guard<std::recursive_mutex> lock(g_mu);
+    W4Shape s{};
+    int rc = w4_shape(w, &s);
+    if (rc) return rc;
+    if (!w->data || (gate && !gate->data)) return fail(MOE_ERR_INVALID, "null argument");
+    if (!aligned16(w->data) || (gate && !aligned16(gate->data)))
+        return fail(MOE_ERR_INVALID, "the packed matrices must be 16-byte aligned");
+    if (gate && (gate->n_experts != w->n_experts || gate->rows != w->rows || gate->K != w->K || gate->group != w->group ||
+                 gate->scale_type != w->scale_type || (gate->has_zeros != 0) != (w->has_zeros != 0)))
+        return fail(MOE_ERR_INVALID, "the gate must have the up matrices' shape, group, scale type and zeros");
+    if (gate_bias && !gate) return fail(MOE_ERR_INVALID, "gate_bias without a gate");
+    if (gate && (glu_op < MOE_GLU_SWIGLU || glu_op > MOE_GLU_PRODUCT)) return fail(MOE_ERR_INVALID, "unknown glu_op %d", glu_op);
+    if (mx_elem(x_type) < 0) return fail(MOE_ERR_UNSUPPORTED, "x must be F32, F16 or BF16");
+    if (n_tok < 0 || k < 1 || x_row_stride < w->K || (ids && ids_stride < k))
+        return fail(MOE_ERR_INVALID, "need n_tok >= 0, k >= 1, ids_stride >= k, x_row_stride >= K");
+    if (n_tok > (int64_t{1} << 30) / k) return fail(MOE_ERR_UNSUPPORTED, "too many picks in one call");
+    if (n_tok == 0) return MOE_OK;
+    if (!ids && (w->n_experts != 1 || k != 1)) return fail(MOE_ERR_INVALID, "without ids there is one matrix and one pick");
+    if (!x || !dst || !aligned_elem(x, x_type)) return fail(MOE_ERR_INVALID, "null or misaligned argument");
+    const int xt = mx_elem(x_type);
+    const W4Ws ws = w4_ws(w->n_experts, n_tok, k, xt, ids == nullptr, static_cast<char *>(workspace));
+    if (ws.bytes && (!workspace || workspace_bytes < ws.bytes))
+        return fail(MOE_ERR_INVALID, "workspace too small (%zu < %zu bytes)", workspace_bytes, ws.bytes);
+    if (!aligned16(workspace)) return fail(MOE_ERR_INVALID, "workspace must be 16-byte aligned");
+    if (ws.max_chunks * s.RT > (int64_t{1} << 30)) return fail(MOE_ERR_UNSUPPORTED, "too many tiles in one call");
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    moe::W4Args a{};
+    rc = error_word(st, &a.err);
+    if (rc) return rc;
+    a.mats = gate ? 2 : 1;
+    a.w[a.mats - 1] = w4_matrix(w, s);
+    a.bias[a.mats - 1] = bias;
+    if (gate) {
+        a.w[0] = w4_matrix(gate, s);
+        a.bias[0] = gate_bias;
+    }
+    a.n_experts = static_cast<int32_t>(w->n_experts);
+    a.rows = static_cast<int32_t>(w->rows);
+    a.K = static_cast<int32_t>(w->K);
+    a.RT = static_cast<int32_t>(s.RT);
+    a.KS = static_cast<int32_t>(s.KS);
+    a.G = static_cast<int32_t>(s.G);
+    a.gshift = s.gshift;
+    a.scale_type = mx_elem(w->scale_type);
+    a.glu_op = glu_op;
+    a.glu_limit = glu_limit;
+    a.x = x;
+    a.x_stride = x_row_stride;
+    a.x_type = xt;
+    a.x_vec = aligned16(x) && x_row_stride * static_cast<int64_t>(elem_size(x_type)) % 16 == 0;
+    a.per_pick = x_per_pick != 0;
+    a.k = static_cast<int32_t>(k);
+    a.n_entries = static_cast<int32_t>(n_tok * k);
+    a.ids = ids;
+    a.ids_stride = ids_stride;
+    a.dst = dst;
+    if (ws.bytes) {
+        a.entries = ws.entries;
+        a.chunks = ws.chunks;
+        a.n_chunks = ws.n_chunks;
+        CK(moe::launch_mmq_group(ids, ids_stride, static_cast<int>(n_tok), a.k, a.n_experts,
+                                 moe::w4_chunk_entries(n_tok, k, w->n_experts, false, xt), ws.entries, ws.chunks, ws.n_chunks, a.err,
+                                 st, true));
+    }
+    CK(moe::launch_w4(a, n_tok, ws.max_chunks, s.g32, st));
     return MOE_OK;
 }
 

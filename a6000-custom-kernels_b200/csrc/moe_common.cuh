@@ -21,7 +21,7 @@ enum : int { ACT_Q8_1 = 0, ACT_CPU = 1 };
 enum : int {
     DERR_NONE = 0, DERR_BAD_ID = 1, DERR_TOO_MANY_KEYS = 2, DERR_TIMEOUT_FULL = 3,
     DERR_TIMEOUT_EMPTY = 4, DERR_TOO_MANY_SEGMENTS = 5, DERR_DRAIN = 6, DERR_GRID_BARRIER = 7,
-    DERR_TIMEOUT_TAG = 8, DERR_EP_OVERFLOW = 9,
+    DERR_TIMEOUT_TAG = 8, DERR_EP_OVERFLOW = 9, DERR_BAD_ZERO = 10,
 };
 
 template <int T> struct fmt;
@@ -363,6 +363,43 @@ __device__ __forceinline__ float glu_apply(int op, float g, float up, float limi
             return (x / (1.0f + expf(-x))) * u;
         }
         default: return up * g;
+    }
+}
+
+// The GLU ops of glu_apply, for every form of the product: a token's results do not depend on how many
+// share its call. The epilogue is issue bound: the quotient is the approximate one, off by 2 units of its
+// last place whatever g is (rounded to the nearest: 161 us for a call of 32768 entries, K = 2048, 1024 rows,
+// instead of 138); exp is expf, as __expf's error grows with |g| (135 us).
+__device__ __forceinline__ float mx_sigmoid_times(float x, float t) { return __fdividef(x, 1.0f + expf(-t)); }
+// (fminf and fmaxf would take the clamp's bound for a NaN)
+__device__ __forceinline__ float mx_min(float a, float b) {
+    float c;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+    return c;
+}
+__device__ __forceinline__ float mx_clamp(float a, float b) {   // to [-b, b]
+    float c;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(mx_min(a, b)), "f"(-b));
+    return c;
+}
+template <int OP>
+__device__ __forceinline__ float mx_glu(float g, float up, float limit) {
+    if constexpr (OP == 0) return up * mx_sigmoid_times(g, g);
+    else if constexpr (OP == 2) {
+        const float x = mx_min(g, 7.0f);
+        return mx_sigmoid_times(x, 1.702f * x) * (mx_clamp(up, 7.0f) + 1.0f);
+    } else if constexpr (OP == 3) {
+        const float x = mx_min(g, limit);
+        return mx_sigmoid_times(x, x) * mx_clamp(up, limit);
+    } else return glu_apply(OP, g, up, limit);
+}
+__device__ __forceinline__ float mx_glu_any(int op, float g, float up, float limit) {
+    switch (op) {
+        case 0: return mx_glu<0>(g, up, limit);
+        case 1: return mx_glu<1>(g, up, limit);
+        case 2: return mx_glu<2>(g, up, limit);
+        case 3: return mx_glu<3>(g, up, limit);
+        default: return mx_glu<4>(g, up, limit);
     }
 }
 

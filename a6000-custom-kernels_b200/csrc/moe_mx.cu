@@ -808,43 +808,6 @@ __device__ __forceinline__ bool mx_wait_warp(MxCtl<NT> &C, uint64_t *bar, uint32
     return __all_sync(0xffffffffu, mx_wait(C, bar, parity, a)) != 0;
 }
 
-// The GLU ops of glu_apply, for every form of the product: a token's results do not depend on how many
-// share its call. The epilogue is issue bound: the quotient is the approximate one, off by 2 units of its
-// last place whatever g is (rounded to the nearest: 161 us for a call of 32768 entries, K = 2048, 1024 rows,
-// instead of 138); exp is expf, as __expf's error grows with |g| (135 us).
-__device__ __forceinline__ float mx_sigmoid_times(float x, float t) { return __fdividef(x, 1.0f + expf(-t)); }
-// (fminf and fmaxf would take the clamp's bound for a NaN)
-__device__ __forceinline__ float mx_min(float a, float b) {
-    float c;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
-    return c;
-}
-__device__ __forceinline__ float mx_clamp(float a, float b) {   // to [-b, b]
-    float c;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(mx_min(a, b)), "f"(-b));
-    return c;
-}
-template <int OP>
-__device__ __forceinline__ float mx_glu(float g, float up, float limit) {
-    if constexpr (OP == 0) return up * mx_sigmoid_times(g, g);
-    else if constexpr (OP == 2) {
-        const float x = mx_min(g, 7.0f);
-        return mx_sigmoid_times(x, 1.702f * x) * (mx_clamp(up, 7.0f) + 1.0f);
-    } else if constexpr (OP == 3) {
-        const float x = mx_min(g, limit);
-        return mx_sigmoid_times(x, x) * mx_clamp(up, limit);
-    } else return glu_apply(OP, g, up, limit);
-}
-__device__ __forceinline__ float mx_glu_any(int op, float g, float up, float limit) {
-    switch (op) {
-        case 0: return mx_glu<0>(g, up, limit);
-        case 1: return mx_glu<1>(g, up, limit);
-        case 2: return mx_glu<2>(g, up, limit);
-        case 3: return mx_glu<3>(g, up, limit);
-        default: return mx_glu<4>(g, up, limit);
-    }
-}
-
 // The direct form's chunks, by one warp from the ids of up to 64 entries: lane l
 // looks at entries l and l + 32. Experts follow one another as they first appear.
 template <int NT>

@@ -160,7 +160,7 @@ def device_error(stream=None):
 
 
 # device error codes (moe_b200_device_error)
-DERR_BAD_ID, DERR_TIMEOUT_FULL, DERR_TIMEOUT_EMPTY, DERR_TIMEOUT_TAG, DERR_EP_OVERFLOW = 1, 3, 4, 8, 9
+DERR_BAD_ID, DERR_TIMEOUT_FULL, DERR_TIMEOUT_EMPTY, DERR_TIMEOUT_TAG, DERR_EP_OVERFLOW, DERR_BAD_ZERO = 1, 3, 4, 8, 9, 10
 
 
 def set_wait_limits(kernel_wait_ns=0, exchange_wait_ns=0):

@@ -192,6 +192,7 @@ int moe_b200_set_wait_limits(int64_t kernel_wait_ns, int64_t exchange_wait_ns);
 #define MOE_DERR_GRID_BARRIER    7
 #define MOE_DERR_TIMEOUT_TAG     8   /* a wait for another CTA's results ran out */
 #define MOE_DERR_EP_OVERFLOW     9   /* an expert-parallel receive region was full */
+#define MOE_DERR_BAD_ZERO        10  /* a zero of a 4-bit matrix above 127 */
 
 /* No counterpart in the reference: message of the last failed call. */
 const char *moe_b200_last_error(void);
@@ -582,6 +583,93 @@ size_t moe_b200_mxfp4_layer_workspace_size(const moe_mxfp4_layer *layer, int64_t
 int moe_b200_mxfp4_layer_run(const moe_mxfp4_layer *layer, const void *x, int32_t x_type, int64_t x_row_stride,
                              const void *logits, int32_t logits_type, int64_t logits_row_stride, float *out, int64_t n_tok,
                              void *workspace, size_t workspace_bytes, moe_stream_t stream);
+
+/* ---- tokens sorted by expert, and back (no counterpart in the reference) ----
+ * For experts that run outside this library, or on rows of their own: the
+ * (token, pick) entries i = t * k + j in the order of their experts, the tokens'
+ * rows in that order, and the weighted sum of the sorted rows back into the
+ * tokens, with the gradients of both. An entry has a sorted row when its id is in
+ * [0, n_experts); -1 marks an empty slot, any other id counts as one and sets the
+ * device error word (MOE_DERR_BAD_ID). Elements are MOE_TYPE_F32, _F16 or _BF16,
+ * row strides in elements, aligned to their size. Nothing is allocated, except that
+ * moe_b200_sort_by_expert's first call on a device makes its error word (not during
+ * capture: MOE_ERR_STATE); calls may overlap. n_tok may be 0, n_tok * k <= 2^30. */
+
+/* The order: entries by (expert, i), n_experts <= 1024. rows[p] = the entry of sorted
+ * row p and experts[p] its expert, -1 behind the last; positions[t][j] = the sorted
+ * row of an entry, -1 for none; offsets[e] = entries of experts below e, so
+ * offsets[n_experts] is the number of sorted rows. All int32: rows and experts
+ * [n_tok * k], positions [n_tok][k], offsets [n_experts + 1]; ids' rows ids_stride apart. */
+int moe_b200_sort_by_expert(const int32_t *ids, int64_t ids_stride, int64_t n_tok, int64_t k, int64_t n_experts,
+                            int32_t *rows, int32_t *positions, int32_t *experts, int32_t *offsets, moe_stream_t stream);
+
+/* out[p] = x's row of the token of sorted row p, zeros behind the last: out
+ * [n_tok * k][H]. n_sorted: device address of the number of sorted rows
+ * (&offsets[n_experts]). */
+int moe_b200_gather_sorted(const void *x, int32_t type, int64_t x_row_stride, int64_t n_tok, int64_t k, int64_t H,
+                           const int32_t *positions, const int32_t *n_sorted, void *out, moe_stream_t stream);
+
+/* out[t] = sum over the picks j, in order, of weights[t][j] * y[positions[t][j]], plus
+ * shared[t] (or NULL), in 32 bits, rounded once. weights f32 [n_tok][k] or NULL (all 1;
+ * the gradient of moe_b200_gather_sorted is this of the rows' gradients). Picks without
+ * a sorted row add nothing, whatever weights holds for them. out [n_tok][H]. */
+int moe_b200_combine_sorted(const void *y, int32_t type, int64_t y_row_stride, int64_t n_tok, int64_t k, int64_t H,
+                            const int32_t *positions, const float *weights, const void *shared, int64_t shared_row_stride,
+                            void *out, moe_stream_t stream);
+
+/* Its gradients: d_y[positions[t][j]] = weights[t][j] * d_out[t] and zeros behind the last
+ * sorted row ([n_tok * k][H], or NULL), d_weights[t][j] = <d_out[t], y[positions[t][j]]>
+ * in 32 bits, 0 for a pick without a row (f32 [n_tok][k], or NULL: y is not read then). */
+int moe_b200_combine_sorted_grad(const void *d_out, int32_t type, int64_t d_row_stride, const void *y, int64_t y_row_stride,
+                                 int64_t n_tok, int64_t k, int64_t H, const int32_t *positions, const int32_t *n_sorted,
+                                 const float *weights, void *d_y, float *d_weights, moe_stream_t stream);
+
+/* ---- 4-bit matrices with group scales (no counterpart in the reference) ------
+ * value[r][c] = scale[r][c / group] * (code[r][c] - zero[r][c / group]), codes 0..15,
+ * zeros 0..127 (8 where there are none): the integer 4-bit form of most checkpoints,
+ * multiplied by activations as they are (no rounding of x). group: 32, 64, 128, ... (a
+ * power of two), or any length >= K: one group a row; a row's last group may be short. */
+typedef struct {
+    const void *data;              /* laid out by moe_b200_w4_pack, 16-byte aligned */
+    int64_t     n_experts, rows, K, group;
+    int32_t     scale_type;        /* MOE_TYPE_F16 or _BF16 */
+    int32_t     has_zeros;
+} moe_w4;
+
+/* moe_b200_w4_packed_size: bytes of the laid-out matrices of w (data is not read; 0 for a
+ * shape the path does not take). moe_b200_w4_pack writes them to dst (w->data is not read):
+ * codes [n_experts][rows][ceil(K / 2)] bytes, value 2 i in the low nibble of byte i;
+ * scales [n_experts][rows][ceil(K / group)] of scale_type; zeros of that shape, one byte
+ * each, or NULL with has_zeros 0. Done once per matrix; the sources are not needed
+ * afterwards. A zero above 127 is taken as 127 and sets the device error word
+ * (MOE_DERR_BAD_ZERO). */
+size_t moe_b200_w4_packed_size(const moe_w4 *w);
+int moe_b200_w4_pack(const moe_w4 *w, const void *codes, const void *scales, const void *zeros, void *dst, size_t dst_bytes,
+                     moe_stream_t stream);
+
+/* MUL_MAT_ID of 4-bit experts, for one token or a batch:
+ *   dst[(t * k + p) * rows + r] = row r of expert ids[t * ids_stride + p] . x
+ * (+ bias[expert][r]), with x's row t, or t * k + p with x_per_pick; with `gate` (the shape,
+ * group, scale_type and has_zeros of w) GLU(gate . x + gate_bias, w . x + bias), glu_op and
+ * glu_limit as in moe_fusion_device. ids NULL: w is one matrix (n_experts 1), which every
+ * token meets (k 1). x_type MOE_TYPE_F32, _F16 or _BF16, x_row_stride in elements; biases
+ * f32 [n_experts][rows] or NULL. Products and sums of 64 values are the tensor cores',
+ * everything in 32 bits; x is not rounded (F32 as three bf16 planes that add up to it).
+ * Equal calls give equal bits. Made for batches that read a matrix once (up to 32 rows of
+ * F16 / BF16 or 10 of F32 per expert; more are taken in such chunks).
+ * An id of -1 marks an empty slot: its row of dst is left as it was. Any other id outside
+ * [0, n_experts) also leaves its row and sets the device error word (MOE_DERR_BAD_ID). A
+ * NaN or an infinity in a row of x stays in that row's outputs. n_tok may be 0.
+ * Workspace: moe_b200_w4_workspace_size bytes of device memory, 16-byte aligned, no
+ * initialisation needed (0, and NULL does, for up to 64 picks and without ids; 0 also for
+ * arguments that the call refuses); calls that overlap on the GPU must not share one,
+ * captured graphs included. Allocates nothing, except that the first call on a device
+ * makes its error word: not during stream capture (MOE_ERR_STATE). */
+size_t moe_b200_w4_workspace_size(const moe_w4 *w, int64_t n_tok, int64_t k, int32_t x_type);
+int moe_b200_w4_mul_mat_id(const moe_w4 *w, const moe_w4 *gate, const float *bias, const float *gate_bias, int32_t glu_op,
+                           float glu_limit, const void *x, int32_t x_type, int64_t x_row_stride, int32_t x_per_pick,
+                           int64_t n_tok, const int32_t *ids, int64_t k, int64_t ids_stride, float *dst, void *workspace,
+                           size_t workspace_bytes, moe_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,288 @@
+"""Products with 4-bit matrices of group scales against the plain 64-bit
+implementation (sorted_ref)."""
+import numpy as np
+import pytest
+import torch
+
+import sorted_ref as R
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+class Case:
+    def __init__(self, pkg, cuda, rng, E, rows, K, group, zeros, scale="f16", flat=False):
+        n = -(-K // group)
+        self.K, self.group = K, group
+        shape = (rows,) if flat else (E, rows)
+        self.codes = rng.integers(0, 256, size=(*shape, (K + 1) // 2), dtype=np.uint8)
+        s = torch.from_numpy((0.01 * (0.2 + rng.random((*shape, n))) * rng.choice([-1, 1], (*shape, n))).astype(np.float32)).to(DT[scale])
+        self.zeros = rng.integers(0, 16, size=(*shape, n), dtype=np.uint8) if zeros else None
+        self.scales = s.double().numpy()
+        t = lambda a: None if a is None else torch.from_numpy(a).to(cuda)   # noqa: E731
+        self.w = pkg.W4Weights(t(self.codes), s.to(cuda), K, group, zeros=t(self.zeros))
+        self.values = R.w4_values(self.codes, self.scales, self.zeros, K, group).reshape(E, rows, K)
+
+
+def make_x(rng, shape, dtype, cuda):
+    x = torch.from_numpy(rng.normal(size=shape).astype(np.float32)).to(cuda).to(DT[dtype])
+    return x, x.double().cpu().numpy()
+
+
+def product(values, x, ids):
+    """([n, k, rows], sums of magnitudes); x [n, K] or [n, k, K]"""
+    n, k = ids.shape
+    x = np.broadcast_to(x[:, None], (n, k, x.shape[-1])) if x.ndim == 2 else x
+    y, mag = (np.zeros((n, k, values.shape[1])) for _ in range(2))
+    for t in range(n):
+        for p in range(k):
+            if 0 <= ids[t, p] < values.shape[0]:
+                W = values[ids[t, p]]
+                y[t, p], mag[t, p] = W @ x[t, p], np.abs(W) @ np.abs(x[t, p])
+    return y, mag
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,rows,K,group,zeros", [
+    (1, 1, 1, 32, False), (1, 16, 64, 64, True), (1, 17, 33, 32, True), (2, 30, 31, 32, False), (3, 100, 96, 32, True),
+    (1, 768, 2048, 128, False), (5, 1000, 1446, 128, True), (7, 40, 700, 1024, True), (4, 64, 999, 256, False),
+    (8, 33, 4096, 32, True), (9, 129, 512, 64, False), (16, 48, 1024, 128, True), (17, 50, 2000, 64, True),
+    (24, 256, 4096, 32, True), (33, 20, 320, 128, False), (70, 130, 640, 64, True), (2, 5000, 128, 32, True),
+    (11, 64, 20000, 128, True), (32, 64, 9000, 32, False),                       # K in several passes
+])
+def test_one_matrix(pkg, cuda, n, rows, K, group, zeros, dtype):
+    rng = np.random.default_rng(rows + K)
+    c = Case(pkg, cuda, rng, 1, rows, K, group, zeros, scale=("f16", "bf16")[n % 2], flat=n % 2 == 0)
+    x, x64 = make_x(rng, (n, K), dtype, cuda)
+    got = pkg.w4_mul_mat(c.w, x).double().cpu().numpy()
+    ref, mag = product(c.values, x64, np.zeros((n, 1), np.int32))
+    assert got.shape == (n, rows)
+    err = np.abs(got - ref[:, 0])
+    assert (err <= R.w4_tol(mag[:, 0], K)).all(), (err / R.w4_tol(mag[:, 0], K)).max()
+    assert pkg.moe_cache.device_error() == 0
+
+
+EXPERTS = [
+    # n, E, k, rows, K, group, zeros, per_pick
+    (1, 8, 4, 48, 256, 128, False, False), (1, 4, 4, 20, 64, 32, True, True), (3, 5, 2, 100, 1446, 64, True, False),
+    (8, 64, 8, 64, 768, 32, False, True), (16, 3, 4, 33, 512, 128, True, False),        # 64 picks: grouped in the kernel
+    (13, 3, 5, 33, 512, 128, True, True), (64, 16, 8, 96, 448, 64, False, False), (100, 2, 3, 40, 320, 32, True, True),
+    (40, 300, 6, 16, 96, 32, False, False), (5, 1, 1, 31, 62, 32, True, False), (90, 1, 1, 31, 62, 64, True, False),
+    (12, 4, 5, 24, 6000, 128, True, False),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,E,k,rows,K,group,zeros,per_pick", EXPERTS)
+def test_experts(pkg, cuda, n, E, k, rows, K, group, zeros, per_pick, dtype):
+    """Picks dropped and repeated; their rows of dst stay as they were; biases."""
+    rng = np.random.default_rng(n + E + K)
+    c = Case(pkg, cuda, rng, E, rows, K, group, zeros, scale=("f16", "bf16")[E % 2])
+    ids = rng.integers(0, E, size=(n, k)).astype(np.int32)
+    ids[rng.random((n, k)) < 0.15] = -1
+    x, x64 = make_x(rng, (n, k, K) if per_pick else (n, K), dtype, cuda)
+    bias = rng.normal(size=(E, rows)).astype(np.float32)
+    dst = torch.full((n, k, rows), 7.25, device=cuda)
+    tids = torch.from_numpy(ids).to(cuda)
+    got = pkg.w4_mul_mat_id(c.w, x, tids, bias=torch.from_numpy(bias).to(cuda), dst=dst)
+    assert got is dst
+    got = got.double().cpu().numpy()
+    ref, mag = product(c.values, x64, ids)
+    held = ids >= 0
+    assert (got[~held] == 7.25).all()
+    b = bias.astype(np.float64)[np.maximum(ids, 0)]
+    assert (np.abs(got - ref - b)[held] <= R.w4_tol(mag + np.abs(b), K)[held]).all()
+    again = pkg.w4_mul_mat_id(c.w, x, tids, bias=torch.from_numpy(bias).to(cuda))
+    assert torch.equal(again[tids >= 0], dst[tids >= 0])
+    assert pkg.moe_cache.device_error() == 0
+
+
+@pytest.mark.parametrize("op", [0, 1, 2, 3, 4])
+@pytest.mark.parametrize("n,E,k,rows,K,group,zeros,dtype,biases", [
+    (1, 8, 4, 100, 2048, 128, False, "f32", False), (9, 3, 4, 40, 320, 32, True, "f16", True), (30, 5, 3, 33, 700, 64, True, "bf16", True),
+    (20, 2, 2, 64, 9000, 128, False, "bf16", True), (2, 1, 1, 64, 5000, 32, True, "f32", False),
+])
+def test_gate(pkg, cuda, n, E, k, rows, K, group, zeros, dtype, biases, op):
+    rng = np.random.default_rng(K + op)
+    up, gate = (Case(pkg, cuda, rng, E, rows, K, group, zeros) for _ in range(2))
+    ids = rng.integers(0, E, size=(n, k)).astype(np.int32)
+    x, x64 = make_x(rng, (n, K), dtype, cuda)
+    b = [rng.normal(size=(E, rows)).astype(np.float32) if biases else np.zeros((E, rows), np.float32) for _ in range(2)]
+    kw = dict(bias=torch.from_numpy(b[0]).to(cuda), gate_bias=torch.from_numpy(b[1]).to(cuda)) if biases else {}
+    if E == 1:
+        got = pkg.w4_mul_mat(up.w, x, gate=gate.w, glu_op=op, glu_limit=1.25, **kw)[:, None]
+    else:
+        got = pkg.w4_mul_mat_id(up.w, x, torch.from_numpy(ids).to(cuda), gate=gate.w, glu_op=op, glu_limit=1.25, **kw)
+    (u, mu), (g, mg) = (product(c.values, x64, ids) for c in (up, gate))
+    u, g = u + b[0].astype(np.float64)[ids], g + b[1].astype(np.float64)[ids]
+    eu, eg = R.w4_tol(mu + np.abs(b[0])[ids], K), R.w4_tol(mg + np.abs(b[1])[ids], K)
+    err = np.abs(got.double().cpu().numpy() - R.glu(op, g, u, 1.25))
+    assert (err <= R.glu_tol(op, g, u, eg, eu, 1.25)).all()
+
+
+def test_exact_values(pkg, cuda):
+    """Every code against every zero, scales that are powers of two, x a unit vector: the values come back exactly."""
+    K, rows = 64, 128
+    codes = np.tile((np.arange(32, dtype=np.uint8) * 2 % 16) | ((np.arange(32, dtype=np.uint8) * 2 + 1) % 16 << 4), (rows, 1))
+    zeros = np.stack([np.arange(rows), 127 - np.arange(rows)], 1).astype(np.uint8)
+    scales = np.exp2((np.arange(rows * 2) % 7 - 3).reshape(rows, 2)).astype(np.float16)
+    ref = R.w4_values(codes, scales.astype(np.float64), zeros, K, 32)
+    t = lambda a: torch.from_numpy(a).to(cuda)   # noqa: E731
+    w = pkg.W4Weights(t(codes), t(scales), K, 32, zeros=t(zeros))
+    assert pkg.moe_cache.device_error() == 0
+    for dt in DT.values():
+        np.testing.assert_array_equal(pkg.w4_mul_mat(w, torch.eye(K, device=cuda, dtype=dt)).cpu().numpy().T, ref)
+
+
+def test_x_of_32_bits_is_not_rounded(pkg, cuda):
+    """x of full 24-bit mantissas over the whole range of exponents that products leave finite, one value at a time: the
+    product is x times a power of two, exactly -- down to where the third plane (2^-16 of x) is a bf16 that is no
+    longer exact, at 2^-117."""
+    K = 32
+    codes = torch.full((16, 16), 0x99, dtype=torch.uint8, device=cuda)          # q - 8 = 1
+    w = pkg.W4Weights(codes, torch.full((16, 1), 0.5, dtype=torch.float16, device=cuda), K, 32)
+    rng = np.random.default_rng(1)
+    x = torch.zeros((200, K), device=cuda)
+    vals = (rng.uniform(1, 2, 200) * np.exp2(rng.integers(-100, 120, 200)) * rng.choice([-1, 1], 200)).astype(np.float32)
+    for i, v in enumerate(vals):
+        x[i, i % K] = float(v)
+    y = pkg.w4_mul_mat(w, x)
+    np.testing.assert_array_equal(y.cpu().numpy(), np.repeat(vals[:, None] * np.float32(0.5), 16, 1))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_nan_and_inf_stay_in_their_row(pkg, cuda, dtype):
+    rng = np.random.default_rng(2)
+    c = Case(pkg, cuda, rng, 1, 70, 300, 64, True)
+    x, _ = make_x(rng, (12, 300), dtype, cuda)
+    good = pkg.w4_mul_mat(c.w, x)
+    x[3, 17], x[5, 299], x[8, 0] = float("nan"), float("inf"), float("-inf")
+    y = pkg.w4_mul_mat(c.w, x)
+    hit = [3, 5, 8]
+    assert not torch.isfinite(y[3]).any()
+    rest = [i for i in range(12) if i not in hit]
+    assert torch.equal(y[rest], good[rest])
+    W = torch.from_numpy(c.values[0])
+    for row, col, sign in ((5, 299, 1.0), (8, 0, -1.0)):
+        v = W[:, col]
+        assert torch.equal(torch.isnan(y[row]).cpu(), v == 0)                   # 0 times infinity
+        assert torch.equal((y[row].cpu() == float("inf")), v * sign > 0)
+
+
+def test_bad_ids_and_zeros(pkg, cuda):
+    mc = pkg.moe_cache
+    rng = np.random.default_rng(3)
+    c = Case(pkg, cuda, rng, 4, 40, 128, 64, True)
+    for n in (3, 60):                                                            # both forms
+        x, x64 = make_x(rng, (n, 128), "f32", cuda)
+        ids = rng.integers(0, 4, size=(n, 2)).astype(np.int32)
+        for bad in (4, -2, 2 ** 31 - 1, -2 ** 31):
+            ids[1, 1] = bad
+            dst = torch.full((n, 2, 40), 3.5, device=cuda)
+            pkg.w4_mul_mat_id(c.w, x, torch.from_numpy(ids).to(cuda), dst=dst)
+            assert mc.device_error() == mc.DERR_BAD_ID and mc.device_error() == 0
+            assert (dst[1, 1] == 3.5).all()
+            ref, mag = product(c.values, x64, ids)
+            ok = ids < 4
+            ok[1, 1] = False
+            assert (np.abs(dst.double().cpu().numpy() - ref)[ok] <= R.w4_tol(mag, 128)[ok]).all()
+        none = torch.full((n, 2), -1, dtype=torch.int32, device=cuda)
+        dst = torch.full((n, 2, 40), 3.5, device=cuda)
+        assert (pkg.w4_mul_mat_id(c.w, x, none, dst=dst) == 3.5).all()
+    zeros = torch.full((16, 1), 128, dtype=torch.uint8, device=cuda)
+    pkg.W4Weights(torch.zeros((16, 16), dtype=torch.uint8, device=cuda), torch.ones((16, 1), dtype=torch.float16, device=cuda),
+                  32, 32, zeros=zeros)
+    assert mc.device_error() == mc.DERR_BAD_ZERO
+
+
+def test_rows_of_wider_buffers(pkg, cuda):
+    rng = np.random.default_rng(4)
+    c = Case(pkg, cuda, rng, 3, 50, 320, 64, False)
+    for dtype in DT:
+        big, _ = make_x(rng, (20, 320 + 24), dtype, cuda)
+        ids = torch.from_numpy(rng.integers(0, 3, size=(20, 9)).astype(np.int32)).to(cuda)
+        for at in (0, 1, 8, 24):
+            for sl in (ids[:, :4], ids[:, 3:5], ids[:3, 2:7]):
+                x = big[: sl.shape[0], at:at + 320]
+                assert torch.equal(pkg.w4_mul_mat_id(c.w, x, sl), pkg.w4_mul_mat_id(c.w, x.contiguous(), sl.contiguous()))
+
+
+def test_streams_and_graphs(pkg, cuda):
+    rng = np.random.default_rng(5)
+    c = Case(pkg, cuda, rng, 6, 80, 512, 128, True)
+    for n, k in ((4, 2), (50, 3)):
+        x, _ = make_x(rng, (n, 512), "bf16", cuda)
+        ids = torch.from_numpy(rng.integers(0, 6, size=(n, k)).astype(np.int32)).to(cuda)
+        want = pkg.w4_mul_mat_id(c.w, x, ids)
+        torch.cuda.synchronize()
+        s = torch.cuda.Stream()
+        for stream in (s, s.cuda_stream):
+            y = pkg.w4_mul_mat_id(c.w, x, ids, stream=stream)
+            s.synchronize()
+            assert torch.equal(y, want)
+        graphs = []
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                y = pkg.w4_mul_mat_id(c.w, x, ids)
+            graphs.append((g, y))
+        x.neg_()
+        torch.cuda.synchronize()
+        for g, y in graphs:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                g.replay()
+        torch.cuda.synchronize()
+        for g, y in graphs:
+            assert torch.equal(y, -want)
+    assert pkg.moe_cache.device_error() == 0
+
+
+def test_a_token_alone_and_in_a_batch(pkg, cuda):
+    """A token's result depends on its own row: the same bits wherever the call's sums of a row have the same order
+    (they do: K is shared by the same warps whatever the batch; passes of K add their sums apart)."""
+    rng = np.random.default_rng(6)
+    c = Case(pkg, cuda, rng, 1, 64, 512, 64, True)
+    x, _ = make_x(rng, (40, 512), "bf16", cuda)
+    all_of = pkg.w4_mul_mat(c.w, x)
+    for i in (0, 7, 39):
+        assert torch.equal(pkg.w4_mul_mat(c.w, x[i:i + 1])[0], all_of[i])
+
+
+def test_no_tokens(pkg, cuda):
+    rng = np.random.default_rng(7)
+    c = Case(pkg, cuda, rng, 2, 16, 64, 64, False)
+    x = torch.empty((0, 64), device=cuda)
+    assert pkg.w4_mul_mat_id(c.w, x, torch.empty((0, 3), dtype=torch.int32, device=cuda)).shape == (0, 3, 16)
+
+
+@pytest.mark.parametrize("n", [1, 70])
+def test_routed_experts_sorted_and_combined(pkg, cuda, n):
+    """A layer out of the pieces: route, then either the experts' products by pick, or rows sorted by expert, their
+    products (one pick a row), and the weighted sum back."""
+    rng = np.random.default_rng(8)
+    H, F, E, k = 256, 96, 16, 4
+    up, gate, down = (Case(pkg, cuda, rng, E, r, K, 64, True) for r, K in ((F, H), (F, H), (H, F)))
+    x, x64 = make_x(rng, (n, H), "f32", cuda)
+    shared, s64 = make_x(rng, (n, H), "f32", cuda)
+    logits = torch.from_numpy(rng.normal(size=(n, E)).astype(np.float32)).to(cuda)
+    ids, w = pkg.Router(k, norm_w=True)(logits)
+    rows, order = pkg.dispatch_sorted(x, ids, E)
+    one = order.experts.view(-1, 1)
+    h = pkg.w4_mul_mat_id(up.w, rows, one, gate=gate.w)[:, 0]
+    y = pkg.w4_mul_mat_id(down.w, h, one)[:, 0]
+    out = pkg.combine_sorted(y, order, w, shared=shared)
+    hp = pkg.w4_mul_mat_id(up.w, x, ids, gate=gate.w)
+    yp = pkg.w4_mul_mat_id(down.w, hp, ids)
+    assert torch.equal(h[order.positions.long()], hp) and torch.equal(y[order.positions.long()], yp)
+    i, w64 = ids.cpu().numpy(), w.double().cpu().numpy()
+    (u, mu), (g, mg) = (product(c.values, x64, i) for c in (up, gate))
+    ref_h = R.glu(0, g, u)
+    eh = R.glu_tol(0, g, u, R.w4_tol(mg, H), R.w4_tol(mu, H))
+    ref_y, mag = product(down.values, ref_h, i)
+    ey = R.w4_tol(mag, F) + product(np.abs(down.values), eh, i)[0]
+    ref = (ref_y * w64[..., None]).sum(1) + s64
+    parts = np.abs(ref_y * w64[..., None]).sum(1) + np.abs(s64)
+    tol = (ey * w64[..., None]).sum(1) * 1.01 + R.combine_tol(ref, parts, k, "f32")
+    assert (np.abs(out.double().cpu().numpy() - ref) <= tol).all()
+    assert pkg.moe_cache.device_error() == 0
