@@ -168,10 +168,10 @@ cudaError_t launch_mx_product(MxArgs &a, int NT, int64_t units, cudaStream_t st)
 
 // 4-bit matrices with group scales (moe_w4.cu): their layout; the product of n_tok * k entries, after
 // launch_mmq_group into a.entries / a.chunks (chunks of w4_chunk_entries), or alone for up to W4_DIRECT of them.
-// max_chunks: the largest possible number of chunks; g32: groups of 32.
+// max_chunks: the largest possible number of chunks; per_stage: groups of a stage.
 cudaError_t launch_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, int64_t E, int64_t rows, int64_t K,
-                           int64_t groups, int64_t G, uint8_t *out, int *err, cudaStream_t st);
+                           int64_t group, int per_stage, uint8_t *out, int *err, cudaStream_t st);
 int w4_chunk_entries(int64_t n_tok, int64_t k, int64_t n_experts, bool one_matrix, int x_type);
-cudaError_t launch_w4(W4Args &a, int64_t n_tok, int64_t max_chunks, bool g32, cudaStream_t st);
+cudaError_t launch_w4(W4Args &a, int64_t n_tok, int64_t max_chunks, cudaStream_t st);
 
 }  // namespace moe

@@ -2520,43 +2520,29 @@ int moe_b200_combine_sorted_grad(const void *d_out, int32_t type, int64_t d_row_
 namespace {
 
 struct W4Shape {
-    int64_t RT, KS, groups, G;   // tiles of 16 rows, of 64 values; groups of a row, as the caller and as the layout has them
-    int gshift;
-    bool g32;
-    size_t codes, scales, zeros; // bytes of the parts
+    int64_t RT, KS;       // tiles of 16 rows, stages of 256 values
+    int per_stage;        // groups of a stage
+    size_t expert_bytes, bytes;
 };
 
 int w4_shape(const moe_w4 *w, W4Shape *out) {
     if (!w) return fail(MOE_ERR_INVALID, "null argument");
     if (w->n_experts < 1 || w->rows < 1 || w->K < 1 || w->group < 1)
         return fail(MOE_ERR_INVALID, "need n_experts >= 1, rows >= 1, K >= 1, group >= 1");
-    if (w->n_experts > moe::SORT_MAX_EXPERTS || w->rows > (int64_t{1} << 24) || w->K > (int64_t{1} << 20))
-        return fail(MOE_ERR_UNSUPPORTED, "more than %d experts, rows above 2^24 or K above 2^20", moe::SORT_MAX_EXPERTS);
+    if (w->n_experts > moe::W4_MAX_EXPERTS || w->rows > (int64_t{1} << 24) || w->K > (int64_t{1} << 20))
+        return fail(MOE_ERR_UNSUPPORTED, "more than %d experts, rows above 2^24 or K above 2^20", moe::W4_MAX_EXPERTS);
     if (w->scale_type != MOE_TYPE_F16 && w->scale_type != MOE_TYPE_BF16)
         return fail(MOE_ERR_UNSUPPORTED, "scales must be F16 or BF16");
-    W4Shape s{};
-    const bool row = w->group >= w->K;
-    if (!row && (w->group < 32 || (w->group & (w->group - 1))))
+    if (w->group < w->K && (w->group < 32 || (w->group & (w->group - 1))))
         return fail(MOE_ERR_UNSUPPORTED, "group must be a power of two from 32 on, or at least K");
+    W4Shape s{};
     s.RT = (w->rows + moe::W4_M - 1) / moe::W4_M;
-    s.KS = (w->K + moe::W4_KT - 1) / moe::W4_KT;
-    s.groups = row ? 1 : (w->K + w->group - 1) / w->group;
-    s.g32 = !row && w->group == 32;
-    s.G = s.g32 ? 2 * s.KS : s.groups;
-    s.gshift = 31;
-    if (!row && !s.g32)
-        for (s.gshift = 0; (int64_t{moe::W4_KT} << s.gshift) < w->group;) ++s.gshift;
-    const int64_t tiles = w->n_experts * s.RT;
-    s.codes = static_cast<size_t>(tiles * s.KS) * moe::W4_TILE;
-    s.scales = static_cast<size_t>(tiles * s.G) * 32;
-    s.zeros = w->has_zeros ? static_cast<size_t>(tiles * s.G) * 16 : 0;
+    s.KS = (w->K + moe::W4_KS - 1) / moe::W4_KS;
+    s.per_stage = w->group >= w->K || w->group >= moe::W4_KS ? 1 : static_cast<int>(moe::W4_KS / w->group);
+    s.expert_bytes = static_cast<size_t>(s.RT * s.KS) * moe::w4_stage_bytes(s.per_stage, w->has_zeros != 0);
+    s.bytes = static_cast<size_t>(w->n_experts) * s.expert_bytes;
     *out = s;
     return MOE_OK;
-}
-
-moe::W4Matrix w4_matrix(const moe_w4 *w, const W4Shape &s) {
-    const uint8_t *p = static_cast<const uint8_t *>(w->data);
-    return {p, p + s.codes, w->has_zeros ? p + s.codes + s.scales : nullptr};
 }
 
 struct W4Ws {
@@ -2587,7 +2573,7 @@ extern "C" {
 
 size_t moe_b200_w4_packed_size(const moe_w4 *w) {
     W4Shape s{};
-    return w4_shape(w, &s) ? 0 : s.codes + s.scales + s.zeros;
+    return w4_shape(w, &s) ? 0 : s.bytes;
 }
 
 int moe_b200_w4_pack(const moe_w4 *w, const void *codes, const void *scales, const void *zeros, void *dst, size_t dst_bytes,
@@ -2599,14 +2585,13 @@ int moe_b200_w4_pack(const moe_w4 *w, const void *codes, const void *scales, con
     if (!codes || !scales || !dst || (w->has_zeros != 0) != (zeros != nullptr) || reinterpret_cast<uintptr_t>(scales) % 2)
         return fail(MOE_ERR_INVALID, "null or misaligned argument, or zeros that do not go with has_zeros");
     if (!aligned16(dst)) return fail(MOE_ERR_INVALID, "the packed matrices must be 16-byte aligned");
-    if (dst_bytes < s.codes + s.scales + s.zeros)
-        return fail(MOE_ERR_INVALID, "packed buffer too small (%zu < %zu bytes)", dst_bytes, s.codes + s.scales + s.zeros);
+    if (dst_bytes < s.bytes) return fail(MOE_ERR_INVALID, "packed buffer too small (%zu < %zu bytes)", dst_bytes, s.bytes);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     int *err = nullptr;
     rc = error_word(st, &err);
     if (rc) return rc;
     CK(moe::launch_w4_pack(static_cast<const uint8_t *>(codes), scales, static_cast<const uint8_t *>(zeros), w->n_experts, w->rows,
-                           w->K, s.groups, s.G, static_cast<uint8_t *>(dst), err, st));
+                           w->K, w->group, s.per_stage, static_cast<uint8_t *>(dst), err, st));
     return MOE_OK;
 }
 
@@ -2650,10 +2635,10 @@ int moe_b200_w4_mul_mat_id(const moe_w4 *w, const moe_w4 *gate, const float *bia
     rc = error_word(st, &a.err);
     if (rc) return rc;
     a.mats = gate ? 2 : 1;
-    a.w[a.mats - 1] = w4_matrix(w, s);
+    a.w[a.mats - 1] = static_cast<const uint8_t *>(w->data);
     a.bias[a.mats - 1] = bias;
     if (gate) {
-        a.w[0] = w4_matrix(gate, s);
+        a.w[0] = static_cast<const uint8_t *>(gate->data);
         a.bias[0] = gate_bias;
     }
     a.n_experts = static_cast<int32_t>(w->n_experts);
@@ -2661,8 +2646,8 @@ int moe_b200_w4_mul_mat_id(const moe_w4 *w, const moe_w4 *gate, const float *bia
     a.K = static_cast<int32_t>(w->K);
     a.RT = static_cast<int32_t>(s.RT);
     a.KS = static_cast<int32_t>(s.KS);
-    a.G = static_cast<int32_t>(s.G);
-    a.gshift = s.gshift;
+    a.groups = s.per_stage;
+    a.zeros = w->has_zeros != 0;
     a.scale_type = mx_elem(w->scale_type);
     a.glu_op = glu_op;
     a.glu_limit = glu_limit;
@@ -2684,7 +2669,7 @@ int moe_b200_w4_mul_mat_id(const moe_w4 *w, const moe_w4 *gate, const float *bia
                                  moe::w4_chunk_entries(n_tok, k, w->n_experts, false, xt), ws.entries, ws.chunks, ws.n_chunks, a.err,
                                  st, true));
     }
-    CK(moe::launch_w4(a, n_tok, ws.max_chunks, s.g32, st));
+    CK(moe::launch_w4(a, n_tok, ws.max_chunks, st));
     return MOE_OK;
 }
 

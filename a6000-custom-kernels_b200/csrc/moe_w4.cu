@@ -2,83 +2,98 @@
 //
 //   dst[i][r] = sum over groups of s[r][group] * sum over the group of (q[r][c] - z[r][group]) x[c]
 //
-// A batch of decode tokens reads every weight once, so the weights' bytes bound it, and the
-// instructions between a byte and its product come right behind: at 6.5 TB/s an SM
-// takes in a 512-byte tile every 22 cycles, and a scheduler has 88 issue slots for it. Hence
-// * mma.sync m16n8k16 with the weights as A, straight from the registers they were unpacked
-//   in. Its eight columns are the batch (or the planes of a 32-bit x), so up to eight tokens
-//   cost what one does. (tcgen05 would take the weights through tensor memory, and the groups'
-//   sums back out of it for their scales.)
-// * codes become 16-bit floats by bits: 128 + q in bf16, 1024 + q in f16 are an OR; one
-//   subtraction of 128 + z leaves q - z exactly. Products and the sums of a group's 64 values
-//   are the tensor cores', in 32 bits; the scale is applied to those, in 32 bits.
-// * a 32-bit x is split into three bf16 planes that add up to it exactly (8 + 8 + 8 bits), each
-//   a column; 16-bit x are one plane of their own type. So x is never rounded.
-// * each lane copies what it will read itself into a ring in shared memory (cp.async, 16 bytes of
-//   codes and 4 of scales): no barrier between copy and use, and the ring, not the
-//   registers, holds what is in flight.
-// * the warps of a CTA share K (sums meet in shared memory in a fixed order), because
-//   rows / 16 tiles are too few for the 2368 warps of the GPU.
+// A batch of decode tokens reads every weight once, so the weights' bytes would bound it, but the
+// instructions between a byte and its product come right behind: at 6.5 TB/s an SM takes in 512
+// bytes (1024 codes) every 22 cycles, and a scheduler has 88 issue slots for them. Hence
+// * mma.sync m16n8k16 in f16 with the weights as A, straight from the registers they were unpacked
+//   in. Its eight columns are the batch, so up to eight tokens cost what one does. (tcgen05 would
+//   take the weights through tensor memory, and the groups' sums back out of it for their scales.)
+// * four bits at the bottom of an f16 are a number as they are: the subnormal q 2^-24 (q 2^-20 four bits
+//   further up, where the tile's other eight rows lie). So unpacking eight codes is four ANDs and a
+//   shift; the tensor cores multiply subnormals exactly, and the powers of two come off at the end.
+// * zeros: sum (q - z) x = sum q x - z sum x. The sums of x per group are made once, when x is staged
+//   (32 bits; the difference costs about one bit, sums of q x being twice those of (q - z) x).
+// * x: f16 as it is. bf16 times a power of two per 256 values, so that their largest is just below
+//   2^15: what f16 then cuts off is below 2^-39 of that largest. f32 likewise in two planes (two columns)
+//   of 11 bits each, off by 2^-22 of the value at most. Everything behind the products is in 32 bits.
+// * a warp copies what it will read itself into a ring in shared memory (cp.async): no barrier
+//   between copy and use but the warp's, and the ring, not the registers, holds what is in
+//   flight. A stage is 16 rows x 256 values with their scales and zeros, one piece of memory.
+// * warps that share no K need no barrier; where rows are few, the warps of a CTA, and where rows are
+//   very few or x is large the CTAs of a cluster, share K (the sums meet in shared memory, in a fixed
+//   order), and a CTA then holds its share of x only.
 #include "moe_aux.h"
 #include "moe_mx.cuh"
 #include "moe_w4.cuh"
 
-#include <cuda_bf16.h>
+#include <type_traits>
+#ifdef W4_TUNE
+#include <cstdio>
+#include <cstdlib>
+#endif
 
 namespace moe {
 
 namespace {
 
-constexpr int W4_WARPS = 8;
-constexpr int W4_THREADS = 32 * W4_WARPS;
+constexpr int W4_WARPS = 8;              // of a CTA at most
 constexpr int W4_RED = 20;               // floats between two columns of a warp's sums: no bank conflicts
 constexpr int W4_PAD = 64;               // bytes behind a column of x: two columns fill the banks
-constexpr int W4_SMEM = 111 * 1024;      // of a CTA: two fit an SM
-constexpr int W4_ACC = 16 * 1024;        // of it at most for sums kept over K passes
+constexpr int W4_SMEM = 112 * 1024;      // of a CTA: two fit an SM
+constexpr int W4_ACC = 8 * 1024;         // of it at most for sums kept to a run's end, where one block's fit
+constexpr float W4_CODE = 0x1p-24f;      // a code's unit in rows g (times 16 in rows g + 8)
+constexpr float W4_UP = 4096.f;          // which comes off in two factors: with x's power of two, and at the end
+constexpr float W4_PLANE = 4096.f;       // the second plane of an f32 x holds what the first one leaves, times this
+
+// What the plan counts with: a warp's stage where the SM is full, and by itself; adding up a row tile's sums; a row's
+// 256 values of x
+constexpr double W4_STAGE_US = 0.055, W4_STAGE_LATENCY_US = 0.35, W4_SUM_US = 0.03, W4_X_US = 0.02;
+
+// stages in flight per warp
+template <int NT>
+__host__ __device__ constexpr int w4_stages() { return NT == 4 ? 2 : 3; }
 
 // ---- layout ----------------------------------------------------------------------
-// one thread per word of codes, scales or zeros
+// one thread per word
 __global__ void __launch_bounds__(256) w4_pack_kernel(const uint8_t *__restrict__ codes, const uint16_t *__restrict__ scales,
-                                                      const uint8_t *__restrict__ zeros, int64_t E, int rows, int K, int groups,
-                                                      int RT, int KS, int G, uint32_t *out, int64_t n_codes, int64_t n_scales,
-                                                      int64_t n_zeros, int *err) {
+                                                      const uint8_t *__restrict__ zeros, int rows, int K, int group, int groups,
+                                                      int RT, int KS, int per_stage, uint32_t *out, int64_t n, int *err) {
     const int64_t half_k = (K + 1) / 2;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n_codes + n_scales + n_zeros;
-         i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int words = w4_stage_bytes(per_stage, zeros != nullptr) / 4;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
         uint32_t word = 0;
-        if (i < n_codes) {
-            const int w = static_cast<int>(i & 3), lane = static_cast<int>(i >> 2) & 31, g = lane >> 2, t = lane & 3;
-            const int64_t tile = i >> 7;
-            const int s = static_cast<int>(tile % KS);
-            const int64_t et = tile / KS, e = et / RT;
-            const int rt = static_cast<int>(et % RT);
+        const int64_t stage = i / words, et = stage / KS, e = et / RT;
+        const int s = static_cast<int>(stage - et * KS), r0 = static_cast<int>(et - e * RT) * W4_M;
+        int o = static_cast<int>(i - stage * words);
+        if (o < W4_CODES / 4) {
+            const int w = o & 3, lane = (o >> 2) & 31, g = lane >> 2, t = lane & 3;
+            const int c0 = s * W4_KS + (o >> 7) * W4_KT + 32 * (w >> 1) + 8 * t + 4 * (w & 1);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int r = rt * W4_M + g + 8 * (j & 1), c = s * W4_KT + 32 * (w >> 1) + 8 * t + 4 * (w & 1) + 2 * (j >> 1);
+                const int r = r0 + g + 8 * (j & 1), c = c0 + 2 * (j >> 1);
                 if (r < rows && c < K) {
                     const uint32_t b = codes[(e * rows + r) * half_k + (c >> 1)];
                     word |= ((b & 15u) << (4 * j)) | ((c + 1 < K ? b >> 4 : 0u) << (16 + 4 * j));
                 }
             }
-        } else if (i < n_codes + n_scales) {
-            const int64_t o = i - n_codes, eg = o >> 3;
-            const int g = static_cast<int>(o & 7), gi = static_cast<int>(eg % G);
-            const int64_t et = eg / G, e = et / RT;
-            const int rt = static_cast<int>(et % RT);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int r = rt * W4_M + g + 8 * h;
-                if (r < rows && gi < groups) word |= static_cast<uint32_t>(scales[(e * rows + r) * groups + gi]) << (16 * h);
-            }
         } else {
-            const int64_t o = i - n_codes - n_scales, eg = o >> 2;
-            const int g2 = static_cast<int>(o & 3), gi = static_cast<int>(eg % G);
-            const int64_t et = eg / G, e = et / RT;
-            const int rt = static_cast<int>(et % RT);
+            o -= W4_CODES / 4;
+            const bool zero = o >= 8 * per_stage;
+            if (zero) o -= 8 * per_stage;
+            const int gi_stage = zero ? o >> 2 : o >> 3;
+            const int64_t c = static_cast<int64_t>(s) * W4_KS + gi_stage * (W4_KS / per_stage);
+            const int64_t gi = c / group;
+            if (c < K && !zero) {
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const int r = rt * W4_M + 2 * g2 + (b >> 1) + 8 * (b & 1);
-                if (r < rows && gi < groups) {
+                for (int h = 0; h < 2; ++h) {
+                    const int r = r0 + (o & 7) + 8 * h;
+                    if (r < rows) word |= static_cast<uint32_t>(scales[(e * rows + r) * groups + gi]) << (16 * h);
+                }
+            } else if (c < K) {
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const int r = r0 + 2 * (o & 3) + (b >> 1) + 8 * (b & 1);
+                    if (r >= rows) continue;
                     uint32_t z = zeros[(e * rows + r) * groups + gi];
                     if (z > W4_MAX_ZERO) {
                         set_error(err, DERR_BAD_ZERO);
@@ -97,457 +112,665 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const uint8_t *__restrict_
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp4(uint32_t dst, const void *src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ uint4 lds16(uint32_t a) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint32_t lds4(uint32_t a) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-    return v;
-}
+// (those not committed to a group, too)
+__device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ uint4 lds16(const uint8_t *p) { return *reinterpret_cast<const uint4 *>(p); }
+__device__ __forceinline__ uint32_t lds4(const uint8_t *p) { return *reinterpret_cast<const uint32_t *>(p); }
 
-template <int T>
+// d = a b + c; the first of a chain starts from zeros
+template <bool FIRST>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (T == MX_F16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    if constexpr (FIRST)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t add2(uint32_t a, uint32_t b, __half2 *) {
-    const __half2 r = __hadd2(reinterpret_cast<const __half2 &>(a), reinterpret_cast<const __half2 &>(b));
-    return reinterpret_cast<const uint32_t &>(r);
-}
-__device__ __forceinline__ uint32_t add2(uint32_t a, uint32_t b, __nv_bfloat162 *) {
-    const __nv_bfloat162 r = __hadd2(reinterpret_cast<const __nv_bfloat162 &>(a), reinterpret_cast<const __nv_bfloat162 &>(b));
-    return reinterpret_cast<const uint32_t &>(r);
-}
-__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
-    const __half2 r = __hfma2(reinterpret_cast<const __half2 &>(a), reinterpret_cast<const __half2 &>(b),
-                              reinterpret_cast<const __half2 &>(c));
-    return reinterpret_cast<const uint32_t &>(r);
+// A word's eight codes as the A fragment of one MMA: rows g as q 2^-24, rows g + 8 as q 2^-20
+__device__ __forceinline__ void unpack_codes(uint32_t w, uint32_t (&a)[4]) {
+    a[0] = w & 0x000F000Fu;
+    a[1] = w & 0x00F000F0u;
+    a[2] = (w >> 8) & 0x000F000Fu;
+    a[3] = (w >> 8) & 0x00F000F0u;
 }
 
-// What a group subtracts, for rows g and g + 8: -(128 + z) twice in bf16; -(1024 + z) and -(64 + z) in f16.
-template <int T>
-struct Zeros {
-    uint32_t a[2], b[2];
-    // byte 2 (g & 1) + h of the word is row g + 8 h's zero
-    __device__ __forceinline__ void set(uint32_t word, bool odd) {
-        constexpr uint32_t top = T == MX_F16 ? 0xE4E4E4E4u : 0xC3C3C3C3u;
-        a[0] = __byte_perm(word, top, odd ? 0x4242 : 0x4040);
-        a[1] = __byte_perm(word, top, odd ? 0x4343 : 0x4141);
-        if constexpr (T == MX_F16) {
+__device__ __forceinline__ void w4_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t saddr, int rank) {
+    uint32_t a;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+
+// Groups up to W4_DIRECT picks, every CTA for itself: entry[] by (expert, pick), chunk[] = {expert | count << 16,
+// first entry}; returns the number of chunks. Every CTA has to find the same order, so counts belong to
+// warps (count[W4_WARPS][E], scratch) and a warp's picks are ranked by its ballots.
+__device__ int w4_group(const W4Args &a, int2 *chunk, uint16_t *entry, int *count) {
+    __shared__ int warp_sum[W4_WARPS];
+    // (CTAs of the grouped form have all W4_WARPS warps)
+    constexpr int THREADS = 32 * W4_WARPS, PER = W4_DIRECT / THREADS, EPT = W4_MAX_EXPERTS / THREADS;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n_entries, E = a.n_experts;
+    for (int e = tid; e < W4_WARPS * E; e += THREADS) count[e] = 0;
+    __syncthreads();
+    int id[PER], at[PER];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) b[h] = add2(a[h], 0x63806380u, static_cast<__half2 *>(nullptr));   // + 960, exact
+    for (int u = 0; u < PER; ++u) {
+        const int i = (warp * PER + u) * 32 + lane;
+        id[u] = -1;
+        if (i < n) {
+            const int t = i / a.k;
+            id[u] = a.ids[static_cast<int64_t>(t) * a.ids_stride + (i - t * a.k)];
+            if (id[u] < 0 || id[u] >= E) {
+                if (id[u] != -1 && blockIdx.x == 0) set_error(a.err, DERR_BAD_ID);
+                id[u] = -1;
+            }
         }
     }
-};
-
-// A word's eight codes as the A fragment of one MMA, less the zeros.
-template <int T>
-__device__ __forceinline__ void unpack_codes(uint32_t w, const Zeros<T> &z, uint32_t (&a)[4]) {
-    if constexpr (T == MX_F16) {
-        // 1024 + q from bits 0..3, 1024 + 16 q from bits 4..7 (times 2^-4: 64 + q)
-        const uint32_t hi = w >> 8;
-        a[0] = add2((w & 0x000F000Fu) | 0x64006400u, z.a[0], static_cast<__half2 *>(nullptr));
-        a[1] = fma2((w & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, z.b[1]);
-        a[2] = add2((hi & 0x000F000Fu) | 0x64006400u, z.a[0], static_cast<__half2 *>(nullptr));
-        a[3] = fma2((hi & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, z.b[1]);
-    } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            a[j] = add2(((w >> (4 * j)) & 0x000F000Fu) | 0x43004300u, z.a[j & 1], static_cast<__nv_bfloat162 *>(nullptr));
+    for (int u = 0; u < PER; ++u) {
+        if ((warp * PER + u) * 32 >= n) break;
+        const unsigned peers = __match_any_sync(0xffffffffu, id[u]);
+        const int leader = __ffs(peers) - 1;
+        int before = 0;
+        if (id[u] >= 0 && lane == leader) {
+            before = count[warp * E + id[u]];
+            count[warp * E + id[u]] = before + __popc(peers);
+        }
+        at[u] = __shfl_sync(0xffffffffu, before, leader) + __popc(peers & ((1u << lane) - 1u));
+        __syncwarp();
+    }
+    __syncthreads();
+    // first entries and first chunks: scans over the experts, EPT consecutive ones per thread (halves of a word)
+    int c[EPT], sum = 0;
+#pragma unroll
+    for (int u = 0; u < EPT; ++u) {
+        const int e = EPT * tid + u;
+        c[u] = 0;
+        if (e < E)
+            for (int w = 0; w < W4_WARPS; ++w) c[u] += count[w * E + e];
+        sum += c[u] + ((c[u] + a.nc - 1) / a.nc << 16);
+    }
+    int incl = sum;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += o;
+    }
+    if (lane == 31) warp_sum[warp] = incl;
+    __syncthreads();
+    int at0 = incl - sum, total = 0;
+#pragma unroll
+    for (int w = 0; w < W4_WARPS; ++w) {
+        at0 += w < warp ? warp_sum[w] : 0;
+        total += warp_sum[w];
+    }
+#pragma unroll
+    for (int u = 0; u < EPT; ++u) {
+        const int e = EPT * tid + u;
+        if (e >= E) break;
+        int first = at0 & 0xFFFF, q = at0 >> 16, next = first;
+        at0 += c[u] + ((c[u] + a.nc - 1) / a.nc << 16);
+        for (int w = 0; w < W4_WARPS; ++w) {
+            const int mine = count[w * E + e];
+            count[w * E + e] = next;
+            next += mine;
+        }
+        for (int left = c[u]; left > 0; left -= a.nc, first += a.nc)
+            chunk[q++] = make_int2(e | min(left, a.nc) << 16, first);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < PER; ++u)
+        if (id[u] >= 0) entry[count[warp * E + id[u]] + at[u]] = static_cast<uint16_t>((warp * PER + u) * 32 + lane);
+    __syncthreads();
+    return total >> 16;
+}
+
+// A warp brings 256 values of a row of x (from kk on, zeros behind K) to shared memory, eight per lane: the column (two,
+// pitch bytes apart, for f32), the sums of its groups (negative, in units of the codes', gap floats apart) and
+// the power of two that takes the column's products back. A NaN or an infinity makes the sums NaN, and so the row's outputs.
+template <int GROUPS>
+__device__ __forceinline__ void stage_x(const W4Args &a, int64_t row, int kk, int lane, uint8_t *to, int pitch, float *sums,
+                                        float *back, int gap) {
+    kk += 8 * lane;
+    float v[8];
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (a.x_type == MX_F32) {
+        const float *src = static_cast<const float *>(a.x) + row * a.x_stride + kk;
+        if (a.x_vec && kk + 8 <= a.K) {
+            *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(src);
+            *reinterpret_cast<float4 *>(v + 4) = *reinterpret_cast<const float4 *>(src + 4);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = kk + i < a.K ? src[i] : 0.f;
+        }
+    } else {
+        const uint16_t *src = static_cast<const uint16_t *>(a.x) + row * a.x_stride + kk;
+        if (a.x_vec && kk + 8 <= a.K) {
+            raw = *reinterpret_cast<const uint4 *>(src);
+        } else {
+            uint32_t h[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[i] = kk + i < a.K ? src[i] : 0u;
+            raw = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+        }
+        const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (a.x_type == MX_BF16) {
+                v[2 * i] = __uint_as_float(words[i] << 16);
+                v[2 * i + 1] = __uint_as_float(words[i] & 0xFFFF0000u);
+            } else {
+                const float2 f = __half22float2(reinterpret_cast<const __half2 &>(words[i]));
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
+            }
+        }
+    }
+    uint32_t top = 0;
+    bool odd = false;   // a NaN or an infinity
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const bool fin = fabsf(v[i]) < INFINITY;
+        odd |= !fin;
+        v[i] = fin ? v[i] : 0.f;
+        top = max(top, __float_as_uint(fabsf(v[i])));
+    }
+    odd = __any_sync(0xffffffffu, odd);
+    int e = 0;
+    if (a.x_type != MX_F16) {
+        // the largest to [2^14, 2^15); above 2^-106 (values that small lose f16's subnormals at 2^-144)
+        top = __reduce_max_sync(0xffffffffu, top);
+        e = top ? min(141 - static_cast<int>(top >> 23), 120) : 0;
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        uint32_t h[4];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= up;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 p = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            h[i] = reinterpret_cast<const uint32_t &>(p);
+        }
+        raw = make_uint4(h[0], h[1], h[2], h[3]);
+        if (a.x_type == MX_F32) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = __half22float2(reinterpret_cast<const __half2 &>(h[i]));
+                const __half2 p = __floats2half2_rn((v[2 * i] - f.x) * W4_PLANE, (v[2 * i + 1] - f.y) * W4_PLANE);
+                h[i] = reinterpret_cast<const uint32_t &>(p);
+                const float2 l = __half22float2(p);   // the sums are of what the planes hold
+                v[2 * i] = fmaf(l.x, 1.f / W4_PLANE, f.x);
+                v[2 * i + 1] = fmaf(l.y, 1.f / W4_PLANE, f.y);
+            }
+            *reinterpret_cast<uint4 *>(to + pitch + 16 * lane) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+    } else if (odd) {
+        raw = make_uint4(0, 0, 0, 0);
+    }
+    *reinterpret_cast<uint4 *>(to + 16 * lane) = raw;
+    float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+#pragma unroll
+    for (int off = 1; off < 32 / GROUPS; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if (lane % (32 / GROUPS) == 0) {
+        sums[lane / (32 / GROUPS) * gap] = odd ? NAN : sum * -W4_CODE;
+        if (a.x_type == MX_F32) sums[lane / (32 / GROUPS) * gap + 1] = 0.f;
+    }
+    if (lane == 0) {
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        back[0] = down * W4_UP;
+        if (a.x_type == MX_F32) back[1] = down * (W4_UP / W4_PLANE);
     }
 }
 
-// A warp's way through the tiles of its CTA: chunks (an expert and up to nc entries) x row blocks, the row
-// blocks of a run (of one chunk, at most seg of them where K takes several passes) once for each pass,
-// the gate's matrix before the other's, then this warp's steps of the pass.
+// A warp's way through its stages, ahead of their use: chunks (an expert and up to nc entries) x row blocks, the
+// row blocks of a run (of one chunk, at most seg of them) once for each pass over K, the gate's matrix before the
+// other's, then this warp's stages of the pass. Nothing here divides: it runs for every row block.
 struct Cursor {
-    int item, run_end;      // within [item of the run's first block, run_end)
-    int run0, pass, mat, s, s_end;
-    const uint8_t *codes, *scales, *zeros;
+    int left, chunk, tile0, len, i, pass, mat;   // blocks left; the run [tile0, tile0 + len) and the block in it
+    int begin, mine;                             // this warp's stages of the pass: first, number
+    int todo;                                    // of them left at src
+    const uint8_t *src;
+    int64_t expert;                              // offset of the expert's matrix
 };
 
-struct W4Ctl {              // the direct form's chunks
-    int expert[W4_DIRECT], first[W4_DIRECT], count[W4_DIRECT], entry[W4_DIRECT];
-    int n;
-};
-
-// Groups up to 64 ids, every CTA for itself: experts follow one another as they first appear.
-__device__ void w4_group(const W4Args &a, W4Ctl &C, int *ids) {
-    const int i = threadIdx.x, n = a.n_entries;
-    if (i < n) {
-        const int t = i / a.k;
-        int id = a.ids[static_cast<int64_t>(t) * a.ids_stride + (i - t * a.k)];
-        if (id < 0 || id >= a.n_experts) {
-            if (id != -1 && blockIdx.x == 0) set_error(a.err, DERR_BAD_ID);
-            id = -1;
-        }
-        ids[i] = id;
-    }
-    __syncthreads();
-    if (i < n) {
-        const int id = ids[i];
-        int before = 0, all = 0, first = i;
-        for (int j = 0; j < n; ++j) {
-            const bool same = ids[j] == id;
-            all += same;
-            before += same && j < i;
-            if (same && j < first) first = j;
-        }
-        // entries and chunks of the experts that appeared before this one did
-        int e0 = 0, c0 = 0;
-        for (int j = 0; j < first; ++j) {
-            if (ids[j] < 0 || id < 0) continue;
-            int seen = 0, cnt = 0;
-            for (int q = 0; q < n; ++q) {
-                const bool same = ids[q] == ids[j];
-                seen += same && q < j;
-                cnt += same;
-            }
-            if (seen == 0) {
-                e0 += cnt;
-                c0 += (cnt + a.nc - 1) / a.nc;
-            }
-        }
-        if (id >= 0) {
-            C.entry[e0 + before] = i;
-            if (before % a.nc == 0) {
-                const int c = c0 + before / a.nc;
-                C.expert[c] = id;
-                C.first[c] = e0 + before;
-                C.count[c] = min(a.nc, all - before);
-            }
-            atomicMax(&C.n, c0 + (all + a.nc - 1) / a.nc);
-        }
-    }
-    __syncthreads();
-}
-
-template <int T, int NT, bool ZERO, bool G32>
-__global__ void __launch_bounds__(W4_THREADS, 2) w4_kernel(const __grid_constant__ W4Args a) {
-    constexpr int D = NT == 1 ? 8 : NT == 2 ? 6 : 4;                     // tiles in flight per warp
-    constexpr int GW = G32 ? 2 : 1;                                      // groups of a tile
-    constexpr uint32_t STAGE = W4_TILE + 128 * GW * (ZERO ? 2 : 1);
+template <int NT, bool ZERO, int GROUPS, bool SCALE_BF16>
+__global__ void __launch_bounds__(32 * W4_WARPS, 2) w4_kernel(const __grid_constant__ W4Args a) {
+    constexpr int D = w4_stages<NT>(), GW = GROUPS == 8 ? 2 : 1;   // groups of a stage, of a tile
+    constexpr int COLS = 8 * NT, XGAP = (GROUPS + 1) * COLS;       // floats of a stage's sums of x, and its powers of two
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ W4Ctl C;
-    __shared__ int ids[W4_DIRECT];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int WK = 1 << a.wk_shift, wk = warp & (WK - 1), wm = warp >> a.wk_shift, WM = W4_WARPS >> a.wk_shift;
+    // warps wm * WK.. share K of row block row tile wm; warps behind the last of WM * WK have nothing to do
+    const int WK = 1 << a.wk_shift, wk = warp & (WK - 1), wm = warp >> a.wk_shift, WM = a.wm;
+    const int S = 1 << a.split_shift, rank = static_cast<int>(blockIdx.x) & (S - 1);
+    float *red = reinterpret_cast<float *>(smem + a.red_off);
+    int2 *chunk_tab = reinterpret_cast<int2 *>(smem + a.tab_off);
+    uint16_t *entry_tab = reinterpret_cast<uint16_t *>(chunk_tab + a.n_entries);
     int n_chunks;
-    if (a.chunks) {
-        n_chunks = *a.n_chunks;
-    } else if (!a.ids) {
-        n_chunks = (a.n_entries + a.nc - 1) / a.nc;
-    } else {
-        if (tid == 0) C.n = 0;
-        w4_group(a, C, ids);
-        n_chunks = C.n;
-    }
-    const int items = n_chunks * a.tiles;
-    const int i0 = static_cast<int>(static_cast<int64_t>(items) * blockIdx.x / gridDim.x);
-    const int i1 = static_cast<int>(static_cast<int64_t>(items) * (blockIdx.x + 1) / gridDim.x);
-    if (i0 == i1) return;
+    if (a.chunks) n_chunks = *a.n_chunks;
+    else if (!a.ids) n_chunks = (a.n_entries + a.nc - 1) / a.nc;
+    else n_chunks = w4_group(a, chunk_tab, entry_tab, reinterpret_cast<int *>(smem));   // (the ring is not in use yet)
+    const int items = n_chunks * a.tiles, cluster = static_cast<int>(blockIdx.x) >> a.split_shift;
+    const int clusters = static_cast<int>(gridDim.x) >> a.split_shift;
+    const int i0 = static_cast<int>(static_cast<int64_t>(items) * cluster / clusters);
+    int left = static_cast<int>(static_cast<int64_t>(items) * (cluster + 1) / clusters) - i0;
+    if (left == 0) return;   // the whole cluster's
+    int chunk = i0 / a.tiles, tile0 = i0 - chunk * a.tiles;
 
-    auto expert_of = [&](int c) { return a.chunks ? a.chunks[c].x : a.ids ? C.expert[c] : 0; };
-    auto first_of = [&](int c) { return a.chunks ? a.chunks[c].y : a.ids ? C.first[c] : c * a.nc; };
-    auto count_of = [&](int c) {
-        return a.chunks ? a.chunks[c].z : a.ids ? C.count[c] : min(a.nc, a.n_entries - c * a.nc);
+    auto expert_of = [&](int c) { return a.chunks ? a.chunks[c].x : a.ids ? chunk_tab[c].x & 0xFFFF : 0; };
+    auto entry_of = [&](int i) { return a.chunks ? a.entries[i] : a.ids ? static_cast<int>(entry_tab[i]) : i; };
+    auto run_of = [&](int left, int tile0) { return min(min(left, a.tiles - tile0), a.seg); };
+    // the first of rank r's stages of a pass
+    auto share = [&](int pass, int r) {
+        const int s0 = pass * a.sp, n = min(a.KS, s0 + a.sp) - s0;
+        return s0 + (n * r >> a.split_shift);
     };
-    auto run_of = [&](int item) {   // the run's end
-        const int end = min(i1, (item / a.tiles + 1) * a.tiles);
-        return a.passes > 1 ? min(end, item + a.seg) : end;
-    };
-    auto steps_of = [&](int pass) { return min(a.KS, (pass + 1) * a.sp); };   // the pass's end
 
-    // prefetch
-    const uint32_t ring = smem_u32(smem) + warp * D * STAGE;
+    constexpr uint32_t stage_bytes = w4_stage_bytes(GROUPS, ZERO);
+    uint8_t *const ring = smem + warp * D * stage_bytes, *const ring_end = ring + D * stage_bytes;
     Cursor P{};
-    auto seek = [&]() {   // the matrices' addresses at the cursor
-        const int chunk = P.item / a.tiles, rt = min((P.item - chunk * a.tiles) * WM + wm, a.RT - 1);
-        const int64_t row = static_cast<int64_t>(expert_of(chunk)) * a.RT + rt;
-        const W4Matrix &m = a.w[P.mat];
-        P.s = P.pass * a.sp + wk;
-        P.s_end = steps_of(P.pass);
-        P.codes = m.codes + (row * a.KS + P.s) * W4_TILE + 16 * lane;
-        P.scales = m.scales + row * a.G * 32 + 4 * g;
-        if (ZERO) P.zeros = m.zeros + row * a.G * 16 + 4 * (g >> 1);
+    auto seek_chunk = [&]() {
+        P.expert = static_cast<int64_t>(expert_of(P.chunk)) * a.RT * a.KS * stage_bytes + 16 * lane;
     };
-    auto next = [&]() {   // the next matrix, row block, pass or run; false behind the last
-        if (++P.mat < a.mats) return true;
-        P.mat = 0;
-        if (++P.item < P.run_end) return true;
-        if (++P.pass < a.passes) {
-            P.item = P.run0;
-            return true;
-        }
-        P.pass = 0;
-        if (P.item >= i1) return false;
-        P.run0 = P.item;
-        P.run_end = run_of(P.item);
-        return true;
+    auto seek_pass = [&]() {
+        P.begin = share(P.pass, rank) + wk;
+        P.mine = max(0, (share(P.pass, rank + 1) - P.begin + WK - 1) >> a.wk_shift);
     };
-    bool more = true;
-    P.item = P.run0 = i0;
-    P.run_end = run_of(i0);
-    P.pass = P.mat = 0;
-    seek();
-    auto fetch = [&](int slot) {
-        while (more && P.s >= P.s_end) {
-            more = next();
-            if (more) seek();
-        }
-        if (more) {
-            const uint32_t at = ring + slot * STAGE;
-            cp16(at + 16 * lane, P.codes);
-#pragma unroll
-            for (int h = 0; h < GW; ++h) {
-                const int gi = G32 ? 2 * P.s + h : P.s >> a.gshift;
-                cp4(at + W4_TILE + 128 * h + 4 * lane, P.scales + 32 * static_cast<int64_t>(gi));
-                if (ZERO) cp4(at + W4_TILE + 128 * (GW + h) + 4 * lane, P.zeros + 16 * static_cast<int64_t>(gi));
+    auto seek = [&]() {   // the first of the warp's stages of a matrix and pass
+        const int rt = (P.tile0 + P.i) * WM + wm;
+        P.src = (P.mat ? a.w[1] : a.w[0]) + P.expert + (static_cast<int64_t>(rt) * a.KS + P.begin) * stage_bytes;
+        P.todo = rt < a.RT ? P.mine : 0;
+    };
+    auto next = [&]() {   // the next matrix, row block, pass or run; nothing behind the last (left 0)
+        if (++P.mat == a.mats) {
+            P.mat = 0;
+            if (++P.i == P.len) {
+                P.i = 0;
+                if (++P.pass == a.passes) {
+                    P.pass = 0;
+                    P.left -= P.len;
+                    if (P.left == 0) return;
+                    P.tile0 += P.len;
+                    if (P.tile0 == a.tiles) {
+                        P.tile0 = 0;
+                        ++P.chunk;
+                        seek_chunk();
+                    }
+                    P.len = run_of(P.left, P.tile0);
+                }
+                if (a.passes > 1) seek_pass();
             }
-            P.codes += static_cast<int64_t>(WK) * W4_TILE;
-            P.s += WK;
+        }
+        seek();
+    };
+    if (wm < WM) {
+        P.left = left;
+        P.chunk = chunk;
+        P.tile0 = tile0;
+        P.len = run_of(left, tile0);
+        seek_chunk();
+        seek_pass();
+        seek();
+    }
+    const uint32_t step = stage_bytes << a.wk_shift;
+    auto fetch = [&](const uint8_t *stage) {
+        while (P.todo == 0 && P.left) next();
+        if (P.todo) {
+            const uint32_t to = smem_u32(stage) + 16 * lane;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) cp16(to + 512 * i, P.src + 512 * i);
+            if (16 * lane < stage_bytes - W4_CODES) cp16(to + W4_CODES, P.src + W4_CODES);
+            P.src += step;
+            --P.todo;
         }
         cp_commit();
     };
-#pragma unroll
-    for (int d = 0; d < D; ++d) fetch(d);
+#pragma unroll 1
+    for (int d = 0; d < D; ++d) fetch(ring + d * stage_bytes);
 
-    float *red = reinterpret_cast<float *>(smem + a.red_off);
     float *acc = reinterpret_cast<float *>(smem + a.acc_off);
-    const int pitch = 2 * W4_KT * a.sp + W4_PAD;   // bytes of a staged column
-    const uint32_t xs = smem_u32(smem) + a.x_off;
-    constexpr uint32_t RED_BUF = W4_WARPS * NT * 8 * W4_RED;
-    int slot = 0, buf = 0;
+    const int outs1 = a.nc * W4_M;        // sums of a row tile
+    const bool hold = S > 1 || a.passes > 1;
+    constexpr int RED_BUF = W4_WARPS * COLS * W4_RED;
+    const uint8_t *at = ring;
+    int buf = 0, x_chunk = -1;            // whose x is staged
 
-    for (int run0 = i0; run0 < i1;) {
-        const int run_end = run_of(run0), chunk = run0 / a.tiles, count = count_of(chunk), first = first_of(chunk);
-        const int expert = expert_of(chunk), cols = count * a.planes;
-        for (int pass = 0; pass < a.passes; ++pass) {
-            const int s0 = pass * a.sp, s1 = steps_of(pass);
-            __syncthreads();   // everyone is done with the x of the pass before
-            {
-                const int per = (s1 - s0) * (W4_KT / 8), n = per * count;
-                for (int v = tid; v < n; v += W4_THREADS) {
-                    const int col = v / per, c8 = v - col * per, kk = s0 * W4_KT + 8 * c8;
-                    int entry = first + col;
-                    if (a.chunks) entry = a.entries[entry];
-                    else if (a.ids) entry = C.entry[entry];
-                    const int64_t row = a.per_pick ? entry : entry / a.k;
-                    uint8_t *to = smem + a.x_off + static_cast<int64_t>(col) * a.planes * pitch + 16 * c8;
-                    if (a.x_type == MX_F32) {
-                        const float *src = static_cast<const float *>(a.x) + row * a.x_stride + kk;
-                        float f[8];
-                        if (a.x_vec && kk + 8 <= a.K) {
-                            *reinterpret_cast<float4 *>(f) = *reinterpret_cast<const float4 *>(src);
-                            *reinterpret_cast<float4 *>(f + 4) = *reinterpret_cast<const float4 *>(src + 4);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) f[i] = kk + i < a.K ? src[i] : 0.f;
-                        }
-                        uint32_t p[3][4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                // by truncation: 8 bits, the next 8, the last 8. A NaN keeps a quiet payload
-                                const float v0 = f[2 * i + h];
-                                const bool fin = fabsf(v0) < INFINITY;
-                                uint32_t u0 = __float_as_uint(v0) & 0xFFFF0000u;
-                                if (v0 != v0) u0 |= 0x00400000u;
-                                const float r1 = fin ? v0 - __uint_as_float(u0) : 0.f;
-                                const uint32_t u1 = __float_as_uint(r1) & 0xFFFF0000u;
-                                const uint32_t u2 = __float_as_uint(r1 - __uint_as_float(u1));
-                                p[0][i] = h ? p[0][i] | u0 : u0 >> 16;
-                                p[1][i] = h ? p[1][i] | u1 : u1 >> 16;
-                                p[2][i] = h ? p[2][i] | (u2 & 0xFFFF0000u) : u2 >> 16;
-                            }
-                        }
-#pragma unroll
-                        for (int q = 0; q < 3; ++q)
-                            *reinterpret_cast<uint4 *>(to + q * pitch) = make_uint4(p[q][0], p[q][1], p[q][2], p[q][3]);
-                    } else {
-                        const uint16_t *src = static_cast<const uint16_t *>(a.x) + row * a.x_stride + kk;
-                        uint4 q;
-                        if (a.x_vec && kk + 8 <= a.K) {
-                            q = *reinterpret_cast<const uint4 *>(src);
-                        } else {
-                            uint32_t h[8];
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) h[i] = kk + i < a.K ? src[i] : 0u;
-                            q = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
-                        }
-                        *reinterpret_cast<uint4 *>(to) = q;
-                    }
-                }
+    while (left) {
+        const int len = run_of(left, tile0);
+        int count, first, expert;
+        if (a.chunks) {
+            const int4 c = a.chunks[chunk];
+            expert = c.x, first = c.y, count = c.z;
+        } else if (a.ids) {
+            const int2 c = chunk_tab[chunk];
+            expert = c.x & 0xFFFF, first = c.y, count = c.x >> 16;
+        } else {
+            expert = 0, first = chunk * a.nc, count = min(a.nc, a.n_entries - first);
+        }
+        const int cols = count * a.planes, outs = count * W4_M;
+        const int64_t row_base = static_cast<int64_t>(expert) * a.rows;
+        auto emit = [&](int row, int col, float v, float gate) {   // the biases, the GLU, the result
+            if (a.mats > 1) {
+                if (a.bias[0]) gate += a.bias[0][row_base + row];
+                if (a.bias[1]) v += a.bias[1][row_base + row];
+                v = mx_glu_any(a.glu_op, gate, v, a.glu_limit);
+            } else if (a.bias[0]) {
+                v += a.bias[0][row_base + row];
             }
-            __syncthreads();
-            for (int item = run0; item < run_end; ++item) {
+            a.dst[static_cast<int64_t>(entry_of(first + col)) * a.rows + row] = v;
+        };
+        for (int pass = 0; pass < a.passes; ++pass) {
+            const int s0 = share(pass, rank), n_st = share(pass, rank + 1) - s0;
+            const int pitch = n_st * 2 * W4_KS + W4_PAD;   // bytes of a column of x
+            float *xsum = reinterpret_cast<float *>(smem + a.x_off + cols * pitch);   // [stage][GROUPS + 1][COLS]
+            if (chunk != x_chunk || a.passes > 1) {
+                __syncthreads();   // everyone is done with the x of before
+                for (int u = warp; u < count * n_st; u += W4_WARPS) {
+                    const int col = u / n_st, st = u - col * n_st, entry = entry_of(first + col);
+                    float *sums = xsum + st * XGAP + col * a.planes;
+                    stage_x<GROUPS>(a, a.per_pick ? entry : entry / a.k, (s0 + st) * W4_KS, lane,
+                                    smem + a.x_off + col * a.planes * pitch + st * 2 * W4_KS, pitch, sums, sums + GROUPS * COLS,
+                                    COLS);
+                }
+                __syncthreads();
+                x_chunk = chunk;
+            }
+            const uint8_t *xcol[NT];   // (columns past the last repeat the first one's: nothing reads their sums)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                xcol[j] = smem + a.x_off + (8 * j + g < cols ? 8 * j + g : 0) * pitch + 16 * t + wk * 2 * W4_KS;
+            const int mine = wm < WM ? max(0, (n_st - wk + WK - 1) >> a.wk_shift) : 0;
+            for (int it = 0; it < len; ++it) {
+                const int rt = (tile0 + it) * WM + wm;
+                if (wm >= WM || rt >= a.RT) break;
                 for (int mat = 0; mat < a.mats; ++mat) {
                     float sum[NT][4] = {};
-                    for (int s = s0 + wk; s < s1; s += WK) {
-                        cp_wait<D - 1>();
-                        const uint32_t at = ring + slot * STAGE;
-                        const uint4 w = lds16(at + 16 * lane);
-                        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-                        uint32_t A[4][4];
-                        float sc[GW][2];
+                    // this warp's stages, for J tiles of columns
+                    auto run = [&](auto tiles) {
+                        constexpr int J = decltype(tiles)::value;
+                        uint32_t xk = 0;
+                        const float *xs = xsum + wk * XGAP + 2 * t;
+                        for (int s = 0; s < mine; ++s) {
+                            cp_wait<D - 1>();
+                            __syncwarp();
+                            float part[J][4];
 #pragma unroll
-                        for (int h = 0; h < GW; ++h) {
-                            const uint32_t sw = lds4(at + W4_TILE + 128 * h + 4 * lane);
-                            if (a.scale_type == W4_BF16) {
-                                sc[h][0] = __uint_as_float(sw << 16);
-                                sc[h][1] = __uint_as_float(sw & 0xFFFF0000u);
-                            } else {
-                                const float2 f = __half22float2(reinterpret_cast<const __half2 &>(sw));
-                                sc[h][0] = f.x;
-                                sc[h][1] = f.y;
-                            }
-                            Zeros<T> z;
-                            z.set(ZERO ? lds4(at + W4_TILE + 128 * (GW + h) + 4 * lane) : 0x08080808u, ZERO && (g & 1));
+                            for (int i = 0; i < W4_KS / W4_KT; ++i) {
+                                const uint4 w = lds16(at + 16 * lane + W4_TILE * i);
+                                uint32_t A[4][4];
+                                unpack_codes(w.x, A[0]);
+                                unpack_codes(w.y, A[1]);
+                                unpack_codes(w.z, A[2]);
+                                unpack_codes(w.w, A[3]);
+                                float sc[GW][2], sz[GW][2];
 #pragma unroll
-                            for (int i = 4 / GW * h; i < 4 / GW * (h + 1); ++i) unpack_codes<T>(words[i], z, A[i]);
-                        }
-                        const uint32_t xk = xs + (s - s0) * 2 * W4_KT + 16 * t;
-#pragma unroll
-                        for (int j = 0; j < NT; ++j) {
-                            if (NT > 1 && 8 * j >= cols) break;
-                            // (columns past the last repeat the first one's: nothing reads their sums)
-                            const uint32_t xc = xk + (8 * j + g < cols ? 8 * j + g : 0) * pitch;
-                            const uint4 b0 = lds16(xc), b1 = lds16(xc + 64);
-#pragma unroll
-                            for (int h = 0; h < GW; ++h) {
-                                float d[4] = {};
-                                if (GW == 1 || h == 0) {
-                                    mma<T>(d, A[0], b0.x, b0.y);
-                                    mma<T>(d, A[1], b0.z, b0.w);
+                                for (int h = 0; h < GW; ++h) {
+                                    const int gi = GW == 2 ? 2 * i + h : i * GROUPS / 4;
+                                    const uint32_t sw = lds4(at + W4_CODES + 32 * gi + 4 * g);
+                                    if constexpr (SCALE_BF16) {
+                                        sc[h][0] = __uint_as_float(sw << 16);
+                                        sc[h][1] = __uint_as_float(sw & 0xFFFF0000u);
+                                    } else {
+                                        const float2 f = __half22float2(reinterpret_cast<const __half2 &>(sw));
+                                        sc[h][0] = f.x;
+                                        sc[h][1] = f.y;
+                                    }
+                                    // scale * zero where a group begins; rows g + 8 in their codes' units
+                                    if (GW == 1 && i * GROUPS % 4) continue;
+                                    if constexpr (ZERO) {
+                                        const uint32_t zw = lds4(at + W4_CODES + 32 * GROUPS + 16 * gi + 4 * (g >> 1));
+                                        // 2^23 + zero, by bits
+                                        const float z0 = __uint_as_float(__byte_perm(zw, 0x4B000000u, g & 1 ? 0x7552 : 0x7550));
+                                        const float z1 = __uint_as_float(__byte_perm(zw, 0x4B000000u, g & 1 ? 0x7553 : 0x7551));
+                                        sz[h][0] = sc[h][0] * (z0 - 8388608.f);
+                                        sz[h][1] = sc[h][1] * fmaf(z1, 16.f, -16.f * 8388608.f);
+                                    } else {
+                                        sz[h][0] = sc[h][0] * 8.f;
+                                        sz[h][1] = sc[h][1] * 128.f;
+                                    }
                                 }
-                                if (GW == 1 || h == 1) {
-                                    mma<T>(d, A[2], b1.x, b1.y);
-                                    mma<T>(d, A[3], b1.z, b1.w);
-                                }
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) sum[j][i] = fmaf(sc[h][i >> 1], d[i], sum[j][i]);
+                                for (int j = 0; j < J; ++j) {
+                                    const uint8_t *xb = xcol[j] + xk + 2 * W4_KT * i;
+                                    const uint4 b0 = lds16(xb), b1 = lds16(xb + 64);
+                                    float d[GW][4];
+                                    mma<true>(d[0], A[0], b0.x, b0.y);
+                                    mma<false>(d[0], A[1], b0.z, b0.w);
+                                    mma<GW == 2>(d[GW - 1], A[2], b1.x, b1.y);
+                                    mma<false>(d[GW - 1], A[3], b1.z, b1.w);
+#pragma unroll
+                                    for (int h = 0; h < GW; ++h) {
+#pragma unroll
+                                        for (int q = 0; q < 4; ++q)
+                                            part[j][q] = i + h == 0 ? sc[h][q >> 1] * d[h][q] : fmaf(sc[h][q >> 1], d[h][q], part[j][q]);
+                                        if (GW == 1 && i * GROUPS % 4) continue;
+                                        const int gi = GW == 2 ? 2 * i + h : i * GROUPS / 4;
+                                        const float2 x = *reinterpret_cast<const float2 *>(xs + gi * COLS + 8 * j);
+#pragma unroll
+                                        for (int q = 0; q < 4; ++q) part[j][q] = fmaf(sz[h][q >> 1], q & 1 ? x.y : x.x, part[j][q]);
+                                    }
+                                }
                             }
+#pragma unroll
+                            for (int j = 0; j < J; ++j) {
+                                const float2 x = *reinterpret_cast<const float2 *>(xs + GROUPS * COLS + 8 * j);
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) sum[j][q] = fmaf(q & 1 ? x.y : x.x, part[j][q], sum[j][q]);
+                            }
+                            xk += 2 * W4_KS << a.wk_shift;
+                            xs += XGAP << a.wk_shift;
+                            __syncwarp();   // all lanes have read the stage
+                            fetch(at);
+                            at = at + stage_bytes == ring_end ? ring : at + stage_bytes;
                         }
-                        fetch(slot);
-                        slot = slot + 1 == D ? 0 : slot + 1;
+                    };
+                    if constexpr (NT == 1) {
+                        run(std::integral_constant<int, 1>{});
+                    } else if constexpr (NT == 2) {
+                        if (cols <= 8) run(std::integral_constant<int, 1>{});
+                        else run(std::integral_constant<int, 2>{});
+                    } else {
+                        if (cols <= 16) run(std::integral_constant<int, 2>{});
+                        else if (cols <= 24) run(std::integral_constant<int, 3>{});
+                        else run(std::integral_constant<int, 4>{});
                     }
-                    // the warps' sums meet
-                    float *mine = red + buf * RED_BUF + warp * NT * 8 * W4_RED;
+                    // the sums of the warps that share K meet; codes' units come off
+                    float *mine_at = red + buf * RED_BUF + warp * COLS * W4_RED + 2 * t * W4_RED + g;
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) mine[(8 * j + 2 * t + (i & 1)) * W4_RED + g + 8 * (i >> 1)] = sum[j][i];
-                    __syncthreads();
-                    const int outs = count * WM * W4_M;
-                    const bool last = pass + 1 == a.passes;
-                    const int tile = item - chunk * a.tiles;
-                    float *keep = acc + ((a.passes > 1 ? item - run0 : 0) * a.mats + mat) * a.nc * WM * W4_M;
-                    for (int o = tid; o < outs; o += W4_THREADS) {
-                        const int r = o & (W4_M - 1), m = (o >> 4) & (WM - 1), col = o >> (4 + 3 - a.wk_shift);
-                        const float *from = red + buf * RED_BUF + (m << a.wk_shift) * NT * 8 * W4_RED + r;
+                        for (int q = 0; q < 4; ++q)
+                            mine_at[(8 * j + (q & 1)) * W4_RED + 8 * (q >> 1)] = sum[j][q] * (q < 2 ? W4_UP : W4_UP / 16.f);
+                    auto group_sync = [&]() {
+                        if (WK == 1) __syncwarp();
+                        else asm volatile("bar.sync %0, %1;" ::"r"(1 + wm), "r"(32 << a.wk_shift) : "memory");
+                    };
+                    group_sync();
+                    const float *from = red + buf * RED_BUF + (wm << a.wk_shift) * COLS * W4_RED;
+                    float *keep = acc + (((hold ? it : 0) * a.mats + mat) * WM + wm) * outs1;
+                    for (int o = 32 * wk + lane; o < outs; o += 32 << a.wk_shift) {
+                        const int r = o & (W4_M - 1), col = o / W4_M;
                         float v = 0.f;
-                        for (int q = a.planes - 1; q >= 0; --q)   // the small planes first
-                            for (int w = 0; w < WK; ++w) v += from[(w * NT * 8 + col * a.planes + q) * W4_RED];
+                        for (int q = a.planes - 1; q >= 0; --q)   // the small plane first
+                            for (int w = 0; w < WK; ++w) v += from[(w * COLS + col * a.planes + q) * W4_RED + r];
                         if (pass > 0) v += keep[o];
-                        if (!last || mat + 1 < a.mats) {
-                            keep[o] = v;
-                            continue;
-                        }
-                        const int row = (tile * WM + m) * W4_M + r;
-                        if (row >= a.rows) continue;
-                        int entry = first + col;
-                        if (a.chunks) entry = a.entries[entry];
-                        else if (a.ids) entry = C.entry[entry];
-                        const int64_t b = static_cast<int64_t>(expert) * a.rows + row;
-                        if (a.mats > 1) {
-                            float gate = keep[o - a.nc * WM * W4_M];
-                            if (a.bias[0]) gate += a.bias[0][b];
-                            if (a.bias[1]) v += a.bias[1][b];
-                            v = mx_glu_any(a.glu_op, gate, v, a.glu_limit);
-                        } else if (a.bias[0]) {
-                            v += a.bias[0][b];
-                        }
-                        a.dst[static_cast<int64_t>(entry) * a.rows + row] = v;
+                        if (S > 1 || pass + 1 < a.passes || mat + 1 < a.mats) keep[o] = v;
+                        else if (rt * W4_M + r < a.rows) emit(rt * W4_M + r, col, v, a.mats > 1 ? keep[o - WM * outs1] : 0.f);
                     }
-                    if (NT > 2) __syncthreads();   // one buffer
+                    if (NT > 2) group_sync();   // one buffer
                     else buf ^= 1;
                 }
             }
         }
-        run0 = run_end;
+        if (S > 1) {   // the run's outputs, from the sums of every CTA of the cluster
+            w4_cluster_sync();
+            for (int b = 0; b < len * WM; ++b) {
+                const int it = b / WM, m = b - it * WM, rt = (tile0 + it) * WM + m;
+                if (rt >= a.RT) break;
+                for (int o = (rank * W4_WARPS + ((warp + W4_WARPS - b) & (W4_WARPS - 1))) * 32 + lane; o < outs; o += 32 * W4_WARPS << a.split_shift) {
+                    const int row = rt * W4_M + (o & (W4_M - 1));
+                    if (row >= a.rows) continue;
+                    auto total = [&](int mat) {
+                        const uint32_t from = smem_u32(acc + ((it * a.mats + mat) * WM + m) * outs1 + o);
+                        float u = 0.f;
+                        for (int q = 0; q < S; ++q) u += ld_cluster(from, q);
+                        return u;
+                    };
+                    const float v = total(0);
+                    if (a.mats > 1) emit(row, o / W4_M, total(1), v);
+                    else emit(row, o / W4_M, v, 0.f);
+                }
+            }
+            w4_cluster_sync();   // the sums stay until every CTA has read them
+        }
+        left -= len;
+        tile0 += len;
+        if (tile0 == a.tiles) {
+            tile0 = 0;
+            ++chunk;
+        }
     }
-    cp_wait<0>();
+    cp_wait_all();
 }
 
-template <int T, int NT, bool ZERO, bool G32>
+// How the rows and K are shared out: the plan with the least time by this count, in us. A CTA has up to eight
+// warps at work: wm row tiles, K of each shared by 1 << wk_shift warps and `split` CTAs.
+struct W4Plan {
+    int split, wk_shift, wm, passes, sp, seg;
+    uint32_t acc;
+    double us;
+};
+
+W4Plan w4_plan(const W4Args &a, uint32_t fixed, int cols, int x_stage, int64_t chunks, int n_sm) {
+    W4Plan best{};
+    best.us = 1e30;
+    for (int split = 1; split <= 8 && (split == 1 || split <= a.KS); split *= 2)
+        for (int wk = 0; wk <= 3; ++wk)
+            for (int wm = 1; wm << wk <= W4_WARPS; ++wm) {
+                const int WK = 1 << wk, spr = (a.KS + split - 1) / split;
+                if ((WK > 1 && WK / 2 >= spr) || (wm > 1 && wm > a.RT)) continue;
+                const uint32_t one = static_cast<uint32_t>(a.nc * wm * W4_M * a.mats) * 4;   // a row block's sums
+                W4Plan p{split, wk, wm, 1, a.KS, 1 << 29, 0, 0.0};
+                bool hold = split > 1;
+                auto room_for_x = [&]() {   // stages of x that fit
+                    p.acc = hold ? (one > W4_ACC ? one : W4_ACC / one * one) : a.mats > 1 ? one : 0;
+                    const int64_t left = static_cast<int64_t>(W4_SMEM) - fixed - p.acc - cols * W4_PAD;
+                    return left < 0 ? 0 : static_cast<int>(left / (cols * 2 * W4_KS + x_stage));
+                };
+                int fit = room_for_x();
+                if (fit < spr) {
+                    hold = true;
+                    fit = room_for_x();
+                    if (fit < 1) continue;
+                    p.passes = (spr + fit - 1) / fit;
+                    p.sp = (a.KS + p.passes - 1) / p.passes;
+                    if ((p.sp + split - 1) / split > fit) p.sp = fit * split;
+                    p.passes = (a.KS + p.sp - 1) / p.sp;
+                }
+                if (hold) p.seg = static_cast<int>(p.acc / one);
+                const int mine = (p.sp + split - 1) / split;                    // stages of a CTA in a pass
+                const int deep = a.mats * p.passes * ((mine + WK - 1) / WK);    // of a warp for a row block
+                const int64_t items = chunks * ((a.RT + wm - 1) / wm), slots = 2 * n_sm / split;
+                const int64_t rounds = (items + slots - 1) / slots, of_sm = (items * split + n_sm - 1) / n_sm;
+                const double full = of_sm * (wm * WK) * (deep * W4_STAGE_US + a.mats * p.passes * W4_SUM_US);
+                const double deepest = rounds * (deep * W4_STAGE_LATENCY_US + a.mats * p.passes * 0.2);
+                const int64_t runs = p.passes > 1 || split > 1 ? (rounds + p.seg - 1) / p.seg : 1;
+                const double x = (p.passes > 1 ? runs * p.passes : 1) * (0.3 + cols / a.planes * mine * W4_X_US);
+                p.us = (full > deepest ? full : deepest) + x + (split > 1 ? 0.8 * runs : 0.0);
+#ifdef W4_TUNE
+                static const char *force = getenv("W4_FORCE");
+                if (force && (atoi(force) / 100 != split || atoi(force) / 10 % 10 != wk || atoi(force) % 10 != wm)) continue;
+#endif
+                if (p.us < best.us) best = p;
+            }
+    return best;
+}
+
+template <int NT, bool ZERO, int GROUPS, bool SCALE_BF16>
 cudaError_t w4_t(W4Args &a, int64_t max_chunks, cudaStream_t st) {
-    constexpr int D = NT == 1 ? 8 : NT == 2 ? 6 : 4;
-    constexpr uint32_t STAGE = W4_TILE + 128 * (G32 ? 2 : 1) * (ZERO ? 2 : 1);
-    constexpr uint32_t ring = W4_WARPS * D * STAGE, red = (NT > 2 ? 1 : 2) * W4_WARPS * NT * 8 * W4_RED * 4;
-    // warps that share K: at least three tiles each
-    a.wk_shift = a.KS >= 24 ? 3 : a.KS >= 12 ? 2 : a.KS >= 6 ? 1 : 0;
-    const int WM = W4_WARPS >> a.wk_shift, WK = 1 << a.wk_shift;
-    a.tiles = (a.RT + WM - 1) / WM;
-    const uint32_t one = static_cast<uint32_t>(a.nc * WM * W4_M * a.mats) * 4;     // a row block's sums
-    const int cols = (a.n_entries < a.nc ? a.n_entries : a.nc) * a.planes;
-    const uint32_t room = W4_SMEM - ring - red - (a.mats > 1 ? one : 0);
-    const int fit = static_cast<int>((room / cols - W4_PAD) / (2 * W4_KT));
-    a.passes = 1;
-    a.seg = 1;
-    a.sp = a.KS;
-    uint32_t acc = a.mats > 1 ? one : 0;
-    if (fit < a.KS) {
-        acc = one > W4_ACC ? one : W4_ACC / one * one;
-        a.seg = static_cast<int32_t>(acc / one);
-        int sp = static_cast<int>(((W4_SMEM - ring - red - acc) / cols - W4_PAD) / (2 * W4_KT));
-        sp = sp / WK * WK;
-        if (sp < 1) return cudaErrorInvalidConfiguration;
-        a.passes = (a.KS + sp - 1) / sp;
-        a.sp = (a.KS + a.passes - 1) / a.passes;
-        a.sp = (a.sp + WK - 1) / WK * WK;
-        a.passes = (a.KS + a.sp - 1) / a.sp;
-    }
-    a.red_off = ring;
-    a.acc_off = ring + red;
-    a.x_off = (ring + red + acc + 15) / 16 * 16;
-    const size_t smem = a.x_off + static_cast<size_t>(cols) * (2 * W4_KT * a.sp + W4_PAD);
     static bool configured[64] = {};
-    int dev = 0, n_sm = 148;
+    static int sms[64] = {};
+    int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, dev);
     if (!configured[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(w4_kernel<T, NT, ZERO, G32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   W4_SMEM + 16);
+        cudaError_t e = cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(w4_kernel<NT, ZERO, GROUPS, SCALE_BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_SMEM);
         if (e != cudaSuccess) return e;
         configured[dev] = true;
     }
-    const int64_t items = max_chunks * a.tiles;
-    const int64_t grid = items < 2 * n_sm ? items : 2 * n_sm;
-    w4_kernel<T, NT, ZERO, G32><<<static_cast<unsigned>(grid), W4_THREADS, smem, st>>>(a);
-    return cudaGetLastError();
+    static_assert(W4_WARPS * w4_stages<NT>() * W4_CODES >= W4_WARPS * W4_MAX_EXPERTS * 4, "the grouping counts in the ring");
+    const uint32_t ring = W4_WARPS * w4_stages<NT>() * w4_stage_bytes(GROUPS, ZERO);
+    const uint32_t red = (NT > 2 ? 1 : 2) * W4_WARPS * NT * 8 * W4_RED * 4;
+    const uint32_t tab = a.ids && !a.chunks ? (static_cast<uint32_t>(a.n_entries) * 10 + 15) / 16 * 16 : 0;
+    constexpr int x_stage = (GROUPS + 1) * 8 * NT * 4;   // bytes of a stage's sums of x
+    const int most = a.n_entries < a.nc ? a.n_entries : a.nc, cols = most * a.planes;
+    // chunks to expect: those of the experts that even picks would touch
+    int64_t chunks = max_chunks;
+    if (a.ids) {
+        const int64_t touched = a.n_entries < a.n_experts ? a.n_entries : a.n_experts;
+        chunks = touched + a.n_entries / (2 * a.nc);
+        chunks = chunks < max_chunks ? chunks : max_chunks;
+    }
+    const W4Plan p = w4_plan(a, ring + red + tab, cols, x_stage, chunks, sms[dev]);
+    if (p.split == 0) return cudaErrorInvalidConfiguration;
+    a.split_shift = p.split == 1 ? 0 : p.split == 2 ? 1 : p.split == 4 ? 2 : 3;
+    a.wk_shift = p.wk_shift;
+    a.wm = p.wm;
+    a.passes = p.passes;
+    a.sp = p.sp;
+    a.seg = p.seg;
+    a.tiles = (a.RT + p.wm - 1) / p.wm;
+    a.red_off = ring;
+    a.tab_off = ring + red;
+    a.acc_off = a.tab_off + tab;
+    a.x_off = a.acc_off + p.acc;
+    const int mine = (p.sp + p.split - 1) / p.split;
+    const size_t smem = a.x_off + static_cast<size_t>(cols) * (mine * 2 * W4_KS + W4_PAD) + static_cast<size_t>(mine) * x_stage;
+#ifdef W4_TUNE
+    if (getenv("W4_SHOW")) fprintf(stderr, "NT %d cols %d chunks %ld split %d wk %d wm %d passes %d sp %d seg %d acc %u smem %zu us %.1f\n", NT, cols, (long)chunks, p.split, p.wk_shift, p.wm, p.passes, p.sp, p.seg, p.acc, smem, p.us);
+#endif
+    if (smem > W4_SMEM) return cudaErrorInvalidConfiguration;
+    const int64_t items = max_chunks * a.tiles, slots = 2 * sms[dev] / p.split;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>((items < slots ? items : slots) * p.split));
+    cfg.blockDim = dim3(32 * W4_WARPS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = static_cast<unsigned>(p.split);
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = p.split > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, w4_kernel<NT, ZERO, GROUPS, SCALE_BF16>, a);
 }
 
-template <int T, int NT>
-cudaError_t w4_nt(W4Args &a, int64_t max_chunks, bool g32, cudaStream_t st) {
-    const bool zero = a.w[0].zeros != nullptr;
-    if (zero) return g32 ? w4_t<T, NT, true, true>(a, max_chunks, st) : w4_t<T, NT, true, false>(a, max_chunks, st);
-    return g32 ? w4_t<T, NT, false, true>(a, max_chunks, st) : w4_t<T, NT, false, false>(a, max_chunks, st);
+template <int NT, bool ZERO, bool SCALE_BF16>
+cudaError_t w4_groups(W4Args &a, int64_t max_chunks, cudaStream_t st) {
+    switch (a.groups) {
+        case 8: return w4_t<NT, ZERO, 8, SCALE_BF16>(a, max_chunks, st);
+        case 4: return w4_t<NT, ZERO, 4, SCALE_BF16>(a, max_chunks, st);
+        case 2: return w4_t<NT, ZERO, 2, SCALE_BF16>(a, max_chunks, st);
+        default: return w4_t<NT, ZERO, 1, SCALE_BF16>(a, max_chunks, st);
+    }
+}
+
+template <int NT>
+cudaError_t w4_nt(W4Args &a, int64_t max_chunks, cudaStream_t st) {
+    if (a.scale_type == MX_BF16)
+        return a.zeros ? w4_groups<NT, true, true>(a, max_chunks, st) : w4_groups<NT, false, true>(a, max_chunks, st);
+    return a.zeros ? w4_groups<NT, true, false>(a, max_chunks, st) : w4_groups<NT, false, false>(a, max_chunks, st);
 }
 
 // MMA columns of 8: as few as hold a call's rows, for experts the average load and a half
@@ -563,32 +786,27 @@ int w4_tiles_n(int64_t n_tok, int64_t k, int64_t n_experts, bool one_matrix, int
 }  // namespace
 
 int w4_chunk_entries(int64_t n_tok, int64_t k, int64_t n_experts, bool one_matrix, int x_type) {
-    const int planes = x_type == MX_F32 ? 3 : 1;
+    const int planes = x_type == MX_F32 ? 2 : 1;
     return 8 * w4_tiles_n(n_tok, k, n_experts, one_matrix, planes) / planes;
 }
 
 cudaError_t launch_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, int64_t E, int64_t rows, int64_t K,
-                           int64_t groups, int64_t G, uint8_t *out, int *err, cudaStream_t st) {
-    const int64_t RT = (rows + W4_M - 1) / W4_M, KS = (K + W4_KT - 1) / W4_KT;
-    const int64_t nc = E * RT * KS * (W4_TILE / 4), ns = E * RT * G * 8, nz = zeros ? E * RT * G * 4 : 0;
-    const int64_t blocks = (nc + ns + nz + 255) / 256;
+                           int64_t group, int per_stage, uint8_t *out, int *err, cudaStream_t st) {
+    const int64_t RT = (rows + W4_M - 1) / W4_M, KS = (K + W4_KS - 1) / W4_KS, g = group < K ? group : K;
+    const int64_t n = E * RT * KS * (w4_stage_bytes(per_stage, zeros != nullptr) / 4), blocks = (n + 255) / 256;
     w4_pack_kernel<<<static_cast<unsigned>(blocks < 148 * 64 ? blocks : 148 * 64), 256, 0, st>>>(
-        codes, static_cast<const uint16_t *>(scales), zeros, E, static_cast<int>(rows), static_cast<int>(K),
-        static_cast<int>(groups), static_cast<int>(RT), static_cast<int>(KS), static_cast<int>(G),
-        reinterpret_cast<uint32_t *>(out), nc, ns, nz, err);
+        codes, static_cast<const uint16_t *>(scales), zeros, static_cast<int>(rows), static_cast<int>(K), static_cast<int>(g),
+        static_cast<int>((K + g - 1) / g), static_cast<int>(RT), static_cast<int>(KS), per_stage, reinterpret_cast<uint32_t *>(out),
+        n, err);
     return cudaGetLastError();
 }
 
-cudaError_t launch_w4(W4Args &a, int64_t n_tok, int64_t max_chunks, bool g32, cudaStream_t st) {
-    a.planes = a.x_type == MX_F32 ? 3 : 1;
+cudaError_t launch_w4(W4Args &a, int64_t n_tok, int64_t max_chunks, cudaStream_t st) {
+    a.planes = a.x_type == MX_F32 ? 2 : 1;
     const int NT = w4_tiles_n(n_tok, a.k, a.n_experts, a.ids == nullptr, a.planes);
     a.nc = 8 * NT / a.planes;
-    if (a.x_type == MX_F16) {
-        if (NT == 1) return w4_nt<MX_F16, 1>(a, max_chunks, g32, st);
-        return NT == 2 ? w4_nt<MX_F16, 2>(a, max_chunks, g32, st) : w4_nt<MX_F16, 4>(a, max_chunks, g32, st);
-    }
-    if (NT == 1) return w4_nt<MX_BF16, 1>(a, max_chunks, g32, st);
-    return NT == 2 ? w4_nt<MX_BF16, 2>(a, max_chunks, g32, st) : w4_nt<MX_BF16, 4>(a, max_chunks, g32, st);
+    if (NT == 1) return w4_nt<1>(a, max_chunks, st);
+    return NT == 2 ? w4_nt<2>(a, max_chunks, st) : w4_nt<4>(a, max_chunks, st);
 }
 
 }  // namespace moe

@@ -53,7 +53,7 @@ class W4Weights:
 
 
 def w4_workspace_size(w, n_tok, k, dtype):
-    """Bytes of device workspace w4_mul_mat_id needs (moe_b200_w4_workspace_size): 0 for up to 64 picks."""
+    """Bytes of device workspace w4_mul_mat_id needs (moe_b200_w4_workspace_size): 0 for up to 1024 picks."""
     n = w._ws_bytes.get((n_tok, k, dtype))
     if n is None:
         if len(w._ws_bytes) >= 1024:
@@ -82,7 +82,7 @@ def _gate(gate, gate_bias, w):
 def w4_mul_mat(w, x, gate=None, bias=None, gate_bias=None, glu_op=GLU_SWIGLU, glu_limit=0.0, dst=None, stream=None):
     """x f32 / f16 / bf16 [n_tok, K] times one 4-bit matrix (W4Weights with E = 1) -> dst f32
     [n_tok, rows] = w . x (+ bias), or GLU(gate . x + gate_bias, w . x + bias) with
-    `gate`. x is not rounded; sums are in 32 bits."""
+    `gate`. x is not quantised; sums are in 32 bits."""
     stride = dense_rows(x, "x")
     dev, n_tok = w.device, x.shape[0]
     if w.E != 1:
@@ -107,7 +107,7 @@ def w4_mul_mat_id(w, x, ids, gate=None, bias=None, gate_bias=None, glu_op=GLU_SW
     """MUL_MAT_ID of 4-bit experts (moe_b200_w4_mul_mat_id): x f32 / f16 / bf16 [n_tok, K],
     or [n_tok, k, K] with a row per pick, ids i32 [n_tok, k] -> dst f32 [n_tok, k, rows] =
     experts w . x (+ bias), or GLU(gate . x + gate_bias, w . x + bias) with `gate`. Picks
-    with id -1 leave their rows of dst as they were. x is not rounded; sums are in 32 bits."""
+    with id -1 leave their rows of dst as they were. x is not quantised; sums are in 32 bits."""
     if not (isinstance(ids, torch.Tensor) and ids.is_cuda and ids.dtype == torch.int32 and ids.dim() == 2):
         raise bad("ids must be an i32 CUDA tensor [n_tok, k]")
     n_tok, k = ids.shape

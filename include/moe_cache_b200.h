@@ -627,7 +627,7 @@ int moe_b200_combine_sorted_grad(const void *d_out, int32_t type, int64_t d_row_
 /* ---- 4-bit matrices with group scales (no counterpart in the reference) ------
  * value[r][c] = scale[r][c / group] * (code[r][c] - zero[r][c / group]), codes 0..15,
  * zeros 0..127 (8 where there are none): the integer 4-bit form of most checkpoints,
- * multiplied by activations as they are (no rounding of x). group: 32, 64, 128, ... (a
+ * multiplied by activations that are not quantised. group: 32, 64, 128, ... (a
  * power of two), or any length >= K: one group a row; a row's last group may be short. */
 typedef struct {
     const void *data;              /* laid out by moe_b200_w4_pack, 16-byte aligned */
@@ -654,14 +654,15 @@ int moe_b200_w4_pack(const moe_w4 *w, const void *codes, const void *scales, con
  * glu_limit as in moe_fusion_device. ids NULL: w is one matrix (n_experts 1), which every
  * token meets (k 1). x_type MOE_TYPE_F32, _F16 or _BF16, x_row_stride in elements; biases
  * f32 [n_experts][rows] or NULL. Products and sums of 64 values are the tensor cores',
- * everything in 32 bits; x is not rounded (F32 as three bf16 planes that add up to it).
- * Equal calls give equal bits. Made for batches that read a matrix once (up to 32 rows of
- * F16 / BF16 or 10 of F32 per expert; more are taken in such chunks).
+ * everything in 32 bits. x is taken as it is: F16 exactly; BF16 and F32 relative to the largest
+ * of 256 consecutive values, cut off below 2^-39 of it, F32 to 2^-22 of each value. Equal calls
+ * give equal bits. Made for batches that read a matrix once (up to 32 rows of F16 / BF16 or 16
+ * of F32 per expert; more are taken in such chunks).
  * An id of -1 marks an empty slot: its row of dst is left as it was. Any other id outside
  * [0, n_experts) also leaves its row and sets the device error word (MOE_DERR_BAD_ID). A
- * NaN or an infinity in a row of x stays in that row's outputs. n_tok may be 0.
+ * NaN or an infinity in a row of x makes that row's outputs NaN and no other's. n_tok may be 0.
  * Workspace: moe_b200_w4_workspace_size bytes of device memory, 16-byte aligned, no
- * initialisation needed (0, and NULL does, for up to 64 picks and without ids; 0 also for
+ * initialisation needed (0, and NULL does, for up to 1024 picks and without ids; 0 also for
  * arguments that the call refuses); calls that overlap on the GPU must not share one,
  * captured graphs included. Allocates nothing, except that the first call on a device
  * makes its error word: not during stream capture (MOE_ERR_STATE). */

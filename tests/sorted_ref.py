@@ -48,19 +48,23 @@ def combine_tol(s, mag, k, t):
 
 
 def w4_values(codes, scales, zeros, K, group):
-    """uint8 [..., rows, ceil(K / 2)], f64 [..., rows, n], zeros or None -> f64 [..., rows, K]"""
+    """uint8 [..., rows, ceil(K / 2)], f64 [..., rows, n], zeros or None -> f64 [..., rows, K]: scale (code - zero), and
+    |scale| (code + zero)"""
     q = np.stack([codes & 15, codes >> 4], -1).reshape(*codes.shape[:-1], -1)[..., :K].astype(np.float64)
     at = np.arange(K) // group
     z = 8.0 if zeros is None else zeros[..., at].astype(np.float64)
-    return (q - z) * scales[..., at]
+    return (q - z) * scales[..., at], (q + z) * np.abs(scales[..., at])
 
 
 def w4_tol(mag, K):
-    """Of a sum of K products in steps of 64, mag = the sum of their magnitudes: products of 16-bit numbers are exact
-    in 32 bits; each of a step's 64 additions, on the tensor cores, may cut off 2^-23 of at most mag; the step's
-    scale is applied and added with one rounding (2^-24) per step, up to 8 warps' sums and 3 planes follow with one
-    each, and the bias. The last plane of a 32-bit x below 2^-126 may be lost: 2^-133 per product."""
-    return 1.01 * mag * ((64 * 2.0 ** -23) + (K / 64 + 1 + 24 + 1) * 2.0 ** -24) + K * 2.0 ** -120
+    """Of sum s (q - z) x, computed as the sum over groups of s (sum q x) - s z (sum x); mag = the sum of |s| (q + z) |x|,
+    which bounds every partial sum. Each of the 64 additions of a tile, on the tensor cores, may cut off 2^-23 of at most
+    mag. Every tile's scale and every group's s z (two roundings) are applied with a rounding each, 2^-24; so are the
+    sums of a stage, of up to 8 warps and 8 CTAs, of 2 planes and the bias (20), and the sums of x over a group
+    (8 levels). A 32-bit x is held to 2^-22 of its value. What lies more than 2^24 below the largest x of its 256 values is
+    cut off at 2^-39 of that: the largest is one of mag's, times at most 30 / 1 between (q + z) of two places,
+    hence 256 * 30 * 2^-39 < 2^-26 of mag."""
+    return 1.01 * mag * (64 * 2.0 ** -23 + (K / 64 + 3 * (K / 32 + 1) + K / 256 + 20 + 8 + 2) * 2.0 ** -24 + 2.0 ** -22 + 2.0 ** -26) + 1e-36
 
 
 def glu(op, g, u, limit=0.0):

@@ -22,7 +22,7 @@ class Case:
         self.scales = s.double().numpy()
         t = lambda a: None if a is None else torch.from_numpy(a).to(cuda)   # noqa: E731
         self.w = pkg.W4Weights(t(self.codes), s.to(cuda), K, group, zeros=t(self.zeros))
-        self.values = R.w4_values(self.codes, self.scales, self.zeros, K, group).reshape(E, rows, K)
+        self.values, self.parts = (v.reshape(E, rows, K) for v in R.w4_values(self.codes, self.scales, self.zeros, K, group))
 
 
 def make_x(rng, shape, dtype, cuda):
@@ -30,16 +30,17 @@ def make_x(rng, shape, dtype, cuda):
     return x, x.double().cpu().numpy()
 
 
-def product(values, x, ids):
-    """([n, k, rows], sums of magnitudes); x [n, K] or [n, k, K]"""
+def product(c, x, ids):
+    """([n, k, rows], the bound of its partial sums); x [n, K] or [n, k, K]"""
     n, k = ids.shape
+    values, parts = c if isinstance(c, tuple) else (c.values, c.parts)
     x = np.broadcast_to(x[:, None], (n, k, x.shape[-1])) if x.ndim == 2 else x
     y, mag = (np.zeros((n, k, values.shape[1])) for _ in range(2))
     for t in range(n):
         for p in range(k):
             if 0 <= ids[t, p] < values.shape[0]:
-                W = values[ids[t, p]]
-                y[t, p], mag[t, p] = W @ x[t, p], np.abs(W) @ np.abs(x[t, p])
+                e = ids[t, p]
+                y[t, p], mag[t, p] = values[e] @ x[t, p], parts[e] @ np.abs(x[t, p])
     return y, mag
 
 
@@ -56,7 +57,7 @@ def test_one_matrix(pkg, cuda, n, rows, K, group, zeros, dtype):
     c = Case(pkg, cuda, rng, 1, rows, K, group, zeros, scale=("f16", "bf16")[n % 2], flat=n % 2 == 0)
     x, x64 = make_x(rng, (n, K), dtype, cuda)
     got = pkg.w4_mul_mat(c.w, x).double().cpu().numpy()
-    ref, mag = product(c.values, x64, np.zeros((n, 1), np.int32))
+    ref, mag = product(c, x64, np.zeros((n, 1), np.int32))
     assert got.shape == (n, rows)
     err = np.abs(got - ref[:, 0])
     assert (err <= R.w4_tol(mag[:, 0], K)).all(), (err / R.w4_tol(mag[:, 0], K)).max()
@@ -88,7 +89,7 @@ def test_experts(pkg, cuda, n, E, k, rows, K, group, zeros, per_pick, dtype):
     got = pkg.w4_mul_mat_id(c.w, x, tids, bias=torch.from_numpy(bias).to(cuda), dst=dst)
     assert got is dst
     got = got.double().cpu().numpy()
-    ref, mag = product(c.values, x64, ids)
+    ref, mag = product(c, x64, ids)
     held = ids >= 0
     assert (got[~held] == 7.25).all()
     b = bias.astype(np.float64)[np.maximum(ids, 0)]
@@ -114,7 +115,7 @@ def test_gate(pkg, cuda, n, E, k, rows, K, group, zeros, dtype, biases, op):
         got = pkg.w4_mul_mat(up.w, x, gate=gate.w, glu_op=op, glu_limit=1.25, **kw)[:, None]
     else:
         got = pkg.w4_mul_mat_id(up.w, x, torch.from_numpy(ids).to(cuda), gate=gate.w, glu_op=op, glu_limit=1.25, **kw)
-    (u, mu), (g, mg) = (product(c.values, x64, ids) for c in (up, gate))
+    (u, mu), (g, mg) = (product(c, x64, ids) for c in (up, gate))
     u, g = u + b[0].astype(np.float64)[ids], g + b[1].astype(np.float64)[ids]
     eu, eg = R.w4_tol(mu + np.abs(b[0])[ids], K), R.w4_tol(mg + np.abs(b[1])[ids], K)
     err = np.abs(got.double().cpu().numpy() - R.glu(op, g, u, 1.25))
@@ -127,7 +128,7 @@ def test_exact_values(pkg, cuda):
     codes = np.tile((np.arange(32, dtype=np.uint8) * 2 % 16) | ((np.arange(32, dtype=np.uint8) * 2 + 1) % 16 << 4), (rows, 1))
     zeros = np.stack([np.arange(rows), 127 - np.arange(rows)], 1).astype(np.uint8)
     scales = np.exp2((np.arange(rows * 2) % 7 - 3).reshape(rows, 2)).astype(np.float16)
-    ref = R.w4_values(codes, scales.astype(np.float64), zeros, K, 32)
+    ref = R.w4_values(codes, scales.astype(np.float64), zeros, K, 32)[0]
     t = lambda a: torch.from_numpy(a).to(cuda)   # noqa: E731
     w = pkg.W4Weights(t(codes), t(scales), K, 32, zeros=t(zeros))
     assert pkg.moe_cache.device_error() == 0
@@ -135,39 +136,51 @@ def test_exact_values(pkg, cuda):
         np.testing.assert_array_equal(pkg.w4_mul_mat(w, torch.eye(K, device=cuda, dtype=dt)).cpu().numpy().T, ref)
 
 
-def test_x_of_32_bits_is_not_rounded(pkg, cuda):
-    """x of full 24-bit mantissas over the whole range of exponents that products leave finite, one value at a time: the
-    product is x times a power of two, exactly -- down to where the third plane (2^-16 of x) is a bf16 that is no
-    longer exact, at 2^-117."""
-    K = 32
-    codes = torch.full((16, 16), 0x99, dtype=torch.uint8, device=cuda)          # q - 8 = 1
-    w = pkg.W4Weights(codes, torch.full((16, 1), 0.5, dtype=torch.float16, device=cuda), K, 32)
+def test_x_of_32_bits(pkg, cuda):
+    """x of full 24-bit mantissas over the exponents that products leave finite, one value in 256: two planes hold it to
+    2^-22, and (9 - 8) x costs one rounding of 9 x and one of the difference more."""
+    K = 300
+    codes = torch.full((16, 150), 0x99, dtype=torch.uint8, device=cuda)          # q - 8 = 1
+    w = pkg.W4Weights(codes, torch.full((16, 1), 0.5, dtype=torch.float16, device=cuda), K, 512)
     rng = np.random.default_rng(1)
     x = torch.zeros((200, K), device=cuda)
     vals = (rng.uniform(1, 2, 200) * np.exp2(rng.integers(-100, 120, 200)) * rng.choice([-1, 1], 200)).astype(np.float32)
     for i, v in enumerate(vals):
-        x[i, i % K] = float(v)
-    y = pkg.w4_mul_mat(w, x)
-    np.testing.assert_array_equal(y.cpu().numpy(), np.repeat(vals[:, None] * np.float32(0.5), 16, 1))
+        x[i, i] = float(v)
+    y = pkg.w4_mul_mat(w, x).double().cpu().numpy()
+    want = np.repeat(vals[:, None].astype(np.float64) * 0.5, 16, 1)
+    assert (np.abs(y - want) <= (2.0 ** -22 + 18 * 2.0 ** -24) * np.abs(want)).all()
+
+
+def test_bf16_over_its_range(pkg, cuda):
+    """bf16 values 2^24 apart in one block are exact; below 2^-39 of the block's largest nothing is left of them."""
+    K = 256
+    codes = torch.full((16, 128), 0x88, dtype=torch.uint8, device=cuda)          # 0,
+    codes[:, 1:] = 0x98                                                          # and 0, 1 from the third value on
+    w = pkg.W4Weights(codes, torch.ones((16, 1), dtype=torch.float16, device=cuda), K, 256)
+    for p in (-90, 0, 100):
+        for d in (1, 10, 24, 28):
+            x = torch.zeros((1, K), device=cuda, dtype=torch.bfloat16)
+            x[0, 0], x[0, 3] = 1.5 * 2.0 ** p, -1.25 * 2.0 ** (p - d)
+            y = pkg.w4_mul_mat(w, x).double().cpu()
+            # sums of q x: 8 * 1.5 and 9 * 1.25 2^-d against 8 times their sum, in 32 bits
+            assert ((y + 1.25 * 2.0 ** (p - d)).abs() <= 3 * 24.0 * 2.0 ** (p - 24)).all()
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_nan_and_inf_stay_in_their_row(pkg, cuda, dtype):
     rng = np.random.default_rng(2)
-    c = Case(pkg, cuda, rng, 1, 70, 300, 64, True)
-    x, _ = make_x(rng, (12, 300), dtype, cuda)
-    good = pkg.w4_mul_mat(c.w, x)
-    x[3, 17], x[5, 299], x[8, 0] = float("nan"), float("inf"), float("-inf")
-    y = pkg.w4_mul_mat(c.w, x)
-    hit = [3, 5, 8]
-    assert not torch.isfinite(y[3]).any()
-    rest = [i for i in range(12) if i not in hit]
-    assert torch.equal(y[rest], good[rest])
-    W = torch.from_numpy(c.values[0])
-    for row, col, sign in ((5, 299, 1.0), (8, 0, -1.0)):
-        v = W[:, col]
-        assert torch.equal(torch.isnan(y[row]).cpu(), v == 0)                   # 0 times infinity
-        assert torch.equal((y[row].cpu() == float("inf")), v * sign > 0)
+    for n, K in ((12, 300), (2, 70), (12, 3000)):
+        c = Case(pkg, cuda, rng, 1, 70, K, 64, True)
+        x, _ = make_x(rng, (n, K), dtype, cuda)
+        good = pkg.w4_mul_mat(c.w, x)
+        hit = {0: float("nan")} if n < 3 else {3: float("nan"), 5: float("inf"), 8: float("-inf")}
+        for i, (row, v) in enumerate(hit.items()):
+            x[row, (17, K - 1, 0)[i]] = v
+        y = pkg.w4_mul_mat(c.w, x)
+        assert all(torch.isnan(y[row]).all() for row in hit)
+        rest = [i for i in range(n) if i not in hit]
+        assert torch.equal(y[rest], good[rest])
 
 
 def test_bad_ids_and_zeros(pkg, cuda):
@@ -183,7 +196,7 @@ def test_bad_ids_and_zeros(pkg, cuda):
             pkg.w4_mul_mat_id(c.w, x, torch.from_numpy(ids).to(cuda), dst=dst)
             assert mc.device_error() == mc.DERR_BAD_ID and mc.device_error() == 0
             assert (dst[1, 1] == 3.5).all()
-            ref, mag = product(c.values, x64, ids)
+            ref, mag = product(c, x64, ids)
             ok = ids < 4
             ok[1, 1] = False
             assert (np.abs(dst.double().cpu().numpy() - ref)[ok] <= R.w4_tol(mag, 128)[ok]).all()
@@ -276,11 +289,11 @@ def test_routed_experts_sorted_and_combined(pkg, cuda, n):
     yp = pkg.w4_mul_mat_id(down.w, hp, ids)
     assert torch.equal(h[order.positions.long()], hp) and torch.equal(y[order.positions.long()], yp)
     i, w64 = ids.cpu().numpy(), w.double().cpu().numpy()
-    (u, mu), (g, mg) = (product(c.values, x64, i) for c in (up, gate))
+    (u, mu), (g, mg) = (product(c, x64, i) for c in (up, gate))
     ref_h = R.glu(0, g, u)
     eh = R.glu_tol(0, g, u, R.w4_tol(mg, H), R.w4_tol(mu, H))
-    ref_y, mag = product(down.values, ref_h, i)
-    ey = R.w4_tol(mag, F) + product(np.abs(down.values), eh, i)[0]
+    ref_y, mag = product(down, ref_h, i)
+    ey = R.w4_tol(mag, F) + product((np.abs(down.values), down.parts), eh, i)[0]
     ref = (ref_y * w64[..., None]).sum(1) + s64
     parts = np.abs(ref_y * w64[..., None]).sum(1) + np.abs(s64)
     tol = (ey * w64[..., None]).sum(1) * 1.01 + R.combine_tol(ref, parts, k, "f32")
