@@ -172,6 +172,9 @@ cudaError_t launch_mx_product(MxArgs &a, int NT, int64_t units, cudaStream_t st)
 cudaError_t launch_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, int64_t E, int64_t rows, int64_t K,
                            int64_t group, int per_stage, uint8_t *out, int *err, cudaStream_t st);
 int w4_chunk_entries(int64_t n_tok, int64_t k, int64_t n_experts, bool one_matrix, int x_type);
-cudaError_t launch_w4(W4Args &a, int64_t n_tok, int64_t max_chunks, cudaStream_t st);
+// staged: memory for x in the products' form (w4_row_bytes of every row), where w4_staged says so
+int64_t w4_row_bytes(int64_t KS, int groups, int x_type);
+bool w4_staged(int64_t n_tok, int64_t k, int64_t n_experts, bool one_matrix, int64_t KS, int x_type);
+cudaError_t launch_w4(W4Args &a, int64_t n_tok, int64_t max_chunks, uint8_t *staged, cudaStream_t st);
 
 }  // namespace moe

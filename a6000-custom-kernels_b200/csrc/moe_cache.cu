@@ -2546,23 +2546,27 @@ int w4_shape(const moe_w4 *w, W4Shape *out) {
 }
 
 struct W4Ws {
+    uint8_t *staged;
     int32_t *entries, *n_chunks;
     int4 *chunks;
     int64_t max_chunks;
     size_t bytes;
 };
 
-W4Ws w4_ws(int64_t E, int64_t n_tok, int64_t k, int elem, bool one_matrix, char *base) {
+W4Ws w4_ws(int64_t E, const W4Shape &s, int64_t n_tok, int64_t k, int elem, bool per_pick, bool one_matrix, char *base) {
     W4Ws w{};
     const int nc = moe::w4_chunk_entries(n_tok, k, E, one_matrix, elem);
     const int64_t n = n_tok * k;
-    w.max_chunks = one_matrix ? (n + nc - 1) / nc : std::min(n, moe::mmq_max_chunks(n, E, nc));
-    if (one_matrix || n <= moe::W4_DIRECT) return w;
     size_t off = 0;
     auto take = [&](size_t bytes) { char *p = base ? base + off : nullptr; off += align256(bytes); return p; };
-    w.entries = reinterpret_cast<int32_t *>(take(4 * static_cast<size_t>(n)));
-    w.chunks = reinterpret_cast<int4 *>(take(16 * static_cast<size_t>(moe::mmq_max_chunks(n, E, nc))));
-    w.n_chunks = reinterpret_cast<int32_t *>(take(4));
+    if (moe::w4_staged(n_tok, k, E, one_matrix, s.KS, elem))
+        w.staged = reinterpret_cast<uint8_t *>(take(static_cast<size_t>((per_pick ? n : n_tok) * moe::w4_row_bytes(s.KS, s.per_stage, elem))));
+    w.max_chunks = one_matrix ? (n + nc - 1) / nc : std::min(n, moe::mmq_max_chunks(n, E, nc));
+    if (!one_matrix && n > moe::W4_DIRECT) {
+        w.entries = reinterpret_cast<int32_t *>(take(4 * static_cast<size_t>(n)));
+        w.chunks = reinterpret_cast<int4 *>(take(16 * static_cast<size_t>(moe::mmq_max_chunks(n, E, nc))));
+        w.n_chunks = reinterpret_cast<int32_t *>(take(4));
+    }
     w.bytes = off;
     return w;
 }
@@ -2595,10 +2599,11 @@ int moe_b200_w4_pack(const moe_w4 *w, const void *codes, const void *scales, con
     return MOE_OK;
 }
 
-size_t moe_b200_w4_workspace_size(const moe_w4 *w, int64_t n_tok, int64_t k, int32_t x_type) {
+size_t moe_b200_w4_workspace_size(const moe_w4 *w, int64_t n_tok, int64_t k, int32_t x_type, int32_t x_per_pick) {
     W4Shape s{};
-    if (w4_shape(w, &s) || n_tok < 1 || k < 1 || mx_elem(x_type) < 0 || n_tok > (int64_t{1} << 30) / k) return 0;
-    return w4_ws(w->n_experts, n_tok, k, mx_elem(x_type), false, nullptr).bytes;
+    const bool one_matrix = k == 0;
+    if (w4_shape(w, &s) || n_tok < 1 || k < 0 || mx_elem(x_type) < 0 || n_tok > (int64_t{1} << 30) / (k ? k : 1)) return 0;
+    return w4_ws(w->n_experts, s, n_tok, k ? k : 1, mx_elem(x_type), x_per_pick != 0, one_matrix, nullptr).bytes;
 }
 
 int moe_b200_w4_mul_mat_id(const moe_w4 *w, const moe_w4 *gate, const float *bias, const float *gate_bias, int32_t glu_op,
@@ -2625,7 +2630,7 @@ int moe_b200_w4_mul_mat_id(const moe_w4 *w, const moe_w4 *gate, const float *bia
     if (!ids && (w->n_experts != 1 || k != 1)) return fail(MOE_ERR_INVALID, "without ids there is one matrix and one pick");
     if (!x || !dst || !aligned_elem(x, x_type)) return fail(MOE_ERR_INVALID, "null or misaligned argument");
     const int xt = mx_elem(x_type);
-    const W4Ws ws = w4_ws(w->n_experts, n_tok, k, xt, ids == nullptr, static_cast<char *>(workspace));
+    const W4Ws ws = w4_ws(w->n_experts, s, n_tok, k, xt, x_per_pick != 0, ids == nullptr, static_cast<char *>(workspace));
     if (ws.bytes && (!workspace || workspace_bytes < ws.bytes))
         return fail(MOE_ERR_INVALID, "workspace too small (%zu < %zu bytes)", workspace_bytes, ws.bytes);
     if (!aligned16(workspace)) return fail(MOE_ERR_INVALID, "workspace must be 16-byte aligned");
@@ -2661,7 +2666,7 @@ int moe_b200_w4_mul_mat_id(const moe_w4 *w, const moe_w4 *gate, const float *bia
     a.ids = ids;
     a.ids_stride = ids_stride;
     a.dst = dst;
-    if (ws.bytes) {
+    if (ws.n_chunks) {
         a.entries = ws.entries;
         a.chunks = ws.chunks;
         a.n_chunks = ws.n_chunks;
@@ -2669,7 +2674,7 @@ int moe_b200_w4_mul_mat_id(const moe_w4 *w, const moe_w4 *gate, const float *bia
                                  moe::w4_chunk_entries(n_tok, k, w->n_experts, false, xt), ws.entries, ws.chunks, ws.n_chunks, a.err,
                                  st, true));
     }
-    CK(moe::launch_w4(a, n_tok, ws.max_chunks, st));
+    CK(moe::launch_w4(a, n_tok, ws.max_chunks, ws.staged, st));
     return MOE_OK;
 }
 

@@ -51,7 +51,7 @@ constexpr double W4_STAGE_US = 0.055, W4_STAGE_LATENCY_US = 0.35, W4_SUM_US = 0.
 
 // stages in flight per warp
 template <int NT>
-__host__ __device__ constexpr int w4_stages() { return NT == 4 ? 2 : 3; }
+__host__ __device__ constexpr int w4_stages() { return NT == 1 ? 3 : 2; }
 
 // ---- layout ----------------------------------------------------------------------
 // one thread per word
@@ -112,6 +112,9 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const uint8_t *__restrict_
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+__device__ __forceinline__ void cp4(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -144,11 +147,11 @@ __device__ __forceinline__ void unpack_codes(uint32_t w, uint32_t (&a)[4]) {
 __device__ __forceinline__ void w4_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float ld_cluster(uint32_t saddr, int rank) {
+__device__ __forceinline__ float4 ld_cluster(uint32_t saddr, int rank) {
     uint32_t a;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    float4 v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
     return v;
 }
 
@@ -332,6 +335,20 @@ __device__ __forceinline__ void stage_x(const W4Args &a, int64_t row, int kk, in
     }
 }
 
+// The rows of x brought into that form once, for calls whose CTAs would all do it for the same rows: a unit per row and
+// stage, planes x 512 bytes of columns, then [GROUPS + 1][planes] floats. One warp per unit.
+template <int GROUPS>
+__global__ void __launch_bounds__(256) w4_stage_kernel(const __grid_constant__ W4Args a, int64_t units, uint8_t *out) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (the product may come up meanwhile)
+    const int64_t u = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    if (u >= units) return;
+    const int64_t row = u / a.KS;
+    uint8_t *to = out + u * a.unit;
+    float *sums = reinterpret_cast<float *>(to + a.planes * 2 * W4_KS);
+    stage_x<GROUPS>(a, row, static_cast<int>(u - row * a.KS) * W4_KS, threadIdx.x & 31, to, 2 * W4_KS, sums, sums + GROUPS * a.planes,
+                    a.planes);
+}
+
 // A warp's way through its stages, ahead of their use: chunks (an expert and up to nc entries) x row blocks, the
 // row blocks of a run (of one chunk, at most seg of them) once for each pass over K, the gate's matrix before the
 // other's, then this warp's stages of the pass. Nothing here divides: it runs for every row block.
@@ -363,7 +380,10 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 2) w4_kernel(const __grid_const
     const int clusters = static_cast<int>(gridDim.x) >> a.split_shift;
     const int i0 = static_cast<int>(static_cast<int64_t>(items) * cluster / clusters);
     int left = static_cast<int>(static_cast<int64_t>(items) * (cluster + 1) / clusters) - i0;
-    if (left == 0) return;   // the whole cluster's
+    if (left == 0) {   // the whole cluster's
+        if (a.staged) asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+    }
     int chunk = i0 / a.tiles, tile0 = i0 - chunk * a.tiles;
 
     auto expert_of = [&](int c) { return a.chunks ? a.chunks[c].x : a.ids ? chunk_tab[c].x & 0xFFFF : 0; };
@@ -456,31 +476,69 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 2) w4_kernel(const __grid_const
         } else {
             expert = 0, first = chunk * a.nc, count = min(a.nc, a.n_entries - first);
         }
-        const int cols = count * a.planes, outs = count * W4_M;
+        const int cols = count * a.planes, outs = count * (W4_M / 4);   // a thread takes four rows of an entry
         const int64_t row_base = static_cast<int64_t>(expert) * a.rows;
-        auto emit = [&](int row, int col, float v, float gate) {   // the biases, the GLU, the result
-            if (a.mats > 1) {
-                if (a.bias[0]) gate += a.bias[0][row_base + row];
-                if (a.bias[1]) v += a.bias[1][row_base + row];
-                v = mx_glu_any(a.glu_op, gate, v, a.glu_limit);
-            } else if (a.bias[0]) {
-                v += a.bias[0][row_base + row];
+        auto emit = [&](int row, int col, float4 v, float4 gate) {   // the biases, the GLU, the result
+            const int n = min(4, a.rows - row);
+            if (n <= 0) return;
+            float u[4] = {v.x, v.y, v.z, v.w};
+            const float gt[4] = {gate.x, gate.y, gate.z, gate.w};
+            float *to = a.dst + static_cast<int64_t>(entry_of(first + col)) * a.rows + row;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (i >= n) break;
+                if (a.mats > 1) {
+                    const float gi = a.bias[0] ? gt[i] + a.bias[0][row_base + row + i] : gt[i];
+                    if (a.bias[1]) u[i] += a.bias[1][row_base + row + i];
+                    u[i] = mx_glu_any(a.glu_op, gi, u[i], a.glu_limit);
+                } else if (a.bias[0]) {
+                    u[i] += a.bias[0][row_base + row + i];
+                }
             }
-            a.dst[static_cast<int64_t>(entry_of(first + col)) * a.rows + row] = v;
+            if (a.dst_vec) {   // (rows a multiple of 4)
+                *reinterpret_cast<float4 *>(to) = make_float4(u[0], u[1], u[2], u[3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i < n) to[i] = u[i];
+            }
         };
+        auto add4 = [](float4 p, float4 q) { return make_float4(p.x + q.x, p.y + q.y, p.z + q.z, p.w + q.w); };
         for (int pass = 0; pass < a.passes; ++pass) {
             const int s0 = share(pass, rank), n_st = share(pass, rank + 1) - s0;
             const int pitch = n_st * 2 * W4_KS + W4_PAD;   // bytes of a column of x
             float *xsum = reinterpret_cast<float *>(smem + a.x_off + cols * pitch);   // [stage][GROUPS + 1][COLS]
             if (chunk != x_chunk || a.passes > 1) {
                 __syncthreads();   // everyone is done with the x of before
-                for (int u = warp; u < count * n_st; u += W4_WARPS) {
-                    const int col = u / n_st, st = u - col * n_st, entry = entry_of(first + col);
-                    float *sums = xsum + st * XGAP + col * a.planes;
-                    stage_x<GROUPS>(a, a.per_pick ? entry : entry / a.k, (s0 + st) * W4_KS, lane,
-                                    smem + a.x_off + col * a.planes * pitch + st * 2 * W4_KS, pitch, sums, sums + GROUPS * COLS,
-                                    COLS);
+                if (a.staged && x_chunk < 0) asm volatile("griddepcontrol.wait;" ::: "memory");   // (the kernel that staged it)
+                // 1 << x_shift warps to an entry, a stage each at a time
+                const int st0 = warp & ((1 << a.x_shift) - 1), dst_step = 1 << a.x_shift;
+                for (int col = warp >> a.x_shift; col < count; col += W4_WARPS >> a.x_shift) {
+                    const int entry = entry_of(first + col);
+                    const int64_t row = a.per_pick || a.k == 1 ? entry : entry / a.k;
+                    uint8_t *to = smem + a.x_off + col * a.planes * pitch + st0 * 2 * W4_KS;
+                    float *sums = xsum + st0 * XGAP + col * a.planes;
+                    if (a.staged) {   // (cp.async)
+                        const uint8_t *from = a.staged + (row * a.KS + s0 + st0) * a.unit;
+                        const int gi = a.planes > 1 ? lane >> 1 : lane, q = a.planes > 1 ? lane & 1 : 0;
+                        uint32_t to32 = smem_u32(to + 16 * lane), sums32 = smem_u32(sums + gi * COLS + q);
+                        for (int st = st0; st < n_st; st += dst_step) {
+                            cp16(to32, from + 16 * lane);
+                            if (a.planes > 1) cp16(to32 + pitch, from + 2 * W4_KS + 16 * lane);
+                            if (lane < (GROUPS + 1) * a.planes) cp4(sums32, from + a.planes * 2 * W4_KS + 4 * lane);
+                            from += a.unit << a.x_shift;
+                            to32 += 2 * W4_KS << a.x_shift;
+                            sums32 += 4 * XGAP << a.x_shift;
+                        }
+                    } else {
+                        for (int st = st0; st < n_st; st += dst_step) {
+                            stage_x<GROUPS>(a, row, (s0 + st) * W4_KS, lane, to, pitch, sums, sums + GROUPS * COLS, COLS);
+                            to += 2 * W4_KS << a.x_shift;
+                            sums += XGAP << a.x_shift;
+                        }
+                    }
                 }
+                if (a.staged) cp_wait_all();   // (and the stages in flight)
                 __syncthreads();
                 x_chunk = chunk;
             }
@@ -502,7 +560,7 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 2) w4_kernel(const __grid_const
                         for (int s = 0; s < mine; ++s) {
                             cp_wait<D - 1>();
                             __syncwarp();
-                            float part[J][4];
+                            float part[J][4], dots[J][GW][4], sc[GW][2], sz[GW][2];
 #pragma unroll
                             for (int i = 0; i < W4_KS / W4_KT; ++i) {
                                 const uint4 w = lds16(at + 16 * lane + W4_TILE * i);
@@ -511,9 +569,9 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 2) w4_kernel(const __grid_const
                                 unpack_codes(w.y, A[1]);
                                 unpack_codes(w.z, A[2]);
                                 unpack_codes(w.w, A[3]);
-                                float sc[GW][2], sz[GW][2];
 #pragma unroll
                                 for (int h = 0; h < GW; ++h) {
+                                    if (GW == 1 && i * GROUPS % 4) continue;   // the group goes on
                                     const int gi = GW == 2 ? 2 * i + h : i * GROUPS / 4;
                                     const uint32_t sw = lds4(at + W4_CODES + 32 * gi + 4 * g);
                                     if constexpr (SCALE_BF16) {
@@ -524,8 +582,7 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 2) w4_kernel(const __grid_const
                                         sc[h][0] = f.x;
                                         sc[h][1] = f.y;
                                     }
-                                    // scale * zero where a group begins; rows g + 8 in their codes' units
-                                    if (GW == 1 && i * GROUPS % 4) continue;
+                                    // scale * zero; rows g + 8 in their codes' units
                                     if constexpr (ZERO) {
                                         const uint32_t zw = lds4(at + W4_CODES + 32 * GROUPS + 16 * gi + 4 * (g >> 1));
                                         // 2^23 + zero, by bits
@@ -542,17 +599,22 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 2) w4_kernel(const __grid_const
                                 for (int j = 0; j < J; ++j) {
                                     const uint8_t *xb = xcol[j] + xk + 2 * W4_KT * i;
                                     const uint4 b0 = lds16(xb), b1 = lds16(xb + 64);
-                                    float d[GW][4];
-                                    mma<true>(d[0], A[0], b0.x, b0.y);
+                                    // (groups of 128 and more: two tiles' products meet in the tensor cores)
+                                    constexpr bool PAIRS = GROUPS <= 2;
+                                    float (&d)[GW][4] = dots[j];
+                                    if (PAIRS && i % 2) mma<false>(d[0], A[0], b0.x, b0.y);
+                                    else mma<true>(d[0], A[0], b0.x, b0.y);
                                     mma<false>(d[0], A[1], b0.z, b0.w);
                                     mma<GW == 2>(d[GW - 1], A[2], b1.x, b1.y);
                                     mma<false>(d[GW - 1], A[3], b1.z, b1.w);
+                                    if (PAIRS && i % 2 == 0) continue;
 #pragma unroll
                                     for (int h = 0; h < GW; ++h) {
 #pragma unroll
                                         for (int q = 0; q < 4; ++q)
-                                            part[j][q] = i + h == 0 ? sc[h][q >> 1] * d[h][q] : fmaf(sc[h][q >> 1], d[h][q], part[j][q]);
-                                        if (GW == 1 && i * GROUPS % 4) continue;
+                                            part[j][q] = i / (PAIRS ? 2 : 1) + h == 0 ? sc[h][q >> 1] * d[h][q]
+                                                                                      : fmaf(sc[h][q >> 1], d[h][q], part[j][q]);
+                                        if (GW == 1 && (i + 1) * GROUPS % 4) continue;   // the group's last tile
                                         const int gi = GW == 2 ? 2 * i + h : i * GROUPS / 4;
                                         const float2 x = *reinterpret_cast<const float2 *>(xs + gi * COLS + 8 * j);
 #pragma unroll
@@ -598,13 +660,16 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 2) w4_kernel(const __grid_const
                     const float *from = red + buf * RED_BUF + (wm << a.wk_shift) * COLS * W4_RED;
                     float *keep = acc + (((hold ? it : 0) * a.mats + mat) * WM + wm) * outs1;
                     for (int o = 32 * wk + lane; o < outs; o += 32 << a.wk_shift) {
-                        const int r = o & (W4_M - 1), col = o / W4_M;
-                        float v = 0.f;
-                        for (int q = a.planes - 1; q >= 0; --q)   // the small plane first
-                            for (int w = 0; w < WK; ++w) v += from[(w * COLS + col * a.planes + q) * W4_RED + r];
-                        if (pass > 0) v += keep[o];
-                        if (S > 1 || pass + 1 < a.passes || mat + 1 < a.mats) keep[o] = v;
-                        else if (rt * W4_M + r < a.rows) emit(rt * W4_M + r, col, v, a.mats > 1 ? keep[o - WM * outs1] : 0.f);
+                        const int r = 4 * (o & 3), col = o >> 2;
+                        const float *p = from + col * a.planes * W4_RED + r;
+                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (a.planes > 1)   // the small plane first
+                            for (int w = 0; w < WK; ++w) v = add4(v, *reinterpret_cast<const float4 *>(p + (w * COLS + 1) * W4_RED));
+                        for (int w = 0; w < WK; ++w) v = add4(v, *reinterpret_cast<const float4 *>(p + w * COLS * W4_RED));
+                        float4 *kept = reinterpret_cast<float4 *>(keep) + o;
+                        if (pass > 0) v = add4(v, *kept);
+                        if (S > 1 || pass + 1 < a.passes || mat + 1 < a.mats) *kept = v;
+                        else emit(rt * W4_M + r, col, v, a.mats > 1 ? kept[-(WM * outs1 / 4)] : v);
                     }
                     if (NT > 2) group_sync();   // one buffer
                     else buf ^= 1;
@@ -613,23 +678,31 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 2) w4_kernel(const __grid_const
         }
         if (S > 1) {   // the run's outputs, from the sums of every CTA of the cluster
             w4_cluster_sync();
-            for (int b = 0; b < len * WM; ++b) {
-                const int it = b / WM, m = b - it * WM, rt = (tile0 + it) * WM + m;
-                if (rt >= a.RT) break;
-                for (int o = (rank * W4_WARPS + ((warp + W4_WARPS - b) & (W4_WARPS - 1))) * 32 + lane; o < outs; o += 32 * W4_WARPS << a.split_shift) {
-                    const int row = rt * W4_M + (o & (W4_M - 1));
-                    if (row >= a.rows) continue;
-                    auto total = [&](int mat) {
-                        const uint32_t from = smem_u32(acc + ((it * a.mats + mat) * WM + m) * outs1 + o);
-                        float u = 0.f;
-                        for (int q = 0; q < S; ++q) u += ld_cluster(from, q);
-                        return u;
-                    };
-                    const float v = total(0);
-                    if (a.mats > 1) emit(row, o / W4_M, total(1), v);
-                    else emit(row, o / W4_M, v, 0.f);
+            for (int it = 0, turn = 0; it < len; ++it)
+                for (int m = 0; m < WM; ++m, ++turn) {
+                    const int rt = (tile0 + it) * WM + m;
+                    if (rt >= a.RT) break;
+                    // the warps of the cluster in turn
+                    int o = ((rank * W4_WARPS + warp + (turn << 3) - turn) & ((W4_WARPS << a.split_shift) - 1)) * 32 + lane;
+                    for (; o < outs; o += 32 * W4_WARPS << a.split_shift) {
+                        auto total = [&](int mat) {
+                            const uint32_t at4 = smem_u32(reinterpret_cast<float4 *>(acc + ((it * a.mats + mat) * WM + m) * outs1) + o);
+                            float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (S == 2) {
+                                const float4 p = ld_cluster(at4, 0), q = ld_cluster(at4, 1);
+                                return add4(p, q);
+                            }
+                            for (int q = 0; q < S; q += 4) {   // (loads of four CTAs in flight)
+                                const float4 p0 = ld_cluster(at4, q), p1 = ld_cluster(at4, q + 1), p2 = ld_cluster(at4, q + 2),
+                                             p3 = ld_cluster(at4, q + 3);
+                                u = add4(u, add4(add4(p0, p1), add4(p2, p3)));
+                            }
+                            return u;
+                        };
+                        const float4 v = total(0);
+                        emit(rt * W4_M + 4 * (o & 3), o >> 2, a.mats > 1 ? total(1) : v, v);
+                    }
                 }
-            }
             w4_cluster_sync();   // the sums stay until every CTA has read them
         }
         left -= len;
@@ -687,7 +760,7 @@ W4Plan w4_plan(const W4Args &a, uint32_t fixed, int cols, int x_stage, int64_t c
                 const double x = (p.passes > 1 ? runs * p.passes : 1) * (0.3 + cols / a.planes * mine * W4_X_US);
                 p.us = (full > deepest ? full : deepest) + x + (split > 1 ? 0.8 * runs : 0.0);
 #ifdef W4_TUNE
-                static const char *force = getenv("W4_FORCE");
+                const char *force = getenv("W4_FORCE");
                 if (force && (atoi(force) / 100 != split || atoi(force) / 10 % 10 != wk || atoi(force) % 10 != wm)) continue;
 #endif
                 if (p.us < best.us) best = p;
@@ -727,6 +800,8 @@ cudaError_t w4_t(W4Args &a, int64_t max_chunks, cudaStream_t st) {
     a.split_shift = p.split == 1 ? 0 : p.split == 2 ? 1 : p.split == 4 ? 2 : 3;
     a.wk_shift = p.wk_shift;
     a.wm = p.wm;
+    a.x_shift = most >= 8 ? 0 : most >= 4 ? 1 : most >= 2 ? 2 : 3;
+    a.dst_vec = a.rows % 4 == 0 && reinterpret_cast<uintptr_t>(a.dst) % 16 == 0;
     a.passes = p.passes;
     a.sp = p.sp;
     a.seg = p.seg;
@@ -747,12 +822,14 @@ cudaError_t w4_t(W4Args &a, int64_t max_chunks, cudaStream_t st) {
     cfg.blockDim = dim3(32 * W4_WARPS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = static_cast<unsigned>(p.split);
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // (behind w4_stage_kernel only)
+    at[0].val.programmaticStreamSerializationAllowed = a.staged ? 1 : 0;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = static_cast<unsigned>(p.split);
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = p.split > 1 ? 1 : 0;
+    cfg.numAttrs = p.split > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, w4_kernel<NT, ZERO, GROUPS, SCALE_BF16>, a);
 }
 
@@ -780,6 +857,9 @@ int w4_tiles_n(int64_t n_tok, int64_t k, int64_t n_experts, bool one_matrix, int
         const int64_t mean = (3 * n_tok * k + 2 * n_experts - 1) / (2 * n_experts);
         most = mean < n_tok ? mean : n_tok;
     }
+#ifdef W4_TUNE
+    if (getenv("W4_NT")) return atoi(getenv("W4_NT"));
+#endif
     return most * planes <= 8 ? 1 : most * planes <= 16 ? 2 : 4;
 }
 
@@ -801,8 +881,35 @@ cudaError_t launch_w4_pack(const uint8_t *codes, const void *scales, const uint8
     return cudaGetLastError();
 }
 
-cudaError_t launch_w4(W4Args &a, int64_t n_tok, int64_t max_chunks, cudaStream_t st) {
+// bytes of a row of x brought into the products' form
+int64_t w4_row_bytes(int64_t KS, int groups, int x_type) {
+    const int planes = x_type == MX_F32 ? 2 : 1;
+    return KS * ((planes * (2 * W4_KS + 4 * (groups + 1)) + 15) / 16 * 16);
+}
+
+// Whether a call brings x into that form first, once, rather than in every CTA
+bool w4_staged(int64_t n_tok, int64_t k, int64_t n_experts, bool one_matrix, int64_t KS, int x_type) {
+#ifdef W4_TUNE
+    if (getenv("W4_PRE")) return atoi(getenv("W4_PRE"));
+#endif
+    (void)k, (void)n_experts, (void)one_matrix, (void)x_type;
+    return n_tok * KS > 32;
+}
+
+cudaError_t launch_w4(W4Args &a, int64_t n_tok, int64_t max_chunks, uint8_t *staged, cudaStream_t st) {
     a.planes = a.x_type == MX_F32 ? 2 : 1;
+    if (staged) {
+        a.unit = static_cast<int32_t>(w4_row_bytes(1, a.groups, a.x_type));
+        const int64_t units = (a.per_pick ? static_cast<int64_t>(a.n_entries) : n_tok) * a.KS;
+        const unsigned grid = static_cast<unsigned>((units + 7) / 8);
+        if (a.groups == 8) w4_stage_kernel<8><<<grid, 256, 0, st>>>(a, units, staged);
+        else if (a.groups == 4) w4_stage_kernel<4><<<grid, 256, 0, st>>>(a, units, staged);
+        else if (a.groups == 2) w4_stage_kernel<2><<<grid, 256, 0, st>>>(a, units, staged);
+        else w4_stage_kernel<1><<<grid, 256, 0, st>>>(a, units, staged);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+        a.staged = staged;
+    }
     const int NT = w4_tiles_n(n_tok, a.k, a.n_experts, a.ids == nullptr, a.planes);
     a.nc = 8 * NT / a.planes;
     if (NT == 1) return w4_nt<1>(a, max_chunks, st);

@@ -40,6 +40,8 @@ struct W4Args {
     const void *x;
     int64_t x_stride;                // elements
     int32_t x_type, x_vec;           // MX_*; whether rows may be read 16 bytes at a time
+    const uint8_t *staged;           // x in the products' form (w4_stage_kernel), `unit` bytes for 256 values; null: not yet
+    int32_t unit;
     int32_t per_pick, k, n_entries;
     const int32_t *ids;              // null: one matrix, every entry's
     int64_t ids_stride;
@@ -53,6 +55,8 @@ struct W4Args {
     int32_t split_shift, wk_shift;   // 1 << split_shift CTAs of a cluster, and 1 << wk_shift warps of each, share a row's K
     int32_t wm, tiles;               // row tiles of a block, a CTA's at a time; blocks
     int32_t passes, sp;              // K passes of sp stages (of the whole cluster)
+    int32_t x_shift;                 // 1 << x_shift warps bring an entry's x
+    int32_t dst_vec;                 // whether four rows of dst may be written at once
     int32_t seg;                     // blocks of a run, whose sums are held over passes or for the cluster
     uint32_t x_off, red_off, acc_off, tab_off;
 };

@@ -49,17 +49,32 @@ class W4Weights:
         self.desc.data = self.data.data_ptr()
         keep(stream, codes, scales, zeros)
         self.shape = (self.E, self.rows, K, group, scales.dtype, zeros is not None, self.device)
-        self._ws_bytes = {}      # workspace sizes by (n_tok, k, type)
+        self._ws_bytes = {}      # workspace sizes by call
 
 
-def w4_workspace_size(w, n_tok, k, dtype):
-    """Bytes of device workspace w4_mul_mat_id needs (moe_b200_w4_workspace_size): 0 for up to 1024 picks."""
-    n = w._ws_bytes.get((n_tok, k, dtype))
+def w4_workspace_size(w, n_tok, k, dtype, per_pick=False):
+    """Bytes of device workspace that w4_mul_mat (k = 0) or w4_mul_mat_id need (moe_b200_w4_workspace_size): 0 for few
+    rows of x. per_pick: x is [n_tok, k, K]."""
+    n = w._ws_bytes.get((n_tok, k, dtype, per_pick))
     if n is None:
         if len(w._ws_bytes) >= 1024:
             w._ws_bytes.clear()
-        n = w._ws_bytes[n_tok, k, dtype] = lib().moe_b200_w4_workspace_size(w.ref, n_tok, k, ELEM[dtype])
+        n = w._ws_bytes[n_tok, k, dtype, per_pick] = lib().moe_b200_w4_workspace_size(w.ref, n_tok, k, ELEM[dtype], per_pick)
     return n
+
+
+def _workspace(workspace, w, x, *call):
+    """(tensor, address, bytes) of a call's workspace: the caller's, or one of its own where it needs one."""
+    if workspace is None:
+        n = w4_workspace_size(w, *call)
+        if n == 0:
+            return None, None, 0
+        workspace = x.new_empty(n, dtype=torch.uint8)
+        return workspace, workspace.data_ptr(), n
+    if not isinstance(workspace, torch.Tensor) or workspace.dtype != torch.uint8 or workspace.device != w.device or \
+            not workspace.is_contiguous():
+        raise bad("workspace must be contiguous uint8 on the weights' device")
+    return workspace, workspace.data_ptr(), workspace.numel()
 
 
 def _bias(b, name, w):
@@ -79,7 +94,8 @@ def _gate(gate, gate_bias, w):
         raise bad("gate_bias without a gate")
 
 
-def w4_mul_mat(w, x, gate=None, bias=None, gate_bias=None, glu_op=GLU_SWIGLU, glu_limit=0.0, dst=None, stream=None):
+def w4_mul_mat(w, x, gate=None, bias=None, gate_bias=None, glu_op=GLU_SWIGLU, glu_limit=0.0, dst=None, workspace=None,
+               stream=None):
     """x f32 / f16 / bf16 [n_tok, K] times one 4-bit matrix (W4Weights with E = 1) -> dst f32
     [n_tok, rows] = w . x (+ bias), or GLU(gate . x + gate_bias, w . x + bias) with
     `gate`. x is not quantised; sums are in 32 bits."""
@@ -95,10 +111,11 @@ def w4_mul_mat(w, x, gate=None, bias=None, gate_bias=None, glu_op=GLU_SWIGLU, gl
     with ctx:
         dst = x.new_empty((n_tok, w.rows), dtype=torch.float32) if dst is None else \
             given(dst, "dst", torch.float32, (n_tok, w.rows), dev)
+        workspace, ws_ptr, ws_bytes = _workspace(workspace, w, x, n_tok, 0, x.dtype)
         check(lib().moe_b200_w4_mul_mat_id(w.ref, None if gate is None else gate.ref, b, gb, glu_op, glu_limit, x.data_ptr(),
-                                           ELEM[x.dtype], stride, 0, n_tok, None, 1, 1, dst.data_ptr(), None, 0, st))
+                                           ELEM[x.dtype], stride, 0, n_tok, None, 1, 1, dst.data_ptr(), ws_ptr, ws_bytes, st))
     if stream is not None:
-        keep(stream, w.data, None if gate is None else gate.data, x, bias, gate_bias, dst)
+        keep(stream, w.data, None if gate is None else gate.data, x, bias, gate_bias, dst, workspace)
     return dst
 
 
@@ -129,16 +146,7 @@ def w4_mul_mat_id(w, x, ids, gate=None, bias=None, gate_bias=None, glu_op=GLU_SW
     with ctx:
         dst = x.new_empty((n_tok, k, rows), dtype=torch.float32) if dst is None else \
             given(dst, "dst", torch.float32, (n_tok, k, rows), dev)
-        ws_ptr, ws_bytes = None, 0
-        if workspace is None:
-            ws_bytes = w4_workspace_size(w, n_tok, k, x.dtype)
-            if ws_bytes:
-                workspace = x.new_empty(ws_bytes, dtype=torch.uint8)
-                ws_ptr = workspace.data_ptr()
-        elif workspace.dtype != torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
-            raise bad("workspace must be contiguous uint8 on the weights' device")
-        else:
-            ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel()
+        workspace, ws_ptr, ws_bytes = _workspace(workspace, w, x, n_tok, k, x.dtype, per_pick)
         check(lib().moe_b200_w4_mul_mat_id(w.ref, None if gate is None else gate.ref, b, gb, glu_op, glu_limit, x.data_ptr(),
                                            ELEM[x.dtype], stride, per_pick, n_tok, ids.data_ptr(), k, ids_stride,
                                            dst.data_ptr(), ws_ptr, ws_bytes, st))

@@ -661,12 +661,12 @@ int moe_b200_w4_pack(const moe_w4 *w, const void *codes, const void *scales, con
  * An id of -1 marks an empty slot: its row of dst is left as it was. Any other id outside
  * [0, n_experts) also leaves its row and sets the device error word (MOE_DERR_BAD_ID). A
  * NaN or an infinity in a row of x makes that row's outputs NaN and no other's. n_tok may be 0.
- * Workspace: moe_b200_w4_workspace_size bytes of device memory, 16-byte aligned, no
- * initialisation needed (0, and NULL does, for up to 1024 picks and without ids; 0 also for
+ * Workspace: moe_b200_w4_workspace_size bytes of device memory (k 0: without ids), 16-byte
+ * aligned, no initialisation needed (0, and NULL does, for few rows of x; 0 also for
  * arguments that the call refuses); calls that overlap on the GPU must not share one,
  * captured graphs included. Allocates nothing, except that the first call on a device
  * makes its error word: not during stream capture (MOE_ERR_STATE). */
-size_t moe_b200_w4_workspace_size(const moe_w4 *w, int64_t n_tok, int64_t k, int32_t x_type);
+size_t moe_b200_w4_workspace_size(const moe_w4 *w, int64_t n_tok, int64_t k, int32_t x_type, int32_t x_per_pick);
 int moe_b200_w4_mul_mat_id(const moe_w4 *w, const moe_w4 *gate, const float *bias, const float *gate_bias, int32_t glu_op,
                            float glu_limit, const void *x, int32_t x_type, int64_t x_row_stride, int32_t x_per_pick,
                            int64_t n_tok, const int32_t *ids, int64_t k, int64_t ids_stride, float *dst, void *workspace,

@@ -58,13 +58,13 @@ def w4_values(codes, scales, zeros, K, group):
 
 def w4_tol(mag, K):
     """Of sum s (q - z) x, computed as the sum over groups of s (sum q x) - s z (sum x); mag = the sum of |s| (q + z) |x|,
-    which bounds every partial sum. Each of the 64 additions of a tile, on the tensor cores, may cut off 2^-23 of at most
-    mag. Every tile's scale and every group's s z (two roundings) are applied with a rounding each, 2^-24; so are the
+    which bounds every partial sum. Each of the up to 128 additions of two tiles, on the tensor cores, may cut off 2^-23 of at
+    most mag. Every tile's scale and every group's s z (two roundings) are applied with a rounding each, 2^-24; so are the
     sums of a stage, of up to 8 warps and 8 CTAs, of 2 planes and the bias (20), and the sums of x over a group
     (8 levels). A 32-bit x is held to 2^-22 of its value. What lies more than 2^24 below the largest x of its 256 values is
     cut off at 2^-39 of that: the largest is one of mag's, times at most 30 / 1 between (q + z) of two places,
     hence 256 * 30 * 2^-39 < 2^-26 of mag."""
-    return 1.01 * mag * (64 * 2.0 ** -23 + (K / 64 + 3 * (K / 32 + 1) + K / 256 + 20 + 8 + 2) * 2.0 ** -24 + 2.0 ** -22 + 2.0 ** -26) + 1e-36
+    return 1.01 * mag * (128 * 2.0 ** -23 + (K / 64 + 3 * (K / 32 + 1) + K / 256 + 20 + 8 + 2) * 2.0 ** -24 + 2.0 ** -22 + 2.0 ** -26) + 1e-36
 
 
 def glu(op, g, u, limit=0.0):
