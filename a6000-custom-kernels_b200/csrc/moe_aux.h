@@ -166,15 +166,14 @@ cudaError_t launch_mx_prep(const void *x, int xt, int64_t stride, int64_t n_rows
 // units: the largest possible number of chunks
 cudaError_t launch_mx_product(MxArgs &a, int NT, int64_t units, cudaStream_t st);
 
-// 4-bit matrices with group scales (moe_w4.cu): their layout; the product of n_tok * k entries, after
-// launch_mmq_group into a.entries / a.chunks (chunks of w4_chunk_entries), or alone for up to W4_DIRECT of them.
-// max_chunks: the largest possible number of chunks; per_stage: groups of a stage.
+// 4-bit matrices with group scales (moe_w4.cu): their layout, per_stage groups to a stage; the product of n_tok * k
+// entries. Above W4_DIRECT picks a.entries, a.chunks and a.n_chunks are memory for their grouping (as many chunks as
+// w4_min_chunk entries in each could make); where w4_staged says so `staged` is memory for x, w4_row_bytes a row.
 cudaError_t launch_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, int64_t E, int64_t rows, int64_t K,
                            int64_t group, int per_stage, uint8_t *out, int *err, cudaStream_t st);
-int w4_chunk_entries(int64_t n_tok, int64_t k, int64_t n_experts, bool one_matrix, int x_type);
-// staged: memory for x in the products' form (w4_row_bytes of every row), where w4_staged says so
+int w4_min_chunk(int x_type);
+bool w4_staged(int64_t n_tok, int64_t KS);
 int64_t w4_row_bytes(int64_t KS, int groups, int x_type);
-bool w4_staged(int64_t n_tok, int64_t k, int64_t n_experts, bool one_matrix, int64_t KS, int x_type);
-cudaError_t launch_w4(W4Args &a, int64_t n_tok, int64_t max_chunks, uint8_t *staged, cudaStream_t st);
+cudaError_t launch_w4(W4Args &a, int64_t n_tok, uint8_t *staged, cudaStream_t st);
 
 }  // namespace moe

@@ -2549,22 +2549,19 @@ struct W4Ws {
     uint8_t *staged;
     int32_t *entries, *n_chunks;
     int4 *chunks;
-    int64_t max_chunks;
     size_t bytes;
 };
 
 W4Ws w4_ws(int64_t E, const W4Shape &s, int64_t n_tok, int64_t k, int elem, bool per_pick, bool one_matrix, char *base) {
     W4Ws w{};
-    const int nc = moe::w4_chunk_entries(n_tok, k, E, one_matrix, elem);
     const int64_t n = n_tok * k;
     size_t off = 0;
     auto take = [&](size_t bytes) { char *p = base ? base + off : nullptr; off += align256(bytes); return p; };
-    if (moe::w4_staged(n_tok, k, E, one_matrix, s.KS, elem))
+    if (moe::w4_staged(n_tok, s.KS))
         w.staged = reinterpret_cast<uint8_t *>(take(static_cast<size_t>((per_pick ? n : n_tok) * moe::w4_row_bytes(s.KS, s.per_stage, elem))));
-    w.max_chunks = one_matrix ? (n + nc - 1) / nc : std::min(n, moe::mmq_max_chunks(n, E, nc));
     if (!one_matrix && n > moe::W4_DIRECT) {
         w.entries = reinterpret_cast<int32_t *>(take(4 * static_cast<size_t>(n)));
-        w.chunks = reinterpret_cast<int4 *>(take(16 * static_cast<size_t>(moe::mmq_max_chunks(n, E, nc))));
+        w.chunks = reinterpret_cast<int4 *>(take(16 * static_cast<size_t>(moe::mmq_max_chunks(n, E, moe::w4_min_chunk(elem)))));
         w.n_chunks = reinterpret_cast<int32_t *>(take(4));
     }
     w.bytes = off;
@@ -2634,7 +2631,8 @@ int moe_b200_w4_mul_mat_id(const moe_w4 *w, const moe_w4 *gate, const float *bia
     if (ws.bytes && (!workspace || workspace_bytes < ws.bytes))
         return fail(MOE_ERR_INVALID, "workspace too small (%zu < %zu bytes)", workspace_bytes, ws.bytes);
     if (!aligned16(workspace)) return fail(MOE_ERR_INVALID, "workspace must be 16-byte aligned");
-    if (ws.max_chunks * s.RT > (int64_t{1} << 30)) return fail(MOE_ERR_UNSUPPORTED, "too many tiles in one call");
+    const int64_t most = std::min(n_tok * k, moe::mmq_max_chunks(n_tok * k, w->n_experts, moe::w4_min_chunk(xt)));   // chunks
+    if (most * s.RT > (int64_t{1} << 29)) return fail(MOE_ERR_UNSUPPORTED, "too many tiles in one call");
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     moe::W4Args a{};
     rc = error_word(st, &a.err);
@@ -2670,11 +2668,8 @@ int moe_b200_w4_mul_mat_id(const moe_w4 *w, const moe_w4 *gate, const float *bia
         a.entries = ws.entries;
         a.chunks = ws.chunks;
         a.n_chunks = ws.n_chunks;
-        CK(moe::launch_mmq_group(ids, ids_stride, static_cast<int>(n_tok), a.k, a.n_experts,
-                                 moe::w4_chunk_entries(n_tok, k, w->n_experts, false, xt), ws.entries, ws.chunks, ws.n_chunks, a.err,
-                                 st, true));
     }
-    CK(moe::launch_w4(a, n_tok, ws.max_chunks, ws.staged, st));
+    CK(moe::launch_w4(a, n_tok, ws.staged, st));
     return MOE_OK;
 }
 

@@ -24,13 +24,11 @@
 //   order), and a CTA then holds its share of x only.
 #include "moe_aux.h"
 #include "moe_mx.cuh"
+#include "moe_mmq.cuh"
 #include "moe_w4.cuh"
 
 #include <type_traits>
-#ifdef W4_TUNE
-#include <cstdio>
-#include <cstdlib>
-#endif
+#include <cstring>
 
 namespace moe {
 
@@ -44,10 +42,6 @@ constexpr int W4_ACC = 8 * 1024;         // of it at most for sums kept to a run
 constexpr float W4_CODE = 0x1p-24f;      // a code's unit in rows g (times 16 in rows g + 8)
 constexpr float W4_UP = 4096.f;          // which comes off in two factors: with x's power of two, and at the end
 constexpr float W4_PLANE = 4096.f;       // the second plane of an f32 x holds what the first one leaves, times this
-
-// What the plan counts with: a warp's stage where the SM is full, and by itself; adding up a row tile's sums; a row's
-// 256 values of x
-constexpr double W4_STAGE_US = 0.055, W4_STAGE_LATENCY_US = 0.35, W4_SUM_US = 0.03, W4_X_US = 0.02;
 
 // stages in flight per warp
 template <int NT>
@@ -637,13 +631,9 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 2) w4_kernel(const __grid_const
                     };
                     if constexpr (NT == 1) {
                         run(std::integral_constant<int, 1>{});
-                    } else if constexpr (NT == 2) {
+                    } else {
                         if (cols <= 8) run(std::integral_constant<int, 1>{});
                         else run(std::integral_constant<int, 2>{});
-                    } else {
-                        if (cols <= 16) run(std::integral_constant<int, 2>{});
-                        else if (cols <= 24) run(std::integral_constant<int, 3>{});
-                        else run(std::integral_constant<int, 4>{});
                     }
                     // the sums of the warps that share K meet; codes' units come off
                     float *mine_at = red + buf * RED_BUF + warp * COLS * W4_RED + 2 * t * W4_RED + g;
@@ -671,8 +661,7 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 2) w4_kernel(const __grid_const
                         if (S > 1 || pass + 1 < a.passes || mat + 1 < a.mats) *kept = v;
                         else emit(rt * W4_M + r, col, v, a.mats > 1 ? kept[-(WM * outs1 / 4)] : v);
                     }
-                    if (NT > 2) group_sync();   // one buffer
-                    else buf ^= 1;
+                    buf ^= 1;
                 }
             }
         }
@@ -715,28 +704,53 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 2) w4_kernel(const __grid_const
     cp_wait_all();
 }
 
-// How the rows and K are shared out: the plan with the least time by this count, in us. A CTA has up to eight
-// warps at work: wm row tiles, K of each shared by 1 << wk_shift warps and `split` CTAs.
+// How the columns, the rows and K are shared out. A CTA has up to eight warps at work: wm row tiles, K of each shared by
+// 1 << wk_shift warps and `split` CTAs; chunks have up to 8 NT MMA columns. Of all such plans the one with the least
+// time by the count below is taken; its constants were fitted to 22 calls (one matrix of 768 x 2048 to 32768 x 4096 with 1 to
+// 64 rows of x, experts with 1 to 64 tokens) timed in every plan, and its choice is 4 % slower than the best of them on
+// average, 19 % at most. Plans with 32 columns, or with clusters of eight, were never the best by more than 1 %.
 struct W4Plan {
-    int split, wk_shift, wm, passes, sp, seg;
-    uint32_t acc;
+    int nt, split, wk_shift, wm, passes, sp, seg;
+    uint32_t acc, tab;
     double us;
 };
 
-W4Plan w4_plan(const W4Args &a, uint32_t fixed, int cols, int x_stage, int64_t chunks, int n_sm) {
-    W4Plan best{};
-    best.us = 1e30;
-    for (int split = 1; split <= 8 && (split == 1 || split <= a.KS); split *= 2)
+// what a plan depends on
+struct W4Key {
+    int64_t n_tok, RT, KS;
+    int32_t k, n_experts, one_matrix, planes, mats, groups, zeros, n_sm;
+};
+
+int w4_ring(int nt) { return nt == 1 ? w4_stages<1>() : w4_stages<2>(); }
+uint32_t w4_red_bytes(int nt) { return 2 * W4_WARPS * nt * 8 * W4_RED * 4; }
+
+void w4_plan(const W4Key &c, int nt, W4Plan &best) {
+    const int nc = 8 * nt / c.planes;
+    const int64_t n = c.n_tok * c.k;
+    const int cols = static_cast<int>(n < nc ? n : nc) * c.planes;
+    const uint32_t tab = !c.one_matrix && n <= W4_DIRECT ? (static_cast<uint32_t>(n) * 10 + 15) / 16 * 16 : 0;
+    const int64_t fixed = static_cast<int64_t>(W4_WARPS) * w4_ring(nt) * w4_stage_bytes(c.groups, c.zeros != 0) + w4_red_bytes(nt) + tab;
+    const int x_stage = (c.groups + 1) * 8 * nt * 4;   // bytes of a stage's sums of x
+    // chunks to expect: those of the experts that even picks would touch, and some of the crowded ones'
+    int64_t chunks = (n + nc - 1) / nc;
+    if (!c.one_matrix) {
+        const int64_t touched = n < c.n_experts ? n : c.n_experts;
+        chunks = touched + n / (2 * nc) < n ? touched + n / (2 * nc) : n;
+    }
+    const double mean = c.one_matrix ? cols / c.planes : static_cast<double>(n) / static_cast<double>(chunks);
+    const double entries = mean < 1.0 ? 1.0 : mean < nc ? mean : nc;   // of a chunk
+    const bool wide = entries * c.planes > 8, staged = w4_staged(c.n_tok, c.KS);
+    for (int split = 1; split <= 4 && (split == 1 || split <= c.KS); split *= 2)
         for (int wk = 0; wk <= 3; ++wk)
             for (int wm = 1; wm << wk <= W4_WARPS; ++wm) {
-                const int WK = 1 << wk, spr = (a.KS + split - 1) / split;
-                if ((WK > 1 && WK / 2 >= spr) || (wm > 1 && wm > a.RT)) continue;
-                const uint32_t one = static_cast<uint32_t>(a.nc * wm * W4_M * a.mats) * 4;   // a row block's sums
-                W4Plan p{split, wk, wm, 1, a.KS, 1 << 29, 0, 0.0};
+                const int WK = 1 << wk, KS = static_cast<int>(c.KS), spr = (KS + split - 1) / split;
+                if ((WK > 1 && WK / 2 >= spr) || (wm > 1 && wm > c.RT)) continue;
+                const uint32_t one = static_cast<uint32_t>(nc * wm * W4_M * c.mats) * 4;   // a row block's sums
+                W4Plan p{nt, split, wk, wm, 1, KS, 1 << 29, 0, tab, 0.0};
                 bool hold = split > 1;
                 auto room_for_x = [&]() {   // stages of x that fit
-                    p.acc = hold ? (one > W4_ACC ? one : W4_ACC / one * one) : a.mats > 1 ? one : 0;
-                    const int64_t left = static_cast<int64_t>(W4_SMEM) - fixed - p.acc - cols * W4_PAD;
+                    p.acc = hold ? (one > W4_ACC ? one : W4_ACC / one * one) : c.mats > 1 ? one : 0;
+                    const int64_t left = W4_SMEM - fixed - p.acc - cols * W4_PAD;
                     return left < 0 ? 0 : static_cast<int>(left / (cols * 2 * W4_KS + x_stage));
                 };
                 int fit = room_for_x();
@@ -745,59 +759,66 @@ W4Plan w4_plan(const W4Args &a, uint32_t fixed, int cols, int x_stage, int64_t c
                     fit = room_for_x();
                     if (fit < 1) continue;
                     p.passes = (spr + fit - 1) / fit;
-                    p.sp = (a.KS + p.passes - 1) / p.passes;
+                    p.sp = (KS + p.passes - 1) / p.passes;
                     if ((p.sp + split - 1) / split > fit) p.sp = fit * split;
-                    p.passes = (a.KS + p.sp - 1) / p.sp;
+                    p.passes = (KS + p.sp - 1) / p.sp;
                 }
                 if (hold) p.seg = static_cast<int>(p.acc / one);
                 const int mine = (p.sp + split - 1) / split;                    // stages of a CTA in a pass
-                const int deep = a.mats * p.passes * ((mine + WK - 1) / WK);    // of a warp for a row block
-                const int64_t items = chunks * ((a.RT + wm - 1) / wm), slots = 2 * n_sm / split;
-                const int64_t rounds = (items + slots - 1) / slots, of_sm = (items * split + n_sm - 1) / n_sm;
-                const double full = of_sm * (wm * WK) * (deep * W4_STAGE_US + a.mats * p.passes * W4_SUM_US);
-                const double deepest = rounds * (deep * W4_STAGE_LATENCY_US + a.mats * p.passes * 0.2);
-                const int64_t runs = p.passes > 1 || split > 1 ? (rounds + p.seg - 1) / p.seg : 1;
-                const double x = (p.passes > 1 ? runs * p.passes : 1) * (0.3 + cols / a.planes * mine * W4_X_US);
-                p.us = (full > deepest ? full : deepest) + x + (split > 1 ? 0.8 * runs : 0.0);
-#ifdef W4_TUNE
-                const char *force = getenv("W4_FORCE");
-                if (force && (atoi(force) / 100 != split || atoi(force) / 10 % 10 != wk || atoi(force) % 10 != wm)) continue;
-#endif
+                const int sums = c.mats * p.passes, deep = sums * ((mine + WK - 1) / WK);   // of a warp, for a row block
+                const int64_t blocks = (c.RT + wm - 1) / wm, items = chunks * blocks, slots = 2 * c.n_sm / split;
+                const double rounds = static_cast<double>((items + slots - 1) / slots);
+                const double of_sm = static_cast<double>((items * split + c.n_sm - 1) / c.n_sm);
+                // the SM's issue slots, and the way through one CTA's row blocks
+                const double full = of_sm * (wm * WK) *
+                                    (deep * (0.0464 + (wide ? 0.0051 : 0.0) + (c.groups == 8 ? 0.0084 : 0.0)) + sums * 0.0806 * (0.5 + entries / 8));
+                const double one_by_one = rounds * (deep * (wide ? 0.717 : 0.393) + sums * 0.544);
+                // bringing x, once for every chunk that a CTA meets, or for every pass of every run
+                const double runs = p.passes > 1 || split > 1 ? static_cast<double>((static_cast<int64_t>(rounds) + p.seg - 1) / p.seg) : 1.0;
+                const double met = 1.0 + rounds / static_cast<double>(blocks);
+                const double bring = 1.3 + entries * mine * c.planes * (staged ? 0.0079 : 0.039);
+                p.us = (full > one_by_one ? full : one_by_one) + (p.passes > 1 ? runs * p.passes : rounds < met ? rounds : met) * bring +
+                       (split > 1 ? runs * (1.7 + 0.0154 * wm * entries) : 0.0);
                 if (p.us < best.us) best = p;
             }
-    return best;
+}
+
+// the plan of a call, remembered by its sizes (working it out takes some microseconds; the caller holds the library's lock)
+const W4Plan &w4_plan_of(const W4Key &c) {
+    static struct { W4Key key; W4Plan plan; } seen[256];
+    uint64_t h = 0;
+    for (size_t i = 0; i < sizeof(W4Key) / 4; ++i) {
+        uint32_t v;
+        memcpy(&v, reinterpret_cast<const char *>(&c) + 4 * i, 4);
+        h = (h ^ v) * 0x9E3779B97F4A7C15ull;
+    }
+    auto &slot = seen[h >> 56];
+    if (slot.plan.nt == 0 || memcmp(&slot.key, &c, sizeof(c))) {
+        W4Plan best{};
+        best.us = 1e30;
+        w4_plan(c, 1, best);
+        w4_plan(c, 2, best);
+        slot.key = c;
+        slot.plan = best;
+    }
+    return slot.plan;
 }
 
 template <int NT, bool ZERO, int GROUPS, bool SCALE_BF16>
-cudaError_t w4_t(W4Args &a, int64_t max_chunks, cudaStream_t st) {
+cudaError_t w4_t(W4Args &a, const W4Plan &p, int64_t max_chunks, int n_sm, cudaStream_t st) {
     static bool configured[64] = {};
-    static int sms[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     if (!configured[dev]) {
-        cudaError_t e = cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
-        if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(w4_kernel<NT, ZERO, GROUPS, SCALE_BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_SMEM);
+        const cudaError_t e = cudaFuncSetAttribute(w4_kernel<NT, ZERO, GROUPS, SCALE_BF16>,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, W4_SMEM);
         if (e != cudaSuccess) return e;
         configured[dev] = true;
     }
     static_assert(W4_WARPS * w4_stages<NT>() * W4_CODES >= W4_WARPS * W4_MAX_EXPERTS * 4, "the grouping counts in the ring");
-    const uint32_t ring = W4_WARPS * w4_stages<NT>() * w4_stage_bytes(GROUPS, ZERO);
-    const uint32_t red = (NT > 2 ? 1 : 2) * W4_WARPS * NT * 8 * W4_RED * 4;
-    const uint32_t tab = a.ids && !a.chunks ? (static_cast<uint32_t>(a.n_entries) * 10 + 15) / 16 * 16 : 0;
-    constexpr int x_stage = (GROUPS + 1) * 8 * NT * 4;   // bytes of a stage's sums of x
-    const int most = a.n_entries < a.nc ? a.n_entries : a.nc, cols = most * a.planes;
-    // chunks to expect: those of the experts that even picks would touch
-    int64_t chunks = max_chunks;
-    if (a.ids) {
-        const int64_t touched = a.n_entries < a.n_experts ? a.n_entries : a.n_experts;
-        chunks = touched + a.n_entries / (2 * a.nc);
-        chunks = chunks < max_chunks ? chunks : max_chunks;
-    }
-    const W4Plan p = w4_plan(a, ring + red + tab, cols, x_stage, chunks, sms[dev]);
-    if (p.split == 0) return cudaErrorInvalidConfiguration;
-    a.split_shift = p.split == 1 ? 0 : p.split == 2 ? 1 : p.split == 4 ? 2 : 3;
+    const int most = a.n_entries < a.nc ? a.n_entries : a.nc, mine = (p.sp + p.split - 1) / p.split;
+    a.split_shift = p.split == 1 ? 0 : p.split == 2 ? 1 : 2;
     a.wk_shift = p.wk_shift;
     a.wm = p.wm;
     a.x_shift = most >= 8 ? 0 : most >= 4 ? 1 : most >= 2 ? 2 : 3;
@@ -806,17 +827,14 @@ cudaError_t w4_t(W4Args &a, int64_t max_chunks, cudaStream_t st) {
     a.sp = p.sp;
     a.seg = p.seg;
     a.tiles = (a.RT + p.wm - 1) / p.wm;
-    a.red_off = ring;
-    a.tab_off = ring + red;
-    a.acc_off = a.tab_off + tab;
+    a.red_off = W4_WARPS * w4_stages<NT>() * w4_stage_bytes(GROUPS, ZERO);
+    a.tab_off = a.red_off + w4_red_bytes(NT);
+    a.acc_off = a.tab_off + p.tab;
     a.x_off = a.acc_off + p.acc;
-    const int mine = (p.sp + p.split - 1) / p.split;
-    const size_t smem = a.x_off + static_cast<size_t>(cols) * (mine * 2 * W4_KS + W4_PAD) + static_cast<size_t>(mine) * x_stage;
-#ifdef W4_TUNE
-    if (getenv("W4_SHOW")) fprintf(stderr, "NT %d cols %d chunks %ld split %d wk %d wm %d passes %d sp %d seg %d acc %u smem %zu us %.1f\n", NT, cols, (long)chunks, p.split, p.wk_shift, p.wm, p.passes, p.sp, p.seg, p.acc, smem, p.us);
-#endif
+    const size_t smem = a.x_off + static_cast<size_t>(most * a.planes) * (mine * 2 * W4_KS + W4_PAD) +
+                        static_cast<size_t>(mine) * (GROUPS + 1) * 8 * NT * 4;
     if (smem > W4_SMEM) return cudaErrorInvalidConfiguration;
-    const int64_t items = max_chunks * a.tiles, slots = 2 * sms[dev] / p.split;
+    const int64_t items = max_chunks * a.tiles, slots = 2 * n_sm / p.split;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>((items < slots ? items : slots) * p.split));
     cfg.blockDim = dim3(32 * W4_WARPS);
@@ -834,41 +852,36 @@ cudaError_t w4_t(W4Args &a, int64_t max_chunks, cudaStream_t st) {
 }
 
 template <int NT, bool ZERO, bool SCALE_BF16>
-cudaError_t w4_groups(W4Args &a, int64_t max_chunks, cudaStream_t st) {
+cudaError_t w4_groups(W4Args &a, const W4Plan &p, int64_t max_chunks, int n_sm, cudaStream_t st) {
     switch (a.groups) {
-        case 8: return w4_t<NT, ZERO, 8, SCALE_BF16>(a, max_chunks, st);
-        case 4: return w4_t<NT, ZERO, 4, SCALE_BF16>(a, max_chunks, st);
-        case 2: return w4_t<NT, ZERO, 2, SCALE_BF16>(a, max_chunks, st);
-        default: return w4_t<NT, ZERO, 1, SCALE_BF16>(a, max_chunks, st);
+        case 8: return w4_t<NT, ZERO, 8, SCALE_BF16>(a, p, max_chunks, n_sm, st);
+        case 4: return w4_t<NT, ZERO, 4, SCALE_BF16>(a, p, max_chunks, n_sm, st);
+        case 2: return w4_t<NT, ZERO, 2, SCALE_BF16>(a, p, max_chunks, n_sm, st);
+        default: return w4_t<NT, ZERO, 1, SCALE_BF16>(a, p, max_chunks, n_sm, st);
     }
 }
 
 template <int NT>
-cudaError_t w4_nt(W4Args &a, int64_t max_chunks, cudaStream_t st) {
+cudaError_t w4_nt(W4Args &a, const W4Plan &p, int64_t max_chunks, int n_sm, cudaStream_t st) {
     if (a.scale_type == MX_BF16)
-        return a.zeros ? w4_groups<NT, true, true>(a, max_chunks, st) : w4_groups<NT, false, true>(a, max_chunks, st);
-    return a.zeros ? w4_groups<NT, true, false>(a, max_chunks, st) : w4_groups<NT, false, false>(a, max_chunks, st);
-}
-
-// MMA columns of 8: as few as hold a call's rows, for experts the average load and a half
-int w4_tiles_n(int64_t n_tok, int64_t k, int64_t n_experts, bool one_matrix, int planes) {
-    int64_t most = n_tok;
-    if (!one_matrix) {
-        const int64_t mean = (3 * n_tok * k + 2 * n_experts - 1) / (2 * n_experts);
-        most = mean < n_tok ? mean : n_tok;
-    }
-#ifdef W4_TUNE
-    if (getenv("W4_NT")) return atoi(getenv("W4_NT"));
-#endif
-    return most * planes <= 8 ? 1 : most * planes <= 16 ? 2 : 4;
+        return a.zeros ? w4_groups<NT, true, true>(a, p, max_chunks, n_sm, st) : w4_groups<NT, false, true>(a, p, max_chunks, n_sm, st);
+    return a.zeros ? w4_groups<NT, true, false>(a, p, max_chunks, n_sm, st) : w4_groups<NT, false, false>(a, p, max_chunks, n_sm, st);
 }
 
 }  // namespace
 
-int w4_chunk_entries(int64_t n_tok, int64_t k, int64_t n_experts, bool one_matrix, int x_type) {
+// Whether a call brings x into the products' form first, once, rather than in every CTA: the launch costs 0.5 us of a
+// token's 5 (K = 2048), and saves 6 of 16 rows' 29 (one matrix, K = 4096, 32768 rows: 30.4 us for 8 rows without, 23.3 with).
+bool w4_staged(int64_t n_tok, int64_t KS) { return n_tok * KS > 32; }
+
+// bytes of a row of x in that form
+int64_t w4_row_bytes(int64_t KS, int groups, int x_type) {
     const int planes = x_type == MX_F32 ? 2 : 1;
-    return 8 * w4_tiles_n(n_tok, k, n_experts, one_matrix, planes) / planes;
+    return KS * ((planes * (2 * W4_KS + 4 * (groups + 1)) + 15) / 16 * 16);
 }
+
+// entries of a chunk at least
+int w4_min_chunk(int x_type) { return x_type == MX_F32 ? 4 : 8; }
 
 cudaError_t launch_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, int64_t E, int64_t rows, int64_t K,
                            int64_t group, int per_stage, uint8_t *out, int *err, cudaStream_t st) {
@@ -881,23 +894,35 @@ cudaError_t launch_w4_pack(const uint8_t *codes, const void *scales, const uint8
     return cudaGetLastError();
 }
 
-// bytes of a row of x brought into the products' form
-int64_t w4_row_bytes(int64_t KS, int groups, int x_type) {
-    const int planes = x_type == MX_F32 ? 2 : 1;
-    return KS * ((planes * (2 * W4_KS + 4 * (groups + 1)) + 15) / 16 * 16);
-}
-
-// Whether a call brings x into that form first, once, rather than in every CTA
-bool w4_staged(int64_t n_tok, int64_t k, int64_t n_experts, bool one_matrix, int64_t KS, int x_type) {
-#ifdef W4_TUNE
-    if (getenv("W4_PRE")) return atoi(getenv("W4_PRE"));
-#endif
-    (void)k, (void)n_experts, (void)one_matrix, (void)x_type;
-    return n_tok * KS > 32;
-}
-
-cudaError_t launch_w4(W4Args &a, int64_t n_tok, int64_t max_chunks, uint8_t *staged, cudaStream_t st) {
+cudaError_t launch_w4(W4Args &a, int64_t n_tok, uint8_t *staged, cudaStream_t st) {
+    static int sms[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!sms[dev]) {
+        const cudaError_t e = cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
+        if (e != cudaSuccess) return e;
+    }
     a.planes = a.x_type == MX_F32 ? 2 : 1;
+    W4Key c;
+    memset(&c, 0, sizeof(c));   // (compared byte by byte)
+    c.n_tok = n_tok, c.RT = a.RT, c.KS = a.KS;
+    c.k = a.k, c.n_experts = a.n_experts, c.one_matrix = a.ids == nullptr, c.planes = a.planes, c.mats = a.mats;
+    c.groups = a.groups, c.zeros = a.zeros, c.n_sm = sms[dev];
+    const W4Plan p = w4_plan_of(c);
+    if (p.nt == 0) return cudaErrorInvalidConfiguration;
+    a.nc = 8 * p.nt / a.planes;
+    int64_t max_chunks = (a.n_entries + a.nc - 1) / a.nc;
+    if (a.ids) {
+        max_chunks = mmq_max_chunks(a.n_entries, a.n_experts, a.nc);
+        if (max_chunks > a.n_entries) max_chunks = a.n_entries;
+    }
+    if (a.chunks) {
+        const cudaError_t e = launch_mmq_group(a.ids, a.ids_stride, static_cast<int>(n_tok), a.k, a.n_experts, a.nc,
+                                               const_cast<int32_t *>(a.entries), const_cast<int4 *>(a.chunks),
+                                               const_cast<int32_t *>(a.n_chunks), a.err, st, true);
+        if (e != cudaSuccess) return e;
+    }
     if (staged) {
         a.unit = static_cast<int32_t>(w4_row_bytes(1, a.groups, a.x_type));
         const int64_t units = (a.per_pick ? static_cast<int64_t>(a.n_entries) : n_tok) * a.KS;
@@ -910,10 +935,7 @@ cudaError_t launch_w4(W4Args &a, int64_t n_tok, int64_t max_chunks, uint8_t *sta
         if (e != cudaSuccess) return e;
         a.staged = staged;
     }
-    const int NT = w4_tiles_n(n_tok, a.k, a.n_experts, a.ids == nullptr, a.planes);
-    a.nc = 8 * NT / a.planes;
-    if (NT == 1) return w4_nt<1>(a, max_chunks, st);
-    return NT == 2 ? w4_nt<2>(a, max_chunks, st) : w4_nt<4>(a, max_chunks, st);
+    return p.nt == 1 ? w4_nt<1>(a, p, max_chunks, c.n_sm, st) : w4_nt<2>(a, p, max_chunks, c.n_sm, st);
 }
 
 }  // namespace moe
