@@ -165,6 +165,7 @@ def _declare(L):
                                             ctypes.c_float, vp, i32, i64, i32, i64, vp, i64, i64, i32, vp, vp, sz, vp]),
         "moe_b200_sort_by_expert": (i32, [vp, i64, i64, i64, i64, vp, vp, vp, vp, vp]),
         "moe_b200_gather_sorted": (i32, [vp, i32, i64, i64, i64, i64, vp, vp, vp, vp]),
+        "moe_b200_dispatch_sorted": (i32, [vp, i32, i64, i64, vp, i64, i64, i64, i64, vp, vp, vp, vp, vp, vp]),
         "moe_b200_combine_sorted": (i32, [vp, i32, i64, i64, i64, i64, vp, vp, vp, i64, vp, vp]),
         "moe_b200_combine_sorted_grad": (i32, [vp, i32, i64, vp, i64, i64, i64, i64, vp, vp, vp, vp, vp, vp]),
         "moe_b200_w4_packed_size": (sz, [ctypes.POINTER(MoeW4)]),

@@ -145,6 +145,7 @@ struct RowArgs {
     int32_t tpt, per_cta;    // set by the launchers: log2 of a token's threads, of a CTA's tokens
 };
 cudaError_t launch_gather_sorted(RowArgs a, int type, cudaStream_t st);
+cudaError_t launch_dispatch_sorted(const SortArgs &s, RowArgs a, int type, cudaStream_t st);   // both of the above
 cudaError_t launch_combine_sorted(RowArgs a, int type, cudaStream_t st);
 cudaError_t launch_combine_sorted_grad(const RowArgs &a, int type, cudaStream_t st);
 

@@ -2421,6 +2421,43 @@ moe::RowArgs row_args(int32_t type, int64_t n_tok, int64_t k, int64_t H, const i
     return a;
 }
 
+int sort_args(const int32_t *ids, int64_t ids_stride, int64_t n_tok, int64_t k, int64_t n_experts, int32_t *rows,
+              int32_t *positions, int32_t *experts, int32_t *offsets, moe_stream_t stream, moe::SortArgs *a) {
+    const int rc = sorted_check(MOE_TYPE_F32, n_tok, k, 1);
+    if (rc) return rc;
+    if (n_experts < 1 || n_experts > moe::SORT_MAX_EXPERTS)
+        return fail(MOE_ERR_UNSUPPORTED, "need 1 <= n_experts <= %d", moe::SORT_MAX_EXPERTS);
+    if (ids_stride < k) return fail(MOE_ERR_INVALID, "need ids_stride >= k");
+    if (!offsets || (n_tok && (!ids || !rows || !positions || !experts))) return fail(MOE_ERR_INVALID, "null argument");
+    const int erc = error_word(reinterpret_cast<cudaStream_t>(stream), &a->err);
+    if (erc) return erc;
+    a->ids = ids;
+    a->ids_stride = ids_stride;
+    a->n_entries = static_cast<int32_t>(n_tok * k);
+    a->k = static_cast<int32_t>(k);
+    a->n_experts = static_cast<int32_t>(n_experts);
+    a->rows = rows;
+    a->positions = positions;
+    a->experts = experts;
+    a->offsets = offsets;
+    return MOE_OK;
+}
+
+int gather_args(const void *x, int32_t type, int64_t x_row_stride, int64_t n_tok, int64_t k, int64_t H, const int32_t *positions,
+                const int32_t *n_sorted, void *out, moe::RowArgs *a) {
+    const int rc = sorted_check(type, n_tok, k, H);
+    if (rc) return rc;
+    if (x_row_stride < H) return fail(MOE_ERR_INVALID, "row stride below H");
+    if (n_tok && (!x || !positions || !n_sorted || !out || !aligned_elem(x, type) || !aligned_elem(out, type)))
+        return fail(MOE_ERR_INVALID, "null or misaligned argument");
+    *a = row_args(type, n_tok, k, H, positions);
+    a->src = static_cast<const char *>(x);
+    a->src_stride = x_row_stride * static_cast<int64_t>(elem_size(type));
+    a->out = static_cast<char *>(out);
+    a->live = n_sorted;
+    return MOE_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -2428,44 +2465,34 @@ extern "C" {
 int moe_b200_sort_by_expert(const int32_t *ids, int64_t ids_stride, int64_t n_tok, int64_t k, int64_t n_experts,
                             int32_t *rows, int32_t *positions, int32_t *experts, int32_t *offsets, moe_stream_t stream) {
     std::lock_guard<std::recursive_mutex> lock(g_mu);
-    const int rc = sorted_check(MOE_TYPE_F32, n_tok, k, 1);
-    if (rc) return rc;
-    if (n_experts < 1 || n_experts > moe::SORT_MAX_EXPERTS)
-        return fail(MOE_ERR_UNSUPPORTED, "need 1 <= n_experts <= %d", moe::SORT_MAX_EXPERTS);
-    if (ids_stride < k) return fail(MOE_ERR_INVALID, "need ids_stride >= k");
-    if (!offsets || (n_tok && (!ids || !rows || !positions || !experts))) return fail(MOE_ERR_INVALID, "null argument");
-    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     moe::SortArgs a{};
-    const int erc = error_word(st, &a.err);
-    if (erc) return erc;
-    a.ids = ids;
-    a.ids_stride = ids_stride;
-    a.n_entries = static_cast<int32_t>(n_tok * k);
-    a.k = static_cast<int32_t>(k);
-    a.n_experts = static_cast<int32_t>(n_experts);
-    a.rows = rows;
-    a.positions = positions;
-    a.experts = experts;
-    a.offsets = offsets;
-    CK(moe::launch_sort(a, st));
+    const int rc = sort_args(ids, ids_stride, n_tok, k, n_experts, rows, positions, experts, offsets, stream, &a);
+    if (rc) return rc;
+    CK(moe::launch_sort(a, reinterpret_cast<cudaStream_t>(stream)));
     return MOE_OK;
 }
 
 int moe_b200_gather_sorted(const void *x, int32_t type, int64_t x_row_stride, int64_t n_tok, int64_t k, int64_t H,
                            const int32_t *positions, const int32_t *n_sorted, void *out, moe_stream_t stream) {
     std::lock_guard<std::recursive_mutex> lock(g_mu);
-    const int rc = sorted_check(type, n_tok, k, H);
-    if (rc) return rc;
-    if (x_row_stride < H) return fail(MOE_ERR_INVALID, "row stride below H");
-    if (n_tok == 0) return MOE_OK;
-    if (!x || !positions || !n_sorted || !out || !aligned_elem(x, type) || !aligned_elem(out, type))
-        return fail(MOE_ERR_INVALID, "null or misaligned argument");
-    moe::RowArgs a = row_args(type, n_tok, k, H, positions);
-    a.src = static_cast<const char *>(x);
-    a.src_stride = x_row_stride * static_cast<int64_t>(elem_size(type));
-    a.out = static_cast<char *>(out);
-    a.live = n_sorted;
+    moe::RowArgs a{};
+    const int rc = gather_args(x, type, x_row_stride, n_tok, k, H, positions, n_sorted, out, &a);
+    if (rc || n_tok == 0) return rc;
     CK(moe::launch_gather_sorted(a, mx_elem(type), reinterpret_cast<cudaStream_t>(stream)));
+    return MOE_OK;
+}
+
+int moe_b200_dispatch_sorted(const void *x, int32_t type, int64_t x_row_stride, int64_t H, const int32_t *ids, int64_t ids_stride,
+                             int64_t n_tok, int64_t k, int64_t n_experts, int32_t *rows, int32_t *positions, int32_t *experts,
+                             int32_t *offsets, void *out, moe_stream_t stream) {
+    std::lock_guard<std::recursive_mutex> lock(g_mu);
+    moe::SortArgs s{};
+    moe::RowArgs a{};
+    int rc = gather_args(x, type, x_row_stride, n_tok, k, H, positions, offsets ? offsets + n_experts : nullptr, out, &a);
+    if (rc) return rc;
+    rc = sort_args(ids, ids_stride, n_tok, k, n_experts, rows, positions, experts, offsets, stream, &s);
+    if (rc) return rc;
+    CK(moe::launch_dispatch_sorted(s, a, mx_elem(type), reinterpret_cast<cudaStream_t>(stream)));
     return MOE_OK;
 }
 

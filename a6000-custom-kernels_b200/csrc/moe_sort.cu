@@ -27,6 +27,7 @@ namespace {
 // shared memory.
 constexpr int SORT_THREADS = 1024;
 constexpr int SORT_CTAS = 8;
+constexpr int SORT_AHEAD = 8;   // loads in flight per lane
 
 __device__ __forceinline__ void sort_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -37,6 +38,20 @@ __device__ __forceinline__ int ld_cluster_s32(uint32_t saddr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
     asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
     return v;
+}
+
+// The places of a warp's entries among its earlier ones of their expert, whose counts go up; -1 for id -1.
+__device__ __forceinline__ int warp_rank(int *count, int id, int lane) {
+    const unsigned peers = __match_any_sync(0xffffffffu, id);
+    const int leader = __ffs(peers) - 1;
+    int before = 0;
+    if (id >= 0 && lane == leader) {
+        before = count[id];
+        count[id] = before + __popc(peers);
+    }
+    before = __shfl_sync(0xffffffffu, before, leader);
+    __syncwarp();
+    return id >= 0 ? before + __popc(peers & ((1u << lane) - 1u)) : -1;
 }
 
 template <int CTAS>
@@ -58,22 +73,23 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(const SortArgs a) {
         const int t = i / k;
         return a.ids[static_cast<int64_t>(t) * a.ids_stride + (i - t * k)];
     };
-    for (int64_t i0 = lo; i0 < hi; i0 += 32) {
-        const int i = static_cast<int>(i0) + lane;
-        const int id = i < N ? id_of(i) : -1;
-        const bool ok = id >= 0 && id < E;
-        if (!ok && id != -1) set_error(a.err, DERR_BAD_ID);
-        const unsigned peers = __match_any_sync(0xffffffffu, ok ? id : -1);
-        const int leader = __ffs(peers) - 1;
-        int before = 0;
-        if (ok && lane == leader) {
-            before = count[id];
-            count[id] = before + __popc(peers);
+    for (int64_t i0 = lo; i0 < hi; i0 += 32 * SORT_AHEAD) {
+        int id[SORT_AHEAD];
+#pragma unroll
+        for (int u = 0; u < SORT_AHEAD; ++u) {
+            const int64_t i = i0 + 32 * u + lane;
+            id[u] = i < hi ? id_of(static_cast<int>(i)) : -1;
         }
-        before = __shfl_sync(0xffffffffu, before, leader);
-        // (the place in the warp's stretch, until the counts of the others are known)
-        if (i < N) a.positions[i] = ok ? before + __popc(peers & ((1u << lane) - 1u)) : -1;
-        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < SORT_AHEAD; ++u) {
+            const int64_t i = i0 + 32 * u + lane;
+            if (i0 + 32 * u >= hi) break;
+            const bool ok = id[u] >= 0 && id[u] < E;
+            if (!ok && id[u] != -1) set_error(a.err, DERR_BAD_ID);
+            const int local = warp_rank(count, ok ? id[u] : -1, lane);
+            // (the place in the warp's stretch, until the counts of the others are known)
+            if (i < hi) a.positions[i] = local;
+        }
     }
     __syncthreads();
     for (int e = tid; e < E; e += nth) {
@@ -126,16 +142,22 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(const SortArgs a) {
     }
     if (rank == 0 && tid == 0) a.offsets[E] = carry;
     __syncthreads();
-    for (int64_t i0 = lo; i0 < hi; i0 += 32) {
-        const int i = static_cast<int>(i0) + lane;
-        if (i >= N) continue;
-        const int local = a.positions[i];
-        if (local < 0) continue;
-        const int id = id_of(i);
-        const int p = first[id] + count[id] + local;
-        a.positions[i] = p;
-        a.rows[p] = i;
-        a.experts[p] = id;
+    for (int64_t i0 = lo; i0 < hi; i0 += 32 * SORT_AHEAD) {
+        int id[SORT_AHEAD], local[SORT_AHEAD];
+#pragma unroll
+        for (int u = 0; u < SORT_AHEAD; ++u) {
+            const int64_t i = i0 + 32 * u + lane;
+            local[u] = i < hi ? a.positions[i] : -1;
+            id[u] = i < hi ? id_of(static_cast<int>(i)) : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < SORT_AHEAD; ++u) {
+            if (local[u] < 0) continue;
+            const int i = static_cast<int>(i0) + 32 * u + lane, p = first[id[u]] + count[id[u]] + local[u];
+            a.positions[i] = p;
+            a.rows[p] = i;
+            a.experts[p] = id[u];
+        }
     }
     for (int64_t p = static_cast<int64_t>(carry) + rank * nth + tid; p < N; p += CTAS * nth) {
         a.rows[p] = -1;
@@ -215,6 +237,103 @@ __global__ void __launch_bounds__(ROW_THREADS) gather_kernel(const RowArgs a) {
         }
     }
     if (blockIdx.y == 0) zero_tail<V>(a.out, a.row_bytes, *a.live, a.n_entries);
+}
+
+// Both in one launch for few entries: every CTA finds the whole order by itself (as sort_kernel's CTAs do; two
+// microseconds, against those of a second launch) and copies its tokens' rows; the first one writes the order down.
+constexpr int DISPATCH_PER = 8;   // entries of a thread at most
+
+template <int V>
+__global__ void __launch_bounds__(ROW_THREADS) dispatch_kernel(const SortArgs s, const RowArgs a) {
+    using vt = typename vec<V>::t;
+    constexpr int WARPS = ROW_THREADS / 32;
+    extern __shared__ int sort_smem[];   // counts [WARPS][E], then the positions [N]
+    __shared__ int warp_sum[WARPS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, E = s.n_experts, N = s.n_entries, k = s.k;
+    const bool writes = blockIdx.x == 0 && blockIdx.y == 0;
+    int *count = sort_smem + warp * E, *positions = sort_smem + WARPS * E;
+    for (int i = tid; i < WARPS * E; i += ROW_THREADS) sort_smem[i] = 0;
+    __syncthreads();
+    const int per = (N + 32 * WARPS - 1) / (32 * WARPS);   // groups of 32 entries of a warp
+    int id[DISPATCH_PER], local[DISPATCH_PER];
+#pragma unroll
+    for (int u = 0; u < DISPATCH_PER; ++u) {
+        const int i = (warp * per + u) * 32 + lane;
+        id[u] = -1;
+        if (u < per && i < N) {
+            const int t = i / k;
+            id[u] = s.ids[static_cast<int64_t>(t) * s.ids_stride + (i - t * k)];
+            if (id[u] < 0 || id[u] >= E) {
+                if (id[u] != -1 && writes) set_error(s.err, DERR_BAD_ID);
+                id[u] = -1;
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < DISPATCH_PER; ++u)
+        if (u < per) local[u] = warp_rank(count, id[u], lane);
+    __syncthreads();
+    int carry = 0;
+    for (int base = 0; base < E; base += ROW_THREADS) {
+        const int e = base + tid;
+        int all = 0;
+        if (e < E)
+            for (int w = 0; w < WARPS; ++w) all += sort_smem[w * E + e];
+        int incl = all;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, incl, off);
+            if (lane >= off) incl += o;
+        }
+        if (lane == 31) warp_sum[warp] = incl;
+        __syncthreads();
+        int first = carry + incl - all;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            first += w < warp ? warp_sum[w] : 0;
+            carry += warp_sum[w];
+        }
+        if (e < E) {
+            if (writes) s.offsets[e] = first;
+            for (int w = 0; w < WARPS; ++w) {
+                const int c = sort_smem[w * E + e];
+                sort_smem[w * E + e] = first;
+                first += c;
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int u = 0; u < DISPATCH_PER; ++u) {
+        const int i = (warp * per + u) * 32 + lane;
+        if (u >= per || i >= N) continue;
+        const int p = id[u] >= 0 ? count[id[u]] + local[u] : -1;
+        positions[i] = p;
+        if (writes) {
+            s.positions[i] = p;
+            if (p >= 0) {
+                s.rows[p] = i;
+                s.experts[p] = id[u];
+            }
+        }
+    }
+    if (writes) {
+        if (tid == 0) s.offsets[E] = carry;
+        for (int p = carry + tid; p < N; p += ROW_THREADS) s.rows[p] = s.experts[p] = -1;
+    }
+    __syncthreads();
+    const int64_t t = (static_cast<int64_t>(blockIdx.x) << a.per_cta) + (tid >> a.tpt);
+    const int nv = static_cast<int>(a.row_bytes / V), step = static_cast<int>(gridDim.y) << a.tpt;
+    if (t < a.n_tok) {
+        const vt *src = reinterpret_cast<const vt *>(a.src + t * a.src_stride);
+        const int *pos = positions + t * k;
+        for (int c = (static_cast<int>(blockIdx.y) << a.tpt) + (tid & ((1 << a.tpt) - 1)); c < nv; c += step) {
+            const vt v = src[c];
+            for (int j = 0; j < k; ++j)
+                if (pos[j] >= 0) reinterpret_cast<vt *>(a.out + pos[j] * a.row_bytes)[c] = v;
+        }
+    }
+    if (blockIdx.y == 0) zero_tail<V>(a.out, a.row_bytes, carry, N);
 }
 
 // The sum of a token's rows in pick order, in 32 bits, rounded once; WEIGHTED: times the
@@ -424,6 +543,32 @@ cudaError_t launch_gather_sorted(RowArgs a, int type, cudaStream_t st) {
     else if (v == 4) gather_kernel<4><<<grid, ROW_THREADS, 0, st>>>(a);
     else gather_kernel<2><<<grid, ROW_THREADS, 0, st>>>(a);
     return cudaGetLastError();
+}
+
+template <int V>
+cudaError_t dispatch_v(const SortArgs &s, const RowArgs &a, dim3 grid, cudaStream_t st) {
+    static bool configured[64] = {};
+    constexpr size_t most = sizeof(int) * (ROW_THREADS / 32 * static_cast<size_t>(SORT_MAX_EXPERTS) + DISPATCH_PER * ROW_THREADS);
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!configured[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(dispatch_kernel<V>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        if (e != cudaSuccess) return e;
+        configured[dev] = true;
+    }
+    dispatch_kernel<V><<<grid, ROW_THREADS, sizeof(int) * (ROW_THREADS / 32 * static_cast<size_t>(s.n_experts) + s.n_entries), st>>>(s, a);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_dispatch_sorted(const SortArgs &s, RowArgs a, int type, cudaStream_t st) {
+    if (a.n_tok == 0 || s.n_entries > DISPATCH_PER * ROW_THREADS) {
+        const cudaError_t e = launch_sort(s, st);
+        return e == cudaSuccess ? launch_gather_sorted(a, type, st) : e;
+    }
+    const int v = vec_bytes(a, type == MX_F32 ? 4 : 2);
+    const dim3 grid = row_grid(a, v);
+    return v == 16 ? dispatch_v<16>(s, a, grid, st) : v == 4 ? dispatch_v<4>(s, a, grid, st) : dispatch_v<2>(s, a, grid, st);
 }
 
 cudaError_t launch_combine_sorted(RowArgs a, int type, cudaStream_t st) {

@@ -10,8 +10,12 @@ stream; outputs are allocated on it. With a torch.cuda.Stream the inputs may be
 dropped right behind the call, with a raw handle the caller keeps them until the
 stream has run it. gather_sorted, dispatch_sorted and combine_sorted are
 differentiable once (in x, y, weights and shared); their backward pass runs on the
-stream of the call.
+stream of the call. A pass may be captured into a graph while no autograd graph of the
+same leaves that was made on another stream is alive (autograd would make the capture
+wait for that stream): such a call is refused.
 """
+import weakref
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -25,113 +29,164 @@ class ExpertOrder:
     i32 [n_tok, k], the sorted row of a pick or -1; `offsets` i32 [n_experts + 1], the
     first sorted row of each expert, then their number."""
 
-    def __init__(self, ids, n_experts, stream=None):
+    def __init__(self, ids, n_experts):
+        """(dispatch_sorted and sort_by_expert make orders)"""
         if not (isinstance(ids, torch.Tensor) and ids.is_cuda and ids.dtype == torch.int32 and ids.dim() == 2):
             raise bad("ids must be an i32 CUDA tensor [n_tok, k]")
         n_tok, k = ids.shape
-        stride = k
+        self._stride = k
         if not ids.is_contiguous() and n_tok > 0:
-            stride = ids.stride(0) if n_tok > 1 else k
-            if (ids.stride(1) != 1 and k > 1) or stride < k:
+            self._stride = ids.stride(0) if n_tok > 1 else k
+            if (ids.stride(1) != 1 and k > 1) or self._stride < k:
                 raise bad("ids' rows must be dense and must not overlap in memory")
         if k < 1 or n_experts < 1:
             raise bad("need k >= 1 and n_experts >= 1")
-        ctx, st = on(ids.device, stream)
-        n = n_tok * k
-        with ctx:
-            buf = ids.new_empty(3 * n + n_experts + 1)
-            self.rows, pos, self.experts, self.offsets = buf.split([n, n, n, n_experts + 1])
-            at = buf.data_ptr()
-            check(lib().moe_b200_sort_by_expert(ids.data_ptr(), stride, n_tok, k, n_experts, at, at + 4 * n, at + 8 * n,
-                                                at + 12 * n, st))
-        self.positions = pos.view(n_tok, k)
         self.n_tok, self.k, self.n_experts, self.device = n_tok, k, n_experts, ids.device
-        keep(stream, ids, buf)
+        self._views = None
+
+    def _allocate(self, ids):
+        """Memory for the order (rows, positions, experts, offsets behind one another) and their addresses."""
+        n = self.n_tok * self.k
+        self._buf = ids.new_empty(3 * n + self.n_experts + 1)
+        at = self._buf.data_ptr()
+        self._at = at, at + 4 * n, at + 8 * n, at + 12 * n
+        return self._at
+
+    def _view(self, i):
+        if self._views is None:
+            n = self.n_tok * self.k
+            self._views = self._buf.split([n, n, n, self.n_experts + 1])
+        return self._views[i]
+
+    @property
+    def rows(self):
+        return self._view(0)
+
+    @property
+    def positions(self):
+        return self._view(1).view(self.n_tok, self.k)
+
+    @property
+    def experts(self):
+        return self._view(2)
+
+    @property
+    def offsets(self):
+        return self._view(3)
 
 
 def sort_by_expert(ids, n_experts, stream=None):
     """ids i32 [n_tok, k] (a Router's; -1: an empty slot) -> the ExpertOrder of its
     picks: by expert, and within one in the order of (token, pick)."""
-    return ExpertOrder(ids, n_experts, stream)
+    order = ExpertOrder(ids, n_experts)
+    ctx, st = on(ids.device, stream)
+    with ctx:
+        check(lib().moe_b200_sort_by_expert(ids.data_ptr(), order._stride, order.n_tok, order.k, n_experts, *order._allocate(ids), st))
+    keep(stream, ids, order._buf)
+    return order
 
 
-def _tensors(order):
-    """The order's tensors that the row calls read: positions, and the number of sorted rows behind the offsets."""
-    return order.positions, order.offsets
-
-
-def _gather(x, stride, positions, offsets, stream):
-    n_tok, k = positions.shape
-    H = x.shape[1]
+# The row calls take the order's memory (_buf) and its sizes: positions start n_tok k words in, the number of
+# sorted rows is its last word.
+def _gather(x, stride, buf, n_tok, k, stream):
+    n, H = n_tok * k, x.shape[1]
     ctx, st = on(x.device, stream)
     with ctx:
-        out = x.new_empty((n_tok * k, H))
-        check(lib().moe_b200_gather_sorted(x.data_ptr(), ELEM[x.dtype], stride, n_tok, k, H, positions.data_ptr(),
-                                           offsets.data_ptr() + 4 * (offsets.shape[0] - 1), out.data_ptr(), st))
-    keep(stream, x, positions, offsets, out)
+        out = x.new_empty((n, H))
+        at = buf.data_ptr()
+        check(lib().moe_b200_gather_sorted(x.data_ptr(), ELEM[x.dtype], stride, n_tok, k, H, at + 4 * n,
+                                           at + 4 * (buf.shape[0] - 1), out.data_ptr(), st))
+    if stream is not None:
+        keep(stream, x, buf, out)
     return out
 
 
-def _combine(y, stride, positions, weights, shared, shared_stride, stream):
-    n_tok, k = positions.shape
+def _combine(y, stride, buf, n_tok, k, weights, shared, shared_stride, stream):
     H = y.shape[1]
     ctx, st = on(y.device, stream)
     with ctx:
         out = y.new_empty((n_tok, H))
-        check(lib().moe_b200_combine_sorted(y.data_ptr(), ELEM[y.dtype], stride, n_tok, k, H, positions.data_ptr(),
+        check(lib().moe_b200_combine_sorted(y.data_ptr(), ELEM[y.dtype], stride, n_tok, k, H, buf.data_ptr() + 4 * n_tok * k,
                                             None if weights is None else weights.data_ptr(),
                                             None if shared is None else shared.data_ptr(), shared_stride, out.data_ptr(), st))
-    keep(stream, y, positions, weights, shared, out)
+    if stream is not None:
+        keep(stream, y, buf, weights, shared, out)
     return out
+
+
+# ---- gradients -----------------------------------------------------------------
+
+_alive = weakref.WeakSet()      # autograd nodes of the calls below, with the stream and the leaves of each
+
+
+def _leaves(*tensors):
+    return tuple(id(t) for t in tensors if t is not None and t.requires_grad and t.is_leaf)
+
+
+def _check_capture(st, *tensors):
+    if torch.cuda.is_current_stream_capturing():
+        leaves = set(_leaves(*tensors))
+        if any(made != st and not leaves.isdisjoint(of) for made, of in [node.made for node in _alive]):
+            raise bad("an autograd graph of the same leaves, made on another stream, is alive: drop it before the capture")
 
 
 def _grad_rows(g):
     """A gradient as rows that the calls take (autograd may hand over an expanded one) and their stride."""
-    if g.stride(1) != 1 or g.stride(0) < g.shape[1]:
+    H = g.shape[1]
+    if not g.is_contiguous() and (g.stride(1) != 1 or g.stride(0) < H):
         g = g.contiguous()
-    return g, max(g.stride(0), g.shape[1])
+    return g, max(g.stride(0), H)
+
+
+def _differentiable_once(backward):
+    """once_differentiable where a graph of the gradients is being made, the plain call (faster) where it is not."""
+    checked = once_differentiable(backward)
+    return lambda ctx, *g: (checked if torch.is_grad_enabled() else backward)(ctx, *g)
 
 
 class _Gather(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, stride, positions, offsets, stream):
-        ctx.save_for_backward(positions)
-        return _gather(x, stride, positions, offsets, stream)
+    def forward(ctx, x, stride, buf, n_tok, k, made, rows, stream):
+        ctx.save_for_backward(buf)
+        ctx.call, ctx.made = (n_tok, k), (made, _leaves(x))
+        _alive.add(ctx)
+        return _gather(x, stride, buf, n_tok, k, stream) if rows is None else rows
 
     @staticmethod
-    @once_differentiable
+    @_differentiable_once
     def backward(ctx, g):
         g, stride = _grad_rows(g)
-        return _combine(g, stride, ctx.saved_tensors[0], None, None, 0, None), None, None, None, None
+        return _combine(g, stride, ctx.saved_tensors[0], *ctx.call, None, None, 0, None), None, None, None, None, None, None, None
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y, stride, positions, offsets, weights, shared, shared_stride, stream):
-        need_y = y if weights.requires_grad else None     # d_y needs the weights alone
-        ctx.save_for_backward(need_y, positions, offsets, weights)
-        ctx.stride = stride
-        return _combine(y, stride, positions, weights, shared, shared_stride, stream)
+    def forward(ctx, y, stride, buf, n_tok, k, weights, shared, shared_stride, made, stream):
+        ctx.save_for_backward(y if weights.requires_grad else None, buf, weights)     # d_y needs the weights alone
+        ctx.call, ctx.made = (stride, n_tok, k), (made, _leaves(y, weights, shared))
+        _alive.add(ctx)
+        return _combine(y, stride, buf, n_tok, k, weights, shared, shared_stride, stream)
 
     @staticmethod
-    @once_differentiable
+    @_differentiable_once
     def backward(ctx, g):
-        y, positions, offsets, weights = ctx.saved_tensors
-        want_y, want_w, want_s = (ctx.needs_input_grad[i] for i in (0, 4, 5))
+        y, buf, weights = ctx.saved_tensors
+        want = ctx.needs_input_grad
         d_y = d_w = None
-        if want_y or want_w:
+        if want[0] or want[5]:
             rows, stride = _grad_rows(g)
-            n_tok, k = positions.shape
-            H = rows.shape[1]
+            y_stride, n_tok, k = ctx.call
+            n, H = n_tok * k, rows.shape[1]
             c, st = on(rows.device, None)
             with c:
-                d_y = rows.new_empty((n_tok * k, H)) if want_y else None
-                d_w = torch.empty_like(weights) if want_w else None
+                d_y = rows.new_empty((n, H)) if want[0] else None
+                d_w = torch.empty_like(weights) if want[5] else None
+                at = buf.data_ptr()
                 check(lib().moe_b200_combine_sorted_grad(
-                    rows.data_ptr(), ELEM[rows.dtype], stride, None if y is None else y.data_ptr(), ctx.stride, n_tok, k, H,
-                    positions.data_ptr(), offsets.data_ptr() + 4 * (offsets.shape[0] - 1), weights.data_ptr(),
-                    None if d_y is None else d_y.data_ptr(), None if d_w is None else d_w.data_ptr(), st))
-        return d_y, None, None, None, d_w, g if want_s else None, None, None
+                    rows.data_ptr(), ELEM[rows.dtype], stride, None if y is None else y.data_ptr(), y_stride, n_tok, k, H,
+                    at + 4 * n, at + 4 * (buf.shape[0] - 1), weights.data_ptr(), None if d_y is None else d_y.data_ptr(),
+                    None if d_w is None else d_w.data_ptr(), st))
+        return d_y, None, None, None, None, d_w, g if want[6] else None, None, None, None
 
 
 def _rows_of(t, name, n, order):
@@ -147,19 +202,32 @@ def gather_sorted(x, order, stream=None):
     """x f32 / f16 / bf16 [n_tok, H] -> [n_tok k, H]: the token of every sorted row,
     zeros behind the last one."""
     stride = _rows_of(x, "x", order.n_tok, order)
-    if x.requires_grad and torch.is_grad_enabled():
-        with on(x.device, stream)[0]:       # (the backward pass runs on the stream that is current here)
-            return _Gather.apply(x, stride, *_tensors(order), stream)
-    return _gather(x, stride, *_tensors(order), stream)
+    if not (x.requires_grad and torch.is_grad_enabled()):
+        return _gather(x, stride, order._buf, order.n_tok, order.k, stream)
+    ctx, st = on(x.device, stream)
+    with ctx:       # (the backward pass runs on the stream that is current here)
+        _check_capture(st, x)
+        return _Gather.apply(x, stride, order._buf, order.n_tok, order.k, st, None, stream)
 
 
 def dispatch_sorted(x, ids, n_experts, stream=None):
-    """sort_by_expert and gather_sorted: (rows [n_tok k, H], order)."""
-    dense_rows(x, "x")
-    if isinstance(ids, torch.Tensor) and ids.dim() == 2 and (x.dim() != 2 or x.shape[0] != ids.shape[0] or x.device != ids.device):
-        raise bad("x must be [n_tok, H] on the ids' device")
-    order = ExpertOrder(ids, n_experts, stream)
-    return gather_sorted(x, order, stream), order
+    """sort_by_expert and gather_sorted in one call: (rows [n_tok k, H], order)."""
+    order = ExpertOrder(ids, n_experts)
+    stride = _rows_of(x, "x", order.n_tok, order)
+    n_tok, k, H = order.n_tok, order.k, x.shape[1]
+    ctx, st = on(x.device, stream)
+    with ctx:
+        grad = x.requires_grad and torch.is_grad_enabled()
+        if grad:
+            _check_capture(st, x)
+        out = x.new_empty((n_tok * k, H))
+        check(lib().moe_b200_dispatch_sorted(x.data_ptr(), ELEM[x.dtype], stride, H, ids.data_ptr(), order._stride, n_tok, k,
+                                             n_experts, *order._allocate(ids), out.data_ptr(), st))
+        if grad:
+            out = _Gather.apply(x, stride, order._buf, n_tok, k, st, out, stream)
+    if stream is not None:
+        keep(stream, x, ids, order._buf, out)
+    return out, order
 
 
 def combine_sorted(y, order, weights, shared=None, stream=None):
@@ -168,20 +236,23 @@ def combine_sorted(y, order, weights, shared=None, stream=None):
     `shared` [n_tok, H] (the shared expert's) of y's type, in 32 bits, rounded once.
     Picks without a sorted row add nothing, whatever their weight is; y's rows behind the
     last sorted one are not read."""
-    stride = _rows_of(y, "y", order.n_tok * order.k, order)
+    n_tok, k = order.n_tok, order.k
+    stride = _rows_of(y, "y", n_tok * k, order)
     if not isinstance(weights, torch.Tensor) or weights.dtype != torch.float32 or weights.device != order.device or \
-            tuple(weights.shape) != (order.n_tok, order.k) or not weights.is_contiguous():
+            weights.shape != (n_tok, k) or not weights.is_contiguous():
         raise bad("weights must be contiguous f32 [n_tok, k] on the order's device")
-    shared_stride = 0
+    shared_stride, grad = 0, y.requires_grad or weights.requires_grad
     if shared is not None:
-        shared_stride = _rows_of(shared, "shared", order.n_tok, order)
+        shared_stride = _rows_of(shared, "shared", n_tok, order)
         if shared.dtype != y.dtype or shared.shape[1] != y.shape[1]:
             raise bad("shared must be [n_tok, H] of y's type")
-    pos, offsets = _tensors(order)
-    if torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad or (shared is not None and shared.requires_grad)):
-        with on(y.device, stream)[0]:
-            return _Combine.apply(y, stride, pos, offsets, weights, shared, shared_stride, stream)
-    return _combine(y, stride, pos, weights, shared, shared_stride, stream)
+        grad = grad or shared.requires_grad
+    if not (grad and torch.is_grad_enabled()):
+        return _combine(y, stride, order._buf, n_tok, k, weights, shared, shared_stride, stream)
+    ctx, st = on(y.device, stream)
+    with ctx:
+        _check_capture(st, y, weights, shared)
+        return _Combine.apply(y, stride, order._buf, n_tok, k, weights, shared, shared_stride, st, stream)
 
 
 __all__ = ["ExpertOrder", "sort_by_expert", "gather_sorted", "dispatch_sorted", "combine_sorted"]

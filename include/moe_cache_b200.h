@@ -592,7 +592,7 @@ int moe_b200_mxfp4_layer_run(const moe_mxfp4_layer *layer, const void *x, int32_
  * [0, n_experts); -1 marks an empty slot, any other id counts as one and sets the
  * device error word (MOE_DERR_BAD_ID). Elements are MOE_TYPE_F32, _F16 or _BF16,
  * row strides in elements, aligned to their size. Nothing is allocated, except that
- * moe_b200_sort_by_expert's first call on a device makes its error word (not during
+ * the first sort on a device makes its error word (not during
  * capture: MOE_ERR_STATE); calls may overlap. n_tok may be 0, n_tok * k <= 2^30. */
 
 /* The order: entries by (expert, i), n_experts <= 1024. rows[p] = the entry of sorted
@@ -608,6 +608,11 @@ int moe_b200_sort_by_expert(const int32_t *ids, int64_t ids_stride, int64_t n_to
  * (&offsets[n_experts]). */
 int moe_b200_gather_sorted(const void *x, int32_t type, int64_t x_row_stride, int64_t n_tok, int64_t k, int64_t H,
                            const int32_t *positions, const int32_t *n_sorted, void *out, moe_stream_t stream);
+
+/* moe_b200_sort_by_expert and moe_b200_gather_sorted in one call (one launch for up to 2048 entries). */
+int moe_b200_dispatch_sorted(const void *x, int32_t type, int64_t x_row_stride, int64_t H, const int32_t *ids, int64_t ids_stride,
+                             int64_t n_tok, int64_t k, int64_t n_experts, int32_t *rows, int32_t *positions, int32_t *experts,
+                             int32_t *offsets, void *out, moe_stream_t stream);
 
 /* out[t] = sum over the picks j, in order, of weights[t][j] * y[positions[t][j]], plus
  * shared[t] (or NULL), in 32 bits, rounded once. weights f32 [n_tok][k] or NULL (all 1;

@@ -295,3 +295,59 @@ def test_no_tokens(pkg, cuda):
     out = pkg.combine_sorted(rows, order, torch.empty((0, 4), device=cuda))
     assert out.shape == (0, 32)
     assert torch.autograd.grad(out.sum(), x)[0].shape == (0, 32)
+
+
+def test_capture_next_to_an_eager_graph_of_the_same_leaves(pkg, cuda):
+    """Autograd would make the capture wait for the eager graph's stream: refused, and fine once that graph is gone or
+    where it was made on the capture's stream."""
+    rng = np.random.default_rng(10)
+    n, k, E, H = 20, 3, 5, 64
+    ids = torch.from_numpy(draw_ids(rng, n, k, E)).to(cuda)
+    x, y = (rand(rng, (m, H), "f32", cuda).requires_grad_() for m in (n, n * k))
+    w = torch.rand((n, k), device=cuda).requires_grad_()
+    d = rand(rng, (n, H), "f32", cuda)
+
+    def step(stream):
+        with torch.cuda.stream(stream):
+            rows, order = pkg.dispatch_sorted(x, ids, E)
+            out = pkg.combine_sorted(y, order, w)
+            return (rows, out), torch.autograd.grad(out, [y, w], d, retain_graph=True)
+    main, side = torch.cuda.current_stream(), torch.cuda.Stream()
+    alive, want = step(main)
+    want = [t.clone() for t in want]
+    torch.cuda.synchronize()
+    order = pkg.sort_by_expert(ids, E)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        for call in (lambda: pkg.dispatch_sorted(x, ids, E), lambda: pkg.gather_sorted(x, order), lambda: pkg.combine_sorted(y, order, w)):
+            with pytest.raises(pkg.MoeError, match="alive"):
+                call()
+        with torch.no_grad():
+            pkg.combine_sorted(y, order, w)
+    del alive
+    kept, _ = step(side)                          # (on the capture's stream)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        outs, grads = step(side)
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, grads))
+    del kept, outs
+
+
+def test_dispatch_is_sort_and_gather(pkg, cuda):
+    """Both forms, about the size where they change."""
+    rng = np.random.default_rng(11)
+    for n, k, E in ((1, 8, 1024), (255, 8, 64), (256, 8, 300), (257, 8, 64), (682, 3, 1000), (2048, 1, 7), (2049, 1, 7)):
+        ids = draw_ids(rng, n, k, E, 0.1)
+        if n > 200:
+            ids[5, 0] = E
+        t = torch.from_numpy(ids).to(cuda)
+        x = rand(rng, (n, 72), "bf16", cuda)
+        rows, order = pkg.dispatch_sorted(x, t, E)
+        check_order(order, ids, E)
+        assert pkg.moe_cache.device_error() == (pkg.moe_cache.DERR_BAD_ID if n > 200 else 0)
+        other = pkg.sort_by_expert(t, E)
+        assert torch.equal(other._buf, order._buf) and torch.equal(rows, pkg.gather_sorted(x, other))
+        assert pkg.moe_cache.device_error() == (pkg.moe_cache.DERR_BAD_ID if n > 200 else 0)
