@@ -40,9 +40,18 @@ __device__ __forceinline__ int ld_cluster_s32(uint32_t saddr, uint32_t rank) {
     return v;
 }
 
-// The places of a warp's entries among its earlier ones of their expert, whose counts go up; -1 for id -1.
-__device__ __forceinline__ int warp_rank(int *count, int id, int lane) {
-    const unsigned peers = __match_any_sync(0xffffffffu, id);
+// The places of a warp's entries among its earlier ones of their expert, whose counts go up; -1 for id -1. Lanes of one
+// expert are found by a ballot per bit of the ids (bits of them), which costs less than __match_any_sync on many
+// different ones.
+__device__ __forceinline__ int warp_rank(int *count, int id, int lane, int bits) {
+    unsigned peers = 0xffffffffu;
+    for (int b = 0; b < bits; ++b) {
+        const bool one = (id >> b) & 1;
+        const unsigned m = __ballot_sync(0xffffffffu, one);
+        peers &= one ? m : ~m;
+    }
+    const unsigned with = __ballot_sync(0xffffffffu, id >= 0);
+    peers &= id >= 0 ? with : ~with;
     const int leader = __ffs(peers) - 1;
     int before = 0;
     if (id >= 0 && lane == leader) {
@@ -58,9 +67,11 @@ template <int CTAS>
 __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(const SortArgs a) {
     extern __shared__ int sort_smem[];   // counts [warps][E], totals of this CTA [E], first places [E]
     __shared__ int warp_sum[32];
+    if (CTAS > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (they wait for the order)
     const int tid = threadIdx.x, nth = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = nth >> 5;
     const int rank = CTAS > 1 ? static_cast<int>(blockIdx.x) : 0;
     const int E = a.n_experts, N = a.n_entries, k = a.k;
+    const int bits = 32 - __clz(E - 1);
     int *count = sort_smem + warp * E, *total = sort_smem + warps * E, *first = total + E;
     for (int i = tid; i < warps * E; i += nth) sort_smem[i] = 0;
     __syncthreads();
@@ -86,7 +97,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(const SortArgs a) {
             if (i0 + 32 * u >= hi) break;
             const bool ok = id[u] >= 0 && id[u] < E;
             if (!ok && id[u] != -1) set_error(a.err, DERR_BAD_ID);
-            const int local = warp_rank(count, ok ? id[u] : -1, lane);
+            const int local = warp_rank(count, ok ? id[u] : -1, lane, bits);
             // (the place in the warp's stretch, until the counts of the others are known)
             if (i < hi) a.positions[i] = local;
         }
@@ -155,15 +166,33 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(const SortArgs a) {
             if (local[u] < 0) continue;
             const int i = static_cast<int>(i0) + 32 * u + lane, p = first[id[u]] + count[id[u]] + local[u];
             a.positions[i] = p;
-            a.rows[p] = i;
-            a.experts[p] = id[u];
+            if (CTAS == 1) {
+                a.rows[p] = i;
+                a.experts[p] = id[u];
+            }
         }
     }
-    for (int64_t p = static_cast<int64_t>(carry) + rank * nth + tid; p < N; p += CTAS * nth) {
-        a.rows[p] = -1;
-        a.experts[p] = -1;
+    if constexpr (CTAS > 1) {
+        sort_cluster_sync();   // the totals stay until every CTA has read them
+    } else {
+        for (int p = carry + tid; p < N; p += nth) a.rows[p] = a.experts[p] = -1;
     }
-    if (CTAS > 1) sort_cluster_sync();   // the totals stay until every CTA has read them
+}
+
+// What the cluster leaves to the whole GPU: rows and experts. These writes are scattered, and an SM sends off one sector
+// per cycle (8 of them took 36 us for 131072 entries, 17 of them for these). The row kernel does it where one follows.
+__device__ __forceinline__ void place_entry(const SortArgs &s, int64_t i, int64_t t, int j) {
+    const int p = s.positions[i];
+    if (p < 0) return;
+    s.rows[p] = static_cast<int>(i);
+    s.experts[p] = s.ids[t * s.ids_stride + j];
+}
+__global__ void __launch_bounds__(256) place_kernel(const SortArgs s) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // (the order)
+    const int i = blockIdx.x * 256 + threadIdx.x, live = s.offsets[s.n_experts];
+    if (i >= s.n_entries) return;
+    place_entry(s, i, i / s.k, i % s.k);
+    if (i >= live) s.rows[i] = s.experts[i] = -1;
 }
 
 // ---- rows -----------------------------------------------------------------------
@@ -218,25 +247,44 @@ __device__ __forceinline__ void zero_tail(char *out, int64_t row_bytes, int live
             reinterpret_cast<typename vec<V>::t *>(out + p * row_bytes)[c] = zero_vec<V>();
 }
 
-// A token's row is read once and written to its picks' places.
-template <int V>
-__global__ void __launch_bounds__(ROW_THREADS) gather_kernel(const RowArgs a) {
+// A token's row is read once and written to its picks' places. PLACES: right behind sort_kernel's cluster, whose rows and
+// experts it writes; a token's first vectors arrive meanwhile.
+template <int V, bool PLACES>
+__global__ void __launch_bounds__(ROW_THREADS) gather_kernel(const RowArgs a, const SortArgs s) {
     using vt = typename vec<V>::t;
     const int64_t t = (static_cast<int64_t>(blockIdx.x) << a.per_cta) + (threadIdx.x >> a.tpt);
     const int nv = static_cast<int>(a.row_bytes / V), step = static_cast<int>(gridDim.y) << a.tpt;
+    const int col = threadIdx.x & ((1 << a.tpt) - 1);
+    int c = (static_cast<int>(blockIdx.y) << a.tpt) + col;
     if (t < a.n_tok) {
         const vt *src = reinterpret_cast<const vt *>(a.src + t * a.src_stride);
         const int32_t *pos = a.positions + t * a.k;
-        for (int c = (static_cast<int>(blockIdx.y) << a.tpt) + (threadIdx.x & ((1 << a.tpt) - 1)); c < nv; c += step) {
-            const vt v = src[c];
+        vt v = c < nv ? src[c] : zero_vec<V>();
+        if (PLACES) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            if (blockIdx.y == 0)
+                for (int j = col; j < a.k; j += 1 << a.tpt) place_entry(s, t * a.k + j, t, j);
+        }
+        for (; c < nv;) {
 #pragma unroll 4
             for (int j = 0; j < a.k; ++j) {
                 const int p = pos[j];
                 if (p >= 0) reinterpret_cast<vt *>(a.out + p * a.row_bytes)[c] = v;
             }
+            c += step;
+            if (c < nv) v = src[c];
         }
+    } else if (PLACES) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
     }
-    if (blockIdx.y == 0) zero_tail<V>(a.out, a.row_bytes, *a.live, a.n_entries);
+    if (blockIdx.y == 0) {
+        const int live = *a.live;
+        zero_tail<V>(a.out, a.row_bytes, live, a.n_entries);
+        if (PLACES)
+            for (int64_t p = static_cast<int64_t>(live) + static_cast<int64_t>(blockIdx.x) * ROW_THREADS + threadIdx.x; p < a.n_entries;
+                 p += static_cast<int64_t>(gridDim.x) * ROW_THREADS)
+                s.rows[p] = s.experts[p] = -1;
+    }
 }
 
 // Both in one launch for few entries: every CTA finds the whole order by itself (as sort_kernel's CTAs do; two
@@ -251,6 +299,7 @@ __global__ void __launch_bounds__(ROW_THREADS) dispatch_kernel(const SortArgs s,
     __shared__ int warp_sum[WARPS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, E = s.n_experts, N = s.n_entries, k = s.k;
     const bool writes = blockIdx.x == 0 && blockIdx.y == 0;
+    const int bits = 32 - __clz(E - 1);
     int *count = sort_smem + warp * E, *positions = sort_smem + WARPS * E;
     for (int i = tid; i < WARPS * E; i += ROW_THREADS) sort_smem[i] = 0;
     __syncthreads();
@@ -271,7 +320,7 @@ __global__ void __launch_bounds__(ROW_THREADS) dispatch_kernel(const SortArgs s,
     }
 #pragma unroll
     for (int u = 0; u < DISPATCH_PER; ++u)
-        if (u < per) local[u] = warp_rank(count, id[u], lane);
+        if (u < per) local[u] = warp_rank(count, id[u], lane, bits);
     __syncthreads();
     int carry = 0;
     for (int base = 0; base < E; base += ROW_THREADS) {
@@ -528,20 +577,49 @@ cudaError_t sort_launch(const SortArgs &a, int threads, cudaStream_t st) {
 
 }  // namespace
 
-cudaError_t launch_sort(const SortArgs &a, cudaStream_t st) {
-    if (a.n_entries > 4096) return sort_launch<SORT_CTAS>(a, SORT_THREADS, st);
+namespace {
+
+// the launch of a kernel that waits for sort_kernel's cluster by itself
+template <typename... P, typename... A>
+cudaError_t behind_sort(void (*kernel)(P...), dim3 grid, cudaStream_t st, const A &...args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(ROW_THREADS);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+bool sort_by_cluster(const SortArgs &a) { return a.n_entries > 4096; }
+
+cudaError_t sort_order(const SortArgs &a, cudaStream_t st) {
+    if (sort_by_cluster(a)) return sort_launch<SORT_CTAS>(a, SORT_THREADS, st);
     int threads = 32;
     while (threads < a.n_entries && threads < SORT_THREADS) threads <<= 1;
     return sort_launch<1>(a, threads, st);
+}
+
+}  // namespace
+
+cudaError_t launch_sort(const SortArgs &a, cudaStream_t st) {
+    const cudaError_t e = sort_order(a, st);
+    if (e != cudaSuccess || !sort_by_cluster(a)) return e;
+    static_assert(ROW_THREADS == 256, "place_kernel's CTAs");
+    return behind_sort(place_kernel, dim3(static_cast<unsigned>((static_cast<int64_t>(a.n_entries) + 255) / 256)), st, a);
 }
 
 cudaError_t launch_gather_sorted(RowArgs a, int type, cudaStream_t st) {
     if (a.n_tok == 0) return cudaSuccess;
     const int v = vec_bytes(a, type == MX_F32 ? 4 : 2);
     const dim3 grid = row_grid(a, v);
-    if (v == 16) gather_kernel<16><<<grid, ROW_THREADS, 0, st>>>(a);
-    else if (v == 4) gather_kernel<4><<<grid, ROW_THREADS, 0, st>>>(a);
-    else gather_kernel<2><<<grid, ROW_THREADS, 0, st>>>(a);
+    const SortArgs none{};
+    if (v == 16) gather_kernel<16, false><<<grid, ROW_THREADS, 0, st>>>(a, none);
+    else if (v == 4) gather_kernel<4, false><<<grid, ROW_THREADS, 0, st>>>(a, none);
+    else gather_kernel<2, false><<<grid, ROW_THREADS, 0, st>>>(a, none);
     return cudaGetLastError();
 }
 
@@ -562,12 +640,16 @@ cudaError_t dispatch_v(const SortArgs &s, const RowArgs &a, dim3 grid, cudaStrea
 }
 
 cudaError_t launch_dispatch_sorted(const SortArgs &s, RowArgs a, int type, cudaStream_t st) {
-    if (a.n_tok == 0 || s.n_entries > DISPATCH_PER * ROW_THREADS) {
-        const cudaError_t e = launch_sort(s, st);
-        return e == cudaSuccess ? launch_gather_sorted(a, type, st) : e;
-    }
+    if (a.n_tok == 0) return launch_sort(s, st);
     const int v = vec_bytes(a, type == MX_F32 ? 4 : 2);
     const dim3 grid = row_grid(a, v);
+    if (s.n_entries > DISPATCH_PER * ROW_THREADS) {
+        const cudaError_t e = sort_order(s, st);
+        if (e != cudaSuccess) return e;
+        if (!sort_by_cluster(s)) return launch_gather_sorted(a, type, st);
+        return v == 16 ? behind_sort(gather_kernel<16, true>, grid, st, a, s)
+             : v == 4 ? behind_sort(gather_kernel<4, true>, grid, st, a, s) : behind_sort(gather_kernel<2, true>, grid, st, a, s);
+    }
     return v == 16 ? dispatch_v<16>(s, a, grid, st) : v == 4 ? dispatch_v<4>(s, a, grid, st) : dispatch_v<2>(s, a, grid, st);
 }
 
