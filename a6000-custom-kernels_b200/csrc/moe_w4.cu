@@ -34,10 +34,10 @@ namespace moe {
 
 namespace {
 
-constexpr int W4_WARPS = 8;              // of a CTA at most
+constexpr int W4_WARPS = 16;             // of a CTA, one to an SM: x lies there once
 constexpr int W4_RED = 20;               // floats between two columns of a warp's sums: no bank conflicts
 constexpr int W4_PAD = 64;               // bytes behind a column of x: two columns fill the banks
-constexpr int W4_SMEM = 112 * 1024;      // of a CTA: two fit an SM
+constexpr int W4_SMEM = 224 * 1024;
 constexpr int W4_ACC = 8 * 1024;         // of it at most for sums kept to a run's end, where one block's fit
 constexpr float W4_CODE = 0x1p-24f;      // a code's unit in rows g (times 16 in rows g + 8)
 constexpr float W4_UP = 4096.f;          // which comes off in two factors: with x's power of two, and at the end
@@ -355,7 +355,7 @@ struct Cursor {
 };
 
 template <int NT, bool ZERO, int GROUPS, bool SCALE_BF16>
-__global__ void __launch_bounds__(32 * W4_WARPS, 2) w4_kernel(const __grid_constant__ W4Args a) {
+__global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_kernel(const __grid_constant__ W4Args a) {
     constexpr int D = w4_stages<NT>(), GW = GROUPS == 8 ? 2 : 1;   // groups of a stage, of a tile
     constexpr int COLS = 8 * NT, XGAP = (GROUPS + 1) * COLS;       // floats of a stage's sums of x, and its powers of two
     extern __shared__ __align__(16) uint8_t smem[];
@@ -741,7 +741,7 @@ void w4_plan(const W4Key &c, int nt, W4Plan &best) {
     const double entries = mean < 1.0 ? 1.0 : mean < nc ? mean : nc;   // of a chunk
     const bool wide = entries * c.planes > 8, staged = w4_staged(c.n_tok, c.KS);
     for (int split = 1; split <= 4 && (split == 1 || split <= c.KS); split *= 2)
-        for (int wk = 0; wk <= 3; ++wk)
+        for (int wk = 0; wk <= 4; ++wk)
             for (int wm = 1; wm << wk <= W4_WARPS; ++wm) {
                 const int WK = 1 << wk, KS = static_cast<int>(c.KS), spr = (KS + split - 1) / split;
                 if ((WK > 1 && WK / 2 >= spr) || (wm > 1 && wm > c.RT)) continue;
@@ -766,7 +766,7 @@ void w4_plan(const W4Key &c, int nt, W4Plan &best) {
                 if (hold) p.seg = static_cast<int>(p.acc / one);
                 const int mine = (p.sp + split - 1) / split;                    // stages of a CTA in a pass
                 const int sums = c.mats * p.passes, deep = sums * ((mine + WK - 1) / WK);   // of a warp, for a row block
-                const int64_t blocks = (c.RT + wm - 1) / wm, items = chunks * blocks, slots = 2 * c.n_sm / split;
+                const int64_t blocks = (c.RT + wm - 1) / wm, items = chunks * blocks, slots = c.n_sm / split;
                 const double rounds = static_cast<double>((items + slots - 1) / slots);
                 const double of_sm = static_cast<double>((items * split + c.n_sm - 1) / c.n_sm);
                 // the SM's issue slots, and the way through one CTA's row blocks
@@ -821,7 +821,7 @@ cudaError_t w4_t(W4Args &a, const W4Plan &p, int64_t max_chunks, int n_sm, cudaS
     a.split_shift = p.split == 1 ? 0 : p.split == 2 ? 1 : 2;
     a.wk_shift = p.wk_shift;
     a.wm = p.wm;
-    a.x_shift = most >= 8 ? 0 : most >= 4 ? 1 : most >= 2 ? 2 : 3;
+    a.x_shift = most >= 16 ? 0 : most >= 8 ? 1 : most >= 4 ? 2 : most >= 2 ? 3 : 4;
     a.dst_vec = a.rows % 4 == 0 && reinterpret_cast<uintptr_t>(a.dst) % 16 == 0;
     a.passes = p.passes;
     a.sp = p.sp;
@@ -834,7 +834,7 @@ cudaError_t w4_t(W4Args &a, const W4Plan &p, int64_t max_chunks, int n_sm, cudaS
     const size_t smem = a.x_off + static_cast<size_t>(most * a.planes) * (mine * 2 * W4_KS + W4_PAD) +
                         static_cast<size_t>(mine) * (GROUPS + 1) * 8 * NT * 4;
     if (smem > W4_SMEM) return cudaErrorInvalidConfiguration;
-    const int64_t items = max_chunks * a.tiles, slots = 2 * n_sm / p.split;
+    const int64_t items = max_chunks * a.tiles, slots = n_sm / p.split;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>((items < slots ? items : slots) * p.split));
     cfg.blockDim = dim3(32 * W4_WARPS);
