@@ -138,6 +138,12 @@ __device__ __forceinline__ void unpack_codes(uint32_t w, uint32_t (&a)[4]) {
     a[3] = (w >> 8) & 0x00F000F0u;
 }
 
+// Programmatic dependent launch: calls follow one another without the gap between kernels. Behind dep_wait everything
+// before this kernel in the stream is complete; ahead of it nothing is read but the matrices, which only w4_pack_kernel
+// writes (it lets nothing start early), and by a product behind w4_stage_kernel the ids, which that one has waited for.
+__device__ __forceinline__ void dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 __device__ __forceinline__ void w4_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -333,7 +339,8 @@ __device__ __forceinline__ void stage_x(const W4Args &a, int64_t row, int kk, in
 // stage, planes x 512 bytes of columns, then [GROUPS + 1][planes] floats. One warp per unit.
 template <int GROUPS>
 __global__ void __launch_bounds__(256) w4_stage_kernel(const __grid_constant__ W4Args a, int64_t units, uint8_t *out) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (the product may come up meanwhile)
+    dep_wait();
+    dep_launch();   // (the product comes up meanwhile; what this call reads is complete then)
     const int64_t u = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
     if (u >= units) return;
     const int64_t row = u / a.KS;
@@ -366,6 +373,9 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_kernel(const __grid_const
     float *red = reinterpret_cast<float *>(smem + a.red_off);
     int2 *chunk_tab = reinterpret_cast<int2 *>(smem + a.tab_off);
     uint16_t *entry_tab = reinterpret_cast<uint16_t *>(chunk_tab + a.n_entries);
+    dep_launch();
+    bool waited = a.ids && !(a.staged && !a.chunks);
+    if (waited) dep_wait();
     int n_chunks;
     if (a.chunks) n_chunks = *a.n_chunks;
     else if (!a.ids) n_chunks = (a.n_entries + a.nc - 1) / a.nc;
@@ -375,7 +385,7 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_kernel(const __grid_const
     const int i0 = static_cast<int>(static_cast<int64_t>(items) * cluster / clusters);
     int left = static_cast<int>(static_cast<int64_t>(items) * (cluster + 1) / clusters) - i0;
     if (left == 0) {   // the whole cluster's
-        if (a.staged) asm volatile("griddepcontrol.wait;" ::: "memory");
+        dep_wait();
         return;
     }
     int chunk = i0 / a.tiles, tile0 = i0 - chunk * a.tiles;
@@ -390,7 +400,7 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_kernel(const __grid_const
     };
 
     constexpr uint32_t stage_bytes = w4_stage_bytes(GROUPS, ZERO);
-    uint8_t *const ring = smem + warp * D * stage_bytes, *const ring_end = ring + D * stage_bytes;
+    const uint32_t ring = warp * D * stage_bytes, ring_end = ring + D * stage_bytes;   // (offsets)
     Cursor P{};
     auto seek_chunk = [&]() {
         P.expert = static_cast<int64_t>(expert_of(P.chunk)) * a.RT * a.KS * stage_bytes + 16 * lane;
@@ -435,14 +445,14 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_kernel(const __grid_const
         seek_pass();
         seek();
     }
-    const uint32_t step = stage_bytes << a.wk_shift;
-    auto fetch = [&](const uint8_t *stage) {
-        while (P.todo == 0 && P.left) next();
+    const uint32_t step = stage_bytes << a.wk_shift, lane_at = smem_u32(smem) + 16 * lane;
+    auto fetch = [&](uint32_t stage) {   // (its offset)
+        if (P.todo == 0)
+            while (P.left && P.todo == 0) next();
         if (P.todo) {
-            const uint32_t to = smem_u32(stage) + 16 * lane;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) cp16(to + 512 * i, P.src + 512 * i);
-            if (16 * lane < stage_bytes - W4_CODES) cp16(to + W4_CODES, P.src + W4_CODES);
+            for (int i = 0; i < 4; ++i) cp16(lane_at + stage + 512 * i, P.src + 512 * i);
+            if (16 * lane < stage_bytes - W4_CODES) cp16(lane_at + stage + W4_CODES, P.src + W4_CODES);
             P.src += step;
             --P.todo;
         }
@@ -455,7 +465,7 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_kernel(const __grid_const
     const int outs1 = a.nc * W4_M;        // sums of a row tile
     const bool hold = S > 1 || a.passes > 1;
     constexpr int RED_BUF = W4_WARPS * COLS * W4_RED;
-    const uint8_t *at = ring;
+    uint32_t at = ring;
     int buf = 0, x_chunk = -1;            // whose x is staged
 
     while (left) {
@@ -504,7 +514,10 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_kernel(const __grid_const
             float *xsum = reinterpret_cast<float *>(smem + a.x_off + cols * pitch);   // [stage][GROUPS + 1][COLS]
             if (chunk != x_chunk || a.passes > 1) {
                 __syncthreads();   // everyone is done with the x of before
-                if (a.staged && x_chunk < 0) asm volatile("griddepcontrol.wait;" ::: "memory");   // (the kernel that staged it)
+                if (!waited) {
+                    dep_wait();
+                    waited = true;
+                }
                 // 1 << x_shift warps to an entry, a stage each at a time
                 const int st0 = warp & ((1 << a.x_shift) - 1), dst_step = 1 << a.x_shift;
                 for (int col = warp >> a.x_shift; col < count; col += W4_WARPS >> a.x_shift) {
@@ -557,7 +570,7 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_kernel(const __grid_const
                             float part[J][4], dots[J][GW][4], sc[GW][2], sz[GW][2];
 #pragma unroll
                             for (int i = 0; i < W4_KS / W4_KT; ++i) {
-                                const uint4 w = lds16(at + 16 * lane + W4_TILE * i);
+                                const uint4 w = lds16(smem + at + 16 * lane + W4_TILE * i);
                                 uint32_t A[4][4];
                                 unpack_codes(w.x, A[0]);
                                 unpack_codes(w.y, A[1]);
@@ -567,7 +580,7 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_kernel(const __grid_const
                                 for (int h = 0; h < GW; ++h) {
                                     if (GW == 1 && i * GROUPS % 4) continue;   // the group goes on
                                     const int gi = GW == 2 ? 2 * i + h : i * GROUPS / 4;
-                                    const uint32_t sw = lds4(at + W4_CODES + 32 * gi + 4 * g);
+                                    const uint32_t sw = lds4(smem + at + W4_CODES + 32 * gi + 4 * g);
                                     if constexpr (SCALE_BF16) {
                                         sc[h][0] = __uint_as_float(sw << 16);
                                         sc[h][1] = __uint_as_float(sw & 0xFFFF0000u);
@@ -578,7 +591,7 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_kernel(const __grid_const
                                     }
                                     // scale * zero; rows g + 8 in their codes' units
                                     if constexpr (ZERO) {
-                                        const uint32_t zw = lds4(at + W4_CODES + 32 * GROUPS + 16 * gi + 4 * (g >> 1));
+                                        const uint32_t zw = lds4(smem + at + W4_CODES + 32 * GROUPS + 16 * gi + 4 * (g >> 1));
                                         // 2^23 + zero, by bits
                                         const float z0 = __uint_as_float(__byte_perm(zw, 0x4B000000u, g & 1 ? 0x7552 : 0x7550));
                                         const float z1 = __uint_as_float(__byte_perm(zw, 0x4B000000u, g & 1 ? 0x7553 : 0x7551));
@@ -841,8 +854,8 @@ cudaError_t w4_t(W4Args &a, const W4Plan &p, int64_t max_chunks, int n_sm, cudaS
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // (behind w4_stage_kernel only)
-    at[0].val.programmaticStreamSerializationAllowed = a.staged ? 1 : 0;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
     at[1].id = cudaLaunchAttributeClusterDimension;
     at[1].val.clusterDim.x = static_cast<unsigned>(p.split);
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
@@ -926,12 +939,19 @@ cudaError_t launch_w4(W4Args &a, int64_t n_tok, uint8_t *staged, cudaStream_t st
     if (staged) {
         a.unit = static_cast<int32_t>(w4_row_bytes(1, a.groups, a.x_type));
         const int64_t units = (a.per_pick ? static_cast<int64_t>(a.n_entries) : n_tok) * a.KS;
-        const unsigned grid = static_cast<unsigned>((units + 7) / 8);
-        if (a.groups == 8) w4_stage_kernel<8><<<grid, 256, 0, st>>>(a, units, staged);
-        else if (a.groups == 4) w4_stage_kernel<4><<<grid, 256, 0, st>>>(a, units, staged);
-        else if (a.groups == 2) w4_stage_kernel<2><<<grid, 256, 0, st>>>(a, units, staged);
-        else w4_stage_kernel<1><<<grid, 256, 0, st>>>(a, units, staged);
-        const cudaError_t e = cudaGetLastError();
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(static_cast<unsigned>((units + 7) / 8));
+        cfg.blockDim = dim3(256);
+        cfg.stream = st;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        const cudaError_t e = a.groups == 8   ? cudaLaunchKernelEx(&cfg, w4_stage_kernel<8>, a, units, staged)
+                              : a.groups == 4 ? cudaLaunchKernelEx(&cfg, w4_stage_kernel<4>, a, units, staged)
+                              : a.groups == 2 ? cudaLaunchKernelEx(&cfg, w4_stage_kernel<2>, a, units, staged)
+                                              : cudaLaunchKernelEx(&cfg, w4_stage_kernel<1>, a, units, staged);
         if (e != cudaSuccess) return e;
         a.staged = staged;
     }
