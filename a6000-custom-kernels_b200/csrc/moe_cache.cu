@@ -2659,7 +2659,8 @@ int moe_b200_w4_mul_mat_id(const moe_w4 *w, const moe_w4 *gate, const float *bia
         return fail(MOE_ERR_INVALID, "workspace too small (%zu < %zu bytes)", workspace_bytes, ws.bytes);
     if (!aligned16(workspace)) return fail(MOE_ERR_INVALID, "workspace must be 16-byte aligned");
     const int64_t most = std::min(n_tok * k, moe::mmq_max_chunks(n_tok * k, w->n_experts, moe::w4_min_chunk(xt)));   // chunks
-    if (most * s.RT > (int64_t{1} << 29)) return fail(MOE_ERR_UNSUPPORTED, "too many tiles in one call");
+    if (most * s.RT > (int64_t{1} << 29) || n_tok * k * s.KS > (int64_t{1} << 33))
+        return fail(MOE_ERR_UNSUPPORTED, "too many tiles in one call");
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     moe::W4Args a{};
     rc = error_word(st, &a.err);

@@ -290,6 +290,7 @@ __global__ void __launch_bounds__(ROW_THREADS) gather_kernel(const RowArgs a, co
 // Both in one launch for few entries: every CTA finds the whole order by itself (as sort_kernel's CTAs do; two
 // microseconds, against those of a second launch) and copies its tokens' rows; the first one writes the order down.
 constexpr int DISPATCH_PER = 8;   // entries of a thread at most
+constexpr int DISPATCH_CTAS = 592;   // more would sort in several waves (2048 tokens' one expert each)
 
 template <int V>
 __global__ void __launch_bounds__(ROW_THREADS) dispatch_kernel(const SortArgs s, const RowArgs a) {
@@ -643,7 +644,7 @@ cudaError_t launch_dispatch_sorted(const SortArgs &s, RowArgs a, int type, cudaS
     if (a.n_tok == 0) return launch_sort(s, st);
     const int v = vec_bytes(a, type == MX_F32 ? 4 : 2);
     const dim3 grid = row_grid(a, v);
-    if (s.n_entries > DISPATCH_PER * ROW_THREADS) {
+    if (s.n_entries > DISPATCH_PER * ROW_THREADS || grid.x * grid.y > DISPATCH_CTAS) {
         const cudaError_t e = sort_order(s, st);
         if (e != cudaSuccess) return e;
         if (!sort_by_cluster(s)) return launch_gather_sorted(a, type, st);

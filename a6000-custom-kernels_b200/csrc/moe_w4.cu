@@ -43,6 +43,10 @@ constexpr float W4_CODE = 0x1p-24f;      // a code's unit in rows g (times 16 in
 constexpr float W4_UP = 4096.f;          // which comes off in two factors: with x's power of two, and at the end
 constexpr float W4_PLANE = 4096.f;       // the second plane of an f32 x holds what the first one leaves, times this
 
+// What plans count with, in us: a stage of each of the warps that share an SM's issue slots, of one by itself, adding up a block
+constexpr float W4_STAGE = 0.0596f, W4_STAGE_ALONE = 0.325f, W4_BLOCK_US = 0.8f;
+__host__ __device__ __forceinline__ float w4_stage_us(int warps) { return W4_STAGE * warps * powf(16.f / warps, 0.3f); }
+
 // stages in flight per warp
 template <int NT>
 __host__ __device__ constexpr int w4_stages() { return NT == 1 ? 3 : 2; }
@@ -367,8 +371,8 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_kernel(const __grid_const
     constexpr int COLS = 8 * NT, XGAP = (GROUPS + 1) * COLS;       // floats of a stage's sums of x, and its powers of two
     extern __shared__ __align__(16) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    // warps wm * WK.. share K of row block row tile wm; warps behind the last of WM * WK have nothing to do
-    const int WK = 1 << a.wk_shift, wk = warp & (WK - 1), wm = warp >> a.wk_shift, WM = a.wm;
+    // WK warps from wm * WK on share K of the block's row tile wm
+    const int WK = 1 << a.wk_shift, wk = warp & (WK - 1), wm = warp >> a.wk_shift;
     const int S = 1 << a.split_shift, rank = static_cast<int>(blockIdx.x) & (S - 1);
     float *red = reinterpret_cast<float *>(smem + a.red_off);
     int2 *chunk_tab = reinterpret_cast<int2 *>(smem + a.tab_off);
@@ -380,19 +384,27 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_kernel(const __grid_const
     if (a.chunks) n_chunks = *a.n_chunks;
     else if (!a.ids) n_chunks = (a.n_entries + a.nc - 1) / a.nc;
     else n_chunks = w4_group(a, chunk_tab, entry_tab, reinterpret_cast<int *>(smem));   // (the ring is not in use yet)
-    const int items = n_chunks * a.tiles, cluster = static_cast<int>(blockIdx.x) >> a.split_shift;
-    const int clusters = static_cast<int>(gridDim.x) >> a.split_shift;
+    const int cluster = static_cast<int>(blockIdx.x) >> a.split_shift, clusters = static_cast<int>(gridDim.x) >> a.split_shift;
+    // row tiles of a block: as planned, or for experts, whose chunks only the GPU knows, by the plan's count of a round's time
+    int WM = a.wm;
+    if (a.ids) {
+        const int w = lane + 1, rounds = (n_chunks * ((a.RT + w - 1) / w) + clusters - 1) / clusters;
+        const float us = a.deep * fmaxf(W4_STAGE_ALONE, w4_stage_us(w << a.wk_shift)) + a.per_block;
+        const uint32_t cost = w <= a.wm ? __float_as_uint(rounds * us) : 0xFFFFFFFFu;
+        WM = __ffs(__ballot_sync(0xffffffffu, cost == __reduce_min_sync(0xffffffffu, cost)));
+    }
+    const int tiles = (a.RT + WM - 1) / WM, items = n_chunks * tiles;   // blocks of a chunk, of all
     const int i0 = static_cast<int>(static_cast<int64_t>(items) * cluster / clusters);
     int left = static_cast<int>(static_cast<int64_t>(items) * (cluster + 1) / clusters) - i0;
     if (left == 0) {   // the whole cluster's
         dep_wait();
         return;
     }
-    int chunk = i0 / a.tiles, tile0 = i0 - chunk * a.tiles;
+    int chunk = i0 / tiles, tile0 = i0 - chunk * tiles;
 
     auto expert_of = [&](int c) { return a.chunks ? a.chunks[c].x : a.ids ? chunk_tab[c].x & 0xFFFF : 0; };
     auto entry_of = [&](int i) { return a.chunks ? a.entries[i] : a.ids ? static_cast<int>(entry_tab[i]) : i; };
-    auto run_of = [&](int left, int tile0) { return min(min(left, a.tiles - tile0), a.seg); };
+    auto run_of = [&](int left, int tile0) { return min(min(left, tiles - tile0), a.seg); };
     // the first of rank r's stages of a pass
     auto share = [&](int pass, int r) {
         const int s0 = pass * a.sp, n = min(a.KS, s0 + a.sp) - s0;
@@ -424,7 +436,7 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_kernel(const __grid_const
                     P.left -= P.len;
                     if (P.left == 0) return;
                     P.tile0 += P.len;
-                    if (P.tile0 == a.tiles) {
+                    if (P.tile0 == tiles) {
                         P.tile0 = 0;
                         ++P.chunk;
                         seek_chunk();
@@ -560,8 +572,8 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_kernel(const __grid_const
                 for (int mat = 0; mat < a.mats; ++mat) {
                     float sum[NT][4] = {};
                     // this warp's stages, for J tiles of columns
-                    auto run = [&](auto tiles) {
-                        constexpr int J = decltype(tiles)::value;
+                    auto run = [&](auto columns) {
+                        constexpr int J = decltype(columns)::value;
                         uint32_t xk = 0;
                         const float *xs = xsum + wk * XGAP + 2 * t;
                         for (int s = 0; s < mine; ++s) {
@@ -709,7 +721,7 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_kernel(const __grid_const
         }
         left -= len;
         tile0 += len;
-        if (tile0 == a.tiles) {
+        if (tile0 == tiles) {
             tile0 = 0;
             ++chunk;
         }
@@ -717,13 +729,15 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_kernel(const __grid_const
     cp_wait_all();
 }
 
-// How the columns, the rows and K are shared out. A CTA has up to eight warps at work: wm row tiles, K of each shared by
-// 1 << wk_shift warps and `split` CTAs; chunks have up to 8 NT MMA columns. Of all such plans the one with the least
+// How the columns, the rows and K are shared out. A CTA has up to 16 warps at work: wm row tiles, K of each shared by
+// 1 << wk_shift warps and `split` CTAs; chunks have up to 8 nt MMA columns. Of all such plans the one with the least
 // time by the count below is taken; its constants were fitted to 22 calls (one matrix of 768 x 2048 to 32768 x 4096 with 1 to
-// 64 rows of x, experts with 1 to 64 tokens) timed in every plan, and its choice is 4 % slower than the best of them on
-// average, 19 % at most. Plans with 32 columns, or with clusters of eight, were never the best by more than 1 %.
+// 64 rows of x, experts with 1 to 64 tokens) timed in every plan: its choice is 5 % slower than the best of them on average,
+// 27 % at most (1024 x 8192, one row: 6.5 us, 5.1 without a cluster). For experts, whose chunks depend on the picks, the GPU
+// takes wm when it has counted them (64 of them, 4 tokens' 6: 20.2 us, 27.3 with the wm that a guess gave).
+// (Plans with 32 columns or with clusters of eight were never better by more than 1 %.)
 struct W4Plan {
-    int nt, split, wk_shift, wm, passes, sp, seg;
+    int nt, split, wk_shift, wm, passes, sp, seg, deep;
     uint32_t acc, tab;
     double us;
 };
@@ -758,8 +772,9 @@ void w4_plan(const W4Key &c, int nt, W4Plan &best) {
             for (int wm = 1; wm << wk <= W4_WARPS; ++wm) {
                 const int WK = 1 << wk, KS = static_cast<int>(c.KS), spr = (KS + split - 1) / split;
                 if ((WK > 1 && WK / 2 >= spr) || (wm > 1 && wm > c.RT)) continue;
-                const uint32_t one = static_cast<uint32_t>(nc * wm * W4_M * c.mats) * 4;   // a row block's sums
-                W4Plan p{nt, split, wk, wm, 1, KS, 1 << 29, 0, tab, 0.0};
+                const int most = c.one_matrix ? wm : W4_WARPS >> wk;              // row tiles that a block may have
+                const uint32_t one = static_cast<uint32_t>(nc * most * W4_M * c.mats) * 4;   // its sums
+                W4Plan p{nt, split, wk, most, 1, KS, 1 << 24, 0, 0, tab, 0.0};
                 bool hold = split > 1;
                 auto room_for_x = [&]() {   // stages of x that fit
                     p.acc = hold ? (one > W4_ACC ? one : W4_ACC / one * one) : c.mats > 1 ? one : 0;
@@ -779,19 +794,20 @@ void w4_plan(const W4Key &c, int nt, W4Plan &best) {
                 if (hold) p.seg = static_cast<int>(p.acc / one);
                 const int mine = (p.sp + split - 1) / split;                    // stages of a CTA in a pass
                 const int sums = c.mats * p.passes, deep = sums * ((mine + WK - 1) / WK);   // of a warp, for a row block
+                p.deep = deep;
                 const int64_t blocks = (c.RT + wm - 1) / wm, items = chunks * blocks, slots = c.n_sm / split;
                 const double rounds = static_cast<double>((items + slots - 1) / slots);
                 const double of_sm = static_cast<double>((items * split + c.n_sm - 1) / c.n_sm);
                 // the SM's issue slots, and the way through one CTA's row blocks
-                const double full = of_sm * (wm * WK) *
-                                    (deep * (0.0464 + (wide ? 0.0051 : 0.0) + (c.groups == 8 ? 0.0084 : 0.0)) + sums * 0.0806 * (0.5 + entries / 8));
-                const double one_by_one = rounds * (deep * (wide ? 0.717 : 0.393) + sums * 0.544);
+                const double full = of_sm * (deep * (w4_stage_us(wm * WK) + (wide ? 0.0086 * wm * WK : 0.0)) +
+                                             sums * 0.0588 * wm * WK * (0.5 + entries / 8));
+                const double one_by_one = rounds * (deep * (wide ? 0.63 : W4_STAGE_ALONE) + sums * W4_BLOCK_US);
                 // bringing x, once for every chunk that a CTA meets, or for every pass of every run
                 const double runs = p.passes > 1 || split > 1 ? static_cast<double>((static_cast<int64_t>(rounds) + p.seg - 1) / p.seg) : 1.0;
                 const double met = 1.0 + rounds / static_cast<double>(blocks);
-                const double bring = 1.3 + entries * mine * c.planes * (staged ? 0.0079 : 0.039);
+                const double bring = 1.15 + entries * mine * c.planes * (staged ? 0.001 : 0.026);
                 p.us = (full > one_by_one ? full : one_by_one) + (p.passes > 1 ? runs * p.passes : rounds < met ? rounds : met) * bring +
-                       (split > 1 ? runs * (1.7 + 0.0154 * wm * entries) : 0.0);
+                       (split > 1 ? runs * (1.55 + 0.0107 * wm * entries) : 0.0);
                 if (p.us < best.us) best = p;
             }
 }
@@ -834,12 +850,13 @@ cudaError_t w4_t(W4Args &a, const W4Plan &p, int64_t max_chunks, int n_sm, cudaS
     a.split_shift = p.split == 1 ? 0 : p.split == 2 ? 1 : 2;
     a.wk_shift = p.wk_shift;
     a.wm = p.wm;
+    a.deep = static_cast<float>(p.deep);
+    a.per_block = static_cast<float>(a.mats * p.passes) * W4_BLOCK_US;
     a.x_shift = most >= 16 ? 0 : most >= 8 ? 1 : most >= 4 ? 2 : most >= 2 ? 3 : 4;
     a.dst_vec = a.rows % 4 == 0 && reinterpret_cast<uintptr_t>(a.dst) % 16 == 0;
     a.passes = p.passes;
     a.sp = p.sp;
     a.seg = p.seg;
-    a.tiles = (a.RT + p.wm - 1) / p.wm;
     a.red_off = W4_WARPS * w4_stages<NT>() * w4_stage_bytes(GROUPS, ZERO);
     a.tab_off = a.red_off + w4_red_bytes(NT);
     a.acc_off = a.tab_off + p.tab;
@@ -847,7 +864,7 @@ cudaError_t w4_t(W4Args &a, const W4Plan &p, int64_t max_chunks, int n_sm, cudaS
     const size_t smem = a.x_off + static_cast<size_t>(most * a.planes) * (mine * 2 * W4_KS + W4_PAD) +
                         static_cast<size_t>(mine) * (GROUPS + 1) * 8 * NT * 4;
     if (smem > W4_SMEM) return cudaErrorInvalidConfiguration;
-    const int64_t items = max_chunks * a.tiles, slots = n_sm / p.split;
+    const int64_t blocks = a.ids ? a.RT : (a.RT + p.wm - 1) / p.wm, items = max_chunks * blocks, slots = n_sm / p.split;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>((items < slots ? items : slots) * p.split));
     cfg.blockDim = dim3(32 * W4_WARPS);

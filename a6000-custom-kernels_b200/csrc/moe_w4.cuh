@@ -53,7 +53,8 @@ struct W4Args {
     // plan (launch_w4)
     int32_t planes, nc;              // MMA columns of an entry; entries of a chunk
     int32_t split_shift, wk_shift;   // 1 << split_shift CTAs of a cluster, and 1 << wk_shift warps of each, share a row's K
-    int32_t wm, tiles;               // row tiles of a block, a CTA's at a time; blocks
+    int32_t wm;                      // row tiles of a block, a CTA's at a time (for experts: at most)
+    float deep, per_block;           // a warp's stages for a block, and what a block costs besides (w4_plan)
     int32_t passes, sp;              // K passes of sp stages (of the whole cluster)
     int32_t x_shift;                 // 1 << x_shift warps bring an entry's x
     int32_t dst_vec;                 // whether four rows of dst may be written at once

@@ -14,6 +14,7 @@ stream of the call. A pass may be captured into a graph while no autograd graph 
 same leaves that was made on another stream is alive (autograd would make the capture
 wait for that stream): such a call is refused.
 """
+import threading
 import weakref
 
 import torch
@@ -116,7 +117,12 @@ def _combine(y, stride, buf, n_tok, k, weights, shared, shared_stride, stream):
 
 # ---- gradients -----------------------------------------------------------------
 
-_alive = weakref.WeakSet()      # autograd nodes of the calls below, with the stream and the leaves of each
+_alive, _alive_lock = weakref.WeakSet(), threading.Lock()      # autograd nodes of the calls below: `made`, a stream and leaves
+
+
+def _remember(node):
+    with _alive_lock:
+        _alive.add(node)
 
 
 def _leaves(*tensors):
@@ -126,7 +132,9 @@ def _leaves(*tensors):
 def _check_capture(st, *tensors):
     if torch.cuda.is_current_stream_capturing():
         leaves = set(_leaves(*tensors))
-        if any(made != st and not leaves.isdisjoint(of) for made, of in [node.made for node in _alive]):
+        with _alive_lock:
+            alive = [node.made for node in _alive]
+        if any(made != st and not leaves.isdisjoint(of) for made, of in alive):
             raise bad("an autograd graph of the same leaves, made on another stream, is alive: drop it before the capture")
 
 
@@ -146,17 +154,17 @@ def _differentiable_once(backward):
 
 class _Gather(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, stride, buf, n_tok, k, made, rows, stream):
+    def forward(ctx, x, buf, n_tok, k, made, rows):
         ctx.save_for_backward(buf)
         ctx.call, ctx.made = (n_tok, k), (made, _leaves(x))
-        _alive.add(ctx)
-        return _gather(x, stride, buf, n_tok, k, stream) if rows is None else rows
+        _remember(ctx)
+        return rows()
 
     @staticmethod
     @_differentiable_once
     def backward(ctx, g):
         g, stride = _grad_rows(g)
-        return _combine(g, stride, ctx.saved_tensors[0], *ctx.call, None, None, 0, None), None, None, None, None, None, None, None
+        return _combine(g, stride, ctx.saved_tensors[0], *ctx.call, None, None, 0, None), None, None, None, None, None
 
 
 class _Combine(torch.autograd.Function):
@@ -164,7 +172,7 @@ class _Combine(torch.autograd.Function):
     def forward(ctx, y, stride, buf, n_tok, k, weights, shared, shared_stride, made, stream):
         ctx.save_for_backward(y if weights.requires_grad else None, buf, weights)     # d_y needs the weights alone
         ctx.call, ctx.made = (stride, n_tok, k), (made, _leaves(y, weights, shared))
-        _alive.add(ctx)
+        _remember(ctx)
         return _combine(y, stride, buf, n_tok, k, weights, shared, shared_stride, stream)
 
     @staticmethod
@@ -207,7 +215,8 @@ def gather_sorted(x, order, stream=None):
     ctx, st = on(x.device, stream)
     with ctx:       # (the backward pass runs on the stream that is current here)
         _check_capture(st, x)
-        return _Gather.apply(x, stride, order._buf, order.n_tok, order.k, st, None, stream)
+        return _Gather.apply(x, order._buf, order.n_tok, order.k, st,
+                             lambda: _gather(x, stride, order._buf, order.n_tok, order.k, stream))
 
 
 def dispatch_sorted(x, ids, n_experts, stream=None):
@@ -216,15 +225,20 @@ def dispatch_sorted(x, ids, n_experts, stream=None):
     stride = _rows_of(x, "x", order.n_tok, order)
     n_tok, k, H = order.n_tok, order.k, x.shape[1]
     ctx, st = on(x.device, stream)
-    with ctx:
-        grad = x.requires_grad and torch.is_grad_enabled()
-        if grad:
-            _check_capture(st, x)
+
+    def rows():
         out = x.new_empty((n_tok * k, H))
         check(lib().moe_b200_dispatch_sorted(x.data_ptr(), ELEM[x.dtype], stride, H, ids.data_ptr(), order._stride, n_tok, k,
-                                             n_experts, *order._allocate(ids), out.data_ptr(), st))
-        if grad:
-            out = _Gather.apply(x, stride, order._buf, n_tok, k, st, out, stream)
+                                             n_experts, *at, out.data_ptr(), st))
+        return out
+    with ctx:
+        if x.requires_grad and torch.is_grad_enabled():
+            _check_capture(st, x)
+            at = order._allocate(ids)
+            out = _Gather.apply(x, order._buf, n_tok, k, st, rows)
+        else:
+            at = order._allocate(ids)
+            out = rows()
     if stream is not None:
         keep(stream, x, ids, order._buf, out)
     return out, order

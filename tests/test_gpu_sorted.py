@@ -351,3 +351,75 @@ def test_dispatch_is_sort_and_gather(pkg, cuda):
         other = pkg.sort_by_expert(t, E)
         assert torch.equal(other._buf, order._buf) and torch.equal(rows, pkg.gather_sorted(x, other))
         assert pkg.moe_cache.device_error() == (pkg.moe_cache.DERR_BAD_ID if n > 200 else 0)
+
+
+def test_results_may_be_written_in_place(pkg, cuda):
+    rng = np.random.default_rng(12)
+    n, k, E, H = 30, 2, 4, 16
+    ids = torch.from_numpy(draw_ids(rng, n, k, E)).to(cuda)
+    x = rand(rng, (n, H), "f32", cuda).requires_grad_()
+    w = torch.rand((n, k), device=cuda)
+    rows, order = pkg.dispatch_sorted(x, ids, E)
+    rows.mul_(2.0)
+    other = pkg.gather_sorted(x, order).mul_(2.0)
+    assert torch.equal(rows, other)
+    out = pkg.combine_sorted(rows, order, w).add_(1.0)
+    g, = torch.autograd.grad(out, x, torch.ones_like(out))
+    want = 2.0 * w.sum(1, keepdim=True).expand(n, H)
+    assert (g - want).abs().max() <= 1e-6 * want.abs().max()       # sums of two products: 3 roundings of 2^-24
+    rows, order = pkg.dispatch_sorted(x, ids, E)
+    out = pkg.combine_sorted(rows, order, w.requires_grad_())
+    with torch.no_grad():
+        rows.add_(1.0)                                              # saved for d_weights
+    with pytest.raises(RuntimeError, match="modified"):
+        out.sum().backward()
+
+
+def test_calls_at_once_on_two_streams(pkg, cuda):
+    rng = np.random.default_rng(13)
+    jobs = []
+    for n, k, E, H in ((5000, 4, 40, 96), (700, 3, 16, 33)):
+        ids = torch.from_numpy(draw_ids(rng, n, k, E, 0.1)).to(cuda)
+        x, w = rand(rng, (n, H), "bf16", cuda), torch.rand((n, k), device=cuda)
+        rows, order = pkg.dispatch_sorted(x, ids, E)
+        jobs.append((ids, E, x, w, rows, order._buf.clone(), pkg.combine_sorted(rows, order, w), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(8):
+        got = []
+        for ids, E, x, w, *_, st in jobs:
+            with torch.cuda.stream(st):
+                rows, order = pkg.dispatch_sorted(x, ids, E)
+                got.append((rows, order._buf, pkg.combine_sorted(rows, order, w)))
+        torch.cuda.synchronize()
+        for job, g in zip(jobs, got):
+            assert all(torch.equal(a, b) for a, b in zip(job[4:7], g))
+
+
+def test_refusals(pkg, cuda):
+    ids = torch.zeros((4, 2), dtype=torch.int32, device=cuda)
+    x, y, w = torch.zeros((4, 8), device=cuda), torch.zeros((8, 8), device=cuda), torch.zeros((4, 2), device=cuda)
+    order = pkg.sort_by_expert(ids, 3)
+    for f in (lambda: pkg.sort_by_expert(ids.long(), 3), lambda: pkg.sort_by_expert(ids[:, 0], 3), lambda: pkg.sort_by_expert(ids.t(), 3),
+              lambda: pkg.sort_by_expert(ids[:1].expand(4, 2), 3), lambda: pkg.sort_by_expert(ids, 0), lambda: pkg.sort_by_expert(ids, 1025),
+              lambda: pkg.gather_sorted(x[:3], order), lambda: pkg.gather_sorted(x.double(), order), lambda: pkg.gather_sorted(x.t(), order),
+              lambda: pkg.gather_sorted(x.cpu(), order), lambda: pkg.gather_sorted(x[:, :0], order), lambda: pkg.gather_sorted(x[0], order),
+              lambda: pkg.gather_sorted(x[:1].expand(4, 8), order), lambda: pkg.dispatch_sorted(x[:3], ids, 3),
+              lambda: pkg.combine_sorted(x, order, w), lambda: pkg.combine_sorted(y, order, w.half()), lambda: pkg.combine_sorted(y, order, w[:3]),
+              lambda: pkg.combine_sorted(y, order, w.t().contiguous().t()), lambda: pkg.combine_sorted(y, order, None),
+              lambda: pkg.combine_sorted(y, order, w, shared=x.half()), lambda: pkg.combine_sorted(y, order, w, shared=x[:, :4]),
+              lambda: pkg.combine_sorted(y, order, w, shared=x[:3])):
+        with pytest.raises(pkg.MoeError):
+            f()
+    assert pkg.moe_cache.device_error() == 0
+
+
+def test_uses_between_the_forms(pkg, cuda):
+    """Rows long enough that few entries would fill the GPU several times with CTAs that all sort."""
+    rng = np.random.default_rng(14)
+    for n, k, E, H in ((2000, 1, 30, 2048), (300, 2, 9, 9000)):
+        ids = draw_ids(rng, n, k, E, 0.1)
+        x = rand(rng, (n, H), "bf16", cuda)
+        rows, order = pkg.dispatch_sorted(x, torch.from_numpy(ids).to(cuda), E)
+        ref_rows = check_order(order, ids, E)[0]
+        live = torch.from_numpy(ref_rows[ref_rows >= 0]).to(cuda).long()
+        assert torch.equal(rows[: live.numel()], x[live // k]) and not rows[live.numel():].any()

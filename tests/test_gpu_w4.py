@@ -299,3 +299,126 @@ def test_routed_experts_sorted_and_combined(pkg, cuda, n):
     tol = (ey * w64[..., None]).sum(1) * 1.01 + R.combine_tol(ref, parts, k, "f32")
     assert (np.abs(out.double().cpu().numpy() - ref) <= tol).all()
     assert pkg.moe_cache.device_error() == 0
+
+
+def test_calls_behind_one_another_and_at_once(pkg, cuda):
+    """Calls that overlap: each one's x is the result before it, and its ids those of an order; on two streams at a time."""
+    rng = np.random.default_rng(9)
+    E, F, H, k = 12, 160, 320, 3
+    up, down = Case(pkg, cuda, rng, E, F, H, 64, True), Case(pkg, cuda, rng, E, H, F, 32, False)
+    one = Case(pkg, cuda, rng, 1, H, H, 128, False)
+    sets = []
+    for n in (1, 30, 400):
+        x, _ = make_x(rng, (n, H), "f32", cuda)
+        sets.append((x, torch.from_numpy(rng.integers(0, E, size=(n, k)).astype(np.int32)).to(cuda)))
+
+    def chain(x, ids, wait=lambda: None):
+        for _ in range(3):
+            rows, order = pkg.dispatch_sorted(x, ids, E)
+            wait()
+            ex = order.experts.view(-1, 1)
+            h = pkg.w4_mul_mat_id(up.w, rows, ex)[:, 0]
+            wait()
+            y = pkg.w4_mul_mat_id(down.w, h, ex)[:, 0]
+            wait()
+            x = pkg.combine_sorted(y, order, torch.full(ids.shape, 1.0 / k, device=cuda))
+            wait()
+            x = pkg.w4_mul_mat(one.w, x)
+            wait()
+            x = x / x.abs().amax()
+        return x
+    want = [chain(*s, wait=torch.cuda.synchronize) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, st in zip(sets, streams):
+            with torch.cuda.stream(st):
+                got.append(chain(*s))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = [chain(*s) for s in sets]
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, outs))
+    assert pkg.moe_cache.device_error() == 0
+
+
+def test_given_workspaces(pkg, cuda):
+    rng = np.random.default_rng(10)
+    c, one = Case(pkg, cuda, rng, 5, 70, 300, 64, True), Case(pkg, cuda, rng, 1, 70, 300, 64, True)
+    for n, k, per_pick in ((40, 2, False), (600, 2, True)):
+        x, _ = make_x(rng, (n, k, 300) if per_pick else (n, 300), "bf16", cuda)
+        ids = torch.from_numpy(rng.integers(0, 5, size=(n, k)).astype(np.int32)).to(cuda)
+        need = pkg.w4_workspace_size(c.w, n, k, x.dtype, per_pick)
+        assert need > 0
+        ws = torch.full((need + 64,), 255, dtype=torch.uint8, device=cuda)
+        assert torch.equal(pkg.w4_mul_mat_id(c.w, x, ids, workspace=ws[:need]), pkg.w4_mul_mat_id(c.w, x, ids))
+        assert (ws[need:] == 255).all()
+        with pytest.raises(pkg.MoeError, match="too small"):
+            pkg.w4_mul_mat_id(c.w, x, ids, workspace=ws[: need - 16])
+        with pytest.raises(pkg.MoeError, match="aligned"):
+            pkg.w4_mul_mat_id(c.w, x, ids, workspace=ws[1: need + 1])
+    x, _ = make_x(rng, (40, 300), "f32", cuda)
+    ws = torch.empty(pkg.w4_workspace_size(one.w, 40, 0, x.dtype), dtype=torch.uint8, device=cuda)
+    assert torch.equal(pkg.w4_mul_mat(one.w, x, workspace=ws), pkg.w4_mul_mat(one.w, x))
+
+
+def test_many_experts_and_picks(pkg, cuda):
+    """1024 experts; 1024 picks, the last that every CTA groups by itself, and the first that a launch of its own does."""
+    rng = np.random.default_rng(11)
+    c = Case(pkg, cuda, rng, 1024, 16, 32, 32, False)
+    for n, k in ((512, 2), (205, 5), (1024, 1), (1, 1)):
+        ids = rng.integers(0, 1024, size=(n, k)).astype(np.int32)
+        x, x64 = make_x(rng, (n, 32), "f16", cuda)
+        got = pkg.w4_mul_mat_id(c.w, x, torch.from_numpy(ids).to(cuda)).double().cpu().numpy()
+        ref, mag = product(c, x64, ids)
+        assert (np.abs(got - ref) <= R.w4_tol(mag, 32)).all()
+
+
+def test_offsets_past_32_bits(pkg, cuda):
+    """Matrices of more than 2^32 bytes: the last experts' values."""
+    E, rows, K = 600, 2048, 8192
+    g = torch.Generator(device=cuda).manual_seed(1)
+    codes = torch.empty((E, rows, K // 2), dtype=torch.uint8, device=cuda)
+    codes.random_(0, 256, generator=g)
+    scales = torch.full((E, rows, K // 256), 0.01, dtype=torch.bfloat16, device=cuda)
+    w = pkg.W4Weights(codes, scales, K, 256)
+    x = torch.randn((2, K), generator=g, device=cuda)
+    ids = torch.tensor([[E - 1, 0], [E - 2, E // 2]], dtype=torch.int32, device=cuda)
+    y = pkg.w4_mul_mat_id(w, x, ids)
+    for t in range(2):
+        for p in range(2):
+            e = int(ids[t, p])
+            q = torch.stack([codes[e] & 15, codes[e] >> 4], -1).view(rows, K).double()
+            s = float(torch.tensor(0.01, dtype=torch.bfloat16))
+            ref, mag = ((q - 8) * s) @ x[t].double(), ((q + 8) * s) @ x[t].double().abs()
+            assert ((y[t, p].double() - ref).abs().cpu().numpy() <= R.w4_tol(mag.cpu().numpy(), K)).all()
+
+
+def test_refusals(pkg, cuda):
+    codes, scales = torch.zeros((3, 8, 32), dtype=torch.uint8, device=cuda), torch.ones((3, 8, 2), dtype=torch.float16, device=cuda)
+    zeros = torch.zeros((3, 8, 2), dtype=torch.uint8, device=cuda)
+    W = pkg.W4Weights
+    w, one = W(codes, scales, 64, 32), W(codes[0], scales[0], 64, 32)
+    x, ids = torch.zeros((4, 64), device=cuda), torch.zeros((4, 2), dtype=torch.int32, device=cuda)
+    b = torch.zeros((3, 8), device=cuda)
+    for f in (lambda: W(codes.int(), scales, 64, 32), lambda: W(codes, scales.float(), 64, 32), lambda: W(codes, scales, 66, 32),
+              lambda: W(codes, scales, 64, 64), lambda: W(codes, scales, 64, 16), lambda: W(codes, scales[:2], 64, 32),
+              lambda: W(codes, scales, 64, 32, zeros=zeros.float()), lambda: W(codes, scales, 64, 32, zeros=zeros[..., :1]),
+              lambda: W(codes[..., ::2], scales, 32, 32), lambda: W(codes[0, 0], scales[0, 0], 64, 32),
+              lambda: pkg.w4_mul_mat(w, x), lambda: pkg.w4_mul_mat(one, x[:, :32]), lambda: pkg.w4_mul_mat(one, x.double()),
+              lambda: pkg.w4_mul_mat(one, x[0]), lambda: pkg.w4_mul_mat(one, x, gate=w), lambda: pkg.w4_mul_mat(one, x, gate_bias=b[:1]),
+              lambda: pkg.w4_mul_mat(one, x, bias=b), lambda: pkg.w4_mul_mat(one, x, dst=torch.empty((4, 8), device=cuda, dtype=torch.float16)),
+              lambda: pkg.w4_mul_mat(one, x, gate=W(codes[0], scales[0], 64, 32, zeros=zeros[0])), lambda: pkg.w4_mul_mat(one, x, gate=one, glu_op=9),
+              lambda: pkg.w4_mul_mat_id(w, x, ids.long()), lambda: pkg.w4_mul_mat_id(w, x[:3], ids), lambda: pkg.w4_mul_mat_id(w, x, ids[0]),
+              lambda: pkg.w4_mul_mat_id(w, x, ids, bias=b[:2]), lambda: pkg.w4_mul_mat_id(w, x, ids, bias=b.half()),
+              lambda: pkg.w4_mul_mat_id(w, x.cpu(), ids), lambda: pkg.w4_mul_mat_id(w, x, ids, dst=torch.empty((4, 2, 9), device=cuda)),
+              lambda: pkg.w4_mul_mat_id(w, x, ids, workspace=torch.empty(4, device=cuda))):
+        with pytest.raises(pkg.MoeError):
+            f()
+    assert pkg.w4_mul_mat(one, x, bias=b[0]).shape == pkg.w4_mul_mat(one, x, bias=b[:1]).shape == (4, 8)
+    assert pkg.moe_cache.device_error() == 0
