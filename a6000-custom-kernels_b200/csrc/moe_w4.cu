@@ -8,9 +8,10 @@
 // * mma.sync m16n8k16 in f16 with the weights as A, straight from the registers they were unpacked
 //   in. Its eight columns are the batch, so up to eight tokens cost what one does. (tcgen05 would
 //   take the weights through tensor memory, and the groups' sums back out of it for their scales.)
-// * four bits at the bottom of an f16 are a number as they are: the subnormal q 2^-24 (q 2^-20 four bits
-//   further up, where the tile's other eight rows lie). So unpacking eight codes is four ANDs and a
-//   shift; the tensor cores multiply subnormals exactly, and the powers of two come off at the end.
+// * four bits in an f16's mantissa are a number as they are: the subnormal q 2^-22 at bits 2 to 5, q 2^-18 at bits 6
+//   to 9 (the tile's other eight rows). So unpacking eight codes is four ANDs and a rotation; the powers of two
+//   come off at the end. The tensor cores line products up by their exponents, so zeros ahead of a subnormal's
+//   bits cost the sums as many of theirs: at bits 0 and 4 results were off by 1e-6, here by 3e-7.
 // * zeros: sum (q - z) x = sum q x - z sum x. The sums of x per group are made once, when x is staged
 //   (32 bits; the difference costs about one bit, sums of q x being twice those of (q - z) x).
 // * x: f16 as it is. bf16 times a power of two per 256 values, so that their largest is just below
@@ -39,8 +40,8 @@ constexpr int W4_RED = 20;               // floats between two columns of a warp
 constexpr int W4_PAD = 64;               // bytes behind a column of x: two columns fill the banks
 constexpr int W4_SMEM = 224 * 1024;
 constexpr int W4_ACC = 8 * 1024;         // of it at most for sums kept to a run's end, where one block's fit
-constexpr float W4_CODE = 0x1p-24f;      // a code's unit in rows g (times 16 in rows g + 8)
-constexpr float W4_UP = 4096.f;          // which comes off in two factors: with x's power of two, and at the end
+constexpr float W4_CODE = 0x1p-22f;      // a code's unit in rows g (times 16 in rows g + 8)
+constexpr float W4_UP = 2048.f;          // which comes off in two factors: with x's power of two, and at the end
 constexpr float W4_PLANE = 4096.f;       // the second plane of an f32 x holds what the first one leaves, times this
 
 // What plans count with, in us: a stage of each of the warps that share an SM's issue slots, of one by itself, adding up a block
@@ -71,7 +72,8 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const uint8_t *__restrict_
                 const int r = r0 + g + 8 * (j & 1), c = c0 + 2 * (j >> 1);
                 if (r < rows && c < K) {
                     const uint32_t b = codes[(e * rows + r) * half_k + (c >> 1)];
-                    word |= ((b & 15u) << (4 * j)) | ((c + 1 < K ? b >> 4 : 0u) << (16 + 4 * j));
+                    const uint32_t hi = c + 1 < K ? b >> 4 : 0u;
+                    word |= ((b & 15u) << (2 + 4 * j)) | __funnelshift_l(hi, hi, 18 + 4 * j);
                 }
             }
         } else {
@@ -134,12 +136,13 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// A word's eight codes as the A fragment of one MMA: rows g as q 2^-24, rows g + 8 as q 2^-20
+// A word's eight codes as the A fragment of one MMA: rows g as q 2^-22, rows g + 8 as q 2^-18
 __device__ __forceinline__ void unpack_codes(uint32_t w, uint32_t (&a)[4]) {
-    a[0] = w & 0x000F000Fu;
-    a[1] = w & 0x00F000F0u;
-    a[2] = (w >> 8) & 0x000F000Fu;
-    a[3] = (w >> 8) & 0x00F000F0u;
+    const uint32_t r = __funnelshift_r(w, w, 8);
+    a[0] = w & 0x003C003Cu;
+    a[1] = w & 0x03C003C0u;
+    a[2] = r & 0x003C003Cu;
+    a[3] = r & 0x03C003C0u;
 }
 
 // Programmatic dependent launch: calls follow one another without the gap between kernels. Behind dep_wait everything

@@ -7,7 +7,7 @@
 //   codes   4 tiles of 16 x 64 values, 512 bytes, 16 bytes per lane
 //   scales  [groups of the stage][8] words: rows g (low half) and g + 8, 16 bits each
 //   zeros   [groups of the stage][4] words: bytes of rows g, g + 8, g + 1, g + 9 (g even)
-// Word i of lane 4 g + t feeds MMA i of its tile: bits 4 j..4 j + 3 and 16 + 4 j..16 + 4 j + 3
+// Word i of lane 4 g + t feeds MMA i of its tile: the four bits from 4 j + 2 and from 4 j + 18 on (bit 32 is bit 0)
 // hold values 32 (i >> 1) + 8 t + 4 (i & 1) + 2 (j >> 1) and + 1 of row g + 8 (j & 1).
 // The order of the values along K is the kernel's own: x is read from shared memory in
 // the same order, 16 consecutive bytes of a lane for the two MMAs of a half of the tile.
