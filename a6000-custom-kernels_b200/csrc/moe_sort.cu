@@ -23,10 +23,10 @@ namespace {
 // consecutive entries and a column of counts of its own, so that an entry's
 // place is (entries of lower experts) + (of its expert in earlier CTAs) + (in
 // earlier warps) + (earlier in its warp), the same whatever ran first. Few entries
-// take one CTA, many one cluster of SORT_CTAS, whose totals meet in distributed
-// shared memory.
+// take one CTA, many one cluster, whose totals meet in distributed shared memory: of 8 CTAs,
+// or of 16 (where the GPU runs such clusters) from 32768 entries on. Its time is the instructions of so few SMs: 65536 entries
+// 12.6 us by 8 and 9.9 by 16, 131072 20.9 and 13.9.
 constexpr int SORT_THREADS = 1024;
-constexpr int SORT_CTAS = 8;
 constexpr int SORT_AHEAD = 8;   // loads in flight per lane
 
 __device__ __forceinline__ void sort_cluster_sync() {
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(const SortArgs a) {
 }
 
 // What the cluster leaves to the whole GPU: rows and experts. These writes are scattered, and an SM sends off one sector
-// per cycle (8 of them took 36 us for 131072 entries, 17 of them for these). The row kernel does it where one follows.
+// per cycle (8 of them took 31 us for 131072 entries, 21 without these writes). The row kernel does it where one follows.
 __device__ __forceinline__ void place_entry(const SortArgs &s, int64_t i, int64_t t, int j) {
     const int p = s.positions[i];
     if (p < 0) return;
@@ -550,22 +550,17 @@ cudaError_t grad_t(const RowArgs &a, cudaStream_t st) {
 
 size_t sort_smem_bytes(int warps, int E) { return sizeof(int) * static_cast<size_t>(warps + 2) * E; }
 
+// the launch of one CTA or cluster; cudaErrorNotSupported where the GPU runs no such cluster
 template <int CTAS>
 cudaError_t sort_launch(const SortArgs &a, int threads, cudaStream_t st) {
-    static bool configured[64] = {};
+    static int state[64] = {};   // by device: 1 fit to run, -1 not
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if (!configured[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(sort_kernel<CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   static_cast<int>(sort_smem_bytes(SORT_THREADS / 32, SORT_MAX_EXPERTS)));
-        if (e != cudaSuccess) return e;
-        configured[dev] = true;
-    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(CTAS);
     cfg.blockDim = dim3(static_cast<unsigned>(threads));
-    cfg.dynamicSmemBytes = sort_smem_bytes(threads / 32, a.n_experts);
+    cfg.dynamicSmemBytes = sort_smem_bytes(SORT_THREADS / 32, SORT_MAX_EXPERTS);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -573,6 +568,23 @@ cudaError_t sort_launch(const SortArgs &a, int threads, cudaStream_t st) {
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = CTAS > 1 ? 1 : 0;
+    if (!state[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(sort_kernel<CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             static_cast<int>(cfg.dynamicSmemBytes));
+        if (e != cudaSuccess) return e;
+        state[dev] = 1;
+        if (CTAS > 8) {
+            int clusters = 0;
+            e = cudaFuncSetAttribute(sort_kernel<CTAS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&clusters, sort_kernel<CTAS>, &cfg);
+            if (e != cudaSuccess || clusters < 1) {
+                cudaGetLastError();
+                state[dev] = -1;
+            }
+        }
+    }
+    if (state[dev] < 0) return cudaErrorNotSupported;
+    cfg.dynamicSmemBytes = sort_smem_bytes(threads / 32, a.n_experts);
     return cudaLaunchKernelEx(&cfg, sort_kernel<CTAS>, a);
 }
 
@@ -598,7 +610,11 @@ cudaError_t behind_sort(void (*kernel)(P...), dim3 grid, cudaStream_t st, const 
 bool sort_by_cluster(const SortArgs &a) { return a.n_entries > 4096; }
 
 cudaError_t sort_order(const SortArgs &a, cudaStream_t st) {
-    if (sort_by_cluster(a)) return sort_launch<SORT_CTAS>(a, SORT_THREADS, st);
+    if (a.n_entries >= 32768) {
+        const cudaError_t e = sort_launch<16>(a, SORT_THREADS, st);
+        if (e != cudaErrorNotSupported) return e;
+    }
+    if (sort_by_cluster(a)) return sort_launch<8>(a, SORT_THREADS, st);
     int threads = 32;
     while (threads < a.n_entries && threads < SORT_THREADS) threads <<= 1;
     return sort_launch<1>(a, threads, st);
