@@ -23,6 +23,11 @@
 // * warps that share no K need no barrier; where rows are few, the warps of a CTA, and where rows are
 //   very few or x is large the CTAs of a cluster, share K (the sums meet in shared memory, in a fixed
 //   order), and a CTA then holds its share of x only.
+// Measured (one B200, us per call among others, bytes of the weights a second): 32768 x 4096, groups of 64 with zeros, one
+// bf16 token 18.1 (4.0 TB/s); 64 tokens' 8 of 64 experts, gate and up of 1024 x 2048 50.8 (2.8 TB/s of all experts' weights);
+// 4096 x 4096, groups of 32 with zeros, 24 f16 tokens 14.2; 768 x 2048, one f32 token 3.0 in a graph (weights in L2: latency).
+// The first: 322 warp instructions per stage, 58 % of the issue slots with 3.7 warps per scheduler, the ALU 47 %, the
+// tensor pipe 22 %, DRAM 42 %: no unit is full; warps wait for issue, for fixed latencies and for the math pipes.
 #include "moe_aux.h"
 #include "moe_mx.cuh"
 #include "moe_mmq.cuh"
@@ -167,7 +172,6 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t saddr, int rank) {
 // warps (count[W4_WARPS][E], scratch) and a warp's picks are ranked by its ballots.
 __device__ int w4_group(const W4Args &a, int2 *chunk, uint16_t *entry, int *count) {
     __shared__ int warp_sum[W4_WARPS];
-    // (CTAs of the grouped form have all W4_WARPS warps)
     constexpr int THREADS = 32 * W4_WARPS, PER = W4_DIRECT / THREADS, EPT = W4_MAX_EXPERTS / THREADS;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n_entries, E = a.n_experts;
     for (int e = tid; e < W4_WARPS * E; e += THREADS) count[e] = 0;
@@ -737,7 +741,7 @@ __global__ void __launch_bounds__(32 * W4_WARPS, 1) w4_kernel(const __grid_const
 // time by the count below is taken; its constants were fitted to 22 calls (one matrix of 768 x 2048 to 32768 x 4096 with 1 to
 // 64 rows of x, experts with 1 to 64 tokens) timed in every plan: its choice is 5 % slower than the best of them on average,
 // 27 % at most (1024 x 8192, one row: 6.5 us, 5.1 without a cluster). For experts, whose chunks depend on the picks, the GPU
-// takes wm when it has counted them (64 of them, 4 tokens' 6: 20.2 us, 27.3 with the wm that a guess gave).
+// takes wm when it has counted them (64 of them, 4 tokens' 6: 20.5 us, 27.3 with the wm that a guess gave).
 // (Plans with 32 columns or with clusters of eight were never better by more than 1 %.)
 struct W4Plan {
     int nt, split, wk_shift, wm, passes, sp, seg, deep;
@@ -903,8 +907,10 @@ cudaError_t w4_nt(W4Args &a, const W4Plan &p, int64_t max_chunks, int n_sm, cuda
 
 }  // namespace
 
-// Whether a call brings x into the products' form first, once, rather than in every CTA: the launch costs 0.5 us of a
-// token's 5 (K = 2048), and saves 6 of 16 rows' 29 (one matrix, K = 4096, 32768 rows: 30.4 us for 8 rows without, 23.3 with).
+// Whether a call brings x into the products' form first, once, rather than in every CTA (us in a graph, every CTA / once):
+// n_tok KS up to 32 the launch costs 0.7 to 1.3 (one bf16 token 2048 x 2048 4.7 / 5.9); 40 to 64 it costs up to 0.7 (12 tokens
+// 2048 x 1024 5.5 / 6.2) or saves up to 6 (4 f32 tokens 4096 x 4096 14.1 / 8.2, 6 tokens' 4 of 16 experts 20.0 / 16.4); from
+// 128 on it saves (8 bf16 tokens 4096 x 4096 14.7 / 8.7) but for 32 tokens 2048 x 2048 (7.9 / 8.1).
 bool w4_staged(int64_t n_tok, int64_t KS) { return n_tok * KS > 32; }
 
 // bytes of a row of x in that form

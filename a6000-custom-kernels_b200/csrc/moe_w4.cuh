@@ -24,7 +24,7 @@ constexpr int W4_KS = 256;          // values of a stage
 constexpr int W4_CODES = W4_TILE * W4_KS / W4_KT;
 constexpr int W4_DIRECT = 1024;     // picks up to which every CTA groups them by itself
 constexpr int W4_MAX_EXPERTS = 1024;
-constexpr int W4_MAX_ZERO = 127;    // 128 + zero is exact in bf16
+constexpr int W4_MAX_ZERO = 127;
 
 __host__ __device__ constexpr int w4_stage_bytes(int groups, bool zeros) { return W4_CODES + groups * (zeros ? 48 : 32); }
 

@@ -661,7 +661,7 @@ int moe_b200_w4_pack(const moe_w4 *w, const void *codes, const void *scales, con
  * f32 [n_experts][rows] or NULL. Products and sums of 64 values are the tensor cores',
  * everything in 32 bits. x is taken as it is: F16 exactly; BF16 and F32 relative to the largest
  * of 256 consecutive values, cut off below 2^-39 of it, F32 to 2^-22 of each value. Equal calls
- * give equal bits. Made for batches that read a matrix once (up to 32 rows of F16 / BF16 or 16
+ * give equal bits. Made for batches that read a matrix once (up to 16 rows of F16 / BF16 or 8
  * of F32 per expert; more are taken in such chunks).
  * An id of -1 marks an empty slot: its row of dst is left as it was. Any other id outside
  * [0, n_experts) also leaves its row and sets the device error word (MOE_DERR_BAD_ID). A
