@@ -423,3 +423,26 @@ def test_uses_between_the_forms(pkg, cuda):
         ref_rows = check_order(order, ids, E)[0]
         live = torch.from_numpy(ref_rows[ref_rows >= 0]).to(cuda).long()
         assert torch.equal(rows[: live.numel()], x[live // k]) and not rows[live.numel():].any()
+
+
+@pytest.mark.parametrize("n", [4095, 4096, 9001])      # 8 picks each: below, at and above the larger cluster's first size
+def test_many_entries_of_a_wider_buffer_in_a_graph(pkg, cuda, n):
+    rng = np.random.default_rng(n)
+    E, k, H = 100, 8, 24
+    wide = draw_ids(rng, n, 11, E, 0.1)
+    wide[n // 2, 3], wide[n - 1, 8] = E, -7           # as empty slots, and reported
+    t, x = torch.from_numpy(wide).to(cuda), rand(rng, (n, H), "bf16", cuda)
+    pkg.dispatch_sorted(x, t[:, 2:10], E)
+    assert pkg.moe_cache.device_error() == pkg.moe_cache.DERR_BAD_ID
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        rows, order = pkg.dispatch_sorted(x, t[:, 2:10], E)
+        alone = pkg.sort_by_expert(t[:, 2:10], E)
+    for _ in range(2):
+        g.replay()
+    torch.cuda.synchronize()
+    r, _, _, offsets = check_order(order, wide[:, 2:10], E)
+    check_order(alone, wide[:, 2:10], E)
+    live = offsets[-1]
+    assert torch.equal(rows[:live], x[torch.from_numpy(r[:live] // k).long().to(cuda)]) and not rows[live:].any()
+    assert pkg.moe_cache.device_error() == pkg.moe_cache.DERR_BAD_ID and pkg.moe_cache.device_error() == 0
