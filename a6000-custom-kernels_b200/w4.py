@@ -22,7 +22,8 @@ class W4Weights:
     nibble of byte i), `scales` f16 / bf16 [..., rows, ceil(K / group)], `zeros` uint8 of
     that shape (0 to 127; None: 8). `group` is a power of two from 32 on, or at least K
     (one group a row). The sources may be dropped afterwards; calls on other streams
-    than `stream` wait for it as for any tensor made there."""
+    than `stream` wait for it as for any tensor made there. (`data`, the laid-out bytes,
+    may be copied; see moe_b200_w4_pack for kernels that write such bytes.)"""
 
     def __init__(self, codes, scales, K, group, zeros=None, stream=None):
         for t, name, types in ((codes, "codes", (torch.uint8,)), (scales, "scales", tuple(_SCALES)), (zeros, "zeros", (torch.uint8,))):

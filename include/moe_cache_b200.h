@@ -647,7 +647,10 @@ typedef struct {
  * scales [n_experts][rows][ceil(K / group)] of scale_type; zeros of that shape, one byte
  * each, or NULL with has_zeros 0. Done once per matrix; the sources are not needed
  * afterwards. A zero above 127 is taken as 127 and sets the device error word
- * (MOE_DERR_BAD_ZERO). */
+ * (MOE_DERR_BAD_ZERO). Products read the matrices ahead of the end of the kernel before
+ * them in the stream: packed bytes may be copied elsewhere by any cudaMemcpy, but where a
+ * kernel of the caller's writes them, another one (not a product of this library) or a
+ * synchronisation belongs between it and the first product. */
 size_t moe_b200_w4_packed_size(const moe_w4 *w);
 int moe_b200_w4_pack(const moe_w4 *w, const void *codes, const void *scales, const void *zeros, void *dst, size_t dst_bytes,
                      moe_stream_t stream);
@@ -658,7 +661,7 @@ int moe_b200_w4_pack(const moe_w4 *w, const void *codes, const void *scales, con
  * group, scale_type and has_zeros of w) GLU(gate . x + gate_bias, w . x + bias), glu_op and
  * glu_limit as in moe_fusion_device. ids NULL: w is one matrix (n_experts 1), which every
  * token meets (k 1). x_type MOE_TYPE_F32, _F16 or _BF16, x_row_stride in elements; biases
- * f32 [n_experts][rows] or NULL. Products and sums of 64 values are the tensor cores',
+ * f32 [n_experts][rows] or NULL. Products and sums of up to 128 values are the tensor cores',
  * everything in 32 bits. x is taken as it is: F16 exactly; BF16 and F32 relative to the largest
  * of 256 consecutive values, cut off below 2^-39 of it, F32 to 2^-22 of each value. Equal calls
  * give equal bits. Made for batches that read a matrix once (up to 16 rows of F16 / BF16 or 8

@@ -422,3 +422,33 @@ def test_refusals(pkg, cuda):
             f()
     assert pkg.w4_mul_mat(one, x, bias=b[0]).shape == pkg.w4_mul_mat(one, x, bias=b[:1]).shape == (4, 8)
     assert pkg.moe_cache.device_error() == 0
+
+
+def test_products_right_behind_the_packing(pkg, cuda):
+    """Equal bits with and without a pause between the layout of the matrix and its first products, in a graph too."""
+    rng = np.random.default_rng(21)
+    rows, K, group = 4096, 4096, 128
+    t = lambda a: torch.from_numpy(a).to(cuda)   # noqa: E731
+    codes = [t(rng.integers(0, 256, size=(rows, K // 2), dtype=np.uint8)) for _ in range(3)]
+    scales = t((0.01 * rng.random((rows, K // group))).astype(np.float16))
+    xs = [make_x(rng, (n, K), "f16", cuda)[0] for n in (1, 24)]       # 24: x is staged by a launch between
+
+    def products(q, pause=False):
+        w = pkg.W4Weights(q, scales, K, group)
+        if pause:
+            torch.cuda.synchronize()
+        return [pkg.w4_mul_mat(w, x) for x in (*xs, *xs[::-1])]
+    want = [products(q, True) for q in codes]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        got = [products(q) for q in codes]         # the memory of one matrix is the next one's
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for p, q in zip(want, got) for a, b in zip(p, q))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = [products(q) for q in codes]
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for p, q in zip(want, got) for a, b in zip(p, q))
+    assert pkg.moe_cache.device_error() == 0
