@@ -10,7 +10,7 @@
 // All of it moves bytes: nothing is computed that HBM does not hide. 16384 tokens of 2048 bf16 values, 8 of 256
 // experts each (one B200): sort 13.8 us, gather 107 (waiting for the order included; 5.6 TB/s), weighted sum 110 (5.5),
 // gradient of the gather 97 (6.2), of the sum 173 (6.6; up to 126 MB of what a kernel writes may reach HBM after
-// its end); the pass 500. One f32 token with 8 picks: 4.2 us and 3.3, the latency of the steps.
+// its end); the pass 497. One f32 token with 8 picks: 4.2 us and 3.3, the latency of the steps.
 #include "moe_aux.h"
 #include "moe_common.cuh"
 #include "moe_mx.cuh"
