@@ -4,6 +4,7 @@ time."""
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import MOE_ERR_INVALID, MoeError
 from .moe_cache import BF16, F16, F32
@@ -42,6 +43,12 @@ def keep(stream, *tensors):
         for t in tensors:
             if t is not None:
                 t.record_stream(stream)
+
+
+def no_tangents(*tensors):
+    """Refuses tensors with a forward-mode derivative, which a call would drop."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise bad("forward-mode derivatives are not offered")
 
 
 def dense_rows(x, name):

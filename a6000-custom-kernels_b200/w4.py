@@ -4,12 +4,16 @@ with a few tokens (include/moe_cache_b200.h): value = scale * (code - zero).
 Streams, outputs and workspaces as in mxfp4.py: `stream` is a torch.cuda.Stream, a
 raw handle, or None for the device's current stream; what a call makes is allocated
 there; with a raw handle the caller keeps the tensors until the stream has run it.
+
+The products have no derivatives. Where gradients are recorded and x or a bias requires
+one, a result says so (it requires grad, too), and a backward pass through it is refused;
+with `dst` the call itself is. Forward-mode derivatives are refused.
 """
 import ctypes
 
 import torch
 
-from ._call import ELEM, bad, dense_rows, given, keep, on
+from ._call import ELEM, bad, dense_rows, given, keep, no_tangents, on
 from ._lib import MoeW4, check, lib
 from .moe_cache import BF16, F16, GLU_SWIGLU
 
@@ -95,6 +99,26 @@ def _gate(gate, gate_bias, w):
         raise bad("gate_bias without a gate")
 
 
+class _NoGradient(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, call, *inputs):
+        return call()
+
+    @staticmethod
+    def backward(ctx, g):
+        raise bad("products with 4-bit matrices have no gradient: detach their inputs, or call them under torch.no_grad()")
+
+
+def _wants_grad(dst, *inputs):
+    """Whether a call's result has to carry that it depends on these inputs."""
+    no_tangents(*inputs)
+    if not (any(t is not None and t.requires_grad for t in inputs) and torch.is_grad_enabled()):
+        return False
+    if dst is not None:
+        raise bad("with dst an input that requires a gradient is refused: detach it, or call under torch.no_grad()")
+    return True
+
+
 def w4_mul_mat(w, x, gate=None, bias=None, gate_bias=None, glu_op=GLU_SWIGLU, glu_limit=0.0, dst=None, workspace=None,
                stream=None):
     """x f32 / f16 / bf16 [n_tok, K] times one 4-bit matrix (W4Weights with E = 1) -> dst f32
@@ -108,6 +132,9 @@ def w4_mul_mat(w, x, gate=None, bias=None, gate_bias=None, glu_op=GLU_SWIGLU, gl
         raise bad(f"x must be [n_tok, {w.K}] on the weights' device")
     _gate(gate, gate_bias, w)
     b, gb = _bias(bias, "bias", w), _bias(gate_bias, "gate_bias", w)
+    if _wants_grad(dst, x, bias, gate_bias):
+        return _NoGradient.apply(lambda: w4_mul_mat(w, x, gate, bias, gate_bias, glu_op, glu_limit, None, workspace, stream),
+                                 x, bias, gate_bias)
     ctx, st = on(dev, stream)
     with ctx:
         dst = x.new_empty((n_tok, w.rows), dtype=torch.float32) if dst is None else \
@@ -143,6 +170,9 @@ def w4_mul_mat_id(w, x, ids, gate=None, bias=None, gate_bias=None, glu_op=GLU_SW
         raise bad("x, ids and the weights must be on one device")
     _gate(gate, gate_bias, w)
     b, gb = _bias(bias, "bias", w), _bias(gate_bias, "gate_bias", w)
+    if _wants_grad(dst, x, bias, gate_bias):
+        return _NoGradient.apply(lambda: w4_mul_mat_id(w, x, ids, gate, bias, gate_bias, glu_op, glu_limit, None, workspace,
+                                                       stream), x, bias, gate_bias)
     ctx, st = on(dev, stream)
     with ctx:
         dst = x.new_empty((n_tok, k, rows), dtype=torch.float32) if dst is None else \
