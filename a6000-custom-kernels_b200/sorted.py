@@ -9,8 +9,8 @@ back into the tokens, with gradients -- for experts that run outside this librar
 stream; outputs are allocated on it. With a torch.cuda.Stream the inputs may be
 dropped right behind the call, with a raw handle the caller keeps them until the
 stream has run it. gather_sorted, dispatch_sorted and combine_sorted are
-differentiable once (in x, y, weights and shared); their backward pass runs on the
-stream of the call. A pass may be captured into a graph while no autograd graph of the
+differentiable once (in x, y, weights and shared; forward-mode derivatives are refused);
+their backward pass runs on the stream of the call. A pass may be captured into a graph while no autograd graph of the
 same leaves that was made on another stream is alive (autograd would make the capture
 wait for that stream): such a call is refused.
 """
@@ -20,7 +20,7 @@ import weakref
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._call import ELEM, bad, dense_rows, keep, on
+from ._call import ELEM, bad, dense_rows, keep, no_tangents, on
 from ._lib import check, lib
 
 
@@ -210,6 +210,7 @@ def gather_sorted(x, order, stream=None):
     """x f32 / f16 / bf16 [n_tok, H] -> [n_tok k, H]: the token of every sorted row,
     zeros behind the last one."""
     stride = _rows_of(x, "x", order.n_tok, order)
+    no_tangents(x)
     if not (x.requires_grad and torch.is_grad_enabled()):
         return _gather(x, stride, order._buf, order.n_tok, order.k, stream)
     ctx, st = on(x.device, stream)
@@ -223,6 +224,7 @@ def dispatch_sorted(x, ids, n_experts, stream=None):
     """sort_by_expert and gather_sorted in one call: (rows [n_tok k, H], order)."""
     order = ExpertOrder(ids, n_experts)
     stride = _rows_of(x, "x", order.n_tok, order)
+    no_tangents(x)
     n_tok, k, H = order.n_tok, order.k, x.shape[1]
     ctx, st = on(x.device, stream)
 
@@ -261,6 +263,7 @@ def combine_sorted(y, order, weights, shared=None, stream=None):
         if shared.dtype != y.dtype or shared.shape[1] != y.shape[1]:
             raise bad("shared must be [n_tok, H] of y's type")
         grad = grad or shared.requires_grad
+    no_tangents(y, weights, shared)
     if not (grad and torch.is_grad_enabled()):
         return _combine(y, stride, order._buf, n_tok, k, weights, shared, shared_stride, stream)
     ctx, st = on(y.device, stream)

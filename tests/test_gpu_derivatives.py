@@ -1,4 +1,4 @@
-"""Products with 4-bit matrices have no derivatives, and say so where one is asked for."""
+"""Products with 4-bit matrices have no derivatives, the sorted rows none in forward mode: both say so where one is asked for."""
 import numpy as np
 import pytest
 import torch
@@ -72,3 +72,21 @@ def test_the_chain_around_a_product_trains_up_to_it_only(pkg, cuda, matrices):
     # sums of 24 values in 32 bits: 23 additions
     y, at = y.detach().double(), order.positions.long()
     assert ((weights.grad.double() - y.sum(1)[at]).abs() <= 24 * 2.0 ** -24 * y.abs().sum(1)[at]).all() and x.grad is None
+
+
+def test_forward_mode_through_sorted_rows(pkg, cuda):
+    ids = torch.from_numpy(np.arange(12, dtype=np.int32).reshape(6, 2) % 3).to(cuda)
+    x, y, w = torch.randn((6, 40), device=cuda), torch.randn((12, 40), device=cuda), torch.rand((6, 2), device=cuda)
+    order = pkg.sort_by_expert(ids, 3)
+    with forward_ad.dual_level():
+        for grad in (False, True):
+            dx, dy, dw = (forward_ad.make_dual(t.clone().requires_grad_(grad), torch.ones_like(t)) for t in (x, y, w))
+            for f in (lambda: pkg.dispatch_sorted(dx, ids, 3), lambda: pkg.gather_sorted(dx, order),
+                      lambda: pkg.combine_sorted(dy, order, w), lambda: pkg.combine_sorted(y, order, dw),
+                      lambda: pkg.combine_sorted(y, order, w, shared=dx)):
+                with pytest.raises(pkg.MoeError, match="forward"):
+                    f()
+        assert torch.equal(pkg.dispatch_sorted(x, ids, 3)[0], pkg.gather_sorted(x, order))
+    # (torch.func's wrappers have no memory of their own: torch refuses them)
+    with pytest.raises(Exception):
+        torch.func.jvp(lambda t: pkg.gather_sorted(t, order), (x,), (torch.ones_like(x),))
