@@ -10,9 +10,11 @@ stream; outputs are allocated on it. With a torch.cuda.Stream the inputs may be
 dropped right behind the call, with a raw handle the caller keeps them until the
 stream has run it. gather_sorted, dispatch_sorted and combine_sorted are
 differentiable once (in x, y, weights and shared; forward-mode derivatives are refused);
-their backward pass runs on the stream of the call. A pass may be captured into a graph while no autograd graph of the
-same leaves that was made on another stream is alive (autograd would make the capture
-wait for that stream): such a call is refused.
+their backward pass runs on the stream of the call. A pass may be captured into a graph
+while no autograd graph of the same leaves that was made on another stream is alive
+(autograd would make the capture wait for that stream): next to such a graph of these
+calls a call is refused, whether it takes the leaves or what was computed from them.
+Graphs of other operations only are the caller's to drop.
 """
 import threading
 import weakref
@@ -117,7 +119,7 @@ def _combine(y, stride, buf, n_tok, k, weights, shared, shared_stride, stream):
 
 # ---- gradients -----------------------------------------------------------------
 
-_alive, _alive_lock = weakref.WeakSet(), threading.Lock()      # autograd nodes of the calls below: `made`, a stream and leaves
+_alive, _alive_lock = weakref.WeakSet(), threading.Lock()      # autograd nodes of the calls below; `made`: their stream
 
 
 def _remember(node):
@@ -125,16 +127,30 @@ def _remember(node):
         _alive.add(node)
 
 
-def _leaves(*tensors):
-    return tuple(id(t) for t in tensors if t is not None and t.requires_grad and t.is_leaf)
+def _leaves(tensors, nodes):
+    """The leaves (by id; their graphs keep them) that gradients of these tensors, and those that pass these nodes, reach."""
+    leaves = {id(t) for t in tensors if t is not None and t.requires_grad and t.is_leaf}
+    todo = [*nodes, *(t.grad_fn for t in tensors if t is not None and t.grad_fn is not None)]
+    seen = set(todo)
+    while todo:
+        for node, _ in todo.pop().next_functions:
+            if node is None or node in seen:
+                continue
+            seen.add(node)
+            if not node.next_functions and hasattr(node, "variable"):      # where a leaf's gradient is added up
+                leaves.add(id(node.variable))
+            else:
+                todo.append(node)
+    return leaves
 
 
 def _check_capture(st, *tensors):
     if torch.cuda.is_current_stream_capturing():
-        leaves = set(_leaves(*tensors))
         with _alive_lock:
-            alive = [node.made for node in _alive]
-        if any(made != st and not leaves.isdisjoint(of) for made, of in alive):
+            others = [node for node in _alive if node.made != st]
+        meet = others and not _leaves(tensors, ()).isdisjoint(_leaves((), others))
+        del others      # (the error's traceback would keep them)
+        if meet:
             raise bad("an autograd graph of the same leaves, made on another stream, is alive: drop it before the capture")
 
 
@@ -156,7 +172,7 @@ class _Gather(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, buf, n_tok, k, made, rows):
         ctx.save_for_backward(buf)
-        ctx.call, ctx.made = (n_tok, k), (made, _leaves(x))
+        ctx.call, ctx.made = (n_tok, k), made
         _remember(ctx)
         return rows()
 
@@ -171,7 +187,7 @@ class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, stride, buf, n_tok, k, weights, shared, shared_stride, made, stream):
         ctx.save_for_backward(y if weights.requires_grad else None, buf, weights)     # d_y needs the weights alone
-        ctx.call, ctx.made = (stride, n_tok, k), (made, _leaves(y, weights, shared))
+        ctx.call, ctx.made = (stride, n_tok, k), made
         _remember(ctx)
         return _combine(y, stride, buf, n_tok, k, weights, shared, shared_stride, stream)
 

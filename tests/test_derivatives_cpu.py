@@ -32,3 +32,38 @@ def test_a_product_of_4_bit_matrices_keeps_its_place_in_a_graph(pkg):
     with pytest.raises(pkg.MoeError, match="no gradient"):
         y.sum().backward()
     assert x.grad is None
+
+
+class _Made(torch.autograd.Function):
+    """Stands for the calls' autograd nodes."""
+    @staticmethod
+    def forward(ctx, t, made):
+        ctx.made = made
+        import_module("a6000-custom-kernels_b200.sorted")._remember(ctx)
+        return t * 2
+
+    @staticmethod
+    def backward(ctx, g):
+        return 2 * g, None
+
+
+def test_captures_next_to_graphs_of_the_same_leaves(pkg, monkeypatch):
+    """Whether the leaves themselves are taken or what other operations made of them, on either side."""
+    check = import_module("a6000-custom-kernels_b200.sorted")._check_capture
+    p, q = torch.ones(3, requires_grad=True), torch.ones(3, requires_grad=True)
+    for first in (lambda: _Made.apply(p, 7), lambda: _Made.apply(p * 3, 7).sum(), lambda: _Made.apply(p + torch.ones(3) @ torch.ones(3), 7)):
+        kept = first()
+        for of in (lambda: p, lambda: p.sin(), lambda: (p + q).exp(), lambda: _Made.apply(p * 5, 7)):
+            now = of()
+            monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+            for args in ((now,), (None, q, now)):
+                with pytest.raises(pkg.MoeError, match="alive"):
+                    check(8, *args)
+            check(7, now)                                     # (the stream of the kept graph)
+            check(8, q, q.cos(), None, torch.ones(3), p.detach())
+            monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+            check(8, now)
+            del now, args
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        del kept
+        check(8, p, p.sin())

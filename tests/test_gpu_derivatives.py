@@ -90,3 +90,30 @@ def test_forward_mode_through_sorted_rows(pkg, cuda):
     # (torch.func's wrappers have no memory of their own: torch refuses them)
     with pytest.raises(Exception):
         torch.func.jvp(lambda t: pkg.gather_sorted(t, order), (x,), (torch.ones_like(x),))
+
+
+def test_capture_next_to_an_eager_graph_of_what_leaves_became(pkg, cuda):
+    """The calls take no leaf but what another operation made of it: refused next to a live graph of the same leaf."""
+    ids = torch.from_numpy(np.arange(12, dtype=np.int32).reshape(6, 2) % 3).to(cuda)
+    p, d = torch.randn((6, 40), device=cuda, requires_grad=True), torch.randn((12, 40), device=cuda)
+    side = torch.cuda.Stream()
+
+    def step():
+        rows, order = pkg.dispatch_sorted(p * 2, ids, 3)
+        return rows, torch.autograd.grad(rows, p, d)[0], order
+    alive = step()
+    want = alive[1].clone()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        with pytest.raises(pkg.MoeError, match="alive"):
+            pkg.dispatch_sorted(p * 2, ids, 3)
+        with pytest.raises(pkg.MoeError, match="alive"):
+            pkg.gather_sorted(p, alive[2])
+    del alive
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        _, got, _ = step()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
