@@ -172,6 +172,7 @@ cudaError_t launch_mx_product(MxArgs &a, int NT, int64_t units, cudaStream_t st)
 // w4_min_chunk entries in each could make); where w4_staged says so `staged` is memory for x, w4_row_bytes a row.
 cudaError_t launch_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, int64_t E, int64_t rows, int64_t K,
                            int64_t group, int per_stage, uint8_t *out, int *err, cudaStream_t st);
+cudaError_t launch_w4_settle(cudaStream_t st);   // between a kernel that writes packed bytes and their first product
 int w4_min_chunk(int x_type);
 bool w4_staged(int64_t n_tok, int64_t KS);
 int64_t w4_row_bytes(int64_t KS, int groups, int x_type);

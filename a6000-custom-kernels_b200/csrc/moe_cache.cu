@@ -2623,6 +2623,12 @@ int moe_b200_w4_pack(const moe_w4 *w, const void *codes, const void *scales, con
     return MOE_OK;
 }
 
+int moe_b200_w4_settle(moe_stream_t stream) {
+    std::lock_guard<std::recursive_mutex> lock(g_mu);
+    CK(moe::launch_w4_settle(reinterpret_cast<cudaStream_t>(stream)));
+    return MOE_OK;
+}
+
 size_t moe_b200_w4_workspace_size(const moe_w4 *w, int64_t n_tok, int64_t k, int32_t x_type, int32_t x_per_pick) {
     W4Shape s{};
     const bool one_matrix = k == 0;

@@ -150,13 +150,15 @@ __device__ __forceinline__ void unpack_codes(uint32_t w, uint32_t (&a)[4]) {
     a[3] = r & 0x03C003C0u;
 }
 
-// Behind w4_pack_kernel. A product may start when the blocks of the kernel before it have ended, and what those wrote is only
-// sure to be seen behind dep_wait, but products read the matrices ahead of it. This launch is an ordinary one: it starts when
-// the packing is complete, and a product behind it later still.
+// Behind w4_pack_kernel and any other kernel that writes packed bytes. A product may start when the blocks of the kernel before
+// it have ended, and what those wrote is only sure to be seen behind dep_wait, but products read the matrices ahead of it. This
+// launch is an ordinary one: it starts when what is before it is complete, and a product behind it later still. (Matrices
+// read behind dep_wait, only brought to the L2 ahead of it, would need none: us in a graph 3.1 -> 3.7 for 768 x 2048 and one
+// f32 token, 17.5 -> 18.0 for 32768 x 4096 and one bf16 token, 5.6 -> 5.9 for 4096 x 4096.)
 __global__ void w4_settled_kernel() {}
 
 // Programmatic dependent launch: calls follow one another without the gap between kernels. Behind dep_wait everything
-// before this kernel in the stream is complete; ahead of it nothing is read but the matrices, which launch_w4_pack has
+// before this kernel in the stream is complete; ahead of it nothing is read but the matrices, which launch_w4_settle has
 // settled, and by a product behind w4_stage_kernel the ids, which that one has waited for.
 __device__ __forceinline__ void dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
@@ -942,7 +944,10 @@ cudaError_t launch_w4_pack(const uint8_t *codes, const void *scales, const uint8
         static_cast<int>((K + g - 1) / g), static_cast<int>(RT), static_cast<int>(KS), per_stage, reinterpret_cast<uint32_t *>(out),
         n, err);
     const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
+    return e != cudaSuccess ? e : launch_w4_settle(st);
+}
+
+cudaError_t launch_w4_settle(cudaStream_t st) {
     w4_settled_kernel<<<1, 1, 0, st>>>();
     return cudaGetLastError();
 }

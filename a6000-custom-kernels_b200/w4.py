@@ -26,8 +26,12 @@ class W4Weights:
     nibble of byte i), `scales` f16 / bf16 [..., rows, ceil(K / group)], `zeros` uint8 of
     that shape (0 to 127; None: 8). `group` is a power of two from 32 on, or at least K
     (one group a row). The sources may be dropped afterwards; calls on other streams
-    than `stream` wait for it as for any tensor made there. (`data`, the laid-out bytes,
-    may be copied; see moe_b200_w4_pack for kernels that write such bytes.)"""
+    than `stream` wait for it as for any tensor made there.
+
+    `data` is the laid-out bytes, for copies and broadcasts of them. Products read them ahead of
+    the end of the kernel before them; so once `data` has been asked for, which may be to
+    write it, products pay for a small launch that keeps them behind whatever did, until
+    settle() is called behind the last write."""
 
     def __init__(self, codes, scales, K, group, zeros=None, stream=None):
         for t, name, types in ((codes, "codes", (torch.uint8,)), (scales, "scales", tuple(_SCALES)), (zeros, "zeros", (torch.uint8,))):
@@ -48,13 +52,26 @@ class W4Weights:
         self.ref = ctypes.byref(self.desc)
         ctx, st = on(self.device, stream)
         with ctx:
-            self.data = codes.new_empty(max(1, lib().moe_b200_w4_packed_size(self.ref)))
+            self._data = codes.new_empty(max(1, lib().moe_b200_w4_packed_size(self.ref)))
             check(lib().moe_b200_w4_pack(self.ref, codes.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(),
-                                         self.data.data_ptr(), self.data.numel(), st))
-        self.desc.data = self.data.data_ptr()
+                                         self._data.data_ptr(), self._data.numel(), st))
+        self.desc.data = self._data.data_ptr()
+        self._open = False       # whether others may have written _data
         keep(stream, codes, scales, zeros)
         self.shape = (self.E, self.rows, K, group, scales.dtype, zeros is not None, self.device)
         self._ws_bytes = {}      # workspace sizes by call
+
+    @property
+    def data(self):
+        self._open = True
+        return self._data
+
+    def settle(self, stream=None):
+        """Behind the last write to `data`, on its stream: products need no launch of their own for it any longer."""
+        ctx, st = on(self.device, stream)
+        with ctx:
+            check(lib().moe_b200_w4_settle(st))
+        self._open = False
 
 
 def w4_workspace_size(w, n_tok, k, dtype, per_pick=False):
@@ -80,6 +97,11 @@ def _workspace(workspace, w, x, *call):
             not workspace.is_contiguous():
         raise bad("workspace must be contiguous uint8 on the weights' device")
     return workspace, workspace.data_ptr(), workspace.numel()
+
+
+def _settle(w, gate, st):
+    if w._open or (gate is not None and gate._open):
+        check(lib().moe_b200_w4_settle(st))
 
 
 def _bias(b, name, w):
@@ -140,10 +162,11 @@ def w4_mul_mat(w, x, gate=None, bias=None, gate_bias=None, glu_op=GLU_SWIGLU, gl
         dst = x.new_empty((n_tok, w.rows), dtype=torch.float32) if dst is None else \
             given(dst, "dst", torch.float32, (n_tok, w.rows), dev)
         workspace, ws_ptr, ws_bytes = _workspace(workspace, w, x, n_tok, 0, x.dtype)
+        _settle(w, gate, st)
         check(lib().moe_b200_w4_mul_mat_id(w.ref, None if gate is None else gate.ref, b, gb, glu_op, glu_limit, x.data_ptr(),
                                            ELEM[x.dtype], stride, 0, n_tok, None, 1, 1, dst.data_ptr(), ws_ptr, ws_bytes, st))
     if stream is not None:
-        keep(stream, w.data, None if gate is None else gate.data, x, bias, gate_bias, dst, workspace)
+        keep(stream, w._data, None if gate is None else gate._data, x, bias, gate_bias, dst, workspace)
     return dst
 
 
@@ -178,11 +201,12 @@ def w4_mul_mat_id(w, x, ids, gate=None, bias=None, gate_bias=None, glu_op=GLU_SW
         dst = x.new_empty((n_tok, k, rows), dtype=torch.float32) if dst is None else \
             given(dst, "dst", torch.float32, (n_tok, k, rows), dev)
         workspace, ws_ptr, ws_bytes = _workspace(workspace, w, x, n_tok, k, x.dtype, per_pick)
+        _settle(w, gate, st)
         check(lib().moe_b200_w4_mul_mat_id(w.ref, None if gate is None else gate.ref, b, gb, glu_op, glu_limit, x.data_ptr(),
                                            ELEM[x.dtype], stride, per_pick, n_tok, ids.data_ptr(), k, ids_stride,
                                            dst.data_ptr(), ws_ptr, ws_bytes, st))
     if stream is not None:
-        keep(stream, w.data, None if gate is None else gate.data, x, ids, bias, gate_bias, dst, workspace)
+        keep(stream, w._data, None if gate is None else gate._data, x, ids, bias, gate_bias, dst, workspace)
     return dst
 
 

@@ -649,11 +649,13 @@ typedef struct {
  * afterwards. A zero above 127 is taken as 127 and sets the device error word
  * (MOE_DERR_BAD_ZERO). Products read the matrices ahead of the end of the kernel before
  * them in the stream: packed bytes may be copied elsewhere by any cudaMemcpy, but where a
- * kernel of the caller's writes them, another one (not a product of this library) or a
- * synchronisation belongs between it and the first product. */
+ * kernel of another origin writes them (a broadcast over NCCL, say), moe_b200_w4_settle on its
+ * stream belongs between it and the first product (an empty kernel; one of the caller's or a
+ * synchronisation does as well). */
 size_t moe_b200_w4_packed_size(const moe_w4 *w);
 int moe_b200_w4_pack(const moe_w4 *w, const void *codes, const void *scales, const void *zeros, void *dst, size_t dst_bytes,
                      moe_stream_t stream);
+int moe_b200_w4_settle(moe_stream_t stream);
 
 /* MUL_MAT_ID of 4-bit experts, for one token or a batch:
  *   dst[(t * k + p) * rows + r] = row r of expert ids[t * ids_stride + p] . x
