@@ -952,6 +952,22 @@ cudaError_t launch_w4_settle(cudaStream_t st) {
     return cudaGetLastError();
 }
 
+static W4Key w4_key(const W4Args &a, int64_t n_tok, int n_sm) {
+    W4Key c;
+    memset(&c, 0, sizeof(c));   // (compared byte by byte)
+    c.n_tok = n_tok, c.RT = a.RT, c.KS = a.KS;
+    c.k = a.k, c.n_experts = a.n_experts, c.one_matrix = a.ids == nullptr, c.planes = a.x_type == MX_F32 ? 2 : 1, c.mats = a.mats;
+    c.groups = a.groups, c.zeros = a.zeros, c.n_sm = n_sm;
+    return c;
+}
+
+bool w4_plan_for(const W4Args &a, int64_t n_tok, int n_sm, int32_t (&out)[6]) {
+    const W4Plan p = w4_plan_of(w4_key(a, n_tok, n_sm));
+    if (p.nt == 0) return false;
+    out[0] = p.nt, out[1] = p.split, out[2] = 1 << p.wk_shift, out[3] = p.wm, out[4] = p.passes, out[5] = w4_staged(n_tok, a.KS);
+    return true;
+}
+
 cudaError_t launch_w4(W4Args &a, int64_t n_tok, uint8_t *staged, cudaStream_t st) {
     static int sms[64] = {};
     int dev = 0;
@@ -962,12 +978,7 @@ cudaError_t launch_w4(W4Args &a, int64_t n_tok, uint8_t *staged, cudaStream_t st
         if (e != cudaSuccess) return e;
     }
     a.planes = a.x_type == MX_F32 ? 2 : 1;
-    W4Key c;
-    memset(&c, 0, sizeof(c));   // (compared byte by byte)
-    c.n_tok = n_tok, c.RT = a.RT, c.KS = a.KS;
-    c.k = a.k, c.n_experts = a.n_experts, c.one_matrix = a.ids == nullptr, c.planes = a.planes, c.mats = a.mats;
-    c.groups = a.groups, c.zeros = a.zeros, c.n_sm = sms[dev];
-    const W4Plan p = w4_plan_of(c);
+    const W4Plan p = w4_plan_of(w4_key(a, n_tok, sms[dev]));
     if (p.nt == 0) return cudaErrorInvalidConfiguration;
     a.nc = 8 * p.nt / a.planes;
     int64_t max_chunks = (a.n_entries + a.nc - 1) / a.nc;
@@ -1000,7 +1011,7 @@ cudaError_t launch_w4(W4Args &a, int64_t n_tok, uint8_t *staged, cudaStream_t st
         if (e != cudaSuccess) return e;
         a.staged = staged;
     }
-    return p.nt == 1 ? w4_nt<1>(a, p, max_chunks, c.n_sm, st) : w4_nt<2>(a, p, max_chunks, c.n_sm, st);
+    return p.nt == 1 ? w4_nt<1>(a, p, max_chunks, sms[dev], st) : w4_nt<2>(a, p, max_chunks, sms[dev], st);
 }
 
 }  // namespace moe

@@ -96,3 +96,12 @@ def glu_tol(op, g, u, eg, eu, limit=0.0):
     uf = um + 1.0 if op == 2 else um
     slope = 1.2 * eg * uf + 1.2 * eu * gm
     return slope + v * (16 + 4 * gm) * 2.0 ** -24 + gm * uf * 2.0 ** -22 * (op == 1) + 2.0 ** -100
+
+
+# Of products with codes and zeros even over 0..15 (or no zeros) and x N(0, 1), relative, in the 2-norm over many outputs. A
+# chain of up to 8 tensor-core sums cuts off up to 2^-23 of each partial sum, half of it in the mean; the i-th has
+# sqrt(i / 8) of the last one's rms, so all in the same direction 6.1 * 2^-24 = 3.7e-7 of sums of q x, whose rms is 8.8 for the
+# 4.6 or more of (q - z) x: 6.9e-7. A 32-bit x is held to 2^-22, 1.4e-7 rms. The 32-bit roundings behind the tensor cores (a
+# scale, a zero, stages, warps, CTAs, passes, sums of x: 40 in a chain at most) are off by 2^-24 / sqrt(3) rms each, at
+# random: sqrt(40) * 3.4e-8 * 1.9 = 4.2e-7. Together 1.1e-6.
+W4_NORM = 1.5e-6
