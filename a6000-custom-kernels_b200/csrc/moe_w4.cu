@@ -13,7 +13,8 @@
 //   come off at the end. The tensor cores line products up by their exponents, so zeros ahead of a subnormal's
 //   bits cost the sums as many of theirs: at bits 0 and 4 results were off by 1e-6, here by 3e-7.
 // * zeros: sum (q - z) x = sum q x - z sum x. The sums of x per group are made once, when x is staged
-//   (32 bits; the difference costs about one bit, sums of q x being twice those of (q - z) x).
+//   (32 bits; errors are relative to sum |s| (q + z) |x|: about one bit more than with (q - z) x where x is of one size and
+//   zeros are codes; a large x on a code that is its zero, or zeros up to 127, cost more).
 // * x: f16 as it is. bf16 times a power of two per 256 values, so that their largest is just below
 //   2^15: what f16 then cuts off is below 2^-39 of that largest. f32 likewise in two planes (two columns)
 //   of 11 bits each, off by 2^-22 of the value at most. Everything behind the products is in 32 bits.

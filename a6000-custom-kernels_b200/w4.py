@@ -145,7 +145,11 @@ def w4_mul_mat(w, x, gate=None, bias=None, gate_bias=None, glu_op=GLU_SWIGLU, gl
                stream=None):
     """x f32 / f16 / bf16 [n_tok, K] times one 4-bit matrix (W4Weights with E = 1) -> dst f32
     [n_tok, rows] = w . x (+ bias), or GLU(gate . x + gate_bias, w . x + bias) with
-    `gate`. x is not quantised; sums are in 32 bits."""
+    `gate`. x is not quantised: f16 is exact, f32 is held to 2^-22 of a value, and f32 and
+    bf16 to 2^-39 of the largest of 256. Sums are in 32 bits, of up to 128 values in the
+    tensor cores; their errors are relative to the sum of |scale| (code + zero) |x|. Against
+    64 bits a product with N(0, 1) x is off by 1e-7 to 4e-7 (2-norm); a row's last bits may
+    change with n_tok. A NaN or an infinity in a row of x makes that row's outputs NaN."""
     stride = dense_rows(x, "x")
     dev, n_tok = w.device, x.shape[0]
     if w.E != 1:
@@ -175,7 +179,7 @@ def w4_mul_mat_id(w, x, ids, gate=None, bias=None, gate_bias=None, glu_op=GLU_SW
     """MUL_MAT_ID of 4-bit experts (moe_b200_w4_mul_mat_id): x f32 / f16 / bf16 [n_tok, K],
     or [n_tok, k, K] with a row per pick, ids i32 [n_tok, k] -> dst f32 [n_tok, k, rows] =
     experts w . x (+ bias), or GLU(gate . x + gate_bias, w . x + bias) with `gate`. Picks
-    with id -1 leave their rows of dst as they were. x is not quantised; sums are in 32 bits."""
+    with id -1 leave their rows of dst as they were. x and sums are held as in w4_mul_mat."""
     if not (isinstance(ids, torch.Tensor) and ids.is_cuda and ids.dtype == torch.int32 and ids.dim() == 2):
         raise bad("ids must be an i32 CUDA tensor [n_tok, k]")
     n_tok, k = ids.shape

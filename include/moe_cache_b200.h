@@ -663,10 +663,13 @@ int moe_b200_w4_settle(moe_stream_t stream);
  * group, scale_type and has_zeros of w) GLU(gate . x + gate_bias, w . x + bias), glu_op and
  * glu_limit as in moe_fusion_device. ids NULL: w is one matrix (n_experts 1), which every
  * token meets (k 1). x_type MOE_TYPE_F32, _F16 or _BF16, x_row_stride in elements; biases
- * f32 [n_experts][rows] or NULL. Products and sums of up to 128 values are the tensor cores',
- * everything in 32 bits. x is taken as it is: F16 exactly; BF16 and F32 relative to the largest
- * of 256 consecutive values, cut off below 2^-39 of it, F32 to 2^-22 of each value. Equal calls
- * give equal bits. Made for batches that read a matrix once (up to 16 rows of F16 / BF16 or 8
+ * f32 [n_experts][rows] or NULL. Products and sums of up to 128 values are the tensor cores'
+ * (which cut off where a 32-bit sum would round), everything else is in 32 bits. x is not quantised, but
+ * brought into f16: F16 exactly; BF16 and F32 relative to the largest of 256 consecutive values, cut off
+ * below 2^-39 of it, F32 to 2^-22 of each value. Zeros come off the sums of code * x, so
+ * errors are relative to the sum of |scale| (code + zero) |x|, not to the result: a large x on a
+ * code that is its zero leaves its roundings behind. Equal calls give equal bits; the order of a row's sums, and so
+ * its last bits, may change with n_tok. Made for batches that read a matrix once (up to 16 rows of F16 / BF16 or 8
  * of F32 per expert; more are taken in such chunks).
  * An id of -1 marks an empty slot: its row of dst is left as it was. Any other id outside
  * [0, n_experts) also leaves its row and sets the device error word (MOE_DERR_BAD_ID). A

@@ -110,3 +110,36 @@ def test_norms(pkg, cuda, n, rows, K, group, zeros, dtype):
     x = torch.randn((n, K), generator=g, device=cuda).to(DT[dtype])
     ref = m.product(x, torch.zeros((n, 1), dtype=torch.int32, device=cuda))[0][:, 0]
     assert norm(pkg.w4_mul_mat(m.w, x).double() - ref) <= R.W4_NORM * norm(ref)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_small_values_next_to_large_ones(pkg, cuda, dtype):
+    """Values 2^d below the largest of their 256, which meets code 0 and zero 0: x is held to 2^-39 of the largest (f16's least
+    step 2^-24, half of it, under 2^14 to 2^15), and nothing else is rounded but the 32-bit result."""
+    K, rows = 256, 16
+    codes = torch.zeros((rows, K // 2), dtype=torch.uint8, device=cuda)
+    codes[:, 1:] = 0x11
+    w = pkg.W4Weights(codes, torch.ones((rows, 1), dtype=torch.float16, device=cuda), K, K,
+                      zeros=torch.zeros((rows, 1), dtype=torch.uint8, device=cuda))
+    for p in (-60, 0, 100):
+        for d in (1, 8, 15, 20, 24, 28, 32, 36, 38):
+            x = torch.zeros((1, K), device=cuda, dtype=DT[dtype])
+            x[0, 0], x[0, 77] = 1.5 * 2.0 ** p, -1.25 * 2.0 ** (p - d)
+            y = pkg.w4_mul_mat(w, x).double()
+            want = -1.25 * 2.0 ** (p - d)
+            assert ((y - want).abs() <= 2.0 ** -39 * 1.5 * 2.0 ** p + 2.0 ** -24 * abs(want)).all(), (p, d, float(y[0, 0]), want)
+            assert (y[0, 0] == y[0]).all()
+
+
+def test_large_values_on_their_zeros(pkg, cuda):
+    """What the bound is relative to: a large x whose code is its zero adds nothing, but for roundings of code * x."""
+    K = 2048
+    g = torch.Generator(device=cuda).manual_seed(3)
+    m = Matrices(pkg, cuda, g, 1, 64, K, 64, True, True)
+    m.codes[:, 100] = m.zeros[:, 200 // 64] * 0x11
+    m.w = pkg.W4Weights(m.codes, m.scales, K, 64, zeros=m.zeros)
+    for size in (1.0, 2.0 ** 8, 2.0 ** 16, 2.0 ** 24):
+        x = torch.randn((3, K), generator=g, device=cuda)
+        x[:, 200:202] *= size
+        ref, mag = m.product(x, torch.zeros((3, 1), dtype=torch.int32, device=cuda))
+        assert ((pkg.w4_mul_mat(m.w, x).double() - ref[:, 0]).abs() <= tol(mag[:, 0], K)).all()
