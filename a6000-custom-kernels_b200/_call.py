@@ -46,8 +46,9 @@ def keep(stream, *tensors):
 
 
 def no_tangents(*tensors):
-    """Refuses tensors with a forward-mode derivative, which a call would drop."""
-    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    """Refuses tensors with a forward-mode derivative, which a call would drop. (They exist where
+    forward_ad._current_level >= 0: calls look at that themselves.)"""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise bad("forward-mode derivatives are not offered")
 
 

@@ -20,6 +20,7 @@ import threading
 import weakref
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ._call import ELEM, bad, dense_rows, keep, no_tangents, on
@@ -226,7 +227,8 @@ def gather_sorted(x, order, stream=None):
     """x f32 / f16 / bf16 [n_tok, H] -> [n_tok k, H]: the token of every sorted row,
     zeros behind the last one."""
     stride = _rows_of(x, "x", order.n_tok, order)
-    no_tangents(x)
+    if forward_ad._current_level >= 0:
+        no_tangents(x)
     if not (x.requires_grad and torch.is_grad_enabled()):
         return _gather(x, stride, order._buf, order.n_tok, order.k, stream)
     ctx, st = on(x.device, stream)
@@ -240,7 +242,8 @@ def dispatch_sorted(x, ids, n_experts, stream=None):
     """sort_by_expert and gather_sorted in one call: (rows [n_tok k, H], order)."""
     order = ExpertOrder(ids, n_experts)
     stride = _rows_of(x, "x", order.n_tok, order)
-    no_tangents(x)
+    if forward_ad._current_level >= 0:
+        no_tangents(x)
     n_tok, k, H = order.n_tok, order.k, x.shape[1]
     ctx, st = on(x.device, stream)
 
@@ -279,7 +282,8 @@ def combine_sorted(y, order, weights, shared=None, stream=None):
         if shared.dtype != y.dtype or shared.shape[1] != y.shape[1]:
             raise bad("shared must be [n_tok, H] of y's type")
         grad = grad or shared.requires_grad
-    no_tangents(y, weights, shared)
+    if forward_ad._current_level >= 0:
+        no_tangents(y, weights, shared)
     if not (grad and torch.is_grad_enabled()):
         return _combine(y, stride, order._buf, n_tok, k, weights, shared, shared_stride, stream)
     ctx, st = on(y.device, stream)

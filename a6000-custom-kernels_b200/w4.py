@@ -12,6 +12,7 @@ with `dst` the call itself is. Forward-mode derivatives are refused.
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from ._call import ELEM, bad, dense_rows, given, keep, no_tangents, on
 from ._lib import MoeW4, check, lib
@@ -99,11 +100,6 @@ def _workspace(workspace, w, x, *call):
     return workspace, workspace.data_ptr(), workspace.numel()
 
 
-def _settle(w, gate, st):
-    if w._open or (gate is not None and gate._open):
-        check(lib().moe_b200_w4_settle(st))
-
-
 def _bias(b, name, w):
     if b is None:
         return None
@@ -123,8 +119,8 @@ def _gate(gate, gate_bias, w):
 
 class _NoGradient(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, call, *inputs):
-        return call()
+    def forward(ctx, call, args, *inputs):
+        return call(*args)
 
     @staticmethod
     def backward(ctx, g):
@@ -133,7 +129,8 @@ class _NoGradient(torch.autograd.Function):
 
 def _wants_grad(dst, *inputs):
     """Whether a call's result has to carry that it depends on these inputs."""
-    no_tangents(*inputs)
+    if forward_ad._current_level >= 0:
+        no_tangents(*inputs)
     if not (any(t is not None and t.requires_grad for t in inputs) and torch.is_grad_enabled()):
         return False
     if dst is not None:
@@ -158,15 +155,19 @@ def w4_mul_mat(w, x, gate=None, bias=None, gate_bias=None, glu_op=GLU_SWIGLU, gl
         raise bad(f"x must be [n_tok, {w.K}] on the weights' device")
     _gate(gate, gate_bias, w)
     b, gb = _bias(bias, "bias", w), _bias(gate_bias, "gate_bias", w)
-    if _wants_grad(dst, x, bias, gate_bias):
-        return _NoGradient.apply(lambda: w4_mul_mat(w, x, gate, bias, gate_bias, glu_op, glu_limit, None, workspace, stream),
+    # (what _wants_grad asks is true of few calls)
+    if (x.requires_grad or forward_ad._current_level >= 0 or (bias is not None and bias.requires_grad) or
+            (gate_bias is not None and gate_bias.requires_grad)) and _wants_grad(dst, x, bias, gate_bias):
+        # (no closure: its variables would cost every call 0.3 us)
+        return _NoGradient.apply(w4_mul_mat, (w, x, gate, bias, gate_bias, glu_op, glu_limit, None, workspace, stream),
                                  x, bias, gate_bias)
     ctx, st = on(dev, stream)
     with ctx:
         dst = x.new_empty((n_tok, w.rows), dtype=torch.float32) if dst is None else \
             given(dst, "dst", torch.float32, (n_tok, w.rows), dev)
         workspace, ws_ptr, ws_bytes = _workspace(workspace, w, x, n_tok, 0, x.dtype)
-        _settle(w, gate, st)
+        if w._open or (gate is not None and gate._open):
+            check(lib().moe_b200_w4_settle(st))
         check(lib().moe_b200_w4_mul_mat_id(w.ref, None if gate is None else gate.ref, b, gb, glu_op, glu_limit, x.data_ptr(),
                                            ELEM[x.dtype], stride, 0, n_tok, None, 1, 1, dst.data_ptr(), ws_ptr, ws_bytes, st))
     if stream is not None:
@@ -197,15 +198,18 @@ def w4_mul_mat_id(w, x, ids, gate=None, bias=None, gate_bias=None, glu_op=GLU_SW
         raise bad("x, ids and the weights must be on one device")
     _gate(gate, gate_bias, w)
     b, gb = _bias(bias, "bias", w), _bias(gate_bias, "gate_bias", w)
-    if _wants_grad(dst, x, bias, gate_bias):
-        return _NoGradient.apply(lambda: w4_mul_mat_id(w, x, ids, gate, bias, gate_bias, glu_op, glu_limit, None, workspace,
-                                                       stream), x, bias, gate_bias)
+    # (what _wants_grad asks is true of few calls)
+    if (x.requires_grad or forward_ad._current_level >= 0 or (bias is not None and bias.requires_grad) or
+            (gate_bias is not None and gate_bias.requires_grad)) and _wants_grad(dst, x, bias, gate_bias):
+        return _NoGradient.apply(w4_mul_mat_id, (w, x, ids, gate, bias, gate_bias, glu_op, glu_limit, None, workspace, stream),
+                                 x, bias, gate_bias)
     ctx, st = on(dev, stream)
     with ctx:
         dst = x.new_empty((n_tok, k, rows), dtype=torch.float32) if dst is None else \
             given(dst, "dst", torch.float32, (n_tok, k, rows), dev)
         workspace, ws_ptr, ws_bytes = _workspace(workspace, w, x, n_tok, k, x.dtype, per_pick)
-        _settle(w, gate, st)
+        if w._open or (gate is not None and gate._open):
+            check(lib().moe_b200_w4_settle(st))
         check(lib().moe_b200_w4_mul_mat_id(w.ref, None if gate is None else gate.ref, b, gb, glu_op, glu_limit, x.data_ptr(),
                                            ELEM[x.dtype], stride, per_pick, n_tok, ids.data_ptr(), k, ids_stride,
                                            dst.data_ptr(), ws_ptr, ws_bytes, st))

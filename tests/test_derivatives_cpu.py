@@ -27,7 +27,7 @@ def test_a_product_of_4_bit_matrices_keeps_its_place_in_a_graph(pkg):
         assert not w4._wants_grad(None, x) and not w4._wants_grad(plain, x)
     with pytest.raises(pkg.MoeError, match="dst"):
         w4._wants_grad(plain, x)
-    y = w4._NoGradient.apply(lambda: torch.full((2,), 5.0), x, None, plain)
+    y = w4._NoGradient.apply(torch.full, ((2,), 5.0), x, None, plain)
     assert y.requires_grad and y.tolist() == [5.0, 5.0]
     with pytest.raises(pkg.MoeError, match="no gradient"):
         y.sum().backward()
