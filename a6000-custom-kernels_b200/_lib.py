@@ -170,7 +170,7 @@ def _declare(L):
         "moe_b200_combine_sorted_grad": (i32, [vp, i32, i64, vp, i64, i64, i64, i64, vp, vp, vp, vp, vp, vp]),
         "moe_b200_w4_packed_size": (sz, [ctypes.POINTER(MoeW4)]),
         "moe_b200_w4_pack": (i32, [ctypes.POINTER(MoeW4), vp, vp, vp, vp, sz, vp]),
-        "moe_b200_w4_plan": (i32, [ctypes.POINTER(MoeW4), i32, i64, i64, i32, i32, ctypes.POINTER(i32)]),
+        "moe_b200_w4_plan": (i32, [ctypes.POINTER(MoeW4), i32, i64, i64, i32, ctypes.POINTER(i32), ctypes.POINTER(i32)]),
         "moe_b200_w4_settle": (i32, [vp]),
         "moe_b200_w4_workspace_size": (sz, [ctypes.POINTER(MoeW4), i64, i64, i32, i32]),
         "moe_b200_w4_mul_mat_id": (i32, [ctypes.POINTER(MoeW4), ctypes.POINTER(MoeW4), vp, vp, i32, ctypes.c_float, vp, i32, i64,

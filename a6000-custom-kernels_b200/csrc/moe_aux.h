@@ -176,8 +176,10 @@ cudaError_t launch_w4_settle(cudaStream_t st);   // between a kernel that writes
 int w4_min_chunk(int x_type);
 bool w4_staged(int64_t n_tok, int64_t KS);
 int64_t w4_row_bytes(int64_t KS, int groups, int x_type);
-// how a call's work would be shared on n_sm SMs: columns of 8, CTAs and warps that share K, row tiles, passes over K, x staged
-bool w4_plan_for(const W4Args &a, int64_t n_tok, int n_sm, int32_t (&out)[6]);
+// CTAs, clusters of 2 and of 4 that run at once on the current device, and how a call's work would be shared on so many:
+// columns of 8, CTAs and warps that share K, row tiles, passes over K, x staged
+cudaError_t w4_slots(int32_t (&out)[3]);
+bool w4_plan_for(const W4Args &a, int64_t n_tok, const int32_t (&slots)[3], int32_t (&out)[6]);
 cudaError_t launch_w4(W4Args &a, int64_t n_tok, uint8_t *staged, cudaStream_t st);
 
 }  // namespace moe

@@ -2636,20 +2636,24 @@ size_t moe_b200_w4_workspace_size(const moe_w4 *w, int64_t n_tok, int64_t k, int
     return w4_ws(w->n_experts, s, n_tok, k ? k : 1, mx_elem(x_type), x_per_pick != 0, one_matrix, nullptr).bytes;
 }
 
-int moe_b200_w4_plan(const moe_w4 *w, int32_t with_gate, int64_t n_tok, int64_t k, int32_t x_type, int32_t n_sm, int32_t *out) {
+int moe_b200_w4_plan(const moe_w4 *w, int32_t with_gate, int64_t n_tok, int64_t k, int32_t x_type, const int32_t *slots,
+                     int32_t *out) {
     std::lock_guard<std::recursive_mutex> lock(g_mu);
     W4Shape s{};
     const int rc = w4_shape(w, &s);
     if (rc) return rc;
-    if (n_tok < 1 || k < 0 || n_sm < 4 || !out || mx_elem(x_type) < 0 || n_tok > (int64_t{1} << 30) / (k ? k : 1))
-        return fail(MOE_ERR_INVALID, "need n_tok >= 1, k >= 0, n_sm >= 4, an element type and room for six numbers");
+    if (n_tok < 1 || k < 0 || (slots && slots[0] < 1) || !out || mx_elem(x_type) < 0 || n_tok > (int64_t{1} << 30) / (k ? k : 1))
+        return fail(MOE_ERR_INVALID, "need n_tok >= 1, k >= 0, slots[0] >= 1, an element type and room for six numbers");
+    int32_t n[3];
+    if (slots) std::copy(slots, slots + 3, n);
+    else CK(moe::w4_slots(n));
     moe::W4Args a{};
     int32_t none = 0, got[6];
     a.RT = static_cast<int32_t>(s.RT), a.KS = static_cast<int32_t>(s.KS);
     a.k = static_cast<int32_t>(k ? k : 1), a.ids = k ? &none : nullptr;
     a.n_experts = static_cast<int32_t>(w->n_experts);
     a.x_type = mx_elem(x_type), a.mats = with_gate ? 2 : 1, a.groups = s.per_stage, a.zeros = w->has_zeros != 0;
-    if (!moe::w4_plan_for(a, n_tok, n_sm, got)) return fail(MOE_ERR_UNSUPPORTED, "no plan for this size");
+    if (!moe::w4_plan_for(a, n_tok, n, got)) return fail(MOE_ERR_UNSUPPORTED, "no plan for this size");
     std::copy(got, got + 6, out);
     return MOE_OK;
 }

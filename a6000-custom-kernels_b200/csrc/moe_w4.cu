@@ -766,7 +766,8 @@ struct W4Plan {
 // what a plan depends on
 struct W4Key {
     int64_t n_tok, RT, KS;
-    int32_t k, n_experts, one_matrix, planes, mats, groups, zeros, n_sm;
+    int32_t k, n_experts, one_matrix, planes, mats, groups, zeros;
+    int32_t slots[3];   // CTAs, clusters of 2 and clusters of 4 that run at once
 };
 
 int w4_ring(int nt) { return nt == 1 ? w4_stages<1>() : w4_stages<2>(); }
@@ -788,7 +789,8 @@ void w4_plan(const W4Key &c, int nt, W4Plan &best) {
     const double mean = c.one_matrix ? cols / c.planes : static_cast<double>(n) / static_cast<double>(chunks);
     const double entries = mean < 1.0 ? 1.0 : mean < nc ? mean : nc;   // of a chunk
     const bool wide = entries * c.planes > 8, staged = w4_staged(c.n_tok, c.KS);
-    for (int split = 1; split <= 4 && (split == 1 || split <= c.KS); split *= 2)
+    for (int split = 1; split <= 4 && (split == 1 || split <= c.KS); split *= 2) {
+        if (c.slots[split / 2] < 1) continue;
         for (int wk = 0; wk <= 4; ++wk)
             for (int wm = 1; wm << wk <= W4_WARPS; ++wm) {
                 const int WK = 1 << wk, KS = static_cast<int>(c.KS), spr = (KS + split - 1) / split;
@@ -816,11 +818,10 @@ void w4_plan(const W4Key &c, int nt, W4Plan &best) {
                 const int mine = (p.sp + split - 1) / split;                    // stages of a CTA in a pass
                 const int sums = c.mats * p.passes, deep = sums * ((mine + WK - 1) / WK);   // of a warp, for a row block
                 p.deep = deep;
-                const int64_t blocks = (c.RT + wm - 1) / wm, items = chunks * blocks, slots = c.n_sm / split;
+                const int64_t blocks = (c.RT + wm - 1) / wm, items = chunks * blocks, slots = c.slots[split / 2];
                 const double rounds = static_cast<double>((items + slots - 1) / slots);
-                const double of_sm = static_cast<double>((items * split + c.n_sm - 1) / c.n_sm);
                 // the SM's issue slots, and the way through one CTA's row blocks
-                const double full = of_sm * (deep * (w4_stage_us(wm * WK) + (wide ? 0.0086 * wm * WK : 0.0)) +
+                const double full = rounds * (deep * (w4_stage_us(wm * WK) + (wide ? 0.0086 * wm * WK : 0.0)) +
                                              sums * 0.0588 * wm * WK * (0.5 + entries / 8));
                 const double one_by_one = rounds * (deep * (wide ? 0.63 : W4_STAGE_ALONE) + sums * W4_BLOCK_US);
                 // bringing x, once for every chunk that a CTA meets, or for every pass of every run
@@ -831,6 +832,7 @@ void w4_plan(const W4Key &c, int nt, W4Plan &best) {
                        (split > 1 ? runs * (1.55 + 0.0107 * wm * entries) : 0.0);
                 if (p.us < best.us) best = p;
             }
+    }
 }
 
 // the plan of a call, remembered by its sizes (working it out takes some microseconds; the caller holds the library's lock)
@@ -855,7 +857,7 @@ const W4Plan &w4_plan_of(const W4Key &c) {
 }
 
 template <int NT, bool ZERO, int GROUPS, bool SCALE_BF16>
-cudaError_t w4_t(W4Args &a, const W4Plan &p, int64_t max_chunks, int n_sm, cudaStream_t st) {
+cudaError_t w4_t(W4Args &a, const W4Plan &p, int64_t max_chunks, int slots, cudaStream_t st) {
     static bool configured[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
@@ -885,7 +887,7 @@ cudaError_t w4_t(W4Args &a, const W4Plan &p, int64_t max_chunks, int n_sm, cudaS
     const size_t smem = a.x_off + static_cast<size_t>(most * a.planes) * (mine * 2 * W4_KS + W4_PAD) +
                         static_cast<size_t>(mine) * (GROUPS + 1) * 8 * NT * 4;
     if (smem > W4_SMEM) return cudaErrorInvalidConfiguration;
-    const int64_t blocks = a.ids ? a.RT : (a.RT + p.wm - 1) / p.wm, items = max_chunks * blocks, slots = n_sm / p.split;
+    const int64_t blocks = a.ids ? a.RT : (a.RT + p.wm - 1) / p.wm, items = max_chunks * blocks;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>((items < slots ? items : slots) * p.split));
     cfg.blockDim = dim3(32 * W4_WARPS);
@@ -903,20 +905,20 @@ cudaError_t w4_t(W4Args &a, const W4Plan &p, int64_t max_chunks, int n_sm, cudaS
 }
 
 template <int NT, bool ZERO, bool SCALE_BF16>
-cudaError_t w4_groups(W4Args &a, const W4Plan &p, int64_t max_chunks, int n_sm, cudaStream_t st) {
+cudaError_t w4_groups(W4Args &a, const W4Plan &p, int64_t max_chunks, int slots, cudaStream_t st) {
     switch (a.groups) {
-        case 8: return w4_t<NT, ZERO, 8, SCALE_BF16>(a, p, max_chunks, n_sm, st);
-        case 4: return w4_t<NT, ZERO, 4, SCALE_BF16>(a, p, max_chunks, n_sm, st);
-        case 2: return w4_t<NT, ZERO, 2, SCALE_BF16>(a, p, max_chunks, n_sm, st);
-        default: return w4_t<NT, ZERO, 1, SCALE_BF16>(a, p, max_chunks, n_sm, st);
+        case 8: return w4_t<NT, ZERO, 8, SCALE_BF16>(a, p, max_chunks, slots, st);
+        case 4: return w4_t<NT, ZERO, 4, SCALE_BF16>(a, p, max_chunks, slots, st);
+        case 2: return w4_t<NT, ZERO, 2, SCALE_BF16>(a, p, max_chunks, slots, st);
+        default: return w4_t<NT, ZERO, 1, SCALE_BF16>(a, p, max_chunks, slots, st);
     }
 }
 
 template <int NT>
-cudaError_t w4_nt(W4Args &a, const W4Plan &p, int64_t max_chunks, int n_sm, cudaStream_t st) {
+cudaError_t w4_nt(W4Args &a, const W4Plan &p, int64_t max_chunks, int slots, cudaStream_t st) {
     if (a.scale_type == MX_BF16)
-        return a.zeros ? w4_groups<NT, true, true>(a, p, max_chunks, n_sm, st) : w4_groups<NT, false, true>(a, p, max_chunks, n_sm, st);
-    return a.zeros ? w4_groups<NT, true, false>(a, p, max_chunks, n_sm, st) : w4_groups<NT, false, false>(a, p, max_chunks, n_sm, st);
+        return a.zeros ? w4_groups<NT, true, true>(a, p, max_chunks, slots, st) : w4_groups<NT, false, true>(a, p, max_chunks, slots, st);
+    return a.zeros ? w4_groups<NT, true, false>(a, p, max_chunks, slots, st) : w4_groups<NT, false, false>(a, p, max_chunks, slots, st);
 }
 
 }  // namespace
@@ -953,33 +955,67 @@ cudaError_t launch_w4_settle(cudaStream_t st) {
     return cudaGetLastError();
 }
 
-static W4Key w4_key(const W4Args &a, int64_t n_tok, int n_sm) {
+// How many CTAs, clusters of 2 and clusters of 4 run at once, one CTA to an SM: clusters do not span GPCs (one B200: 148, 74
+// and 33; 37 clusters of 4 ran in two rounds: us for 8 bf16 tokens 4096 x 14336 23.6 -> 13.6, 16 f16 tokens 3718 x 6968
+// 19.7 -> 11.9 in a graph).
+cudaError_t w4_slots(int32_t (&out)[3]) {
+    static int32_t known[64][3] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    int32_t (&n)[3] = known[dev];
+    if (!n[0]) {
+        auto *kern = w4_kernel<1, true, 8, false>;
+        int sms = 0, clusters[2] = {};
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_SMEM);
+        if (e != cudaSuccess) return e;
+        for (int i = 0; i < 2; ++i) {
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(148 * 4);
+            cfg.blockDim = dim3(32 * W4_WARPS);
+            cfg.dynamicSmemBytes = W4_SMEM;
+            cudaLaunchAttribute at[1];
+            at[0].id = cudaLaunchAttributeClusterDimension;
+            at[0].val.clusterDim.x = 2u << i;
+            at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+            cfg.attrs = at;
+            cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&clusters[i], kern, &cfg) != cudaSuccess) {
+                cudaGetLastError();
+                clusters[i] = 0;   // plans do without
+            }
+        }
+        e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+        if (e != cudaSuccess) return e;
+        n[1] = clusters[0], n[2] = clusters[1], n[0] = sms;
+    }
+    for (int i = 0; i < 3; ++i) out[i] = n[i];
+    return cudaSuccess;
+}
+
+static W4Key w4_key(const W4Args &a, int64_t n_tok, const int32_t (&slots)[3]) {
     W4Key c;
     memset(&c, 0, sizeof(c));   // (compared byte by byte)
     c.n_tok = n_tok, c.RT = a.RT, c.KS = a.KS;
     c.k = a.k, c.n_experts = a.n_experts, c.one_matrix = a.ids == nullptr, c.planes = a.x_type == MX_F32 ? 2 : 1, c.mats = a.mats;
-    c.groups = a.groups, c.zeros = a.zeros, c.n_sm = n_sm;
+    c.groups = a.groups, c.zeros = a.zeros;
+    memcpy(c.slots, slots, sizeof(slots));
     return c;
 }
 
-bool w4_plan_for(const W4Args &a, int64_t n_tok, int n_sm, int32_t (&out)[6]) {
-    const W4Plan p = w4_plan_of(w4_key(a, n_tok, n_sm));
+bool w4_plan_for(const W4Args &a, int64_t n_tok, const int32_t (&slots)[3], int32_t (&out)[6]) {
+    const W4Plan p = w4_plan_of(w4_key(a, n_tok, slots));
     if (p.nt == 0) return false;
     out[0] = p.nt, out[1] = p.split, out[2] = 1 << p.wk_shift, out[3] = p.wm, out[4] = p.passes, out[5] = w4_staged(n_tok, a.KS);
     return true;
 }
 
 cudaError_t launch_w4(W4Args &a, int64_t n_tok, uint8_t *staged, cudaStream_t st) {
-    static int sms[64] = {};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if (!sms[dev]) {
-        const cudaError_t e = cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
-        if (e != cudaSuccess) return e;
-    }
+    int32_t slots[3];
+    const cudaError_t known = w4_slots(slots);
+    if (known != cudaSuccess) return known;
     a.planes = a.x_type == MX_F32 ? 2 : 1;
-    const W4Plan p = w4_plan_of(w4_key(a, n_tok, sms[dev]));
+    const W4Plan p = w4_plan_of(w4_key(a, n_tok, slots));
     if (p.nt == 0) return cudaErrorInvalidConfiguration;
     a.nc = 8 * p.nt / a.planes;
     int64_t max_chunks = (a.n_entries + a.nc - 1) / a.nc;
@@ -1012,7 +1048,8 @@ cudaError_t launch_w4(W4Args &a, int64_t n_tok, uint8_t *staged, cudaStream_t st
         if (e != cudaSuccess) return e;
         a.staged = staged;
     }
-    return p.nt == 1 ? w4_nt<1>(a, p, max_chunks, sms[dev], st) : w4_nt<2>(a, p, max_chunks, sms[dev], st);
+    const int n = slots[p.split / 2];
+    return p.nt == 1 ? w4_nt<1>(a, p, max_chunks, n, st) : w4_nt<2>(a, p, max_chunks, n, st);
 }
 
 }  // namespace moe

@@ -685,10 +685,12 @@ int moe_b200_w4_mul_mat_id(const moe_w4 *w, const moe_w4 *gate, const float *bia
                            int64_t n_tok, const int32_t *ids, int64_t k, int64_t ids_stride, float *dst, void *workspace,
                            size_t workspace_bytes, moe_stream_t stream);
 
-/* How such a call is shared out on n_sm SMs (k 0: without ids), for tests and tuning; needs no GPU. out[6]: tiles of
- * 8 MMA columns, CTAs of a cluster and warps of each that share K, row tiles of a block (with ids: at most), passes
- * over K, whether a launch of its own stages x. */
-int moe_b200_w4_plan(const moe_w4 *w, int32_t with_gate, int64_t n_tok, int64_t k, int32_t x_type, int32_t n_sm, int32_t *out);
+/* How such a call is shared out (k 0: without ids), for tests and tuning. slots[3]: the CTAs, clusters of 2 and clusters
+ * of 4 that run at once, NULL: the current device's (only this needs a GPU). out[6]: tiles of 8 MMA columns, CTAs of a
+ * cluster and warps of each that share K, row tiles of a block (with ids: at most), passes over K, whether a launch
+ * of its own stages x. */
+int moe_b200_w4_plan(const moe_w4 *w, int32_t with_gate, int64_t n_tok, int64_t k, int32_t x_type,
+                     const int32_t *slots, int32_t *out);
 
 #ifdef __cplusplus
 }

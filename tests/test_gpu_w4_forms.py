@@ -50,9 +50,8 @@ def norm(t):
 
 @pytest.mark.parametrize("case", F.CASES, ids=lambda c: "-".join(str(int(v) if isinstance(v, bool) else v) for v in (*c[0], *c[1:])))
 def test_form(pkg, cuda, case):
-    n_sm = torch.cuda.get_device_properties(cuda).multi_processor_count
     want, rows, K, group, zeros, dtype, n, E, k, gate = case
-    assert F.form(pkg, case, n_sm) == want
+    assert F.form(pkg, case) == want
     g = torch.Generator(device=cuda).manual_seed(rows + K + n)
     up = Matrices(pkg, cuda, g, E, rows, K, group, zeros, k == 0)
     gt = Matrices(pkg, cuda, g, E, rows, K, group, zeros, k == 0) if gate else None
@@ -88,14 +87,13 @@ def test_form(pkg, cuda, case):
 @pytest.mark.parametrize("group,zeros", [(128, False), (32, True)])
 def test_tokens_alone_and_in_batches(pkg, cuda, dtype, group, zeros):
     """The order of a row's sums goes with the number of tokens: results differ between batches, by roundings only."""
-    n_sm = torch.cuda.get_device_properties(cuda).multi_processor_count
     g = torch.Generator(device=cuda).manual_seed(group)
     m = Matrices(pkg, cuda, g, 1, 4096, 4096, group, zeros, True)
     x = torch.randn((64, 4096), generator=g, device=cuda).to(DT[dtype])
     ref, mag = m.product(x, torch.zeros((64, 1), dtype=torch.int32, device=cuda))
     ref, bound, plans = ref[:, 0], tol(mag[:, 0], 4096), set()
     for n in (1, 2, 8, 24, 40, 64):
-        plans.add(tuple(F.plan(pkg, 4096, 4096, group, zeros, dtype, n, 1, 0, False, n_sm)))
+        plans.add(tuple(F.plan(pkg, 4096, 4096, group, zeros, dtype, n, 1, 0, False)))
         err = pkg.w4_mul_mat(m.w, x[:n]).double() - ref[:n]
         assert (err.abs() <= bound[:n]).all() and norm(err) <= R.W4_NORM * norm(ref[:n])
     assert len({p[2] for p in plans}) > 1          # K shared by more and by fewer warps
