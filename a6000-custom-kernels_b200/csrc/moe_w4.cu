@@ -25,10 +25,13 @@
 //   very few or x is large the CTAs of a cluster, share K (the sums meet in shared memory, in a fixed
 //   order), and a CTA then holds its share of x only.
 // Measured (one B200, us per call among others, bytes of the weights a second): 32768 x 4096, groups of 64 with zeros, one
-// bf16 token 18.0 (4.0 TB/s); 64 tokens' 8 of 64 experts, gate and up of 1024 x 2048 52.3 (2.7 TB/s of all experts' weights);
-// 4096 x 4096, groups of 32 with zeros, 24 f16 tokens 14.3; 768 x 2048, one f32 token 3.0 in a graph (weights in L2: latency).
-// The first: 322 warp instructions per stage, 58 % of the issue slots with 3.7 warps per scheduler, the ALU 47 %, the
-// tensor pipe 22 %, DRAM 42 %: no unit is full; warps wait for issue, for fixed latencies and for the math pipes.
+// bf16 token 18.0 (4.0 TB/s); 64 tokens' 8 of 64 experts, gate and up of 1024 x 2048 52.3 (2.0 TB/s of the 47 experts' that picks
+// drawn with a skew touch); 4096 x 4096, groups of 32 with zeros, 24 f16 tokens 14.3; 768 x 2048, one f32 token 3.0 in a
+// graph (weights in L2: latency).
+// The first: 322 warp instructions per stage, 58 % of the active cycles' issue slots (46 % of all) with 3.7 warps per scheduler,
+// the ALU 47 %, the tensor pipe 22 %, DRAM 42 %: warps wait for issue, for fixed latencies and for the math pipes. The
+// second leaves a third of the SMs' time idle: a CTA's share is a number of blocks, which cost more the more rows a chunk has
+// (cycles at work 38 k to 93 k of 100 k).
 #include "moe_aux.h"
 #include "moe_mx.cuh"
 #include "moe_mmq.cuh"
@@ -178,9 +181,10 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t saddr, int rank) {
 // Groups up to W4_DIRECT picks, every CTA for itself: entry[] by (expert, pick), chunk[] = {expert | count << 16,
 // first entry}; returns the number of chunks. Every CTA has to find the same order, so counts belong to
 // warps (count[W4_WARPS][E], scratch) and a warp's picks are ranked by its ballots.
-// Only the warps that hold picks are counted up, in rolled loops (us in a graph, all 16 warps / these: 4 tokens' 8 of 1000
-// experts 10.0 / 8.8, 3 tokens' 8 of 64 14.3 / 14.0; 64 tokens' 8 of 64 51.5 / 52.0). One warp that orders up to 64 picks by
-// ballots instead was 0.4 to 0.7 faster for three calls, but the longer kernel took 3 % from the last.
+// Only the warps that hold picks are counted up, in rolled loops (us in a graph, all 16 warps / these, both built and timed in
+// turn: 4 tokens' 8 of 1000 experts 9.7 / 8.5, 3 tokens' 8 of 64 13.6 / 13.3, 8 tokens' 8 of 64 15.7 / 15.5, one token's 11.1 /
+// 10.9; 64 tokens' 8 of 64 52.4 / 52.7). One warp that orders up to 64 picks by ballots instead was 0.4 to 0.7 faster for three
+// calls, but the longer kernel took 3 % from the last.
 __device__ int w4_group(const W4Args &a, int2 *chunk, uint16_t *entry, int *count) {
     __shared__ int warp_sum[W4_WARPS];
     constexpr int THREADS = 32 * W4_WARPS, PER = W4_DIRECT / THREADS, EPT = W4_MAX_EXPERTS / THREADS;
