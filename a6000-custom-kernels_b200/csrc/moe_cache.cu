@@ -22,6 +22,8 @@
 //   * Every entry point returns a status instead of aborting; a gate tensor
 //     without a table is read at its expert's offset (the reference reads
 //     expert 0 there, :200).
+#include <sys/mman.h>
+
 #include <algorithm>
 #include <cstdarg>
 #include <cstddef>
@@ -179,6 +181,24 @@ int ptr_kind(const void *p) {
     }
     g.ptr_kind[p] = kind;
     return kind;
+}
+
+// A copy of host memory that goes away behind the call. From pageable memory it has been taken when cudaMemcpyAsync
+// returns; registered memory is read when the stream comes to it, and the heap may hand some out (a block that a caller
+// pinned and freed). So it is taken from pages of our own, which nobody registers.
+cudaError_t upload(void *dst, const void *src, size_t bytes, cudaStream_t st) {
+    static void *pages = nullptr;
+    static size_t room = 0;
+    if (bytes > room) {
+        const size_t want = (std::max(bytes, size_t{1} << 16) + 4095) & ~size_t{4095};
+        void *p = mmap(nullptr, want, PROT_READ | PROT_WRITE, MAP_PRIVATE | MAP_ANONYMOUS, -1, 0);
+        if (p == MAP_FAILED) return cudaErrorMemoryAllocation;
+        if (pages) munmap(pages, room);
+        pages = p;
+        room = want;
+    }
+    if (bytes) memcpy(pages, src, bytes);
+    return cudaMemcpyAsync(dst, pages, bytes, cudaMemcpyHostToDevice, st);
 }
 
 bool contiguous(const moe_tensor *t) {
@@ -350,10 +370,9 @@ int publish(const Tensor &t, cudaStream_t st) {
     d.n_experts = t.n_experts;
     d.n_slots = t.n_slots;
     d.live = (t.tiered && !t.retired) ? 1 : 0;
-    CK(cudaMemcpyAsync(g.d_reg + t.id, &d, sizeof(d), cudaMemcpyHostToDevice, st));
+    CK(upload(g.d_reg + t.id, &d, sizeof(d), st));
     const int32_t n = static_cast<int32_t>(g.tensors.size());
-    CK(cudaMemcpyAsync(reinterpret_cast<char *>(g.dev) + offsetof(moe::CacheDev, n_tensors), &n, sizeof(n),
-                       cudaMemcpyHostToDevice, st));
+    CK(upload(reinterpret_cast<char *>(g.dev) + offsetof(moe::CacheDev, n_tensors), &n, sizeof(n), st));
     return MOE_OK;
 }
 
@@ -462,16 +481,14 @@ int enroll(const moe_tensor *src0, cudaStream_t st, Tensor **out) {
     }
     CK(cudaMemsetAsync(t->stamps, 0, 4 * E, st));
     CK(cudaMemsetAsync(t->seen, 0, E, st));
-    CK(cudaMemcpyAsync(t->slot_map, slot_map.data(), 4 * E, cudaMemcpyHostToDevice, st));
-    if (t->n_slots > 0)
-        CK(cudaMemcpyAsync(t->slot_owner, slot_owner.data(), 4 * static_cast<size_t>(t->n_slots), cudaMemcpyHostToDevice, st));
+    CK(upload(t->slot_map, slot_map.data(), 4 * E, st));
+    if (t->n_slots > 0) CK(upload(t->slot_owner, slot_owner.data(), 4 * static_cast<size_t>(t->n_slots), st));
     // the table goes last: no kernel reads a slot before its expert is copied
-    CK(cudaMemcpyAsync(t->table, table.data(), sizeof(char *) * E, cudaMemcpyHostToDevice, st));
+    CK(upload(t->table, table.data(), sizeof(char *) * E, st));
     g.by_ptr[key] = t;
     g.tensors.push_back(t);
     rc = publish(*t, st);
     if (rc) return rc;
-    // the host vectors above are pageable: the copies have taken them by now
     if (g.debug)
         fprintf(stderr, "[moe_b200] tensor %d %s: type %d, %d experts of %llu B, %s, %d slots (%d seeded)\n", t->id,
                 t->name.c_str(), t->type, t->n_experts, static_cast<unsigned long long>(t->expert_bytes),
@@ -1799,8 +1816,7 @@ int moe_b200_stack_prepare(const moe_layer_desc *layers, int64_t n_layers, const
     if (mixed) g_stack_mixed[workspace] = {used_a, used_b};
     else g_stack_mixed.erase(workspace);
     const StackWs sw = stack_ws(&L0, n_layers, static_cast<char *>(workspace));
-    CK(cudaMemcpyAsync(sw.layers, d.data(), sizeof(moe::StackLayer) * d.size(), cudaMemcpyHostToDevice,
-                       reinterpret_cast<cudaStream_t>(stream)));
+    CK(upload(sw.layers, d.data(), sizeof(moe::StackLayer) * d.size(), reinterpret_cast<cudaStream_t>(stream)));
     return MOE_OK;
 }
 
