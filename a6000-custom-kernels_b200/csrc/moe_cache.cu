@@ -1183,18 +1183,27 @@ int ggml_cuda_moe_cache_pin_host(const moe_tensor *t) {
     std::lock_guard<std::recursive_mutex> lock(g_mu);
     read_env();
     if (!g.enabled || !t || (t->flags & MOE_TENSOR_NO_BUFFER) || !t->data) return 0;
-    cudaPointerAttributes attrs;
-    cudaError_t err = cudaPointerGetAttributes(&attrs, t->data);
-    if (err != cudaSuccess) { cudaGetLastError(); return 0; }
-    if (attrs.type == cudaMemoryTypeHost || attrs.type == cudaMemoryTypeManaged) return 1;
-    if (attrs.type == cudaMemoryTypeDevice) return 0;
     const int64_t bs = blck_size(t->type);
     uint64_t nbytes = static_cast<uint64_t>(t->ne[0] / bs) * t->nb[0];
     for (int i = 1; i < 4; ++i) nbytes += static_cast<uint64_t>(t->ne[i] - 1) * t->nb[i];
-    const uintptr_t page = 4096;
-    const uintptr_t base = reinterpret_cast<uintptr_t>(t->data) & ~(page - 1);
-    const uintptr_t end = (reinterpret_cast<uintptr_t>(t->data) + nbytes + page - 1) & ~(page - 1);
-    err = cudaHostRegister(reinterpret_cast<void *>(base), end - base, cudaHostRegisterPortable | cudaHostRegisterReadOnly);
+    if (nbytes == 0) return 0;
+    cudaMemoryType at[2];
+    const char *ends[2] = {static_cast<const char *>(t->data), static_cast<const char *>(t->data) + nbytes - 1};
+    for (int i = 0; i < 2; ++i) {
+        cudaPointerAttributes attrs;
+        if (cudaPointerGetAttributes(&attrs, ends[i]) != cudaSuccess) { cudaGetLastError(); return 0; }
+        at[i] = attrs.type;
+    }
+    const bool first = at[0] != cudaMemoryTypeUnregistered, last = at[1] != cudaMemoryTypeUnregistered;
+    if (first && last) return at[0] == at[1] && at[0] != cudaMemoryTypeDevice ? 1 : 0;
+    if (first || last) {
+        fail(MOE_ERR_CUDA, "moe-cache: a part of %s is pinned already", t->name ? t->name : "<tensor>");
+        return 0;
+    }
+    // The tensor's bytes and no more: CUDA takes whatever lies in a registered range for pinned, read-only memory, so
+    // whole pages would take in what shares the first and the last one (other tensors, which would then count
+    // as pinned; the heap's blocks, which would be copied when a stream comes to it).
+    cudaError_t err = cudaHostRegister(const_cast<void *>(t->data), nbytes, cudaHostRegisterPortable | cudaHostRegisterReadOnly);
     if (err == cudaSuccess) {
         g.ptr_kind.erase(t->data);
         return 1;

@@ -128,7 +128,8 @@ int ggml_cuda_moe_cache_active(void);
 
 /* Replaces: bool ggml_cuda_moe_cache_pin_host(const ggml_tensor*)
  * (moe-cache.cuh:39, :372-405). 1 when t->data is GPU-readable host memory
- * after the call (registers a plain host range with cudaHostRegister). */
+ * after the call (registers a plain host range with cudaHostRegister: the tensor's
+ * bytes, not the pages they lie in; 0 where a part of them is pinned already). */
 int ggml_cuda_moe_cache_pin_host(const moe_tensor *t);
 
 /* ---- additions (no counterpart in the reference) ------------------------ */
