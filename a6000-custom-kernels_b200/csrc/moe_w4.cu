@@ -158,7 +158,7 @@ __device__ __forceinline__ void unpack_codes(uint32_t w, uint32_t (&a)[4]) {
 // it have ended, and what those wrote is only sure to be seen behind dep_wait, but products read the matrices ahead of it. This
 // launch is an ordinary one: it starts when what is before it is complete, and a product behind it later still. (Matrices
 // read behind dep_wait, only brought to the L2 ahead of it, would need none: us in a graph 3.1 -> 3.7 for 768 x 2048 and one
-// f32 token, 17.5 -> 18.0 for 32768 x 4096 and one bf16 token, 5.6 -> 5.9 for 4096 x 4096.)
+// f32 token, 17.6 -> 18.4 for 32768 x 4096 and one bf16 token, 5.6 -> 6.1 for 4096 x 4096.)
 __global__ void w4_settled_kernel() {}
 
 // Programmatic dependent launch: calls follow one another without the gap between kernels. Behind dep_wait everything
